@@ -637,6 +637,120 @@ int jkv_subtract_codewords(float* residual, int64_t H, int64_t N, int64_t D,
 int jkv_rope_table(const float* inv_freq, int64_t n_pos, void* out,
                    jkv_stream_t stream);
 
+/*
+ * A paged K/V cache for batches whose sequences differ in length: the serving
+ * form of the reference's per-sequence LayerCache
+ * (experiments_followup_mistral/evaluate_mistral_longbench.py:29-124).
+ *   pages        key and value pools of one shape, fp16 or bf16 (dtype
+ *                JKV_F16/JKV_BF16): n_pages pages of page_size slots (a power
+ *                of two, 16 to 4096) of KVH rows of D (64 or 128) elements.
+ *                Both pools have the same element strides (multiples of 8) for
+ *                page, head and slot; rows are contiguous and 16-byte aligned.
+ *   block_tables int32, B rows table_stride apart of table_width page numbers:
+ *                entry j of sequence b is slot j % page_size of page
+ *                tables[b][j / page_size].  A number outside [0, n_pages) is
+ *                never followed: it reads as zeros and nothing is written.
+ *   lengths      int32 [B] entries of each sequence, this call's new tokens
+ *                among them (what exceeds the table's room counts as that)
+ *   starts       int32 [B+1], not decreasing: sequence b's new tokens are the
+ *                packed rows [starts[b], starts[b+1]) and its last entries.
+ *                NULL: one token a sequence, row b (N = B).
+ *   positions    int32 [B] rotary position of each sequence's first new token;
+ *                NULL: its entry index (they differ once entries were evicted)
+ *   rope_theta   rotary base, angle = position * theta^(-2i/D) in 64 bits; 0:
+ *                no rotation
+ * Rows that no sequence owns are neither read nor written.
+ */
+
+/*
+ * Writes new keys (rotated, rounded once) and values into their slots.
+ *   key, value   [N,KVH,D], element strides of token and head (multiples of 8)
+ */
+int jkv_paged_append(const void* key, int64_t key_stride_t, int64_t key_stride_h,
+                     const void* value, int64_t value_stride_t,
+                     int64_t value_stride_h, int32_t dtype, void* key_pages,
+                     void* value_pages, int64_t page_stride, int64_t head_stride,
+                     int64_t slot_stride, int64_t n_pages, int64_t page_size,
+                     const int32_t* block_tables, int64_t table_stride,
+                     int64_t table_width, const int32_t* lengths,
+                     const int32_t* starts, const int32_t* positions, int64_t N,
+                     int64_t B, int64_t KVH, int64_t D, double rope_theta,
+                     jkv_stream_t stream);
+
+/*
+ * Attention of the new tokens over their sequences' entries.  A token at entry
+ * i sees the entries j <= i with j > i - window (window 0: all) or j < sinks.
+ *   q, out       [N,QH,D] of the cache's type, element strides (multiples of 8)
+ *   scale        of the scores (1/sqrt(D) for plain attention)
+ *   lse          fp32 [N,QH] contiguous or NULL: natural log of each row's sum
+ *                of exponentials
+ *   weights      fp32 [B,KVH,weight_width] (rows contiguous) or NULL: entry j <
+ *                lengths[b] receives the sum of its softmax weights over the
+ *                sequence's new tokens and the query heads of the kv head,
+ *                added to what is there with `accumulate`, stored without
+ *   max_new, max_length  the caller's bounds of a sequence's new tokens and
+ *                entries (weight_width >= max_length).  Entries past max_length
+ *                take no part; rows past max_new may be left out.
+ * A token whose entry would lie before the first sees nothing: output 0, lse
+ * -inf.
+ */
+int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                        int32_t dtype, const void* key_pages,
+                        const void* value_pages, int64_t page_stride,
+                        int64_t head_stride, int64_t slot_stride,
+                        int64_t n_pages, int64_t page_size,
+                        const int32_t* block_tables, int64_t table_stride,
+                        int64_t table_width, const int32_t* lengths,
+                        const int32_t* starts, const int32_t* positions,
+                        int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D,
+                        int64_t max_new, int64_t max_length, int64_t window,
+                        int64_t sinks, double rope_theta, float scale, void* out,
+                        int64_t out_stride_t, int64_t out_stride_h, float* lse,
+                        float* weights, int64_t weight_stride_b,
+                        int64_t weight_stride_h, int64_t weight_width,
+                        int32_t accumulate, void* workspace,
+                        int64_t workspace_bytes, jkv_stream_t stream);
+
+/* Workspace of jkv_paged_attention for these sizes (bytes). */
+int64_t jkv_paged_attention_workspace_bytes(int64_t N, int64_t B, int64_t QH,
+                                            int64_t KVH, int64_t D,
+                                            int64_t max_new, int64_t max_length,
+                                            int64_t window, int64_t sinks,
+                                            int32_t with_weights);
+
+/*
+ * The entries of each (sequence, kv head) that stay when `budget` may: the
+ * first `sinks`, the last `recent`, and between them those with the largest
+ * weights, the lower index first among equals (-0 equals 0, NaN lies below
+ * every number).  Sequences of at most `budget` entries keep all.
+ *   weights      fp32 [B,KVH,width], rows contiguous
+ *   kept         int32 [B,KVH,budget]: ascending, -1 behind the last
+ *   new_lengths  int32 [B]: min(lengths[b], budget)
+ */
+int jkv_paged_select(const float* weights, int64_t weight_stride_b,
+                     int64_t weight_stride_h, const int32_t* lengths, int64_t B,
+                     int64_t KVH, int64_t width, int64_t budget, int64_t sinks,
+                     int64_t recent, int32_t* kept, int32_t* new_lengths,
+                     jkv_stream_t stream);
+
+/*
+ * Copies row kept[b][h][j] of a sequence's key and value pages to entry j of
+ * its new pages, which must not be pages that are read (an entry copied onto
+ * itself is fine); negative entries copy nothing.  With `weights`, moved[b][h]
+ * (contiguous [B,KVH,width]) receives their weights in the new order and 0
+ * behind them.
+ */
+int jkv_paged_compact(void* key_pages, void* value_pages, int32_t dtype,
+                      int64_t page_stride, int64_t head_stride,
+                      int64_t slot_stride, int64_t n_pages, int64_t page_size,
+                      const int32_t* block_tables, int64_t table_stride,
+                      int64_t table_width, const int32_t* kept, int64_t budget,
+                      const int32_t* new_tables, int64_t new_table_stride,
+                      int64_t new_table_width, int64_t B, int64_t KVH, int64_t D,
+                      const float* weights, int64_t weight_stride_b,
+                      int64_t weight_stride_h, int64_t width, float* moved,
+                      jkv_stream_t stream);
+
 /* fp32 -> fp16 copy (the deploy round trip tables.half()), n elements. */
 int jkv_f32_to_f16(const float* src, void* dst, int64_t n, jkv_stream_t stream);
 

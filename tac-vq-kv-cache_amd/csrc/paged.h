@@ -1,0 +1,103 @@
+// What the kernels over a paged K/V cache share: the cache's description, the
+// sequences of a packed batch, and the rotary angles.
+//
+// Entry j of sequence b lies in slot j % page_size of page
+// tables[b][j / page_size].  Keys are stored rotated.  A call's new tokens are
+// packed: sequence b owns rows [starts[b], starts[b+1]) and they are its last
+// entries, so token t of T sits at entry lengths[b] - T + t and at position
+// positions[b] + t.  Entry counts and positions differ once entries have been
+// evicted.
+//
+// Device integers are not trusted: starts are clamped to the rows there are,
+// lengths to what a table row can list (and to the caller's bound), and a page number outside the pool
+// is never followed (it reads as zeros, and nothing is written to it).
+#pragma once
+
+#include "jkv_common.h"
+
+namespace jkv {
+
+struct PagedCache {
+  uint8_t* k;  // pools, addressed in bytes; K and V share their strides
+  uint8_t* v;
+  int64_t page_bytes, head_bytes, slot_bytes;
+  int32_t n_pages, page_shift;
+  const int32_t* tables;  // [B] rows table_stride apart, table_width pages each
+  int64_t table_stride, table_width;
+  const int32_t* lengths;    // [B] entries, the new tokens among them
+  const int32_t* starts;     // [B+1] packed rows of each sequence, or null: one token a sequence
+  const int32_t* positions;  // [B] position of each sequence's first new token, or null: its entry index
+  int32_t N, B;              // packed rows, sequences
+  int32_t top;               // entries a sequence can have: what its table row lists and the caller bounds
+};
+
+// one sequence of a batch
+struct PagedSeq {
+  int32_t row0, tokens;  // its packed rows
+  int32_t length;        // entries
+  int32_t pos0;          // position of its first new token
+};
+
+__device__ __forceinline__ int32_t clamp_i32(int32_t v, int32_t lo, int32_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
+
+__device__ __forceinline__ int32_t paged_length(const PagedCache& c, int32_t b) {
+  return clamp_i32(c.lengths[b], 0, c.top);
+}
+
+__device__ __forceinline__ void paged_rows(const PagedCache& c, int32_t b, int32_t* row0, int32_t* tokens) {
+  if (c.starts == nullptr) {
+    *row0 = b;
+    *tokens = 1;
+    return;
+  }
+  *row0 = clamp_i32(c.starts[b], 0, c.N);
+  *tokens = clamp_i32(c.starts[b + 1], *row0, c.N) - *row0;
+}
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedCache& c, int32_t b) {
+  PagedSeq s;
+  paged_rows(c, b, &s.row0, &s.tokens);
+  s.length = paged_length(c, b);
+  s.pos0 = c.positions != nullptr ? c.positions[b] : s.length - s.tokens;
+  return s;
+}
+
+// Turns (angle / 2 pi) per position of the D/2 frequencies, theta^(-2i/D) / 2 pi
+// in 64 bits; by value in the kernel's arguments, so no table is kept.
+struct RopeRates {
+  double turns[64];
+  int32_t on;
+};
+
+// cos and sin of position * frequency: the product and its fraction of a turn
+// in 64 bits (32 lose the angle of far positions), the functions in 32.
+__device__ __forceinline__ void rope_trig(double turns, int32_t pos, float* c, float* s) {
+  const float f = (float)__builtin_amdgcn_fract(turns * (double)pos);
+  *c = __builtin_amdgcn_cosf(f);
+  *s = __builtin_amdgcn_sinf(f);
+}
+
+// Types of the cache and the queries: 16-bit floats.
+template <int DT> struct Half16;
+template <> struct Half16<JKV_F16> {
+  typedef _Float16 T;
+  typedef half8 V8;
+  typedef half4 V4;
+};
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+template <> struct Half16<JKV_BF16> {
+  typedef __bf16 T;
+  typedef bf16x8 V8;
+  typedef bf16x4 V4;
+};
+
+// host side: fills c and the rates, or says what is wrong with them
+int paged_cache_args(PagedCache* c, const void* k, const void* v, int64_t page_stride, int64_t head_stride,
+                     int64_t slot_stride, int64_t n_pages, int64_t page_size, const int32_t* tables,
+                     int64_t table_stride, int64_t table_width, const int32_t* lengths, const int32_t* starts,
+                     const int32_t* positions, int64_t N, int64_t B, int64_t KVH, int64_t D, int64_t max_length,
+                     int32_t dtype);
+int paged_rope_args(RopeRates* r, double theta, int64_t D);
+
+}  // namespace jkv

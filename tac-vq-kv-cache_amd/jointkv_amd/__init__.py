@@ -51,6 +51,7 @@ from .packed_nested import (
     unpack_paired_progressive_indices,
     validate_packed_nested_cache,
 )
+from .paged import PagedKVCache, PagedStep, compact_pages, paged_append, paged_attention, select_entries
 from .uniform_depth_tac import ClosedLoopUniformResidualVQ
 from .v_only import ClosedLoopRunContext, DecoderStack, causal_loss, run_loss, v_only_step
 
@@ -71,10 +72,13 @@ __all__ = [
     "PackedLayoutLedger",
     "PackedNestedKVCache",
     "PackedProgressiveStream",
+    "PagedKVCache",
+    "PagedStep",
     "QuantizedKV",
     "StorageLedger",
     "clip_codebook_gradients",
     "closed_loop_attention",
+    "compact_pages",
     "decode_attention",
     "decode_attention_window",
     "deploy_tables",
@@ -88,6 +92,8 @@ __all__ = [
     "hard_residual_vq_exits",
     "pack_fixed_width",
     "pack_paired_progressive_indices",
+    "paged_append",
+    "paged_attention",
     "prefill_attention",
     "prefill_attention_from_codes",
     "paired_prefix_rates",
@@ -95,6 +101,7 @@ __all__ = [
     "relative_trajectory_attention_mse",
     "residual_vq_ledger",
     "run_loss",
+    "select_entries",
     "sgd_step",
     "unpack_action_depths",
     "unpack_fixed_width",

@@ -28,6 +28,7 @@ _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/jkv.h one for one.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -136,6 +137,25 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "jkv_rope_table": (ctypes.c_int, [_vp, _i64, _vp, _vp]),
     "jkv_f32_to_f16": (ctypes.c_int, [_vp, _vp, _i64, _vp]),
+    "jkv_paged_append": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+         _i64, _i64, _i64, _i64, _f64, _vp],
+    ),
+    "jkv_paged_attention": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+         _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f64, _f32, _vp, _i64, _i64, _vp,
+         _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp],
+    ),
+    "jkv_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32]),
+    "jkv_paged_select": (
+        ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "jkv_paged_compact": (
+        ctypes.c_int,
+        [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
+         _vp, _i64, _i64, _i64, _vp, _vp],
+    ),
 }
 
 # the fp16-output forms take the same arguments

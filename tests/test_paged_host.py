@@ -1,0 +1,145 @@
+"""Paged-cache checks that need no GPU: the definitions against one another,
+the host's page accounting, and what the C entry points refuse."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import jointkv_amd as jkv
+from jointkv_amd import _lib
+from oracle import paged_oracle as ref
+
+
+def test_attend_is_a_softmax_over_what_is_seen():
+    rng = np.random.default_rng(1)
+    q, k, v = rng.standard_normal((5, 4, 8)), rng.standard_normal((11, 2, 8)), rng.standard_normal((11, 2, 8))
+    got = ref.attend(q, k, v, 30, window=4, sinks=2, theta=100.0)
+    turned = ref.rotate(q, 30 + np.arange(5), 100.0)
+    for t in range(5):
+        at = 6 + t
+        seen = [j for j in range(11) if j <= at and (j > at - 4 or j < 2)]
+        for h in range(4):
+            e = np.exp([turned[t, h] @ k[j, h // 2] / np.sqrt(8) for j in seen])
+            want = sum(x * v[j, h // 2] for x, j in zip(e / e.sum(), seen))
+            assert np.allclose(got["out"][t, h], want)
+            assert np.isclose(got["lse"][t, h], np.log(e.sum()))
+    assert np.allclose(got["weights"].sum(), 5 * 4)
+
+
+def test_rotation_keeps_products_of_equal_distance():
+    rng = np.random.default_rng(2)
+    a, b = rng.standard_normal((2, 1, 1, 16))
+    near = (ref.rotate(a, [7], 10000.0) * ref.rotate(b, [4], 10000.0)).sum()
+    far = (ref.rotate(a, [1_000_003], 10000.0) * ref.rotate(b, [1_000_000], 10000.0)).sum()
+    assert np.isclose(near, far, rtol=1e-8)
+
+
+def test_select_prefers_weight_then_the_lower_index():
+    w = np.array([0.0, 5.0, 1.0, 1.0, np.nan, 1.0, 0.0, 0.0], dtype=np.float32)
+    assert ref.select(w, 4, 1, 1).tolist() == [0, 1, 2, 7]
+    assert ref.select(w, 8, 1, 1).tolist() == list(range(8))
+    assert ref.select(w, 7, 0, 0).tolist() == [0, 1, 2, 3, 5, 6, 7]
+
+
+def _attention_call(**overrides):
+    args = dict(q=16, qst=512, qsh=128, dtype=0, k=16, v=16, page=4096, head=2048, slot=128, n_pages=4, page_size=16,
+                tables=1, tstride=4, twidth=4, lengths=1, starts=None, positions=None, N=2, B=2, QH=4, KVH=2, D=128,
+                max_new=1, max_length=64, window=0, sinks=0, theta=10000.0, scale=0.1, out=16, ost=512, osh=128,
+                lse=None, weights=None, wsb=0, wsh=0, width=0, accumulate=0, ws=None, ws_bytes=0, stream=None)
+    args.update(overrides)
+    return _lib.load().jkv_paged_attention(*args.values())
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(dtype=2), b"fp16 or bf16"), (dict(D=96), b"head_dim"), (dict(QH=3), b"multiple"), (dict(B=-1), b"geometry"),
+    (dict(N=3), b"one new token"), (dict(page_size=8), b"power of two"), (dict(page_size=48), b"power of two"),
+    (dict(page=4097), b"strides"), (dict(slot=64), b"strides"), (dict(k=8), b"aligned"), (dict(window=-1), b"negative"),
+    (dict(max_new=-1), b"negative"), (dict(sinks=-1), b"negative"), (dict(theta=-2.0), b"rotary"),
+    (dict(theta=float("nan")), b"rotary"), (dict(scale=float("nan")), b"scale"), (dict(qst=12), b"multiples of 8"),
+    (dict(out=8), b"aligned"), (dict(weights=16, width=10), b"fewer entries"), (dict(lengths=None), b"null"),
+    (dict(out=None), b"null"), (dict(weights=16, width=64, wsb=128, wsh=64), b"workspace"), (dict(n_pages=-1), b"page"),
+])
+def test_attention_refuses_before_the_device_is_touched(change, message):
+    # only calls that fail their checks: one that passes would launch
+    assert _attention_call(**change) == _lib.JKV_EINVAL
+    assert message in _lib.load().jkv_last_error(), _lib.load().jkv_last_error()
+
+
+def test_empty_calls_are_no_ops():
+    assert _attention_call(N=0, B=0) == _lib.JKV_OK
+    lib = _lib.load()
+    assert lib.jkv_paged_append(16, 256, 128, 16, 256, 128, 0, 16, 16, 4096, 2048, 128, 4, 16, 1, 4, 4, 1, None, None, 0,
+                                0, 2, 128, 1e4, None) == _lib.JKV_OK
+    assert lib.jkv_paged_select(16, 0, 0, 1, 0, 2, 5, 4, 1, 1, 1, 1, None) == _lib.JKV_OK
+    assert lib.jkv_paged_compact(16, 16, 0, 4096, 2048, 128, 4, 16, 1, 4, 4, 1, 4, 1, 4, 4, 0, 2, 128, None, 0, 0, 0,
+                                 None, None) == _lib.JKV_OK
+
+
+def test_other_entries_refuse_before_the_device_is_touched():
+    lib = _lib.load()
+    append = [16, 256, 128, 16, 256, 128, 0, 16, 16, 4096, 2048, 128, 4, 16, 1, 4, 4, 1, None, None, 2, 2, 2, 128, 1e4, None]
+    for at, value, message in ((0, None, b"null"), (0, 8, b"aligned"), (1, 100, b"multiples"), (23, 32, b"head_dim"),
+                               (24, -1.0, b"rotary"), (13, 17, b"power of two"), (20, 3, b"one new token")):
+        call = list(append)
+        call[at] = value
+        assert lib.jkv_paged_append(*call) == _lib.JKV_EINVAL and message in lib.jkv_last_error()
+    for budget, sinks, recent in ((0, 0, 0), (4, 3, 2), (4, 5, 0), (4, -1, 0), (4, 0, -1)):
+        assert lib.jkv_paged_select(16, 8, 4, 1, 2, 2, 4, budget, sinks, recent, 1, 1, None) == _lib.JKV_EINVAL
+    assert lib.jkv_paged_select(16, 8, 4, 1, 2, 2, 4, 2, 0, 0, None, 1, None) == _lib.JKV_EINVAL
+    assert lib.jkv_paged_compact(16, 16, 0, 4096, 2048, 128, 4, 16, 1, 4, 4, None, 4, 1, 4, 4, 2, 2, 128, None, 0, 0, 0,
+                                 None, None) == _lib.JKV_EINVAL
+
+
+def test_operators_refuse_cpu_tensors():
+    pages = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
+    ints = torch.zeros(2, 4, dtype=torch.int32)
+    lengths = torch.ones(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="MI355X"):
+        jkv.paged_attention(torch.zeros(2, 2, 64, dtype=torch.float16), pages, pages, ints, lengths)
+    with pytest.raises(ValueError, match="MI355X"):
+        jkv.paged_append(torch.zeros(2, 2, 64, dtype=torch.float16), torch.zeros(2, 2, 64, dtype=torch.float16), pages,
+                         pages, ints, lengths)
+    with pytest.raises(ValueError, match="MI355X"):
+        jkv.select_entries(torch.zeros(2, 2, 8), lengths, 4)
+    with pytest.raises(ValueError, match="MI355X"):
+        jkv.compact_pages(pages, pages, ints, torch.zeros(2, 2, 4, dtype=torch.int32), ints)
+
+
+class _HostCache(jkv.PagedKVCache):
+    def _on_device(self, values):
+        return torch.tensor(values, dtype=torch.int32)
+
+
+def test_page_accounting():
+    cache = _HostCache(1, 3, 10, 1, max_length=100, page_size=16, head_dim=64, device="cpu")
+    step = cache.begin([33, 1, 0])
+    assert cache.free_pages == 6 and step.tokens == 34 and step.max_new == 33 and step.max_length == 33
+    assert step.starts.tolist() == [0, 33, 34, 34] and step.positions.tolist() == [0, 0, 0]
+    assert step.lengths.tolist() == [33, 1, 0]
+    pages = step.block_tables.tolist()
+    assert [sum(p >= 0 for p in row) for row in pages] == [3, 1, 0]
+    assert len({p for row in pages for p in row if p >= 0}) == 4
+    step = cache.begin([1, 1, 1])
+    assert step.starts is None and cache.free_pages == 5 and step.positions.tolist() == [33, 1, 0]
+    with pytest.raises(ValueError, match="are free"):
+        cache.begin([0, 0, 99])
+    with pytest.raises(ValueError, match="holds 100"):
+        cache.begin([0, 0, 100])
+    with pytest.raises(ValueError, match="one count"):
+        cache.begin([1, 1])
+    assert cache.lengths == (34, 2, 1) and cache.free_pages == 5, "a refused step changes nothing"
+    with pytest.raises(ValueError, match="does not track"):
+        cache.evict(4)
+    cache.release(0)
+    assert cache.lengths == (0, 2, 1) and cache.free_pages == 8 and cache.positions == (0, 2, 1)
+
+
+@pytest.mark.parametrize("change", [dict(layers=0), dict(head_dim=32), dict(page_size=24), dict(page_size=8),
+                                    dict(dtype=torch.float32), dict(max_length=0)])
+def test_cache_refuses_geometry(change):
+    args = dict(layers=1, sequences=1, pages=2, kv_heads=1, max_length=32, device="cpu")
+    args.update(change)
+    with pytest.raises(ValueError):
+        jkv.PagedKVCache(**args)

@@ -92,6 +92,56 @@ template <> struct Half16<JKV_BF16> {
   typedef bf16x4 V4;
 };
 
+// What the attention kernels of one call share.
+struct PagedAttnArgs {
+  PagedCache c;
+  RopeRates rope;
+  const uint8_t* q;
+  int64_t qst, qsh;  // byte strides of a token and a head
+  uint8_t* out;
+  int64_t ost, osh;
+  float* lse;      // [N,QH] natural log, or null
+  float* weights;  // [B,KVH,..], or null
+  int64_t wsb, wsh;
+  int32_t accumulate;
+  int32_t QH, KVH, per;   // per: query heads of a kv head
+  int32_t window, sinks;  // at most kPagedMost
+  int32_t max_new;
+  // Scores are q k * scale2, base 2: q is multiplied by q_mul (half, so that a
+  // rotated fp16 query cannot overflow; negative for a negative scale, zero for
+  // a zero one) and the product by scale2 > 0.
+  float q_mul, scale2;
+  // splits of the entries, joined by paged_join_kernel (one split: none)
+  int32_t splits, split_tiles;
+  float2* part_ml;  // [splits][N*QH] reference maximum (base 2) and sum
+  float* part_o;    // [splits][N*QH][D]
+  float* lse2;      // [N,QH] base-2 log-sum-exp for the weights, or null
+  float* scores;    // few rows with weights: [B,KVH,max_new*per,score_width] base-2 scores, or null
+  int64_t score_width;
+};
+
+static const int32_t kPagedMost = 0x3fffffff;  // entries of a sequence: sums of two of them stay in 32 bits
+
+// launches; what they need of the workspace is in the arguments already
+int paged_launch_few(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
+
+// The tiles of `size` entries that rows at entries first..last may see: `lead`
+// tiles from entry 0 on that hold sinks, then those from tile `main` on.
+struct PagedTiles {
+  int32_t lead, main, count;
+};
+__host__ __device__ inline PagedTiles paged_tiles(int32_t first, int32_t last, int32_t window, int32_t sinks, int32_t size) {
+  int32_t low = first - window + 1;  // the first entry of any row's window
+  if (low < 0) low = 0;
+  const int32_t seen = sinks < low ? sinks : low;
+  PagedTiles t;
+  t.main = low / size;
+  t.lead = (seen + size - 1) / size;
+  if (t.lead > t.main) t.lead = t.main;
+  t.count = last < 0 ? 0 : t.lead + last / size - t.main + 1;
+  return t;
+}
+
 // host side: fills c and the rates, or says what is wrong with them
 int paged_cache_args(PagedCache* c, const void* k, const void* v, int64_t page_stride, int64_t head_stride,
                      int64_t slot_stride, int64_t n_pages, int64_t page_size, const int32_t* tables,

@@ -38,7 +38,7 @@ int paged_cache_args(PagedCache* c, const void* k, const void* v, int64_t page_s
   c->tables = tables; c->table_stride = table_stride; c->table_width = table_width;
   c->lengths = lengths; c->starts = starts; c->positions = positions;
   c->N = (int32_t)N; c->B = (int32_t)B;
-  const int64_t room = table_width << shift, most = room < 0x7fffffff ? room : 0x7fffffff;
+  const int64_t room = table_width << shift, most = room < kPagedMost ? room : kPagedMost;
   c->top = (int32_t)(max_length < most ? max_length : most);
   return JKV_OK;
 }

@@ -9,25 +9,11 @@
 // products with the keys, and the dims for those with the values.
 #include <math.h>
 
+#include <algorithm>
+
 #include "paged.h"
 
 namespace jkv {
-
-struct PagedAttnArgs {
-  PagedCache c;
-  RopeRates rope;
-  const uint8_t* q;
-  int64_t qst, qsh;  // byte strides of a token and a head
-  uint8_t* out;
-  int64_t ost, osh;
-  float* lse;  // [N,QH] natural log, or null
-  float* weights;  // [B,KVH,..], or null
-  int64_t wsb, wsh;
-  int32_t accumulate;
-  int32_t QH, KVH, per;  // per: query heads of a kv head
-  int32_t window, sinks;
-  float scale;
-};
 
 // the row of a packed token, or -1
 __device__ __forceinline__ int32_t paged_seq_of(const PagedCache& c, int32_t n) {
@@ -97,7 +83,7 @@ __global__ __launch_bounds__(64) void paged_row_kernel(PagedAttnArgs a) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v = fmaf((float)x[e], qs[d + e], v);
         }
-      v *= a.scale;
+      v *= a.q_mul * a.scale2 * 0.6931471805599453f;
     }
     float mx = v;
 #pragma unroll
@@ -175,7 +161,7 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(PagedAttnArgs a) {
       float v = 0.f;
 #pragma unroll
       for (int d = 0; d < D; ++d) v = fmaf(k[d], qs[d], v);
-      sum += expf(v * a.scale - a.lse[(int64_t)n * a.QH + head]);
+      sum += expf(v * a.q_mul * a.scale2 * 0.6931471805599453f - a.lse[(int64_t)n * a.QH + head]);
     }
   if (j < s.length) {
     float* w = a.weights + b * a.wsb + kvh * a.wsh + j;
@@ -187,8 +173,53 @@ template <int DT, int D>
 static void launch_paged(const PagedAttnArgs& a, int64_t max_length, hipStream_t stream) {
   hipLaunchKernelGGL((paged_row_kernel<DT, D>), dim3(a.c.N, a.QH), dim3(64), 0, stream, a);
   if (a.weights != nullptr)
-    hipLaunchKernelGGL((paged_weights_kernel<DT, D>), dim3((uint32_t)ceil_div(max_length, 256), a.KVH, a.c.B), dim3(256),
+    hipLaunchKernelGGL((paged_weights_kernel<DT, D>), dim3((uint32_t)ceil_div(std::max<int64_t>(max_length, 1), 256), a.KVH, a.c.B), dim3(256),
                        0, stream, a);
+}
+
+// How a call's work is divided and what of the workspace it takes.
+struct PagedPlan {
+  bool few;  // at most 32 rows a sequence and kv head
+  int64_t splits, split_tiles, score_width;
+  int64_t ml_at, o_at, lse_at, lse2_at, scores_at, bytes;
+};
+
+static PagedPlan paged_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t max_new, int64_t max_length,
+                            int64_t window, int64_t sinks, bool weights) {
+  PagedPlan p = {};
+  const int64_t per = QH / KVH;
+  p.few = max_new * per <= 32;
+  p.splits = 1;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t from = at;
+    at += ceil_div(bytes, 256) * 256;
+    return from;
+  };
+  if (p.few) {
+    // the most tiles a sequence can have
+    int64_t tiles = ceil_div(max_length, 32);
+    const int64_t bound = ceil_div(window + max_new, 32) + 1 + ceil_div(sinks, 32);
+    if (bound < tiles) tiles = bound;
+    if (tiles < 1) tiles = 1;
+    // two waves a SIMD of every CU
+    const int64_t want = std::max<int64_t>(1, 2048 / std::max<int64_t>(1, B * KVH));
+    p.split_tiles = std::max<int64_t>(2, ceil_div(tiles, want));
+    p.splits = ceil_div(tiles, p.split_tiles);
+    if (p.splits > 1) {
+      p.ml_at = take(p.splits * N * QH * 8);
+      p.o_at = take(p.splits * N * QH * D * 4);
+    }
+    if (weights) {
+      p.lse2_at = take(N * QH * 4);
+      p.score_width = ceil_div(max_length, 32) * 32;
+      p.scores_at = take(B * KVH * max_new * per * p.score_width * 4);
+    }
+  } else if (weights) {
+    p.lse_at = take(N * QH * 4);
+  }
+  p.bytes = at;
+  return p;
 }
 
 }  // namespace jkv
@@ -197,8 +228,10 @@ extern "C" {
 
 int64_t jkv_paged_attention_workspace_bytes(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t max_new,
                                             int64_t max_length, int64_t window, int64_t sinks, int32_t with_weights) {
-  if (N <= 0 || B <= 0 || QH <= 0 || KVH <= 0) return 0;
-  return with_weights ? N * QH * 4 : 0;
+  if (N <= 0 || B <= 0 || QH <= 0 || KVH <= 0 || QH % KVH != 0) return 0;
+  const int64_t most = jkv::kPagedMost;
+  return jkv::paged_plan(N, B, QH, KVH, D, std::min(max_new, N), std::min(max_length, most),
+                         window > 0 && window < most ? window : most, std::min(sinks, most), with_weights != 0).bytes;
 }
 
 int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, int32_t dtype, const void* key_pages,
@@ -231,18 +264,34 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   JKV_CHECK_ARG(weights == nullptr || weight_width >= max_length, "weights have fewer entries than max_length");
   if (N == 0 || B == 0) return JKV_OK;
   JKV_CHECK_ARG(q && out, "null buffer");
-  const int64_t need = jkv_paged_attention_workspace_bytes(N, B, QH, KVH, D, max_new, max_length, window, sinks,
-                                                           weights != nullptr);
-  JKV_CHECK_ARG(workspace_bytes >= need && (need == 0 || workspace != nullptr),
-                "paged attention needs a workspace of %lld bytes, got %lld", (long long)need, (long long)workspace_bytes);
+  if (max_new > N) max_new = N;
+  a.window = (int32_t)(window > 0 && window < kPagedMost ? window : kPagedMost);
+  a.sinks = (int32_t)(sinks < kPagedMost ? sinks : kPagedMost);
+  const PagedPlan p = paged_plan(N, B, QH, KVH, D, max_new, max_length, a.window, a.sinks, weights != nullptr);
+  JKV_CHECK_ARG(workspace_bytes >= p.bytes && (p.bytes == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0)),
+                "paged attention needs an aligned workspace of %lld bytes, got %lld", (long long)p.bytes,
+                (long long)workspace_bytes);
+  uint8_t* ws = (uint8_t*)workspace;
   a.q = (const uint8_t*)q; a.qst = 2 * q_stride_t; a.qsh = 2 * q_stride_h;
   a.out = (uint8_t*)out; a.ost = 2 * out_stride_t; a.osh = 2 * out_stride_h;
-  a.lse = lse != nullptr ? lse : weights != nullptr ? (float*)workspace : nullptr;
+  a.lse = lse;
   a.weights = weights; a.wsb = weight_stride_b; a.wsh = weight_stride_h; a.accumulate = accumulate;
   a.QH = (int32_t)QH; a.KVH = (int32_t)KVH; a.per = (int32_t)(QH / KVH);
-  a.window = (int32_t)(window > 0 && window < 0x7fffffff ? window : 0x7fffffff);
-  a.sinks = (int32_t)(sinks < 0x7fffffff ? sinks : 0x7fffffff);
-  a.scale = scale;
+  a.max_new = (int32_t)max_new;
+  a.q_mul = scale == 0.f ? 0.f : scale < 0.f ? -0.5f : 0.5f;
+  a.scale2 = scale == 0.f ? 1.f : fabsf(scale) * 2.f * 1.4426950408889634f;
+  a.splits = (int32_t)p.splits; a.split_tiles = (int32_t)p.split_tiles;
+  if (p.few) {
+    a.part_ml = (float2*)(ws + p.ml_at);
+    a.part_o = (float*)(ws + p.o_at);
+    if (weights != nullptr) {
+      a.lse2 = (float*)(ws + p.lse2_at);
+      a.scores = (float*)(ws + p.scores_at);
+      a.score_width = p.score_width;
+    }
+    return paged_launch_few(a, dtype, D, stream);
+  }
+  if (lse == nullptr && weights != nullptr) a.lse = (float*)(ws + p.lse_at);
   if (dtype == JKV_F16 && D == 128) launch_paged<JKV_F16, 128>(a, max_length, stream);
   else if (dtype == JKV_F16) launch_paged<JKV_F16, 64>(a, max_length, stream);
   else if (D == 128) launch_paged<JKV_BF16, 128>(a, max_length, stream);

@@ -1,0 +1,434 @@
+// Attention over a paged K/V cache for sequences with few rows (tokens times
+// query heads of a kv head, at most 32): single tokens above all.
+//
+// The bytes of the cache bound it.  One wave per (sequence, kv head, split of
+// the entries): its rows are the columns of every product, so each key and
+// value is read once for all heads of the group, whole rows at a time.  A tile
+// of 32 entries waits in registers while the one before is worked on from
+// 2 x 32 x D x 2 bytes of LDS of the wave's own, so waves share nothing and
+// meet no barrier, and eight of them a CU hold 128 KiB of loads in flight.
+//
+// On v_mfma_f32_16x16x32: S^T[entry][row] = K Q^T, O^T[dim][row] += V^T P^T
+// (V^T by transposing reads of the row-major tile; the contraction order of
+// P's accumulator layout, 4 entries of each of two groups of 16 a lane).  The
+// matrix cores have time to spare here, so neither q nor p is rounded to 16
+// bits: both enter as a sum of two (q = hi + lo, p = hi + lo), which leaves
+// 32-bit scores and sums and the output's own rounding.
+#include <math.h>
+
+#include <type_traits>
+
+#include "paged.h"
+
+namespace jkv {
+
+static const int kFewTile = 32;
+
+template <int DT>
+__device__ __forceinline__ float4v mfma16(typename Half16<DT>::V8 a, typename Half16<DT>::V8 b, float4v c) {
+  if constexpr (DT == JKV_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// max / sum over lanes l, l^16, l^32, l^48 by row swaps
+__device__ __forceinline__ float lanes4_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float lanes4_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+
+// Slot of 16-byte chunk j of row r in a tile: keys so that 16 rows' equal
+// chunks, values so that 8 rows' equal chunk pairs, fall on distinct banks.
+template <int D> __device__ __forceinline__ int key_slot(int r, int j) {
+  return D == 128 ? j ^ (r & 15) : j ^ ((r >> 1) & 7);
+}
+template <int D> __device__ __forceinline__ int value_slot(int r, int j) {
+  return D == 128 ? j ^ (2 * (r & 7)) : j ^ (2 * ((r >> 1) & 3));
+}
+
+template <int DT, int D, int RG>
+__global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_kernel(PagedAttnArgs a) {
+  typedef typename Half16<DT>::T T;
+  typedef typename Half16<DT>::V8 V8;
+  typedef typename Half16<DT>::V4 V4;
+  constexpr int kSteps = D / 32, kDims = D / 16, kRowBytes = 2 * D;
+  constexpr int kRowsPerLoad = 1024 / kRowBytes, kLoads = kFewTile / kRowsPerLoad, kHalfLoads = kLoads / 2;
+  __shared__ __align__(16) uint8_t k_lds[kFewTile * kRowBytes];
+  __shared__ __align__(16) uint8_t v_lds[kFewTile * kRowBytes];
+
+  const int lane = threadIdx.x, ln = lane & 15, lg = lane >> 4;
+  const uint32_t bid = blockIdx.x;
+  const uint32_t bh = bid / (uint32_t)a.splits;
+  const int32_t split = (int32_t)(bid - bh * (uint32_t)a.splits);
+  const int32_t b = (int32_t)(bh / (uint32_t)a.KVH), kvh = (int32_t)(bh - (uint32_t)b * (uint32_t)a.KVH);
+  const PagedSeq s = paged_seq(a.c, b);
+  const int32_t tokens = s.tokens < a.max_new ? s.tokens : a.max_new;
+  if (tokens == 0) return;
+  const int32_t R = tokens * a.per;  // <= 16 RG, as max_new * per is
+  const int32_t first = s.length - s.tokens, last = first + tokens - 1;
+
+  const PagedTiles pt = paged_tiles(first, last, a.window, a.sinks, kFewTile);
+  const int32_t tile0 = split * a.split_tiles;
+  const int32_t tile1 = split == a.splits - 1 || tile0 + a.split_tiles > pt.count ? pt.count : tile0 + a.split_tiles;
+
+  // the lane's rows, one per row group
+  int32_t row_t[RG], self[RG];
+  bool row_ok[RG];
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    const int32_t r = 16 * g + ln;
+    row_ok[g] = r < R;
+    row_t[g] = (int32_t)((uint32_t)(row_ok[g] ? r : 0) / (uint32_t)a.per);
+    self[g] = first + row_t[g];
+  }
+  auto packed_row = [&](int g) -> int64_t {  // n * QH + head
+    const int32_t r = row_ok[g] ? 16 * g + ln : 0;
+    return (int64_t)(s.row0 + row_t[g]) * a.QH + kvh * a.per + (r - row_t[g] * a.per);
+  };
+
+  float m[RG], l[RG];
+  float4v o[RG][kDims];
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.f;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) o[g][d] = float4v{0.f, 0.f, 0.f, 0.f};
+  }
+
+  if (tile0 < tile1) {
+    // ---- tile loader: 16-entry halves lie in one page (page sizes are multiples
+    // of 16).  A page outside the pool and the entries at or behind the length
+    // lie beyond the resource's bound and load as zeros. ----
+    const int32_t* table = a.c.tables + b * a.c.table_stride;
+    const int32_t mask = (1 << a.c.page_shift) - 1;
+    const int lrow = lane / (64 / kRowsPerLoad), lchunk = lane % (64 / kRowsPerLoad);
+    uint32_t voff[kHalfLoads];
+#pragma unroll
+    for (int i = 0; i < kHalfLoads; ++i) voff[i] = (uint32_t)(i * kRowsPerLoad + lrow) * (uint32_t)a.c.slot_bytes + 16u * lchunk;
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    u4 ks[kLoads], vs[kLoads];
+    const uint8_t* k_head = a.c.k + kvh * a.c.head_bytes;
+    const uint8_t* v_head = a.c.v + kvh * a.c.head_bytes;
+    auto entry_of = [&](int32_t i) { return (i < pt.lead ? i : pt.main + i - pt.lead) * kFewTile; };
+    // lane h holds the page of half h of a run of 32 tiles
+    int32_t pages = -1;
+    auto look_up = [&](int32_t i) {
+      const int32_t e = entry_of(i + (lane >> 1)) + 16 * (lane & 1);
+      pages = -1;
+      if (i + (lane >> 1) < tile1 && e < s.length) pages = table[e >> a.c.page_shift];
+      if ((uint32_t)pages >= (uint32_t)a.c.n_pages) pages = -1;
+    };
+    auto fetch = [&](int32_t i) {
+      const int32_t e0 = entry_of(i), in_run = (i - tile0) & 31;
+      if (in_run == 0) look_up(i);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int32_t e = e0 + 16 * hf;
+        const int32_t left = s.length - e;  // entries of this half that exist
+        const int32_t page = __builtin_amdgcn_readlane(pages, 2 * in_run + hf);
+        const int64_t at = page >= 0 ? page * a.c.page_bytes + (int64_t)(e & mask) * a.c.slot_bytes : 0;
+        const int32_t bytes = page >= 0 ? ((left < 16 ? left : 16) - 1) * (int32_t)a.c.slot_bytes + kRowBytes : 0;
+        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(k_head + at), (short)0, bytes, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(v_head + at), (short)0, bytes, 0x00020000);
+#pragma unroll
+        for (int j = 0; j < kHalfLoads; ++j) {
+          ks[hf * kHalfLoads + j] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)voff[j], 0, 0));
+          vs[hf * kHalfLoads + j] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)voff[j], 0, 0));
+        }
+      }
+    };
+    auto stage = [&]() {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = i * kRowsPerLoad + lrow;
+        *(u4*)(k_lds + r * kRowBytes + 16 * key_slot<D>(r, lchunk)) = ks[i];
+        *(u4*)(v_lds + r * kRowBytes + 16 * value_slot<D>(r, lchunk)) = vs[i];
+      }
+    };
+    fetch(tile0);
+
+    // ---- the rotated queries, in two 16-bit parts (B operand: 8 dims of row ln) ----
+    V8 qh[RG][kSteps], ql[RG][kSteps];
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      const int32_t r = row_ok[g] ? 16 * g + ln : 0;
+      const uint8_t* qp = a.q + (int64_t)(s.row0 + row_t[g]) * a.qst +
+                          (int64_t)(kvh * a.per + (r - row_t[g] * a.per)) * a.qsh;
+#pragma unroll
+      for (int c = 0; c < kSteps / 2; ++c) {
+        const int d0 = 32 * c + 8 * lg;
+        const V8 x0 = *(const V8*)(qp + 2 * d0), x1 = *(const V8*)(qp + 2 * d0 + D);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float u = (float)x0[e], w = (float)x1[e];
+          if (a.rope.on) {
+            float cs, sn;
+            rope_trig(a.rope.turns[d0 + e], s.pos0 + row_t[g], &cs, &sn);
+            const float t = u * cs - w * sn;
+            w = w * cs + u * sn;
+            u = t;
+          }
+          u = row_ok[g] ? u * a.q_mul : 0.f;
+          w = row_ok[g] ? w * a.q_mul : 0.f;
+          const T uh = (T)u, wh = (T)w;
+          qh[g][c][e] = uh;
+          ql[g][c][e] = (T)(u - (float)uh);
+          qh[g][c + kSteps / 2][e] = wh;
+          ql[g][c + kSteps / 2][e] = (T)(w - (float)wh);
+        }
+      }
+    }
+
+    const uint32_t v_base = (uint32_t)(size_t)(const void __attribute__((address_space(3)))*)v_lds;
+    const int tr_row = 4 * lg + (ln >> 2);
+    for (int32_t i = tile0; i < tile1; ++i) {
+      const int32_t e0 = entry_of(i);
+      stage();
+      if (i + 1 < tile1) fetch(i + 1);
+
+      float4v sc[RG][2];
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg) {
+#pragma unroll
+        for (int g = 0; g < RG; ++g) sc[g][kg] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+          const int r = 16 * kg + ln;
+          const V8 ka = *(const V8*)(k_lds + r * kRowBytes + 16 * key_slot<D>(r, 4 * c + lg));
+#pragma unroll
+          for (int g = 0; g < RG; ++g) {
+            sc[g][kg] = mfma16<DT>(ka, qh[g][c], sc[g][kg]);
+            sc[g][kg] = mfma16<DT>(ka, ql[g][c], sc[g][kg]);
+          }
+        }
+      }
+      // every row sees the whole tile, or some entries are masked
+      const bool full = e0 + kFewTile - 1 <= first && (e0 > last - a.window || e0 + kFewTile <= a.sinks);
+      V8 ph[RG], pl[RG];
+      float pr[RG][8];
+#pragma unroll
+      for (int g = 0; g < RG; ++g) {
+        if (!full) {
+#pragma unroll
+          for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int32_t j = e0 + 16 * kg + 4 * lg + e;
+              const bool seen = j <= self[g] && (j > self[g] - a.window || j < a.sinks);
+              sc[g][kg][e] = seen ? sc[g][kg][e] : -INFINITY;
+            }
+        }
+        if (a.scores != nullptr && row_ok[g]) {
+          float* to = a.scores + (((int64_t)b * a.KVH + kvh) * (a.max_new * a.per) + 16 * g + ln) * a.score_width + e0 + 4 * lg;
+#pragma unroll
+          for (int kg = 0; kg < 2; ++kg) *(float4v*)(to + 16 * kg) = sc[g][kg] * a.scale2;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[g][kg][e]);
+        mx = lanes4_max(mx) * a.scale2;
+        // the reference moves only when the maximum passes it by more than 4;
+        // p is 2^10 times its weight against the reference, at most 2^14, so
+        // that fp16 holds weights of 2^-34
+        const float mn = mx > m[g] + 4.f ? mx : m[g], mu = mn == -INFINITY ? 0.f : mn - 10.f;
+        const float alpha = m[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[g] - mn);
+        if (__any(mn != m[g])) {
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) o[g][d] *= alpha;
+          l[g] *= alpha;
+        }
+        m[g] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(sc[g][e >> 2][e & 3], a.scale2, -mu));
+          pr[g][e] = p;
+          sum += p;
+          const T hi = (T)p;
+          ph[g][e] = hi;
+          pl[g][e] = (T)(p - (float)hi);
+        }
+        l[g] += sum;
+      }
+      bool plain = true;
+      if (!full) {
+        // a masked weight is 0, but 0 times an infinite or NaN value is not:
+        // where a masked tile holds one, its values are added one by one
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < kFewTile * kRowBytes / 1024; ++j) {
+          const u4 w = *(const u4*)(v_lds + 1024 * j + 16 * lane);
+          constexpr uint32_t kExp = DT == JKV_F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            top |= (w[e] & kExp) == kExp;
+            top |= ((w[e] >> 16) & kExp) == kExp;
+          }
+        }
+        plain = !__any(top != 0);
+      }
+      if (plain) {
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) {
+          const uint32_t at = v_base + (uint32_t)(tr_row * kRowBytes + 16 * value_slot<D>(tr_row, 2 * d + ((ln & 3) >> 1)) + 8 * (ln & 1));
+          const V4 lo = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(size_t)at));
+          const V4 hi = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(size_t)(at + 16u * kRowBytes)));
+          const V8 va = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+          for (int g = 0; g < RG; ++g) {
+            o[g][d] = mfma16<DT>(va, ph[g], o[g][d]);
+            o[g][d] = mfma16<DT>(va, pl[g], o[g][d]);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int from = 0; from < 4; ++from)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int k = 16 * (e >> 2) + 4 * from + (e & 3);
+            const int32_t j = e0 + k;
+#pragma unroll
+            for (int g = 0; g < RG; ++g) {
+              const float p = __shfl(pr[g][e], ln + 16 * from, 64);
+              const bool seen = j <= self[g] && (j > self[g] - a.window || j < a.sinks);
+              if (seen)
+#pragma unroll
+                for (int d = 0; d < kDims; ++d) {
+                  const V4 x = *(const V4*)(v_lds + k * kRowBytes + 16 * value_slot<D>(k, 2 * d + (lg >> 1)) + 8 * (lg & 1));
+#pragma unroll
+                  for (int i2 = 0; i2 < 4; ++i2) o[g][d][i2] = fmaf(p, (float)x[i2], o[g][d][i2]);
+                }
+            }
+          }
+      }
+    }
+  }
+
+  // ---- out, or this split's part of it: lane holds dims 16d + 4lg + e of row ln ----
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    const float lt = lanes4_sum(l[g]);
+    if (!row_ok[g]) continue;
+    const int64_t row = packed_row(g);
+    if (a.splits > 1) {
+      const int64_t at = (int64_t)split * a.c.N * a.QH + row;
+      if (lg == 0) a.part_ml[at] = float2{m[g] == -INFINITY ? m[g] : m[g] - 10.f, lt};
+      if (tile0 < tile1)
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) *(float4v*)(a.part_o + at * D + 16 * d + 4 * lg) = o[g][d];
+      continue;
+    }
+    const bool none = lt == 0.f;  // sees nothing
+    if (lg == 0) {
+      const float l2 = none ? -INFINITY : (m[g] == -INFINITY ? 0.f : m[g] - 10.f) + log2f(lt);
+      if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
+      if (a.lse2 != nullptr) a.lse2[row] = l2;
+    }
+    const float inv = 1.0f / lt;
+    uint8_t* op = a.out + (int64_t)(s.row0 + row_t[g]) * a.ost + (row - (int64_t)(s.row0 + row_t[g]) * a.QH) * a.osh;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) {
+      V4 h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = (T)(none ? 0.f : o[g][d][e] * inv);
+      *(V4*)(op + 2 * (16 * d + 4 * lg)) = h;
+    }
+  }
+}
+
+// The weights of few rows, from the scores that the attention left: one thread
+// an entry, its rows' sum in their order.
+__global__ __launch_bounds__(256) void paged_few_weights_kernel(PagedAttnArgs a) {
+  const uint32_t bh = blockIdx.y + blockIdx.z * 32768u;
+  const int32_t b = (int32_t)(bh / (uint32_t)a.KVH), kvh = (int32_t)(bh - (uint32_t)b * (uint32_t)a.KVH);
+  if (b >= a.c.B) return;
+  const PagedSeq s = paged_seq(a.c, b);
+  const int32_t j = (int32_t)(blockIdx.x * 256 + threadIdx.x);
+  if (j >= s.length) return;
+  const int32_t tokens = s.tokens < a.max_new ? s.tokens : a.max_new, first = s.length - s.tokens;
+  const float* sc = a.scores + ((int64_t)b * a.KVH + kvh) * (a.max_new * a.per) * a.score_width + j;
+  float sum = 0.f;
+  for (int32_t t = 0; t < tokens; ++t) {
+    const int32_t self = first + t;
+    if (!(j <= self && (j > self - a.window || j < a.sinks))) continue;
+    const float* norm = a.lse2 + (int64_t)(s.row0 + t) * a.QH + kvh * a.per;
+    for (int32_t g = 0; g < a.per; ++g)
+      sum += __builtin_amdgcn_exp2f(sc[(int64_t)(t * a.per + g) * a.score_width] - norm[g]);
+  }
+  float* w = a.weights + b * a.wsb + kvh * a.wsh + j;
+  *w = a.accumulate ? *w + sum : sum;
+}
+
+// One wave a row: the splits' parts by their maxima and sums.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+  typedef typename Half16<DT>::T T;
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = (int64_t)a.c.N * a.QH, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int32_t n = (int32_t)((uint64_t)row / (uint32_t)a.QH), head = (int32_t)(row - (int64_t)n * a.QH);
+  if (a.c.starts != nullptr && (n < a.c.starts[0] || n >= a.c.starts[a.c.B])) return;  // nobody's row
+  float top = -INFINITY;
+  for (int32_t i = lane; i < a.splits; i += 64) top = fmaxf(top, a.part_ml[i * rows + row].x);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  float l = 0.f, o[D / 64];
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int32_t i = 0; i < a.splits; ++i) {
+    const float2 ml = a.part_ml[i * rows + row];
+    if (ml.y == 0.f) continue;  // it saw nothing; an empty one has written no sums
+    const float f = __builtin_amdgcn_exp2f(ml.x - top);
+    l = fmaf(ml.y, f, l);
+    const float* p = a.part_o + (i * rows + row) * D + lane * (D / 64);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] = fmaf(p[e], f, o[e]);
+  }
+  const bool none = l == 0.f;
+  if (lane == 0) {
+    const float l2 = none ? -INFINITY : top + log2f(l);
+    if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
+    if (a.lse2 != nullptr) a.lse2[row] = l2;
+  }
+  T* op = (T*)(a.out + n * a.ost + head * a.osh) + lane * (D / 64);
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) op[e] = (T)(none ? 0.f : o[e] / l);
+}
+
+template <int DT, int D>
+static int launch_few(const PagedAttnArgs& a, hipStream_t stream) {
+  const int64_t blocks = (int64_t)a.c.B * a.KVH * a.splits;
+  JKV_CHECK_ARG(blocks < ((int64_t)1 << 31), "paged attention grid too large");
+  if (a.max_new * a.per <= 16) hipLaunchKernelGGL((paged_few_kernel<DT, D, 1>), dim3((uint32_t)blocks), dim3(64), 0, stream, a);
+  else hipLaunchKernelGGL((paged_few_kernel<DT, D, 2>), dim3((uint32_t)blocks), dim3(64), 0, stream, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((paged_join_kernel<DT, D>), dim3((uint32_t)ceil_div((int64_t)a.c.N * a.QH, 4)), dim3(256), 0, stream, a);
+  if (a.weights != nullptr && a.c.top > 0) {
+    const int64_t bh = (int64_t)a.c.B * a.KVH;
+    hipLaunchKernelGGL(paged_few_weights_kernel, dim3((uint32_t)ceil_div(a.c.top, 256), (uint32_t)(bh < 32768 ? bh : 32768),
+                       (uint32_t)ceil_div(bh, 32768)), dim3(256), 0, stream, a);
+  }
+  JKV_CHECK_LAUNCH();
+  return JKV_OK;
+}
+
+int paged_launch_few(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream) {
+  if (dtype == JKV_F16) return D == 128 ? launch_few<JKV_F16, 128>(a, stream) : launch_few<JKV_F16, 64>(a, stream);
+  return D == 128 ? launch_few<JKV_BF16, 128>(a, stream) : launch_few<JKV_BF16, 64>(a, stream);
+}
+
+}  // namespace jkv

@@ -111,6 +111,7 @@ struct PagedAttnArgs {
   // rotated fp16 query cannot overflow; negative for a negative scale, zero for
   // a zero one) and the product by scale2 > 0.
   float q_mul, scale2;
+  int32_t items;  // chunks: an upper bound of all sequences' row blocks
   // splits of the entries, joined by paged_join_kernel (one split: none)
   int32_t splits, split_tiles;
   float2* part_ml;  // [splits][N*QH] reference maximum (base 2) and sum
@@ -118,12 +119,16 @@ struct PagedAttnArgs {
   float* lse2;      // [N,QH] base-2 log-sum-exp for the weights, or null
   float* scores;    // few rows with weights: [B,KVH,max_new*per,score_width] base-2 scores, or null
   int64_t score_width;
+  uint8_t* q_parts;  // chunks with weights: [N,QH] rotated queries, D of their leading and D of their trailing parts
 };
 
 static const int32_t kPagedMost = 0x3fffffff;  // entries of a sequence: sums of two of them stay in 32 bits
 
 // launches; what they need of the workspace is in the arguments already
 int paged_launch_few(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
+int paged_launch_chunk(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
+int paged_launch_join(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
+static const int kChunkRows = 128;  // packed (token, head) rows of a chunk kernel's workgroup
 
 // The tiles of `size` entries that rows at entries first..last may see: `lead`
 // tiles from entry 0 on that hold sinks, then those from tile `main` on.
@@ -140,6 +145,55 @@ __host__ __device__ inline PagedTiles paged_tiles(int32_t first, int32_t last, i
   if (t.lead > t.main) t.lead = t.main;
   t.count = last < 0 ? 0 : t.lead + last / size - t.main + 1;
   return t;
+}
+
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+
+// Transposing LDS read of 8-byte pieces at LDS byte address at: in each 16-lane
+// block, lane 4j + e receives element e of the pieces that the block's lanes j,
+// j+4, j+8, j+12 address (ds_read_b64_tr_b16).
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+template <typename V4>
+__device__ __forceinline__ V4 lds_read_tr(uint32_t at) {
+  return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(size_t)at));
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(size_t)(const void __attribute__((address_space(3)))*)p;
+}
+
+// A masked weight is 0, but 0 times an infinite or NaN value is not.  Tiles with
+// masked entries are therefore staged with such values as 0, and where one was
+// met a second walk over those tiles adds it to the rows that do see it.
+
+// w with the infinite and NaN halves 0; sets *found if there were any
+template <int DT>
+__device__ __forceinline__ uint4v finite_halves(uint4v w, bool* found) {
+  constexpr uint32_t kExp = DT == JKV_F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool lo = (w[e] & kExp) == kExp, hi = ((w[e] >> 16) & kExp) == kExp;
+    *found = *found || lo || hi;
+    w[e] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+  }
+  return w;
+}
+// `up`: 1 where v is +infinity or NaN; `down`: 1 where it is -infinity or NaN.
+// Their products with the rows' visibility say which sums they belong to (both: NaN).
+template <int DT, typename V8>
+__device__ __forceinline__ void non_finite_marks(V8 v, V8* up, V8* down) {
+  typedef typename Half16<DT>::T T;
+  constexpr uint16_t kExp = DT == JKV_F16 ? 0x7c00 : 0x7f80;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint16_t u = __builtin_bit_cast(uint16_t, (T)v[e]);
+    const bool bad = (u & kExp) == kExp, nan = (u & 0x7fff) > kExp, neg = u >> 15;
+    (*up)[e] = bad && (nan || !neg) ? (T)1.f : (T)0.f;
+    (*down)[e] = bad && (nan || neg) ? (T)1.f : (T)0.f;
+  }
+}
+__device__ __forceinline__ float marked(float o, float up, float down) {
+  return o + (up > 0.f ? INFINITY : 0.f) + (down > 0.f ? -INFINITY : 0.f);
 }
 
 // host side: fills c and the rates, or says what is wrong with them

@@ -1,0 +1,535 @@
+// Attention of chunks of new tokens over a paged K/V cache.
+//
+// The matrix products bound it.  The packed (token, query head) rows of a
+// sequence and kv head go 128 to a workgroup of four waves, 32 rows a wave, so
+// any number of heads shares the keys and values of its group.  Tiles of 64
+// entries lie twice in LDS (keys and values 4 x 64 x D x 2 bytes); the next
+// one's loads are issued before this one's products and stored behind them.
+//
+// On v_mfma_f32_32x32x16, S^T[entry][row] = K Q^T gives a lane one row's
+// scores (16 of 32 entries, the other half-wave the rest): a row's maximum and
+// sum take one swap.  O^T[dim][row] += V^T P^T takes P from those registers,
+// 4 entries of each of two groups of 8 a lane, and V^T by transposing reads of
+// the row-major tile in the same order.  Online softmax in 32 bits; p and the
+// rotated q enter the products rounded once to the cache's type, except that
+// with EXACT (weights or log-sum-exps are asked for) q is a sum of two parts.
+#include <math.h>
+
+#include "paged.h"
+
+namespace jkv {
+
+static const int kChunkTile = 64;
+static const int kChunkWaves = kChunkRows / 32;
+
+template <int DT>
+__device__ __forceinline__ float16v mfma32(typename Half16<DT>::V8 a, typename Half16<DT>::V8 b, float16v c) {
+  if constexpr (DT == JKV_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// max / sum over lanes l and l^32
+__device__ __forceinline__ float lanes2_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float lanes2_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// Slot of 16-byte chunk j of row r in a tile: keys so that 16 rows' equal
+// chunks, values so that 4 rows' 64-byte groups, fall on distinct banks.
+template <int D> __device__ __forceinline__ int chunk_key_slot(int r, int j) {
+  return D == 128 ? j ^ (r & 15) : j ^ ((r >> 1) & 7);
+}
+template <int D> __device__ __forceinline__ int chunk_value_slot(int r, int j) {
+  return D == 128 ? j ^ (4 * (r & 3)) : j ^ (4 * ((r >> 1) & 1));
+}
+
+// The sequence and row block of an item: items are the row blocks of all
+// sequences in turn, a sequence's last one first (it sees most).
+__device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int32_t item, int32_t* b, int32_t* block) {
+  const int lane = threadIdx.x & 63;
+  int32_t before = 0;
+  for (int32_t b0 = 0; b0 < a.c.B; b0 += 64) {
+    int32_t n = 0;
+    if (b0 + lane < a.c.B) {
+      int32_t row0, tokens;
+      paged_rows(a.c, b0 + lane, &row0, &tokens);
+      if (tokens > a.max_new) tokens = a.max_new;
+      n = (tokens * a.per + kChunkRows - 1) / kChunkRows;
+    }
+    int32_t upto = n;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int32_t up = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += up;
+    }
+    const int32_t all = __builtin_amdgcn_readlane(upto, 63);
+    if (item < before + all) {
+      const uint64_t hit = __ballot(item < before + upto);
+      const int at = __builtin_ctzll(hit);
+      *b = b0 + at;
+      *block = before + __builtin_amdgcn_readlane(upto, at) - 1 - item;
+      return true;
+    }
+    before += all;
+  }
+  return false;
+}
+
+template <int DT, int D, bool EXACT>
+__global__ __launch_bounds__(64 * kChunkWaves, EXACT ? 1 : 2) void paged_chunk_kernel(PagedAttnArgs a) {
+  typedef typename Half16<DT>::T T;
+  typedef typename Half16<DT>::V8 V8;
+  typedef typename Half16<DT>::V4 V4;
+  constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D;
+  constexpr int kTileBytes = kChunkTile * kRowBytes;
+  constexpr int kRowsPerLoad = 1024 / kRowBytes, kWaveRows = kChunkTile / kChunkWaves, kLoads = kWaveRows / kRowsPerLoad;
+  __shared__ __align__(16) uint8_t k_lds[2][kTileBytes];
+  __shared__ __align__(16) uint8_t v_lds[2][kTileBytes];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 31, lh = lane >> 5;
+  // an XCD takes neighbouring items of one kv head: their tiles meet in its L2
+  uint32_t bid = xcd_remap(blockIdx.x, gridDim.x);
+  const uint32_t slice = (uint32_t)a.items * (uint32_t)a.splits;
+  const int32_t kvh = (int32_t)(bid / slice);
+  if (kvh >= a.KVH) return;
+  bid -= (uint32_t)kvh * slice;
+  const int32_t item = (int32_t)(bid / (uint32_t)a.splits), split = (int32_t)(bid - (uint32_t)item * (uint32_t)a.splits);
+  int32_t b, block;
+  if (!paged_item(a, item, &b, &block)) return;
+  b = __builtin_amdgcn_readfirstlane(b);
+  block = __builtin_amdgcn_readfirstlane(block);
+  const PagedSeq s = paged_seq(a.c, b);
+  const int32_t tokens = s.tokens < a.max_new ? s.tokens : a.max_new;
+  // (rows, N * QH in all, fit 31 bits: host-checked)
+  const uint32_t per = (uint32_t)a.per;
+  const int32_t R = tokens * a.per;
+  const int32_t r0 = block * kChunkRows, r1 = R - r0 > kChunkRows ? r0 + kChunkRows : R;
+  const int32_t before = s.length - s.tokens;
+  const int32_t first = before + (int32_t)((uint32_t)r0 / per), last = before + (int32_t)((uint32_t)(r1 - 1) / per);
+  // this wave's rows
+  const int32_t wr0 = r0 + 32 * wave, wr1 = wr0 + 32 < r1 ? wr0 + 32 : r1;
+  const bool wave_on = wr0 < r1;
+  const int32_t wfirst = wave_on ? before + (int32_t)((uint32_t)wr0 / per) : kPagedMost;
+  const int32_t wlast = wave_on ? before + (int32_t)((uint32_t)(wr1 - 1) / per) : -1;
+  const bool row_ok = wr0 + ln < r1;
+  const int32_t row_t = row_ok ? (int32_t)((uint32_t)(wr0 + ln) / per) : 0;
+  const int32_t head = kvh * a.per + (row_ok ? wr0 + ln - row_t * a.per : 0);
+  const int32_t self = row_ok ? before + row_t : -1;
+
+  const PagedTiles pt = paged_tiles(first, last, a.window, a.sinks, kChunkTile);
+  int32_t tile0 = 0, tile1 = pt.count;
+  if (a.splits > 1) {
+    const int32_t each = (pt.count + a.splits - 1) / a.splits;
+    tile0 = split * each < pt.count ? split * each : pt.count;
+    tile1 = tile0 + each < pt.count ? tile0 + each : pt.count;
+  }
+
+  // ---- tile loader: a wave's 16 entries lie in one page.  A page outside the
+  // pool and the entries at or behind the length lie beyond the resource's
+  // bound and load as zeros. ----
+  const int32_t* table = a.c.tables + b * a.c.table_stride;
+  const int32_t mask = (1 << a.c.page_shift) - 1;
+  const int lrow = lane / (64 / kRowsPerLoad), lchunk = lane % (64 / kRowsPerLoad);
+  const uint8_t* k_head = a.c.k + kvh * a.c.head_bytes;
+  const uint8_t* v_head = a.c.v + kvh * a.c.head_bytes;
+  uint4v ks[kLoads], vs[kLoads];
+  auto entry_of = [&](int32_t i) { return (i < pt.lead ? i : pt.main + i - pt.lead) * kChunkTile; };
+  // lane h holds the page of this wave's entries in tile h of a run of 64
+  int32_t pages = -1, run0 = -64;
+  auto fetch = [&](int32_t i) {
+    if (i - run0 >= 64) {
+      run0 = i;
+      const int32_t e = entry_of(i + lane) + kWaveRows * wave;
+      pages = -1;
+      if (i + lane < tile1 && e < s.length) pages = table[e >> a.c.page_shift];
+      if ((uint32_t)pages >= (uint32_t)a.c.n_pages) pages = -1;
+    }
+    const int32_t e = entry_of(i) + kWaveRows * wave, left = s.length - e;
+    const int32_t page = __builtin_amdgcn_readlane(pages, i - run0);
+    const int64_t at = page >= 0 ? page * a.c.page_bytes + (int64_t)(e & mask) * a.c.slot_bytes : 0;
+    const int32_t bytes = page >= 0 ? ((left < kWaveRows ? left : kWaveRows) - 1) * (int32_t)a.c.slot_bytes + kRowBytes : 0;
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(k_head + at), (short)0, bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(v_head + at), (short)0, bytes, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const uint32_t off = (uint32_t)(j * kRowsPerLoad + lrow) * (uint32_t)a.c.slot_bytes + 16u * lchunk;
+      ks[j] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)off, 0, 0));
+      vs[j] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)off, 0, 0));
+    }
+  };
+  // every row of the workgroup sees the whole tile, or some entries are masked
+  auto block_full = [&](int32_t e0) {
+    return e0 + kChunkTile - 1 <= first && (e0 > last - a.window || e0 + kChunkTile <= a.sinks);
+  };
+  bool found = false;  // an infinite or NaN value in a masked tile
+  auto stage = [&](int32_t i, int buf) {
+    if (!block_full(entry_of(i))) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) vs[j] = finite_halves<DT>(vs[j], &found);
+    }
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int r = kWaveRows * wave + j * kRowsPerLoad + lrow;
+      *(uint4v*)(k_lds[buf] + r * kRowBytes + 16 * chunk_key_slot<D>(r, lchunk)) = ks[j];
+      *(uint4v*)(v_lds[buf] + r * kRowBytes + 16 * chunk_value_slot<D>(r, lchunk)) = vs[j];
+    }
+  };
+  if (tile0 < tile1) fetch(tile0);
+
+  // ---- the wave's rotated queries (B operand: 8 dims of row ln) ----
+  V8 qf[kSteps], ql[EXACT ? kSteps : 1];
+  {
+    const uint8_t* qp = a.q + (int64_t)(s.row0 + row_t) * a.qst + (int64_t)head * a.qsh;
+    const float mul = row_ok ? a.q_mul : 0.f;
+#pragma unroll
+    for (int c = 0; c < kSteps / 2; ++c) {
+      const int d0 = 16 * c + 8 * lh;
+      const V8 x0 = *(const V8*)(qp + 2 * d0), x1 = *(const V8*)(qp + 2 * d0 + D);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float u = (float)x0[e], w = (float)x1[e];
+        if (a.rope.on) {
+          float cs, sn;
+          rope_trig(a.rope.turns[d0 + e], s.pos0 + row_t, &cs, &sn);
+          const float t = u * cs - w * sn;
+          w = w * cs + u * sn;
+          u = t;
+        }
+        u = row_ok ? u * mul : 0.f;
+        w = row_ok ? w * mul : 0.f;
+        qf[c][e] = (T)u;
+        qf[c + kSteps / 2][e] = (T)w;
+        if constexpr (EXACT) {
+          ql[c][e] = (T)(u - (float)(T)u);
+          ql[c + kSteps / 2][e] = (T)(w - (float)(T)w);
+        }
+      }
+    }
+  }
+  if constexpr (EXACT) {
+    if (a.q_parts != nullptr && split == 0 && row_ok) {
+      uint8_t* to = a.q_parts + ((int64_t)(s.row0 + row_t) * a.QH + head) * (4 * D) + 16 * lh;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        *(V8*)(to + 32 * c) = qf[c];
+        *(V8*)(to + 2 * D + 32 * c) = ql[c];
+      }
+    }
+  }
+  if (tile0 < tile1) stage(tile0, 0);
+  __syncthreads();
+
+  float m = -INFINITY, l = 0.f;
+  float16v o[kDims];
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) o[d] = float16v{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+
+  const int tr_row = 4 * lh + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  auto value_operand = [&](uint32_t base, int d, int st) -> V8 {
+    const int r = 16 * st + tr_row;
+    const uint32_t at = base + (uint32_t)(r * kRowBytes + 16 * chunk_value_slot<D>(r, 4 * d + tr_chunk) + 8 * (lane & 1));
+    const uint32_t at8 = base + (uint32_t)((r + 8) * kRowBytes + 16 * chunk_value_slot<D>(r + 8, 4 * d + tr_chunk) + 8 * (lane & 1));
+    const V4 lo = lds_read_tr<V4>(at), hi = lds_read_tr<V4>(at8);
+    return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  for (int32_t i = tile0; i < tile1; ++i) {
+    const int buf = (i - tile0) & 1;
+    const int32_t e0 = entry_of(i);
+    const bool more = i + 1 < tile1;
+    if (more) fetch(i + 1);
+    // a tile none of the wave's rows sees is left out
+    const bool on = e0 <= wlast && (e0 + kChunkTile - 1 > wfirst - a.window || e0 < a.sinks);
+    if (on) {
+      const uint8_t* kl = k_lds[buf];
+      const uint8_t* vl = v_lds[buf];
+      float16v sc[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        sc[kb] = float16v{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+          const int r = 32 * kb + ln;
+          const V8 ka = *(const V8*)(kl + r * kRowBytes + 16 * chunk_key_slot<D>(r, 2 * c + lh));
+          sc[kb] = mfma32<DT>(ka, qf[c], sc[kb]);
+          if constexpr (EXACT) sc[kb] = mfma32<DT>(ka, ql[c], sc[kb]);
+        }
+      }
+      const bool full = e0 + kChunkTile - 1 <= wfirst && (e0 > wlast - a.window || e0 + kChunkTile <= a.sinks);
+      if (!full) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int32_t j = e0 + 32 * kb + 8 * (e >> 2) + 4 * lh + (e & 3);
+            const bool seen = j <= self && (j > self - a.window || j < a.sinks);
+            sc[kb][e] = seen ? sc[kb][e] : -INFINITY;
+          }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, sc[kb][e]), sc[kb][e + 1]);
+      mx = lanes2_max(mx) * a.scale2;
+      // the reference moves only when the maximum passes it by more than 4; p is
+      // 2^10 times its weight against it, at most 2^14: fp16 holds weights of 2^-34
+      const float mn = mx > m + 4.f ? mx : m, mu = mn == -INFINITY ? 0.f : mn - 10.f;
+      if (__any(mn != m)) {
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) o[d] *= alpha;
+        l *= alpha;
+      }
+      m = mn;
+      V8 pf[4];
+      float t4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(sc[kb][e], a.scale2, -mu));
+          t4[e & 3] += p;
+          pf[2 * kb + (e >> 3)][e & 7] = (T)p;
+        }
+      l += (t4[0] + t4[1]) + (t4[2] + t4[3]);
+      const uint32_t v_base = lds_address(vl);
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int st = 0; st < 4; ++st) o[d] = mfma32<DT>(value_operand(v_base, d, st), pf[st], o[d]);
+    }
+    if (more) stage(i + 1, buf ^ 1);
+    __syncthreads();
+  }
+
+  if (__syncthreads_or(found)) {
+    for (int32_t i = tile0; i < tile1; ++i) {
+      const int32_t e0 = entry_of(i);
+      if (block_full(e0)) continue;
+      run0 = -0x40000000;  // the tile's page anew
+      fetch(i);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int r = kWaveRows * wave + j * kRowsPerLoad + lrow;
+        *(uint4v*)(v_lds[0] + r * kRowBytes + 16 * chunk_value_slot<D>(r, lchunk)) = vs[j];
+      }
+      __syncthreads();
+      V8 seen[4];
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int32_t j = e0 + 16 * st + 8 * (e >> 2) + 4 * lh + (e & 3);
+          seen[st][e] = j <= self && (j > self - a.window || j < a.sinks) ? (T)1.f : (T)0.f;
+        }
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) {
+        float16v up = {}, down = {};
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          V8 vu, vd;
+          non_finite_marks<DT>(value_operand(lds_address(v_lds[0]), d, st), &vu, &vd);
+          up = mfma32<DT>(vu, seen[st], up);
+          down = mfma32<DT>(vd, seen[st], down);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = marked(o[d][e], up[e], down[e]);
+      }
+    }
+  }
+
+  // ---- out, or this split's part of it: lane holds dims 32d + 8(e/4) + 4lh + e%4 of row ln ----
+  const float lt = lanes2_sum(l);
+  if (!row_ok) return;
+  const int64_t n = s.row0 + row_t, row = n * a.QH + head;
+  if (a.splits > 1) {
+    const int64_t at = (int64_t)split * a.c.N * a.QH + row;
+    if (lh == 0) a.part_ml[at] = float2{m == -INFINITY ? m : m - 10.f, lt};
+    if (tile0 < tile1)
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          *(float4v*)(a.part_o + at * D + 32 * d + 8 * q4 + 4 * lh) =
+              float4v{o[d][4 * q4], o[d][4 * q4 + 1], o[d][4 * q4 + 2], o[d][4 * q4 + 3]};
+    return;
+  }
+  const bool none = lt == 0.f;  // sees nothing
+  if (lh == 0) {
+    const float l2 = none ? -INFINITY : (m == -INFINITY ? 0.f : m - 10.f) + log2f(lt);
+    if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
+    if (a.lse2 != nullptr) a.lse2[row] = l2;
+  }
+  const float inv = 1.0f / lt;
+  uint8_t* op = a.out + n * a.ost + (int64_t)head * a.osh;
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      V4 h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = (T)(none ? 0.f : o[d][4 * q4 + e] * inv);
+      *(V4*)(op + 2 * (32 * d + 8 * q4 + 4 * lh)) = h;
+    }
+}
+
+// The weights of chunks.  A wave holds 32 entries' keys in registers, walks the
+// rows that may see them in tiles of 32 (their rotated queries in two parts
+// through LDS, shared by the workgroup's waves) and adds exp2(score - lse) up:
+// S^T[entry][row] leaves 16 entries of one row with a lane, the sum over the
+// rows' lanes comes last.  Every sum has one order.
+static const int kWeightEntries = 128;  // a workgroup's: four waves of 32
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void paged_chunk_weights_kernel(PagedAttnArgs a, int32_t blocks) {
+  typedef typename Half16<DT>::V8 V8;
+  constexpr int kSteps = D / 16, kRowBytes = 4 * D, kChunks = kRowBytes / 16;
+  constexpr int kLoads = 32 * kRowBytes / (256 * 16);
+  __shared__ __align__(16) uint8_t q_lds[2][32 * kRowBytes];
+  const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, lh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint32_t bid = xcd_remap(blockIdx.x, gridDim.x);
+  const int32_t blk = (int32_t)(bid % (uint32_t)blocks);
+  bid /= (uint32_t)blocks;
+  const int32_t b = (int32_t)(bid / (uint32_t)a.KVH), kvh = (int32_t)(bid % (uint32_t)a.KVH);
+  if (b >= a.c.B) return;
+  const PagedSeq s = paged_seq(a.c, b);
+  const int32_t j0 = blk * kWeightEntries;
+  if (j0 >= s.length) return;
+  const int32_t tokens = s.tokens < a.max_new ? s.tokens : a.max_new, before = s.length - s.tokens;
+  const int32_t wj0 = j0 + 32 * wave;
+
+  // the wave's keys (A operand: 8 dims of entry ln)
+  V8 kf[kSteps];
+  {
+    const int32_t j = wj0 + ln;
+    int32_t page = -1;
+    if (j < s.length) page = a.c.tables[b * a.c.table_stride + (j >> a.c.page_shift)];
+    const bool ok = (uint32_t)page < (uint32_t)a.c.n_pages;
+    const uint8_t* kp = a.c.k + (ok ? page * a.c.page_bytes + kvh * a.c.head_bytes +
+                                          (int64_t)(j & ((1 << a.c.page_shift) - 1)) * a.c.slot_bytes : 0) + 16 * lh;
+#pragma unroll
+    for (int c = 0; c < kSteps; ++c) {
+      kf[c] = V8{};
+      if (ok) kf[c] = *(const V8*)(kp + 32 * c);
+    }
+  }
+
+  // the rows that may see one of the workgroup's entries
+  int32_t t0 = j0 - before, t1 = tokens;
+  if (t0 < 0) t0 = 0;
+  if (j0 >= a.sinks) {
+    const int32_t end = j0 + kWeightEntries - 1 + a.window - before;  // the last entry's window ends here
+    if (end < t1) t1 = end;
+  }
+  const uint32_t per = (uint32_t)a.per;
+  const int32_t r0 = t0 * a.per, r1 = t1 * a.per;  // (rows fit 31 bits: host-checked)
+  float acc[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+
+  uint4v qs[kLoads];
+  auto fetch = [&](int32_t r) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = i * 256 + tid;
+      int32_t row = r + at / kChunks;
+      if (row >= r1) row = r1 - 1;
+      const int32_t t = (int32_t)((uint32_t)row / per);
+      qs[i] = *(const uint4v*)(a.q_parts + (int64_t)((s.row0 + t) * a.QH + kvh * a.per + (row - t * a.per)) * kRowBytes +
+                               16 * (at % kChunks));
+    }
+  };
+  auto stage = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = i * 256 + tid, r = at / kChunks;
+      *(uint4v*)(q_lds[buf] + r * kRowBytes + 16 * ((at % kChunks) ^ (r & 15))) = qs[i];
+    }
+  };
+  if (r0 < r1) {
+    fetch(r0);
+    stage(0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int32_t r = r0; r < r1; r += 32, buf ^= 1) {
+    const bool more = r + 32 < r1;
+    if (more) fetch(r + 32);
+    const int32_t row = r + ln;
+    const bool row_ok = row < r1;
+    const int32_t t = row_ok ? (int32_t)((uint32_t)row / per) : 0, self = row_ok ? before + t : -1;
+    float norm = INFINITY;
+    if (row_ok) norm = a.lse2[(int64_t)(s.row0 + t) * a.QH + kvh * a.per + (row - t * a.per)];
+    if (norm == -INFINITY) norm = INFINITY;  // it saw nothing
+    const uint8_t* ql = q_lds[buf];
+    float16v sc = {};
+#pragma unroll
+    for (int c = 0; c < kSteps; ++c) {
+      const V8 hi = *(const V8*)(ql + ln * kRowBytes + 16 * ((2 * c + lh) ^ (ln & 15)));
+      const V8 lo = *(const V8*)(ql + ln * kRowBytes + 16 * ((kChunks / 2 + 2 * c + lh) ^ (ln & 15)));
+      sc = mfma32<DT>(kf[c], hi, sc);
+      sc = mfma32<DT>(kf[c], lo, sc);
+    }
+    const int32_t tf = before + (int32_t)((uint32_t)r / per);
+    const int32_t tl = before + (int32_t)((uint32_t)(r + 31 < r1 ? r + 31 : r1 - 1) / per);
+    const bool full = r + 32 <= r1 && wj0 + 31 <= tf && (wj0 > tl - a.window || wj0 + 32 <= a.sinks);
+    if (!full) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int32_t j = wj0 + 8 * (e >> 2) + 4 * lh + (e & 3);
+        const bool seen = j <= self && (j > self - a.window || j < a.sinks);
+        sc[e] = seen ? sc[e] : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] += __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -norm));
+    if (more) stage(buf ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float v = acc[e];
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    const int32_t j = wj0 + 8 * (e >> 2) + 4 * lh + (e & 3);
+    if (ln == e && j < s.length) {
+      float* w = a.weights + b * a.wsb + kvh * a.wsh + j;
+      *w = a.accumulate ? *w + v : v;
+    }
+  }
+}
+
+template <int DT, int D>
+static int launch_chunk(const PagedAttnArgs& a, hipStream_t stream) {
+  const int64_t blocks = ceil_div((int64_t)a.items * a.KVH * a.splits, 8) * 8;
+  JKV_CHECK_ARG(blocks < ((int64_t)1 << 31), "paged attention grid too large");
+  const dim3 grid((uint32_t)blocks), block(64 * kChunkWaves);
+  if (a.lse != nullptr || a.lse2 != nullptr) hipLaunchKernelGGL((paged_chunk_kernel<DT, D, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((paged_chunk_kernel<DT, D, false>), grid, block, 0, stream, a);
+  if (a.splits > 1) {
+    const int rc = paged_launch_join(a, DT, D, stream);
+    if (rc != JKV_OK) return rc;
+  }
+  if (a.weights != nullptr && a.c.top > 0) {
+    const int64_t each = ceil_div(a.c.top, kWeightEntries), all = ceil_div(each * a.c.B * a.KVH, 8) * 8;
+    JKV_CHECK_ARG(all < ((int64_t)1 << 31), "paged weights grid too large");
+    hipLaunchKernelGGL((paged_chunk_weights_kernel<DT, D>), dim3((uint32_t)all), dim3(256), 0, stream, a, (int32_t)each);
+  }
+  JKV_CHECK_LAUNCH();
+  return JKV_OK;
+}
+
+int paged_launch_chunk(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream) {
+  if (dtype == JKV_F16) return D == 128 ? launch_chunk<JKV_F16, 128>(a, stream) : launch_chunk<JKV_F16, 64>(a, stream);
+  return D == 128 ? launch_chunk<JKV_BF16, 128>(a, stream) : launch_chunk<JKV_BF16, 64>(a, stream);
+}
+
+}  // namespace jkv

@@ -44,9 +44,6 @@ __device__ __forceinline__ float lanes4_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-typedef short short4_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) short4_t lds_short4_t;
-
 // Slot of 16-byte chunk j of row r in a tile: keys so that 16 rows' equal
 // chunks, values so that 8 rows' equal chunk pairs, fall on distinct banks.
 template <int D> __device__ __forceinline__ int key_slot(int r, int j) {
@@ -116,44 +113,53 @@ __global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_ker
     uint32_t voff[kHalfLoads];
 #pragma unroll
     for (int i = 0; i < kHalfLoads; ++i) voff[i] = (uint32_t)(i * kRowsPerLoad + lrow) * (uint32_t)a.c.slot_bytes + 16u * lchunk;
-    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-    u4 ks[kLoads], vs[kLoads];
+    uint4v ks[kLoads], vs[kLoads];
     const uint8_t* k_head = a.c.k + kvh * a.c.head_bytes;
     const uint8_t* v_head = a.c.v + kvh * a.c.head_bytes;
     auto entry_of = [&](int32_t i) { return (i < pt.lead ? i : pt.main + i - pt.lead) * kFewTile; };
     // lane h holds the page of half h of a run of 32 tiles
-    int32_t pages = -1;
+    int32_t pages = -1, run0 = -32;
     auto look_up = [&](int32_t i) {
+      run0 = i;
       const int32_t e = entry_of(i + (lane >> 1)) + 16 * (lane & 1);
       pages = -1;
       if (i + (lane >> 1) < tile1 && e < s.length) pages = table[e >> a.c.page_shift];
       if ((uint32_t)pages >= (uint32_t)a.c.n_pages) pages = -1;
     };
     auto fetch = [&](int32_t i) {
-      const int32_t e0 = entry_of(i), in_run = (i - tile0) & 31;
-      if (in_run == 0) look_up(i);
+      const int32_t e0 = entry_of(i);
+      if (i - run0 >= 32) look_up(i);
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int32_t e = e0 + 16 * hf;
         const int32_t left = s.length - e;  // entries of this half that exist
-        const int32_t page = __builtin_amdgcn_readlane(pages, 2 * in_run + hf);
+        const int32_t page = __builtin_amdgcn_readlane(pages, 2 * (i - run0) + hf);
         const int64_t at = page >= 0 ? page * a.c.page_bytes + (int64_t)(e & mask) * a.c.slot_bytes : 0;
         const int32_t bytes = page >= 0 ? ((left < 16 ? left : 16) - 1) * (int32_t)a.c.slot_bytes + kRowBytes : 0;
         const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(k_head + at), (short)0, bytes, 0x00020000);
         const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(v_head + at), (short)0, bytes, 0x00020000);
 #pragma unroll
         for (int j = 0; j < kHalfLoads; ++j) {
-          ks[hf * kHalfLoads + j] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)voff[j], 0, 0));
-          vs[hf * kHalfLoads + j] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)voff[j], 0, 0));
+          ks[hf * kHalfLoads + j] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)voff[j], 0, 0));
+          vs[hf * kHalfLoads + j] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)voff[j], 0, 0));
         }
       }
     };
-    auto stage = [&]() {
+    // every row sees the whole tile, or some entries are masked
+    auto is_full = [&](int32_t e0) {
+      return e0 + kFewTile - 1 <= first && (e0 > last - a.window || e0 + kFewTile <= a.sinks);
+    };
+    bool found = false;  // an infinite or NaN value in a masked tile
+    auto stage = [&](bool full) {
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) vs[i] = finite_halves<DT>(vs[i], &found);
+      }
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int r = i * kRowsPerLoad + lrow;
-        *(u4*)(k_lds + r * kRowBytes + 16 * key_slot<D>(r, lchunk)) = ks[i];
-        *(u4*)(v_lds + r * kRowBytes + 16 * value_slot<D>(r, lchunk)) = vs[i];
+        *(uint4v*)(k_lds + r * kRowBytes + 16 * key_slot<D>(r, lchunk)) = ks[i];
+        *(uint4v*)(v_lds + r * kRowBytes + 16 * value_slot<D>(r, lchunk)) = vs[i];
       }
     };
     fetch(tile0);
@@ -190,11 +196,17 @@ __global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_ker
       }
     }
 
-    const uint32_t v_base = (uint32_t)(size_t)(const void __attribute__((address_space(3)))*)v_lds;
+    const uint32_t v_base = lds_address(v_lds);
     const int tr_row = 4 * lg + (ln >> 2);
+    auto value_operand = [&](int d) -> V8 {
+      const uint32_t at = v_base + (uint32_t)(tr_row * kRowBytes + 16 * value_slot<D>(tr_row, 2 * d + ((ln & 3) >> 1)) + 8 * (ln & 1));
+      const V4 lo = lds_read_tr<V4>(at), hi = lds_read_tr<V4>(at + 16u * kRowBytes);
+      return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
     for (int32_t i = tile0; i < tile1; ++i) {
       const int32_t e0 = entry_of(i);
-      stage();
+      const bool full = is_full(e0);
+      stage(full);
       if (i + 1 < tile1) fetch(i + 1);
 
       float4v sc[RG][2];
@@ -213,10 +225,7 @@ __global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_ker
           }
         }
       }
-      // every row sees the whole tile, or some entries are masked
-      const bool full = e0 + kFewTile - 1 <= first && (e0 > last - a.window || e0 + kFewTile <= a.sinks);
       V8 ph[RG], pl[RG];
-      float pr[RG][8];
 #pragma unroll
       for (int g = 0; g < RG; ++g) {
         if (!full) {
@@ -255,7 +264,6 @@ __global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_ker
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float p = __builtin_amdgcn_exp2f(fmaf(sc[g][e >> 2][e & 3], a.scale2, -mu));
-          pr[g][e] = p;
           sum += p;
           const T hi = (T)p;
           ph[g][e] = hi;
@@ -263,56 +271,43 @@ __global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_ker
         }
         l[g] += sum;
       }
-      bool plain = true;
-      if (!full) {
-        // a masked weight is 0, but 0 times an infinite or NaN value is not:
-        // where a masked tile holds one, its values are added one by one
-        uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < kFewTile * kRowBytes / 1024; ++j) {
-          const u4 w = *(const u4*)(v_lds + 1024 * j + 16 * lane);
-          constexpr uint32_t kExp = DT == JKV_F16 ? 0x7c00u : 0x7f80u;
+      for (int d = 0; d < kDims; ++d) {
+        const V8 va = value_operand(d);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            top |= (w[e] & kExp) == kExp;
-            top |= ((w[e] >> 16) & kExp) == kExp;
-          }
+        for (int g = 0; g < RG; ++g) {
+          o[g][d] = mfma16<DT>(va, ph[g], o[g][d]);
+          o[g][d] = mfma16<DT>(va, pl[g], o[g][d]);
         }
-        plain = !__any(top != 0);
       }
-      if (plain) {
+    }
+    if (__any(found)) {
+      for (int32_t i = tile0; i < tile1; ++i) {
+        const int32_t e0 = entry_of(i);
+        if (is_full(e0)) continue;
+        look_up(i);
+        fetch(i);
+        stage(true);  // as they are
+        V8 seen[RG];
 #pragma unroll
-        for (int d = 0; d < kDims; ++d) {
-          const uint32_t at = v_base + (uint32_t)(tr_row * kRowBytes + 16 * value_slot<D>(tr_row, 2 * d + ((ln & 3) >> 1)) + 8 * (ln & 1));
-          const V4 lo = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(size_t)at));
-          const V4 hi = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(size_t)(at + 16u * kRowBytes)));
-          const V8 va = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-#pragma unroll
-          for (int g = 0; g < RG; ++g) {
-            o[g][d] = mfma16<DT>(va, ph[g], o[g][d]);
-            o[g][d] = mfma16<DT>(va, pl[g], o[g][d]);
-          }
-        }
-      } else {
-#pragma unroll 1
-        for (int from = 0; from < 4; ++from)
+        for (int g = 0; g < RG; ++g)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int k = 16 * (e >> 2) + 4 * from + (e & 3);
-            const int32_t j = e0 + k;
-#pragma unroll
-            for (int g = 0; g < RG; ++g) {
-              const float p = __shfl(pr[g][e], ln + 16 * from, 64);
-              const bool seen = j <= self[g] && (j > self[g] - a.window || j < a.sinks);
-              if (seen)
-#pragma unroll
-                for (int d = 0; d < kDims; ++d) {
-                  const V4 x = *(const V4*)(v_lds + k * kRowBytes + 16 * value_slot<D>(k, 2 * d + (lg >> 1)) + 8 * (lg & 1));
-#pragma unroll
-                  for (int i2 = 0; i2 < 4; ++i2) o[g][d][i2] = fmaf(p, (float)x[i2], o[g][d][i2]);
-                }
-            }
+            const int32_t j = e0 + 16 * (e >> 2) + 4 * lg + (e & 3);
+            seen[g][e] = j <= self[g] && (j > self[g] - a.window || j < a.sinks) ? (T)1.f : (T)0.f;
           }
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) {
+          V8 vu, vd;
+          non_finite_marks<DT>(value_operand(d), &vu, &vd);
+#pragma unroll
+          for (int g = 0; g < RG; ++g) {
+            const float4v zero = {0.f, 0.f, 0.f, 0.f};
+            const float4v up = mfma16<DT>(vu, seen[g], zero), down = mfma16<DT>(vd, seen[g], zero);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[g][d][e] = marked(o[g][d][e], up[e], down[e]);
+          }
+        }
       }
     }
   }
@@ -409,14 +404,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
   for (int e = 0; e < D / 64; ++e) op[e] = (T)(none ? 0.f : o[e] / l);
 }
 
+int paged_launch_join(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream) {
+  const dim3 grid((uint32_t)ceil_div((int64_t)a.c.N * a.QH, 4)), block(256);
+  if (dtype == JKV_F16 && D == 128) hipLaunchKernelGGL((paged_join_kernel<JKV_F16, 128>), grid, block, 0, stream, a);
+  else if (dtype == JKV_F16) hipLaunchKernelGGL((paged_join_kernel<JKV_F16, 64>), grid, block, 0, stream, a);
+  else if (D == 128) hipLaunchKernelGGL((paged_join_kernel<JKV_BF16, 128>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((paged_join_kernel<JKV_BF16, 64>), grid, block, 0, stream, a);
+  JKV_CHECK_LAUNCH();
+  return JKV_OK;
+}
+
 template <int DT, int D>
 static int launch_few(const PagedAttnArgs& a, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.c.B * a.KVH * a.splits;
   JKV_CHECK_ARG(blocks < ((int64_t)1 << 31), "paged attention grid too large");
   if (a.max_new * a.per <= 16) hipLaunchKernelGGL((paged_few_kernel<DT, D, 1>), dim3((uint32_t)blocks), dim3(64), 0, stream, a);
   else hipLaunchKernelGGL((paged_few_kernel<DT, D, 2>), dim3((uint32_t)blocks), dim3(64), 0, stream, a);
-  if (a.splits > 1)
-    hipLaunchKernelGGL((paged_join_kernel<DT, D>), dim3((uint32_t)ceil_div((int64_t)a.c.N * a.QH, 4)), dim3(256), 0, stream, a);
+  if (a.splits > 1) {
+    const int rc = paged_launch_join(a, DT, D, stream);
+    if (rc != JKV_OK) return rc;
+  }
   if (a.weights != nullptr && a.c.top > 0) {
     const int64_t bh = (int64_t)a.c.B * a.KVH;
     hipLaunchKernelGGL(paged_few_weights_kernel, dim3((uint32_t)ceil_div(a.c.top, 256), (uint32_t)(bh < 32768 ? bh : 32768),

@@ -6,6 +6,7 @@
 // is fp32 products of the 16-bit key with fp32 cos/sin, rounded once to the
 // cache's type.
 #include <math.h>
+#include <string.h>
 
 #include "paged.h"
 
@@ -46,8 +47,18 @@ int paged_cache_args(PagedCache* c, const void* k, const void* v, int64_t page_s
 int paged_rope_args(RopeRates* r, double theta, int64_t D) {
   JKV_CHECK_ARG(theta == 0.0 || (theta > 0.0 && isfinite(theta)), "the rotary base must be positive, or 0 for none");
   r->on = theta > 0.0;
-  for (int i = 0; i < 64; ++i)
-    r->turns[i] = r->on && i < D / 2 ? pow(theta, -2.0 * i / (double)D) / 6.283185307179586476925286766559 : 0.0;
+  if (!r->on) return JKV_OK;
+  // a thread's last rates: 64 powers cost a small call a microsecond or two
+  static thread_local double last_theta = 0.0;
+  static thread_local int64_t last_dim = 0;
+  static thread_local double last[64];
+  if (last_theta != theta || last_dim != D) {
+    for (int i = 0; i < 64; ++i)
+      last[i] = i < D / 2 ? pow(theta, -2.0 * i / (double)D) / 6.283185307179586476925286766559 : 0.0;
+    last_theta = theta;
+    last_dim = D;
+  }
+  memcpy(r->turns, last, sizeof(last));
   return JKV_OK;
 }
 

@@ -6,13 +6,14 @@
 // equals, `budget` in all.  One workgroup per (sequence, kv head) finds the
 // weight of the last one that stays by three histograms over 11, 11 and 10
 // bits of the weights' order-preserving words, then lists the entries that
-// stay in their order with two counts a thread and one scan per 4,096.  Every
+// stay in their order, placed by the waves' ballots and one scan a round.  Every
 // sum is of integers, so a call repeats exactly.
 #include "paged.h"
 
 namespace jkv {
 
 static const int kSelectThreads = 1024;
+static const int kRound = 16 * kSelectThreads;
 
 // Unsigned order of weights: -0 counts as 0, NaN below every number.
 __device__ __forceinline__ uint32_t weight_order(float w) {
@@ -70,6 +71,23 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(SelectArgs
     return;
   }
   const int32_t first = a.sinks, last = length - a.recent;  // the entries that compete
+  const int lane = tid & 63, wave = tid >> 6;
+  // 16 entries a thread and round, entry base + 1,024 k + tid: up to 16,384 are
+  // read once and stay in registers, longer rows are read again by every pass
+  const int32_t rounds = (length + kRound - 1) / kRound;
+  uint32_t u[16];
+  auto load = [&](int32_t base) {
+    float x[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int32_t i = base + 1024 * k + tid;
+      x[k] = w[i < length ? i : 0];
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) u[k] = weight_order(x[k]);
+  };
+  if (rounds == 1) load(0);
+
   uint32_t need = (uint32_t)(a.budget - a.sinks - a.recent);
   uint32_t prefix = 0;  // of the order word of the last entry that stays
   if (need > 0) {
@@ -79,9 +97,22 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(SelectArgs
       hist[tid] = 0u;
       hist[tid + 1024] = 0u;
       __syncthreads();
-      for (int32_t i = first + tid; i < last; i += kSelectThreads) {
-        const uint32_t u = weight_order(w[i]);
-        if (pass == 0 || (u >> (shift + bits)) == prefix) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1u)], 1u);
+      for (int32_t round = 0; round < rounds; ++round) {
+        if (rounds > 1) load(round * kRound);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const int32_t i = round * kRound + 1024 * k + tid;
+          const bool in = i >= first && i < last && (pass == 0 || (u[k] >> (shift + bits)) == prefix);
+          const uint32_t digit = (u[k] >> shift) & ((1u << bits) - 1u);
+          // lanes that share the first one's digit count once (many weights are
+          // equal, or close); the others one by one
+          const uint64_t on = __ballot(in);
+          if (on == 0) continue;
+          const uint32_t lead = __builtin_amdgcn_readlane(digit, __builtin_ctzll(on));
+          const uint64_t same = __ballot(in && digit == lead);
+          if (in && digit != lead) atomicAdd(&hist[digit], 1u);
+          if (lane == __builtin_ctzll(on)) atomicAdd(&hist[lead], (uint32_t)__builtin_popcountll(same));
+        }
       }
       __syncthreads();
       // from the largest digit down, the one that holds the need-th
@@ -102,43 +133,41 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(SelectArgs
   } else {
     prefix = 0xffffffffu;  // above every weight: none of them stays
   }
-  // in order: those above the last one's word, and `need` of those at it
-  uint32_t done = 0, ties = 0;  // kept above or by force, and at the word, so far
-  for (int32_t base = 0; base < length; base += 4 * kSelectThreads) {
-    uint32_t flags = 0, over = 0, at = 0;
+
+  // in order: those above the last one's word, and `need` of those at it.  The
+  // waves' counts of every 1,024 entries meet in LDS (high half: at the word).
+  uint32_t over_done = 0, ties_done = 0;
+  for (int32_t round = 0; round < rounds; ++round) {
+    if (rounds > 1) load(round * kRound);
+    uint64_t over[16], at[16];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int32_t i = base + 4 * tid + e;
-      if (i >= length) continue;
-      if (i < first || i >= last) {
-        flags |= 1u << e;
-        ++over;
-        continue;
-      }
-      const uint32_t u = weight_order(w[i]);
-      if (u > prefix) {
-        flags |= 1u << e;
-        ++over;
-      } else if (u == prefix && need > 0) {
-        flags |= 16u << e;
-        ++at;
-      }
+    for (int k = 0; k < 16; ++k) {
+      const int32_t i = round * kRound + 1024 * k + tid;
+      const bool in = i < length, forced = i < first || i >= last;
+      over[k] = __ballot(in && (forced || u[k] > prefix));
+      at[k] = __ballot(in && !forced && u[k] == prefix && need > 0);
+      if (lane == 0)
+        hist[16 * k + wave] = (uint32_t)__builtin_popcountll(over[k]) | ((uint32_t)__builtin_popcountll(at[k]) << 16);
     }
+    __syncthreads();
+    const uint32_t mine = tid < 256 ? hist[tid] : 0u;
     uint32_t all;
-    const uint32_t mine = over | (at << 16), upto = block_scan(mine, part, &all);
-    uint32_t over_before = done + ((upto - mine) & 0xffffu), at_before = ties + ((upto - mine) >> 16);
+    const uint32_t upto = block_scan(mine, part, &all);
+    if (tid < 256) hist[tid] = upto - mine;
+    __syncthreads();
+    const uint64_t below = (1ull << lane) - 1ull;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool tie = flags & (16u << e);
-      if ((flags & (1u << e)) || (tie && at_before < need)) {
-        const uint32_t to = over_before + (at_before < need ? at_before : need);
-        if (to < (uint32_t)a.budget) kept[to] = base + 4 * tid + e;
-      }
-      over_before += (flags >> e) & 1u;
-      at_before += tie ? 1u : 0u;
+    for (int k = 0; k < 16; ++k) {
+      const uint32_t prior = hist[16 * k + wave];
+      const uint32_t ties = ties_done + (prior >> 16) + (uint32_t)__builtin_popcountll(at[k] & below);
+      const bool stays = (over[k] >> lane & 1ull) || ((at[k] >> lane & 1ull) && ties < need);
+      const uint32_t to = over_done + (prior & 0xffffu) + (uint32_t)__builtin_popcountll(over[k] & below) +
+                          (ties < need ? ties : need);
+      if (stays && to < (uint32_t)a.budget) kept[to] = round * kRound + 1024 * k + tid;
     }
-    done += all & 0xffffu;
-    ties += all >> 16;
+    over_done += all & 0xffffu;
+    ties_done += all >> 16;
+    __syncthreads();
   }
 }
 

@@ -367,49 +367,101 @@ __global__ __launch_bounds__(256) void paged_few_weights_kernel(PagedAttnArgs a)
   *w = a.accumulate ? *w + sum : sum;
 }
 
-// One wave a row: the splits' parts by their maxima and sums.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+// Joins the splits' parts of a row by their maxima and sums.  D/4 lanes hold a
+// row; GROUPS of them share out its splits, several loads in flight each, and
+// meet in LDS, always in the same order.
+template <int DT, int D, int GROUPS>
+__global__ __launch_bounds__(8 * D) void paged_join_kernel(PagedAttnArgs a) {
   typedef typename Half16<DT>::T T;
-  const int lane = threadIdx.x & 63;
-  const int64_t rows = (int64_t)a.c.N * a.QH, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const int32_t n = (int32_t)((uint64_t)row / (uint32_t)a.QH), head = (int32_t)(row - (int64_t)n * a.QH);
-  if (a.c.starts != nullptr && (n < a.c.starts[0] || n >= a.c.starts[a.c.B])) return;  // nobody's row
-  float top = -INFINITY;
-  for (int32_t i = lane; i < a.splits; i += 64) top = fmaxf(top, a.part_ml[i * rows + row].x);
+  typedef typename Half16<DT>::V4 V4;
+  constexpr int kLanes = D / 4, kRows = 32 / GROUPS;
+  __shared__ __align__(16) float o_lds[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kRows : 1][D];
+  __shared__ float2 ml_lds[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kRows : 1];
+  const int tid = threadIdx.x, part = tid % kLanes, g = tid / kLanes % GROUPS, r = tid / (kLanes * GROUPS);
+  const int64_t rows = (int64_t)a.c.N * a.QH, row = (int64_t)blockIdx.x * kRows + r;
+  const int32_t n = (int32_t)((uint32_t)row / (uint32_t)a.QH), head = (int32_t)(row - (int64_t)n * a.QH);
+  // (nobody's rows stay as they are)
+  const bool on = row < rows && (a.c.starts == nullptr || (n >= a.c.starts[0] && n < a.c.starts[a.c.B]));
+  float m = -INFINITY, l = 0.f;
+  float4v o = {0.f, 0.f, 0.f, 0.f};
+  if (on) {
+    for (int32_t i0 = g; i0 < a.splits; i0 += 8 * GROUPS) {
+      float2 ml[8];
+      float4v p[8];
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  float l = 0.f, o[D / 64];
+      for (int j = 0; j < 8; ++j) {
+        const int32_t i = i0 + j * GROUPS < a.splits ? i0 + j * GROUPS : i0;
+        ml[j] = a.part_ml[i * rows + row];
+        p[j] = *(const float4v*)(a.part_o + (i * rows + row) * D + 4 * part);
+      }
+      float top = m;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int32_t i = 0; i < a.splits; ++i) {
-    const float2 ml = a.part_ml[i * rows + row];
-    if (ml.y == 0.f) continue;  // it saw nothing; an empty one has written no sums
-    const float f = __builtin_amdgcn_exp2f(ml.x - top);
-    l = fmaf(ml.y, f, l);
-    const float* p = a.part_o + (i * rows + row) * D + lane * (D / 64);
+      for (int j = 0; j < 8; ++j) {
+        if (i0 + j * GROUPS >= a.splits) ml[j] = float2{-INFINITY, 0.f};
+        top = fmaxf(top, ml[j].x);
+      }
+      const float f0 = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+      l *= f0;
+      o *= f0;
+      m = top;
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] = fmaf(p[e], f, o[e]);
+      for (int j = 0; j < 8; ++j)
+        if (ml[j].y != 0.f) {  // a split that saw nothing may have written no sums
+          const float f = __builtin_amdgcn_exp2f(ml[j].x - top);
+          l = fmaf(ml[j].y, f, l);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = fmaf(p[j][e], f, o[e]);
+        }
+    }
   }
+  if constexpr (GROUPS > 1) {
+    *(float4v*)&o_lds[g][r][4 * part] = o;
+    if (part == 0) ml_lds[g][r] = float2{m, l};
+    __syncthreads();
+    if (g != 0) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) top = fmaxf(top, ml_lds[j][r].x);
+    l = 0.f;
+    o = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
+      const float2 ml = ml_lds[j][r];
+      if (ml.y == 0.f) continue;
+      const float f = __builtin_amdgcn_exp2f(ml.x - top);
+      l = fmaf(ml.y, f, l);
+      const float4v p = *(const float4v*)&o_lds[j][r][4 * part];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(p[e], f, o[e]);
+    }
+    m = top;
+  }
+  if (!on) return;
   const bool none = l == 0.f;
-  if (lane == 0) {
-    const float l2 = none ? -INFINITY : top + log2f(l);
+  if (part == 0) {
+    const float l2 = none ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
     if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
     if (a.lse2 != nullptr) a.lse2[row] = l2;
   }
-  T* op = (T*)(a.out + n * a.ost + head * a.osh) + lane * (D / 64);
+  V4 h;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) op[e] = (T)(none ? 0.f : o[e] / l);
+  for (int e = 0; e < 4; ++e) h[e] = (T)(none ? 0.f : o[e] / l);
+  *(V4*)(a.out + n * a.ost + head * a.osh + 8 * part) = h;
+}
+
+template <int DT, int D>
+static void launch_join(const PagedAttnArgs& a, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.c.N * a.QH;
+  const dim3 block(8 * D);
+  if (a.splits > 8)
+    hipLaunchKernelGGL((paged_join_kernel<DT, D, 8>), dim3((uint32_t)ceil_div(rows, 4)), block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_join_kernel<DT, D, 1>), dim3((uint32_t)ceil_div(rows, 32)), block, 0, stream, a);
 }
 
 int paged_launch_join(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream) {
-  const dim3 grid((uint32_t)ceil_div((int64_t)a.c.N * a.QH, 4)), block(256);
-  if (dtype == JKV_F16 && D == 128) hipLaunchKernelGGL((paged_join_kernel<JKV_F16, 128>), grid, block, 0, stream, a);
-  else if (dtype == JKV_F16) hipLaunchKernelGGL((paged_join_kernel<JKV_F16, 64>), grid, block, 0, stream, a);
-  else if (D == 128) hipLaunchKernelGGL((paged_join_kernel<JKV_BF16, 128>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((paged_join_kernel<JKV_BF16, 64>), grid, block, 0, stream, a);
+  if (dtype == JKV_F16) D == 128 ? launch_join<JKV_F16, 128>(a, stream) : launch_join<JKV_F16, 64>(a, stream);
+  else D == 128 ? launch_join<JKV_BF16, 128>(a, stream) : launch_join<JKV_BF16, 64>(a, stream);
   JKV_CHECK_LAUNCH();
   return JKV_OK;
 }

@@ -34,16 +34,20 @@ from typing import Sequence
 import torch
 
 from . import _lib
+from ._ops import _plain
 from .attention import MISTRAL_ROPE_THETA, MISTRAL_WINDOW
 
 PAGE_TYPES = (torch.float16, torch.bfloat16)
+
+
+_NO_CHANGE = contextlib.nullcontext()
 
 
 def _current(device: torch.device):
     """The device's own context where another device is current."""
 
     if torch._C._cuda_getDevice() == device.index:
-        return contextlib.nullcontext()
+        return _NO_CHANGE
     return torch.cuda.device(device)
 
 
@@ -66,7 +70,7 @@ def _pool_args(key_pages: torch.Tensor, value_pages: torch.Tensor, written: bool
         raise ValueError("key and value pages need identical strides")
     if strides[3] != 1:
         raise ValueError("page rows must be contiguous")
-    pages, heads, size, dim = map(int, key_pages.shape)
+    pages, heads, size, dim = key_pages.shape
     if written and not key_pages.is_contiguous():
         # slots that share memory would be written by more than one entry
         span = 1
@@ -78,22 +82,26 @@ def _pool_args(key_pages: torch.Tensor, value_pages: torch.Tensor, written: bool
 
 
 def _batch_args(block_tables, lengths, starts, positions, rows: int) -> tuple:
-    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or (
-            block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+    if block_tables.dtype != torch.int32 or block_tables.ndim != 2:
         raise ValueError("block tables must be int32 [B,pages] with contiguous rows")
-    batch = int(block_tables.shape[0])
-    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (batch,):
+    batch, width = block_tables.shape
+    row, step = block_tables.stride()
+    if step != 1 and width > 1:
+        raise ValueError("block tables must be int32 [B,pages] with contiguous rows")
+    if lengths.dtype != torch.int32 or lengths.shape != (batch,):
         raise ValueError("lengths must be int32 [B]")
     if starts is None:
         if rows != batch:
             raise ValueError("without starts there is one new token a sequence")
-    elif starts.dtype != torch.int32 or tuple(starts.shape) != (batch + 1,):
-        raise ValueError("starts must be int32 [B+1]")
-    if positions is not None and (positions.dtype != torch.int32 or tuple(positions.shape) != (batch,)):
-        raise ValueError("positions must be int32 [B]")
-    ints = [None if t is None else t.contiguous() for t in (lengths, starts, positions)]
-    table = (block_tables.data_ptr(), block_tables.stride(0), int(block_tables.shape[1]))
-    return batch, table, ints
+    else:
+        if starts.dtype != torch.int32 or starts.shape != (batch + 1,):
+            raise ValueError("starts must be int32 [B+1]")
+        starts = starts.contiguous()
+    if positions is not None:
+        if positions.dtype != torch.int32 or positions.shape != (batch,):
+            raise ValueError("positions must be int32 [B]")
+        positions = positions.contiguous()
+    return batch, (block_tables.data_ptr(), row, width), (lengths.contiguous(), starts, positions)
 
 
 def _theta(rope_theta: float | None) -> float:
@@ -130,11 +138,11 @@ def paged_append(
 
     device = _lib.require_device(key, value, key_pages, value_pages, block_tables, lengths, starts, positions)
     strides, heads, dim = _pool_args(key_pages, value_pages, written=True)
-    if key.ndim != 3 or key.shape != value.shape or tuple(key.shape[1:]) != (heads, dim):
+    if key.ndim != 3 or key.shape != value.shape or key.shape[1:] != (heads, dim):
         raise ValueError("new keys and values must be [N,KVH,D] of the pages' heads and dims")
     if key.dtype != key_pages.dtype or value.dtype != key_pages.dtype:
         raise ValueError("new keys and values must have the pages' type")
-    rows = int(key.shape[0])
+    rows = key.shape[0]
     batch, table, (lengths, starts, positions) = _batch_args(block_tables, lengths, starts, positions, rows)
     key, value = _rows(key), _rows(value)
     with _current(device):
@@ -190,9 +198,11 @@ def paged_attention(
     device = _lib.require_device(query, key_pages, value_pages, block_tables, lengths, starts, positions, weights,
                                  lse, out)
     strides, heads, dim = _pool_args(key_pages, value_pages, written=False)
-    if query.ndim != 3 or query.shape[2] != dim or query.dtype != key_pages.dtype:
+    if query.ndim != 3 or query.dtype != key_pages.dtype:
         raise ValueError("queries must be [N,QH,D] of the pages' type and dims")
-    rows, qheads = int(query.shape[0]), int(query.shape[1])
+    rows, qheads, query_dim = query.shape
+    if query_dim != dim:
+        raise ValueError("queries must be [N,QH,D] of the pages' type and dims")
     if qheads == 0 or qheads % heads:
         raise ValueError("query heads must be a multiple of kv heads")
     batch, table, (lengths, starts, positions) = _batch_args(block_tables, lengths, starts, positions, rows)
@@ -201,24 +211,26 @@ def paged_attention(
         raise ValueError("window must be positive")
     if sinks < 0 or (max_new is not None and max_new < 0) or (max_length is not None and max_length < 0):
         raise ValueError("sinks, max_new and max_length must not be negative")
+    weight_args = (None, 0, 0, 0)
     if weights is not None:
-        if (weights.dtype != torch.float32 or weights.ndim != 3 or tuple(weights.shape[:2]) != (batch, heads)
-                or (weights.shape[2] > 1 and weights.stride(2) != 1)):
+        if weights.dtype != torch.float32 or weights.ndim != 3 or weights.shape[:2] != (batch, heads) or (
+                weights.shape[2] > 1 and weights.stride(2) != 1):
             raise ValueError("weights must be fp32 [B,KVH,C] with contiguous rows")
-        width = int(weights.shape[2])
+        width, (per_batch, per_head, _one) = weights.shape[2], weights.stride()
         if max_length is None:
             max_length = min(room, width)
         elif min(max_length, room) > width:
             raise ValueError("weights have fewer entries than max_length")
-        if batch * heads * width and (0 in (weights.stride(0), weights.stride(1)) and batch * heads > 1
-                                      and (weights.stride(0) == 0 and batch > 1 or weights.stride(1) == 0 and heads > 1)):
+        if (heads > 1 and per_head < width) or (batch > 1 and per_batch < (heads - 1) * per_head + width and (
+                per_batch < width or (heads > 1 and per_head < (batch - 1) * per_batch + width))):
             raise ValueError("weights that are written must not overlap")
+        weight_args = (weights.data_ptr(), per_batch, per_head, width)
     max_length = room if max_length is None else min(int(max_length), room)
     max_new = 1 if starts is None else (rows if max_new is None else min(int(max_new), rows))
-    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (rows, qheads) or not lse.is_contiguous()):
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (rows, qheads) or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous fp32 [N,QH] tensor")
     if out is None:
-        out = torch.empty((rows, qheads, dim), dtype=query.dtype, device=device)
+        out = _plain(query)((rows, qheads, dim))
     elif out.dtype != query.dtype or out.shape != query.shape or out.stride(2) != 1 or out.stride(0) % 8 or (
             out.stride(1) % 8 or out.data_ptr() % 16):
         raise ValueError("out must match the queries, with contiguous 16-byte aligned rows")
@@ -229,8 +241,6 @@ def paged_attention(
         ws_bytes = _lib.workspace_bytes("jkv_paged_attention_workspace_bytes", rows, batch, qheads, heads, dim, max_new,
                                         max_length, span, sinks, int(weights is not None))
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
-        weight_args = (None, 0, 0, 0) if weights is None else (weights.data_ptr(), weights.stride(0),
-                                                               weights.stride(1), int(weights.shape[2]))
         _lib.check(_lib.load().jkv_paged_attention(
             query.data_ptr(), query.stride(0), query.stride(1), _lib.dtype_code(query.dtype), key_pages.data_ptr(),
             value_pages.data_ptr(), *strides, *table, lengths.data_ptr(), _lib.ptr(starts), _lib.ptr(positions), rows,

@@ -114,6 +114,7 @@ struct PagedAttnArgs {
   int32_t items;  // chunks: an upper bound of all sequences' row blocks
   // splits of the entries, joined by paged_join_kernel (one split: none)
   int32_t splits, split_tiles;
+  int32_t waves;  // few rows: 1, or more waves a workgroup that join in LDS
   float2* part_ml;  // [splits][N*QH] reference maximum (base 2) and sum
   float* part_o;    // [splits][N*QH][D]
   float* lse2;      // [N,QH] base-2 log-sum-exp for the weights, or null

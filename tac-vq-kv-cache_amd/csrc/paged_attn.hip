@@ -19,7 +19,7 @@ namespace jkv {
 // How a call's work is divided and what of the workspace it takes.
 struct PagedPlan {
   bool few;  // at most 32 rows a sequence and kv head
-  int64_t items, splits, split_tiles, score_width;
+  int64_t items, waves, splits, split_tiles, score_width;
   int64_t ml_at, o_at, lse2_at, scores_at, q_at, bytes;
 };
 
@@ -41,9 +41,25 @@ static PagedPlan paged_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64
     const int64_t bound = ceil_div(window + max_new, 32) + 1 + ceil_div(sinks, 32);
     if (bound < tiles) tiles = bound;
     if (tiles < 1) tiles = 1;
-    // two waves a SIMD of every CU
-    const int64_t want = std::max<int64_t>(1, 2048 / std::max<int64_t>(1, B * KVH));
-    p.split_tiles = std::max<int64_t>(2, ceil_div(tiles, want));
+    // A wave's tile takes about 1.7 us (its loads), a join 5: up to four tiles
+    // stay with one wave.  More waves of a workgroup that join in LDS save the
+    // join where each has at most two tiles, or eight where the sequences alone
+    // fill half the CUs, and where one round of workgroups holds all (a CU holds
+    // one at 128 dims, two at 64).  us with splits and with eight waves, 32/8
+    // heads of 128: 16 x 128 entries 13.1 and 9.9, 16 x 500 18.4 and 16.7, 16 x
+    // 1,000 23.5 and 21.1; 4 x 1,000 16.4 and 18.7, 64 x 500 36.8 and 40.7.
+    const int64_t bh = B * KVH, many = D == 128 && max_new * per > 16 ? 4 : 8;
+    p.waves = 1;
+    if (tiles <= 4) {
+      p.split_tiles = tiles;
+    } else if (bh <= 256 * (128 / D) && (tiles <= 2 * many || (bh >= 128 && tiles <= 8 * many))) {
+      p.waves = many;
+      p.split_tiles = tiles;
+    } else {
+      // two waves a SIMD of every CU
+      const int64_t want = std::max<int64_t>(1, 2048 / std::max<int64_t>(1, bh));
+      p.split_tiles = std::max<int64_t>(2, ceil_div(tiles, want));
+    }
     p.splits = ceil_div(tiles, p.split_tiles);
     if (p.splits > 1) {
       p.ml_at = take(p.splits * N * QH * 8);
@@ -135,6 +151,7 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   a.scale2 = scale == 0.f ? 1.f : fabsf(scale) * 2.f * 1.4426950408889634f;
   a.splits = (int32_t)p.splits; a.split_tiles = (int32_t)p.split_tiles;
   a.items = (int32_t)p.items;
+  a.waves = (int32_t)p.waves;
   a.part_ml = (float2*)(ws + p.ml_at);
   a.part_o = (float*)(ws + p.o_at);
   if (weights != nullptr) {

@@ -53,17 +53,21 @@ template <int D> __device__ __forceinline__ int value_slot(int r, int j) {
   return D == 128 ? j ^ (2 * (r & 7)) : j ^ (2 * ((r >> 1) & 3));
 }
 
-template <int DT, int D, int RG>
-__global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_kernel(PagedAttnArgs a) {
+template <int DT, int D, int RG, int W>
+__global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few_kernel(PagedAttnArgs a) {
   typedef typename Half16<DT>::T T;
   typedef typename Half16<DT>::V8 V8;
   typedef typename Half16<DT>::V4 V4;
   constexpr int kSteps = D / 32, kDims = D / 16, kRowBytes = 2 * D;
   constexpr int kRowsPerLoad = 1024 / kRowBytes, kLoads = kFewTile / kRowsPerLoad, kHalfLoads = kLoads / 2;
-  __shared__ __align__(16) uint8_t k_lds[kFewTile * kRowBytes];
-  __shared__ __align__(16) uint8_t v_lds[kFewTile * kRowBytes];
+  __shared__ __align__(16) uint8_t lds[W][2 * kFewTile * kRowBytes];
+  static_assert(2 * kFewTile * kRowBytes >= 16 * RG * D * 4, "a wave's sums fit its tile's room");
+  __shared__ float2 ml_lds[W > 1 ? W : 1][W > 1 ? 16 * RG : 1];
 
-  const int lane = threadIdx.x, ln = lane & 15, lg = lane >> 4;
+  const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
+  const int wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  uint8_t* const k_lds = lds[wave];
+  uint8_t* const v_lds = lds[wave] + kFewTile * kRowBytes;
   const uint32_t bid = blockIdx.x;
   const uint32_t bh = bid / (uint32_t)a.splits;
   const int32_t split = (int32_t)(bid - bh * (uint32_t)a.splits);
@@ -75,8 +79,13 @@ __global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_ker
   const int32_t first = s.length - s.tokens, last = first + tokens - 1;
 
   const PagedTiles pt = paged_tiles(first, last, a.window, a.sinks, kFewTile);
-  const int32_t tile0 = split * a.split_tiles;
-  const int32_t tile1 = split == a.splits - 1 || tile0 + a.split_tiles > pt.count ? pt.count : tile0 + a.split_tiles;
+  int32_t tile0 = split * a.split_tiles;
+  int32_t tile1 = split == a.splits - 1 || tile0 + a.split_tiles > pt.count ? pt.count : tile0 + a.split_tiles;
+  if constexpr (W > 1) {  // the workgroup's waves share them out
+    const int32_t each = tile1 > tile0 ? (tile1 - tile0 + W - 1) / W : 0;
+    tile0 += wave * each;
+    if (tile0 + each < tile1) tile1 = tile0 + each;
+  }
 
   // the lane's rows, one per row group
   int32_t row_t[RG], self[RG];
@@ -104,6 +113,17 @@ __global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_ker
   }
 
   if (tile0 < tile1) {
+    // ---- the queries as they are: their loads run beside the look-ups below ----
+    V8 qx[RG][kSteps];
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      const int32_t r = row_ok[g] ? 16 * g + ln : 0;
+      const uint8_t* qp = a.q + (int64_t)(s.row0 + row_t[g]) * a.qst +
+                          (int64_t)(kvh * a.per + (r - row_t[g] * a.per)) * a.qsh;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) qx[g][c] = *(const V8*)(qp + 64 * c + 16 * lg);
+    }
+
     // ---- tile loader: 16-entry halves lie in one page (page sizes are multiples
     // of 16).  A page outside the pool and the entries at or behind the length
     // lie beyond the resource's bound and load as zeros. ----
@@ -168,16 +188,12 @@ __global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_ker
     V8 qh[RG][kSteps], ql[RG][kSteps];
 #pragma unroll
     for (int g = 0; g < RG; ++g) {
-      const int32_t r = row_ok[g] ? 16 * g + ln : 0;
-      const uint8_t* qp = a.q + (int64_t)(s.row0 + row_t[g]) * a.qst +
-                          (int64_t)(kvh * a.per + (r - row_t[g] * a.per)) * a.qsh;
 #pragma unroll
       for (int c = 0; c < kSteps / 2; ++c) {
         const int d0 = 32 * c + 8 * lg;
-        const V8 x0 = *(const V8*)(qp + 2 * d0), x1 = *(const V8*)(qp + 2 * d0 + D);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float u = (float)x0[e], w = (float)x1[e];
+          float u = (float)qx[g][c][e], w = (float)qx[g][c + kSteps / 2][e];
           if (a.rope.on) {
             float cs, sn;
             rope_trig(a.rope.turns[d0 + e], s.pos0 + row_t[g], &cs, &sn);
@@ -312,7 +328,56 @@ __global__ __launch_bounds__(64, RG == 2 && D == 128 ? 1 : 2) void paged_few_ker
     }
   }
 
-  // ---- out, or this split's part of it: lane holds dims 16d + 4lg + e of row ln ----
+  // ---- out, or this split's part of it ----
+  if constexpr (W > 1) {
+    // the waves' sums meet in LDS, in the waves' order
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      const float lt = lanes4_sum(l[g]);
+      if (lg == 0) ml_lds[wave][16 * g + ln] = float2{m[g] == -INFINITY ? m[g] : m[g] - 10.f, lt};
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+        *(float4v*)(lds[wave] + ((16 * g + ln) * D + 16 * d + 4 * lg) * 4) = o[g][d];
+    }
+    __syncthreads();
+    for (int32_t i = threadIdx.x; i < R * (D / 4); i += 64 * W) {
+      const int32_t r = i / (D / 4), part = i % (D / 4);
+      float top = -INFINITY, lt = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) top = fmaxf(top, ml_lds[w][r].x);
+      float4v acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float2 ml = ml_lds[w][r];
+        if (ml.y == 0.f) continue;
+        const float f = __builtin_amdgcn_exp2f(ml.x - top);
+        lt = fmaf(ml.y, f, lt);
+        const float4v p = *(const float4v*)(lds[w] + (r * D + 4 * part) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(p[e], f, acc[e]);
+      }
+      const int32_t t = (int32_t)((uint32_t)r / (uint32_t)a.per), head = kvh * a.per + (r - t * a.per);
+      const int64_t row = (int64_t)(s.row0 + t) * a.QH + head;
+      if (a.splits > 1) {
+        const int64_t at = (int64_t)split * a.c.N * a.QH + row;
+        if (part == 0) a.part_ml[at] = float2{top, lt};
+        *(float4v*)(a.part_o + at * D + 4 * part) = acc;
+        continue;
+      }
+      const bool none = lt == 0.f;  // sees nothing
+      if (part == 0) {
+        const float l2 = none ? -INFINITY : (top == -INFINITY ? 0.f : top) + log2f(lt);
+        if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
+        if (a.lse2 != nullptr) a.lse2[row] = l2;
+      }
+      V4 h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = (T)(none ? 0.f : acc[e] / lt);
+      *(V4*)(a.out + (int64_t)(s.row0 + t) * a.ost + (int64_t)head * a.osh + 8 * part) = h;
+    }
+    return;
+  }
+  // lane holds dims 16d + 4lg + e of row ln
 #pragma unroll
   for (int g = 0; g < RG; ++g) {
     const float lt = lanes4_sum(l[g]);
@@ -370,21 +435,33 @@ __global__ __launch_bounds__(256) void paged_few_weights_kernel(PagedAttnArgs a)
 // Joins the splits' parts of a row by their maxima and sums.  D/4 lanes hold a
 // row; GROUPS of them share out its splits, several loads in flight each, and
 // meet in LDS, always in the same order.
+struct JoinArgs {
+  const float2* part_ml;
+  const float* part_o;
+  const int32_t* starts;
+  uint8_t* out;
+  int64_t ost, osh;
+  float *lse, *lse2;
+  int32_t N, B, QH, splits;
+};
+
 template <int DT, int D, int GROUPS>
-__global__ __launch_bounds__(8 * D) void paged_join_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(8 * D) void paged_join_kernel(JoinArgs a) {
   typedef typename Half16<DT>::T T;
   typedef typename Half16<DT>::V4 V4;
   constexpr int kLanes = D / 4, kRows = 32 / GROUPS;
   __shared__ __align__(16) float o_lds[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kRows : 1][D];
   __shared__ float2 ml_lds[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? kRows : 1];
   const int tid = threadIdx.x, part = tid % kLanes, g = tid / kLanes % GROUPS, r = tid / (kLanes * GROUPS);
-  const int64_t rows = (int64_t)a.c.N * a.QH, row = (int64_t)blockIdx.x * kRows + r;
+  const int64_t rows = (int64_t)a.N * a.QH;
+  int64_t row = (int64_t)blockIdx.x * kRows + r;
+  bool on = row < rows;
+  if (!on) row = rows - 1;
   const int32_t n = (int32_t)((uint32_t)row / (uint32_t)a.QH), head = (int32_t)(row - (int64_t)n * a.QH);
-  // (nobody's rows stay as they are)
-  const bool on = row < rows && (a.c.starts == nullptr || (n >= a.c.starts[0] && n < a.c.starts[a.c.B]));
+  if (a.starts != nullptr) on = on && n >= a.starts[0] && n < a.starts[a.B];  // nobody's rows stay as they are
   float m = -INFINITY, l = 0.f;
   float4v o = {0.f, 0.f, 0.f, 0.f};
-  if (on) {
+  {
     for (int32_t i0 = g; i0 < a.splits; i0 += 8 * GROUPS) {
       float2 ml[8];
       float4v p[8];
@@ -450,8 +527,9 @@ __global__ __launch_bounds__(8 * D) void paged_join_kernel(PagedAttnArgs a) {
 }
 
 template <int DT, int D>
-static void launch_join(const PagedAttnArgs& a, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.c.N * a.QH;
+static void launch_join(const PagedAttnArgs& x, hipStream_t stream) {
+  const JoinArgs a = {x.part_ml, x.part_o, x.c.starts, x.out, x.ost, x.osh, x.lse, x.lse2, x.c.N, x.c.B, x.QH, x.splits};
+  const int64_t rows = (int64_t)a.N * a.QH;
   const dim3 block(8 * D);
   if (a.splits > 8)
     hipLaunchKernelGGL((paged_join_kernel<DT, D, 8>), dim3((uint32_t)ceil_div(rows, 4)), block, 0, stream, a);
@@ -470,8 +548,15 @@ template <int DT, int D>
 static int launch_few(const PagedAttnArgs& a, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.c.B * a.KVH * a.splits;
   JKV_CHECK_ARG(blocks < ((int64_t)1 << 31), "paged attention grid too large");
-  if (a.max_new * a.per <= 16) hipLaunchKernelGGL((paged_few_kernel<DT, D, 1>), dim3((uint32_t)blocks), dim3(64), 0, stream, a);
-  else hipLaunchKernelGGL((paged_few_kernel<DT, D, 2>), dim3((uint32_t)blocks), dim3(64), 0, stream, a);
+  const dim3 grid((uint32_t)blocks);
+  constexpr int W2 = D == 128 ? 4 : 8;
+  if (a.max_new * a.per <= 16) {
+    if (a.waves > 1) hipLaunchKernelGGL((paged_few_kernel<DT, D, 1, 8>), grid, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((paged_few_kernel<DT, D, 1, 1>), grid, dim3(64), 0, stream, a);
+  } else {
+    if (a.waves > 1) hipLaunchKernelGGL((paged_few_kernel<DT, D, 2, W2>), grid, dim3(64 * W2), 0, stream, a);
+    else hipLaunchKernelGGL((paged_few_kernel<DT, D, 2, 1>), grid, dim3(64), 0, stream, a);
+  }
   if (a.splits > 1) {
     const int rc = paged_launch_join(a, DT, D, stream);
     if (rc != JKV_OK) return rc;

@@ -107,9 +107,9 @@ struct PagedAttnArgs {
   int32_t QH, KVH, per;   // per: query heads of a kv head
   int32_t window, sinks;  // at most kPagedMost
   int32_t max_new;
-  // Scores are q k * scale2, base 2: q is multiplied by q_mul (half, so that a
-  // rotated fp16 query cannot overflow; negative for a negative scale, zero for
-  // a zero one) and the product by scale2 > 0.
+  // Base-2 scores are (q * q_mul) k * scale2.  q_mul is the softmax scale times
+  // log2(e); where that passes a half, a power of two of it is left to scale2, so
+  // that a rotated fp16 query (up to sqrt 2 of its size) cannot overflow.
   float q_mul, scale2;
   int32_t items;  // chunks: an upper bound of all sequences' row blocks
   // splits of the entries, joined by paged_join_kernel (one split: none)

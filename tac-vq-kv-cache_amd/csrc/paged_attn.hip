@@ -147,8 +147,12 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   a.weights = weights; a.wsb = weight_stride_b; a.wsh = weight_stride_h; a.accumulate = accumulate;
   a.QH = (int32_t)QH; a.KVH = (int32_t)KVH; a.per = (int32_t)(QH / KVH);
   a.max_new = (int32_t)max_new;
-  a.q_mul = scale == 0.f ? 0.f : scale < 0.f ? -0.5f : 0.5f;
-  a.scale2 = scale == 0.f ? 1.f : fabsf(scale) * 2.f * 1.4426950408889634f;
+  a.q_mul = scale * 1.4426950408889634f;
+  a.scale2 = 1.f;
+  while (fabsf(a.q_mul) > 0.5f) {
+    a.q_mul *= 0.5f;
+    a.scale2 *= 2.f;
+  }
   a.splits = (int32_t)p.splits; a.split_tiles = (int32_t)p.split_tiles;
   a.items = (int32_t)p.items;
   a.waves = (int32_t)p.waves;

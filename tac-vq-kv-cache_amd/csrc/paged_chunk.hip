@@ -3,17 +3,19 @@
 // The matrix products bound it.  The packed (token, query head) rows of a
 // sequence and kv head go 128 to a workgroup of four waves, 32 rows a wave, so
 // any number of heads shares the keys and values of its group.  Tiles of 64
-// entries lie twice in LDS (keys and values 4 x 64 x D x 2 bytes); the next
-// one's loads are issued before this one's products and stored behind them.
+// entries lie twice in LDS (keys and values 4 x 64 x D x 2 bytes), loaded
+// there directly a tile ahead.
 //
 // On v_mfma_f32_32x32x16, S^T[entry][row] = K Q^T gives a lane one row's
 // scores (16 of 32 entries, the other half-wave the rest): a row's maximum and
 // sum take one swap.  O^T[dim][row] += V^T P^T takes P from those registers,
 // 4 entries of each of two groups of 8 a lane, and V^T by transposing reads of
 // the row-major tile in the same order.  Online softmax in 32 bits; p and the
-// rotated q enter the products rounded once to the cache's type, except that
-// with EXACT (weights or log-sum-exps are asked for) q is a sum of two parts.
+// rotated, scaled q enter the products rounded once to the cache's type, except
+// that with EXACT (weights or log-sum-exps are asked for) q is a sum of two parts.
 #include <math.h>
+
+#include <type_traits>
 
 #include "paged.h"
 
@@ -80,15 +82,14 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int32_t item,
 }
 
 template <int DT, int D, bool EXACT>
-__global__ __launch_bounds__(64 * kChunkWaves, EXACT ? 1 : 2) void paged_chunk_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedAttnArgs a) {
   typedef typename Half16<DT>::T T;
   typedef typename Half16<DT>::V8 V8;
   typedef typename Half16<DT>::V4 V4;
   constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D;
   constexpr int kTileBytes = kChunkTile * kRowBytes;
   constexpr int kRowsPerLoad = 1024 / kRowBytes, kWaveRows = kChunkTile / kChunkWaves, kLoads = kWaveRows / kRowsPerLoad;
-  __shared__ __align__(16) uint8_t k_lds[2][kTileBytes];
-  __shared__ __align__(16) uint8_t v_lds[2][kTileBytes];
+  __shared__ __align__(1024) uint8_t lds[4 * kTileBytes];  // two tiles of keys, two of values
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -130,63 +131,75 @@ __global__ __launch_bounds__(64 * kChunkWaves, EXACT ? 1 : 2) void paged_chunk_k
     tile1 = tile0 + each < pt.count ? tile0 + each : pt.count;
   }
 
-  // ---- tile loader: a wave's 16 entries lie in one page.  A page outside the
-  // pool and the entries at or behind the length lie beyond the resource's
-  // bound and load as zeros. ----
+  // ---- tile loader: a wave's 16 entries lie in one page, and go from global
+  // memory into LDS directly.  A page outside the pool and the entries at or
+  // behind the length lie beyond the resource's bound and land as zeros.  (The
+  // loads are asm: for the builtin the compiler holds every LDS read back until
+  // all of them have landed.  They have no result registers, and the waits below
+  // count them.) ----
   const int32_t* table = a.c.tables + b * a.c.table_stride;
   const int32_t mask = (1 << a.c.page_shift) - 1;
-  const int lrow = lane / (64 / kRowsPerLoad), lchunk = lane % (64 / kRowsPerLoad);
-  const uint8_t* k_head = a.c.k + kvh * a.c.head_bytes;
-  const uint8_t* v_head = a.c.v + kvh * a.c.head_bytes;
-  uint4v ks[kLoads], vs[kLoads];
+  const int lrow = lane / (64 / kRowsPerLoad), lslot = lane % (64 / kRowsPerLoad);
+  const uint64_t k_head = (uint64_t)(a.c.k + kvh * a.c.head_bytes), v_head = (uint64_t)(a.c.v + kvh * a.c.head_bytes);
+  const uint32_t lds_base = lds_address(lds);
+  // lane -> row lrow of each load, slot lslot: the chunk that belongs there
+  uint32_t k_off[kLoads], v_off[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const int r = j * kRowsPerLoad + lrow;  // (a wave's first row is a multiple of 16: it does not change the slot)
+    k_off[j] = (uint32_t)r * (uint32_t)a.c.slot_bytes + 16u * (uint32_t)chunk_key_slot<D>(r, lslot);
+    v_off[j] = (uint32_t)r * (uint32_t)a.c.slot_bytes + 16u * (uint32_t)chunk_value_slot<D>(r, lslot);
+  }
   auto entry_of = [&](int32_t i) { return (i < pt.lead ? i : pt.main + i - pt.lead) * kChunkTile; };
-  // lane h holds the page of this wave's entries in tile h of a run of 64
-  int32_t pages = -1, run0 = -64;
-  auto fetch = [&](int32_t i) {
-    if (i - run0 >= 64) {
-      run0 = i;
-      const int32_t e = entry_of(i + lane) + kWaveRows * wave;
-      pages = -1;
-      if (i + lane < tile1 && e < s.length) pages = table[e >> a.c.page_shift];
-      if ((uint32_t)pages >= (uint32_t)a.c.n_pages) pages = -1;
-    }
+  // lane h holds the page of this wave's entries in tile h of a run of 64 (a
+  // tile past the last has none and loads zeros)
+  int32_t pages = -1, run0 = tile0 - 64;
+  auto resource = [&](int32_t i, uint64_t pool) -> uint4v {
     const int32_t e = entry_of(i) + kWaveRows * wave, left = s.length - e;
     const int32_t page = __builtin_amdgcn_readlane(pages, i - run0);
-    const int64_t at = page >= 0 ? page * a.c.page_bytes + (int64_t)(e & mask) * a.c.slot_bytes : 0;
+    const uint64_t at = pool + (page >= 0 ? page * a.c.page_bytes + (int64_t)(e & mask) * a.c.slot_bytes : 0);
     const int32_t bytes = page >= 0 ? ((left < kWaveRows ? left : kWaveRows) - 1) * (int32_t)a.c.slot_bytes + kRowBytes : 0;
-    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(k_head + at), (short)0, bytes, 0x00020000);
-    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(v_head + at), (short)0, bytes, 0x00020000);
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const uint32_t off = (uint32_t)(j * kRowsPerLoad + lrow) * (uint32_t)a.c.slot_bytes + 16u * lchunk;
-      ks[j] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(kr, (int)off, 0, 0));
-      vs[j] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(vr, (int)off, 0, 0));
-    }
+    return uint4v{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, (uint32_t)bytes, 0x00020000u};
   };
+  auto look_up = [&](int32_t i) {
+    if (i - run0 < 64) return;
+    run0 = i;
+    const int32_t e = entry_of(i + lane) + kWaveRows * wave;
+    pages = -1;
+    if (i + lane < tile1 && e < s.length) pages = table[e >> a.c.page_shift];
+    if ((uint32_t)pages >= (uint32_t)a.c.n_pages) pages = -1;
+  };
+  auto load_tile = [&](uint4v rsrc, const uint32_t (&off)[kLoads], uint32_t to) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(to + (uint32_t)(kWaveRows * kRowBytes) * (uint32_t)wave + 1024u * j), "v"(off[j]), "s"(rsrc)
+                   : "memory", "m0");
+  };
+  auto load_keys = [&](int32_t i, int buf) {
+    look_up(i);
+    load_tile(resource(i, k_head), k_off, lds_base + buf * kTileBytes);
+  };
+  auto load_values = [&](int32_t i, int buf) { load_tile(resource(i, v_head), v_off, lds_base + (2 + buf) * kTileBytes); };
+  // every load has landed and every LDS access is done, in all waves
+  auto meet = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
   // every row of the workgroup sees the whole tile, or some entries are masked
   auto block_full = [&](int32_t e0) {
     return e0 + kChunkTile - 1 <= first && (e0 > last - a.window || e0 + kChunkTile <= a.sinks);
   };
-  bool found = false;  // an infinite or NaN value in a masked tile
-  auto stage = [&](int32_t i, int buf) {
-    if (!block_full(entry_of(i))) {
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) vs[j] = finite_halves<DT>(vs[j], &found);
-    }
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int r = kWaveRows * wave + j * kRowsPerLoad + lrow;
-      *(uint4v*)(k_lds[buf] + r * kRowBytes + 16 * chunk_key_slot<D>(r, lchunk)) = ks[j];
-      *(uint4v*)(v_lds[buf] + r * kRowBytes + 16 * chunk_value_slot<D>(r, lchunk)) = vs[j];
-    }
-  };
-  if (tile0 < tile1) fetch(tile0);
+  // a tile that none of the wave's rows sees is left out
+  auto wave_sees = [&](int32_t e0) { return e0 <= wlast && (e0 + kChunkTile - 1 > wfirst - a.window || e0 < a.sinks); };
 
-  // ---- the wave's rotated queries (B operand: 8 dims of row ln) ----
+  const bool any = tile0 < tile1;
+  if (any) {
+    load_keys(tile0, 0);
+    load_values(tile0, 0);
+  }
+
+  // ---- the wave's rotated queries times the scale (B operand: 8 dims of row ln) ----
   V8 qf[kSteps], ql[EXACT ? kSteps : 1];
   {
     const uint8_t* qp = a.q + (int64_t)(s.row0 + row_t) * a.qst + (int64_t)head * a.qsh;
-    const float mul = row_ok ? a.q_mul : 0.f;
 #pragma unroll
     for (int c = 0; c < kSteps / 2; ++c) {
       const int d0 = 16 * c + 8 * lh;
@@ -201,8 +214,8 @@ __global__ __launch_bounds__(64 * kChunkWaves, EXACT ? 1 : 2) void paged_chunk_k
           w = w * cs + u * sn;
           u = t;
         }
-        u = row_ok ? u * mul : 0.f;
-        w = row_ok ? w * mul : 0.f;
+        u = row_ok ? u * a.q_mul : 0.f;
+        w = row_ok ? w * a.q_mul : 0.f;
         qf[c][e] = (T)u;
         qf[c + kSteps / 2][e] = (T)w;
         if constexpr (EXACT) {
@@ -222,105 +235,138 @@ __global__ __launch_bounds__(64 * kChunkWaves, EXACT ? 1 : 2) void paged_chunk_k
       }
     }
   }
-  if (tile0 < tile1) stage(tile0, 0);
-  __syncthreads();
 
-  float m = -INFINITY, l = 0.f;
-  float16v o[kDims];
+  // `shift` is minus the reference maximum plus 10 in all elements: the products
+  // start from it, so that a score leaves them as the exponent of its p.  p is
+  // 2^10 times the weight against the reference, which moves when a maximum
+  // passes it by more than 4 (at first: at once): p stays below 2^14, and fp16
+  // holds weights of 2^-34.  (In units of scale2, a power of two that only
+  // large scales need.)
+  float16v shift = {}, o[kDims];
+  float l = 0.f, limit = -INFINITY;
 #pragma unroll
-  for (int d = 0; d < kDims; ++d) o[d] = float16v{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-
+  for (int d = 0; d < kDims; ++d) o[d] = float16v{};
+  // LDS addresses: a few per lane, the rest are offsets known at compile time
+  uint32_t k_at[kSteps], v_at[kDims];
+#pragma unroll
+  for (int c = 0; c < kSteps; ++c) k_at[c] = lds_base + (uint32_t)(ln * kRowBytes + 16 * chunk_key_slot<D>(ln, 2 * c + lh));
   const int tr_row = 4 * lh + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  auto value_operand = [&](uint32_t base, int d, int st) -> V8 {
-    const int r = 16 * st + tr_row;
-    const uint32_t at = base + (uint32_t)(r * kRowBytes + 16 * chunk_value_slot<D>(r, 4 * d + tr_chunk) + 8 * (lane & 1));
-    const uint32_t at8 = base + (uint32_t)((r + 8) * kRowBytes + 16 * chunk_value_slot<D>(r + 8, 4 * d + tr_chunk) + 8 * (lane & 1));
-    const V4 lo = lds_read_tr<V4>(at), hi = lds_read_tr<V4>(at8);
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+    v_at[d] = lds_base + (uint32_t)(2 * kTileBytes + tr_row * kRowBytes + 16 * chunk_value_slot<D>(tr_row, 4 * d + tr_chunk) + 8 * (lane & 1));
+  auto value_operand = [&](int d, int st, int buf) -> V8 {
+    const uint32_t at = v_at[d] + (uint32_t)(buf * kTileBytes + 16 * st * kRowBytes);
+    const V4 lo = lds_read_tr<V4>(at), hi = lds_read_tr<V4>(at + 8 * kRowBytes);
     return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-  for (int32_t i = tile0; i < tile1; ++i) {
-    const int buf = (i - tile0) & 1;
-    const int32_t e0 = entry_of(i);
-    const bool more = i + 1 < tile1;
-    if (more) fetch(i + 1);
-    // a tile none of the wave's rows sees is left out
-    const bool on = e0 <= wlast && (e0 + kChunkTile - 1 > wfirst - a.window || e0 < a.sinks);
-    if (on) {
-      const uint8_t* kl = k_lds[buf];
-      const uint8_t* vl = v_lds[buf];
-      float16v sc[2];
+  typedef __attribute__((address_space(3))) const V8 lds_v8;
+  auto scores = [&](int buf, float16v (&sc)[2]) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        sc[kb] = float16v{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int kb = 0; kb < 2; ++kb) {
+      sc[kb] = shift;
 #pragma unroll
-        for (int c = 0; c < kSteps; ++c) {
-          const int r = 32 * kb + ln;
-          const V8 ka = *(const V8*)(kl + r * kRowBytes + 16 * chunk_key_slot<D>(r, 2 * c + lh));
-          sc[kb] = mfma32<DT>(ka, qf[c], sc[kb]);
-          if constexpr (EXACT) sc[kb] = mfma32<DT>(ka, ql[c], sc[kb]);
-        }
+      for (int c = 0; c < kSteps; ++c) {
+        const V8 ka = *(lds_v8*)(size_t)(k_at[c] + (uint32_t)(buf * kTileBytes + 32 * kb * kRowBytes));
+        sc[kb] = mfma32<DT>(ka, qf[c], sc[kb]);
+        if constexpr (EXACT) sc[kb] = mfma32<DT>(ka, ql[c], sc[kb]);
       }
-      const bool full = e0 + kChunkTile - 1 <= wfirst && (e0 > wlast - a.window || e0 + kChunkTile <= a.sinks);
-      if (!full) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int32_t j = e0 + 32 * kb + 8 * (e >> 2) + 4 * lh + (e & 3);
-            const bool seen = j <= self && (j > self - a.window || j < a.sinks);
-            sc[kb][e] = seen ? sc[kb][e] : -INFINITY;
-          }
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, sc[kb][e]), sc[kb][e + 1]);
-      mx = lanes2_max(mx) * a.scale2;
-      // the reference moves only when the maximum passes it by more than 4; p is
-      // 2^10 times its weight against it, at most 2^14: fp16 holds weights of 2^-34
-      const float mn = mx > m + 4.f ? mx : m, mu = mn == -INFINITY ? 0.f : mn - 10.f;
-      if (__any(mn != m)) {
-        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) o[d] *= alpha;
-        l *= alpha;
-      }
-      m = mn;
-      V8 pf[4];
-      float t4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(sc[kb][e], a.scale2, -mu));
-          t4[e & 3] += p;
-          pf[2 * kb + (e >> 3)][e & 7] = (T)p;
-        }
-      l += (t4[0] + t4[1]) + (t4[2] + t4[3]);
-      const uint32_t v_base = lds_address(vl);
-#pragma unroll
-      for (int d = 0; d < kDims; ++d)
-#pragma unroll
-        for (int st = 0; st < 4; ++st) o[d] = mfma32<DT>(value_operand(v_base, d, st), pf[st], o[d]);
     }
-    if (more) stage(i + 1, buf ^ 1);
-    __syncthreads();
+  };
+  auto hide = [&](int32_t e0, float16v (&sc)[2]) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int32_t j = e0 + 32 * kb + 8 * (e >> 2) + 4 * lh + (e & 3);
+        const bool seen = j <= self && (j > self - a.window || j < a.sinks);
+        sc[kb][e] = seen ? sc[kb][e] : -INFINITY;
+      }
+  };
+  auto largest = [&](const float16v (&sc)[2]) -> float {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, sc[kb][e]), sc[kb][e + 1]);
+    return lanes2_max(mx);
+  };
+  auto move_reference = [&](float mx, float16v (&sc)[2]) {
+    const bool need = mx > limit;
+    if (!__any(need)) return;
+    const float d = need ? mx - 10.f : 0.f, by = d / a.scale2;
+    const float alpha = limit == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(-d);
+    limit = need ? 14.f : limit;
+    shift -= by;
+    l *= alpha;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) sc[kb] -= d;
+#pragma unroll
+    for (int x = 0; x < kDims; ++x) o[x] *= alpha;
+  };
+  // p of a tile's scores, and O^T += V^T P^T
+  auto weigh = [&](const float16v (&sc)[2], V8 (&pf)[4]) {
+    float t4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float p = __builtin_amdgcn_exp2f(sc[kb][e]);
+        t4[e & 3] += p;
+        pf[2 * kb + (e >> 3)][e & 7] = (T)p;
+      }
+    l += (t4[0] + t4[1]) + (t4[2] + t4[3]);
+  };
+  auto sum_values = [&](int buf, const V8 (&pf)[4]) {
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int st = 0; st < 4; ++st) o[d] = mfma32<DT>(value_operand(d, st, buf), pf[st], o[d]);
+  };
+  auto wave_full = [&](int32_t e0) {
+    return e0 + kChunkTile - 1 <= wfirst && (e0 > wlast - a.window || e0 + kChunkTile <= a.sinks);
+  };
+  const bool unit = a.scale2 == 1.f;
+
+  bool found = false;  // an infinite or NaN value in a masked tile
+  auto clean = [&](int buf) {
+    for (int at = 16 * tid; at < kTileBytes; at += 16 * 64 * kChunkWaves) {
+      uint4v* w = (uint4v*)(lds + (2 + buf) * kTileBytes + at);
+      *w = finite_halves<DT>(*w, &found);
+    }
+    meet();
+  };
+  auto step = [&](int32_t i, auto parity) {
+    constexpr int buf = decltype(parity)::value;
+    const int32_t e0 = entry_of(i);
+    meet();
+    if (!block_full(e0)) clean(buf);
+    load_keys(i + 1, buf ^ 1);
+    load_values(i + 1, buf ^ 1);
+    if (!wave_sees(e0)) return;
+    float16v sc[2];
+    scores(buf, sc);
+    if (!unit)
+      for (int kb = 0; kb < 2; ++kb) sc[kb] *= a.scale2;
+    if (!wave_full(e0)) hide(e0, sc);
+    move_reference(largest(sc), sc);
+    V8 pf[4];
+    weigh(sc, pf);
+    sum_values(buf, pf);
+  };
+  for (int32_t i = tile0; i < tile1; i += 2) {
+    step(i, std::integral_constant<int, 0>());
+    if (i + 1 < tile1) step(i + 1, std::integral_constant<int, 1>());
   }
 
   if (__syncthreads_or(found)) {
     for (int32_t i = tile0; i < tile1; ++i) {
       const int32_t e0 = entry_of(i);
       if (block_full(e0)) continue;
-      run0 = -0x40000000;  // the tile's page anew
-      fetch(i);
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const int r = kWaveRows * wave + j * kRowsPerLoad + lrow;
-        *(uint4v*)(v_lds[0] + r * kRowBytes + 16 * chunk_value_slot<D>(r, lchunk)) = vs[j];
-      }
-      __syncthreads();
+      run0 = i - 64;  // the tile's page anew
+      meet();
+      look_up(i);
+      load_values(i, 0);
+      meet();
       V8 seen[4];
 #pragma unroll
       for (int st = 0; st < 4; ++st)
@@ -335,7 +381,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, EXACT ? 1 : 2) void paged_chunk_k
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
           V8 vu, vd;
-          non_finite_marks<DT>(value_operand(lds_address(v_lds[0]), d, st), &vu, &vd);
+          non_finite_marks<DT>(value_operand(d, st, 0), &vu, &vd);
           up = mfma32<DT>(vu, seen[st], up);
           down = mfma32<DT>(vd, seen[st], down);
         }
@@ -344,6 +390,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, EXACT ? 1 : 2) void paged_chunk_k
       }
     }
   }
+  meet();  // (loads ahead of the last tile land before the LDS is given back)
 
   // ---- out, or this split's part of it: lane holds dims 32d + 8(e/4) + 4lh + e%4 of row ln ----
   const float lt = lanes2_sum(l);
@@ -351,7 +398,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, EXACT ? 1 : 2) void paged_chunk_k
   const int64_t n = s.row0 + row_t, row = n * a.QH + head;
   if (a.splits > 1) {
     const int64_t at = (int64_t)split * a.c.N * a.QH + row;
-    if (lh == 0) a.part_ml[at] = float2{m == -INFINITY ? m : m - 10.f, lt};
+    if (lh == 0) a.part_ml[at] = float2{limit == -INFINITY ? -INFINITY : -shift[0] * a.scale2, lt};
     if (tile0 < tile1)
 #pragma unroll
       for (int d = 0; d < kDims; ++d)
@@ -363,7 +410,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, EXACT ? 1 : 2) void paged_chunk_k
   }
   const bool none = lt == 0.f;  // sees nothing
   if (lh == 0) {
-    const float l2 = none ? -INFINITY : (m == -INFINITY ? 0.f : m - 10.f) + log2f(lt);
+    const float l2 = none ? -INFINITY : log2f(lt) - shift[0] * a.scale2;
     if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
     if (a.lse2 != nullptr) a.lse2[row] = l2;
   }

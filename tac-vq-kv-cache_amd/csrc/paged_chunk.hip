@@ -21,6 +21,8 @@
 
 namespace jkv {
 
+#define JKV_SG(what, n) __builtin_amdgcn_sched_group_barrier(what, n, 0)
+
 static const int kChunkTile = 64;
 static const int kChunkWaves = kChunkRows / 32;
 
@@ -200,29 +202,30 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   V8 qf[kSteps], ql[EXACT ? kSteps : 1];
   {
     const uint8_t* qp = a.q + (int64_t)(s.row0 + row_t) * a.qst + (int64_t)head * a.qsh;
+    V8 x[kSteps];
 #pragma unroll
-    for (int c = 0; c < kSteps / 2; ++c) {
-      const int d0 = 16 * c + 8 * lh;
-      const V8 x0 = *(const V8*)(qp + 2 * d0), x1 = *(const V8*)(qp + 2 * d0 + D);
+    for (int c = 0; c < kSteps; ++c) x[c] = *(const V8*)(qp + 32 * c + 16 * lh);
+    auto put = [&](int c, int e, float v) {
+      v = row_ok ? v * a.q_mul : 0.f;
+      qf[c][e] = (T)v;
+      if constexpr (EXACT) ql[c][e] = (T)(v - (float)(T)v);
+    };
+    if (a.rope.on) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float u = (float)x0[e], w = (float)x1[e];
-        if (a.rope.on) {
+      for (int c = 0; c < kSteps / 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
           float cs, sn;
-          rope_trig(a.rope.turns[d0 + e], s.pos0 + row_t, &cs, &sn);
-          const float t = u * cs - w * sn;
-          w = w * cs + u * sn;
-          u = t;
+          rope_trig(a.rope.turns[16 * c + 8 * lh + e], s.pos0 + row_t, &cs, &sn);
+          const float u = (float)x[c][e], w = (float)x[c + kSteps / 2][e];
+          put(c, e, u * cs - w * sn);
+          put(c + kSteps / 2, e, w * cs + u * sn);
         }
-        u = row_ok ? u * a.q_mul : 0.f;
-        w = row_ok ? w * a.q_mul : 0.f;
-        qf[c][e] = (T)u;
-        qf[c + kSteps / 2][e] = (T)w;
-        if constexpr (EXACT) {
-          ql[c][e] = (T)(u - (float)(T)u);
-          ql[c + kSteps / 2][e] = (T)(w - (float)(T)w);
-        }
-      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) put(c, e, (float)x[c][e]);
     }
   }
   if constexpr (EXACT) {
@@ -303,24 +306,16 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
 #pragma unroll
     for (int x = 0; x < kDims; ++x) o[x] *= alpha;
   };
-  // p of a tile's scores, and O^T += V^T P^T
-  auto weigh = [&](const float16v (&sc)[2], V8 (&pf)[4]) {
+  // p of 32 of a tile's scores
+  auto weigh = [&](const float16v& sc, V8* pf) {
     float t4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p = __builtin_amdgcn_exp2f(sc[kb][e]);
-        t4[e & 3] += p;
-        pf[2 * kb + (e >> 3)][e & 7] = (T)p;
-      }
+    for (int e = 0; e < 16; ++e) {
+      const float p = __builtin_amdgcn_exp2f(sc[e]);
+      t4[e & 3] += p;
+      pf[e >> 3][e & 7] = (T)p;
+    }
     l += (t4[0] + t4[1]) + (t4[2] + t4[3]);
-  };
-  auto sum_values = [&](int buf, const V8 (&pf)[4]) {
-#pragma unroll
-    for (int d = 0; d < kDims; ++d)
-#pragma unroll
-      for (int st = 0; st < 4; ++st) o[d] = mfma32<DT>(value_operand(d, st, buf), pf[st], o[d]);
   };
   auto wave_full = [&](int32_t e0) {
     return e0 + kChunkTile - 1 <= wfirst && (e0 > wlast - a.window || e0 + kChunkTile <= a.sinks);
@@ -345,13 +340,35 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     if (!wave_sees(e0)) return;
     float16v sc[2];
     scores(buf, sc);
-    if (!unit)
+    JKV_SG(0x100, kSteps);
+    for (int x = 0; x < kSteps; ++x) { JKV_SG(0x8, EXACT ? 2 : 1); JKV_SG(0x100, 1); }
+    JKV_SG(0x8, EXACT ? 2 * kSteps : kSteps);
+    if (!unit || !wave_full(e0)) {
       for (int kb = 0; kb < 2; ++kb) sc[kb] *= a.scale2;
-    if (!wave_full(e0)) hide(e0, sc);
-    move_reference(largest(sc), sc);
+      hide(e0, sc);
+    }
+    V8 va[2][kDims];
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) va[st][d] = value_operand(d, st, buf);
+    const float mx = largest(sc);
+    move_reference(mx, sc);
     V8 pf[4];
-    weigh(sc, pf);
-    sum_values(buf, pf);
+    weigh(sc[0], pf);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) o[d] = mfma32<DT>(va[st][d], pf[st], o[d]);
+    weigh(sc[1], pf + 2);
+#pragma unroll
+    for (int st = 2; st < 4; ++st)
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) o[d] = mfma32<DT>(value_operand(d, st, buf), pf[st], o[d]);
+    // the second half's exponentials beside the first half's products
+    for (int x = 0; x < 2 * kDims; ++x) { JKV_SG(0x8, 1); JKV_SG(0x100, 2); JKV_SG(0x2, 40 / (2 * kDims)); }
+    JKV_SG(0x8, 2 * kDims);
   };
   for (int32_t i = tile0; i < tile1; i += 2) {
     step(i, std::integral_constant<int, 0>());

@@ -91,18 +91,16 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D;
   constexpr int kTileBytes = kChunkTile * kRowBytes;
   constexpr int kRowsPerLoad = 1024 / kRowBytes, kWaveRows = kChunkTile / kChunkWaves, kLoads = kWaveRows / kRowsPerLoad;
-  __shared__ __align__(1024) uint8_t lds[4 * kTileBytes];  // two tiles of keys, two of values
+  __shared__ __align__(1024) uint8_t lds[4 * kTileBytes];  // twice a tile of keys, one of values
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 31, lh = lane >> 5;
-  // an XCD takes neighbouring items of one kv head: their tiles meet in its L2
-  uint32_t bid = xcd_remap(blockIdx.x, gridDim.x);
-  const uint32_t slice = (uint32_t)a.items * (uint32_t)a.splits;
-  const int32_t kvh = (int32_t)(bid / slice);
-  if (kvh >= a.KVH) return;
-  bid -= (uint32_t)kvh * slice;
-  const int32_t item = (int32_t)(bid / (uint32_t)a.splits), split = (int32_t)(bid - (uint32_t)item * (uint32_t)a.splits);
+  // kv heads run fastest: with eight of them (or a multiple) each XCD has its
+  // own, and a sequence's tiles meet in one L2; items spread evenly in any case
+  const uint32_t bid = blockIdx.x, at_item = bid / (uint32_t)a.KVH;
+  const int32_t kvh = (int32_t)(bid - at_item * (uint32_t)a.KVH);
+  const int32_t item = (int32_t)(at_item / (uint32_t)a.splits), split = (int32_t)(at_item - (uint32_t)item * (uint32_t)a.splits);
   int32_t b, block;
   if (!paged_item(a, item, &b, &block)) return;
   b = __builtin_amdgcn_readfirstlane(b);
@@ -138,7 +136,8 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   // behind the length lie beyond the resource's bound and land as zeros.  (The
   // loads are asm: for the builtin the compiler holds every LDS read back until
   // all of them have landed.  They have no result registers, and the waits below
-  // count them.) ----
+  // count them.  M0, their place in LDS, is set beside each: nothing else here
+  // uses it.) ----
   const int32_t* table = a.c.tables + b * a.c.table_stride;
   const int32_t mask = (1 << a.c.page_shift) - 1;
   const int lrow = lane / (64 / kRowsPerLoad), lslot = lane % (64 / kRowsPerLoad);
@@ -153,50 +152,56 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     v_off[j] = (uint32_t)r * (uint32_t)a.c.slot_bytes + 16u * (uint32_t)chunk_value_slot<D>(r, lslot);
   }
   auto entry_of = [&](int32_t i) { return (i < pt.lead ? i : pt.main + i - pt.lead) * kChunkTile; };
-  // lane h holds the page of this wave's entries in tile h of a run of 64 (a
-  // tile past the last has none and loads zeros)
-  int32_t pages = -1, run0 = tile0 - 64;
-  auto resource = [&](int32_t i, uint64_t pool) -> uint4v {
-    const int32_t e = entry_of(i) + kWaveRows * wave, left = s.length - e;
-    const int32_t page = __builtin_amdgcn_readlane(pages, i - run0);
-    const uint64_t at = pool + (page >= 0 ? page * a.c.page_bytes + (int64_t)(e & mask) * a.c.slot_bytes : 0);
-    const int32_t bytes = page >= 0 ? ((left < kWaveRows ? left : kWaveRows) - 1) * (int32_t)a.c.slot_bytes + kRowBytes : 0;
-    return uint4v{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, (uint32_t)bytes, 0x00020000u};
-  };
+  // What a tile needs is found 64 tiles at a time, a lane each, and read from
+  // there: the place of this wave's 16 entries in the pools, the bytes that may
+  // be read there (none past the last tile), and
+  enum { kBlockFull = 1 << 28, kWaveFull = 2 << 28, kWaveSees = 4 << 28, kBytes = kBlockFull - 1 };
+  // all rows of the workgroup, or of the wave, see the whole tile; some row of
+  // the wave sees some of it.
+  uint32_t at_lo = 0, at_hi = 0;
+  int32_t what = 0, run0 = tile0 - 64;  // bytes (below 2^27: host-checked strides) and flags
   auto look_up = [&](int32_t i) {
     if (i - run0 < 64) return;
     run0 = i;
-    const int32_t e = entry_of(i + lane) + kWaveRows * wave;
-    pages = -1;
-    if (i + lane < tile1 && e < s.length) pages = table[e >> a.c.page_shift];
-    if ((uint32_t)pages >= (uint32_t)a.c.n_pages) pages = -1;
+    const int32_t e0 = entry_of(i + lane), e = e0 + kWaveRows * wave, left = s.length - e;
+    int32_t page = -1;
+    if (i + lane < tile1 && left > 0) page = table[e >> a.c.page_shift];
+    const bool ok = (uint32_t)page < (uint32_t)a.c.n_pages;
+    const uint64_t at = ok ? page * a.c.page_bytes + (int64_t)(e & mask) * a.c.slot_bytes : 0;
+    at_lo = (uint32_t)at;
+    at_hi = (uint32_t)(at >> 32);
+    what = ok ? ((left < kWaveRows ? left : kWaveRows) - 1) * (int32_t)a.c.slot_bytes + kRowBytes : 0;
+    const bool sunk = e0 + kChunkTile <= a.sinks;
+    what |= (e0 + kChunkTile - 1 <= first && (e0 > last - a.window || sunk) ? kBlockFull : 0) |
+             (e0 + kChunkTile - 1 <= wfirst && (e0 > wlast - a.window || sunk) ? kWaveFull : 0) |
+             (e0 <= wlast && (e0 + kChunkTile - 1 > wfirst - a.window || e0 < a.sinks) ? kWaveSees : 0);
+    asm volatile("" : "+v"(at_lo));  // waited for here, not at every tile's use
+  };
+  auto resource = [&](int32_t i, uint64_t pool) -> uint4v {
+    const uint32_t lo = __builtin_amdgcn_readlane(at_lo, i - run0), hi = __builtin_amdgcn_readlane(at_hi, i - run0);
+    const uint64_t at = pool + (((uint64_t)hi << 32) | lo);
+    return uint4v{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, (uint32_t)__builtin_amdgcn_readlane(what, i - run0) & kBytes, 0x00020000u};
   };
   auto load_tile = [&](uint4v rsrc, const uint32_t (&off)[kLoads], uint32_t to) {
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                    :: "s"(to + (uint32_t)(kWaveRows * kRowBytes) * (uint32_t)wave + 1024u * j), "v"(off[j]), "s"(rsrc)
-                   : "memory", "m0");
+                   : "memory");
   };
-  auto load_keys = [&](int32_t i, int buf) {
+  auto load_values = [&](int32_t i, int stage) {
+    load_tile(resource(i, v_head), v_off, lds_base + (2 * stage + 1) * kTileBytes);
+  };
+  auto load_stage = [&](int32_t i, int stage) {
     look_up(i);
-    load_tile(resource(i, k_head), k_off, lds_base + buf * kTileBytes);
+    load_tile(resource(i, k_head), k_off, lds_base + 2 * stage * kTileBytes);
+    load_values(i, stage);
   };
-  auto load_values = [&](int32_t i, int buf) { load_tile(resource(i, v_head), v_off, lds_base + (2 + buf) * kTileBytes); };
   // every load has landed and every LDS access is done, in all waves
   auto meet = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-  // every row of the workgroup sees the whole tile, or some entries are masked
-  auto block_full = [&](int32_t e0) {
-    return e0 + kChunkTile - 1 <= first && (e0 > last - a.window || e0 + kChunkTile <= a.sinks);
-  };
-  // a tile that none of the wave's rows sees is left out
-  auto wave_sees = [&](int32_t e0) { return e0 <= wlast && (e0 + kChunkTile - 1 > wfirst - a.window || e0 < a.sinks); };
 
   const bool any = tile0 < tile1;
-  if (any) {
-    load_keys(tile0, 0);
-    load_values(tile0, 0);
-  }
+  if (any) load_stage(tile0, 0);
 
   // ---- the wave's rotated queries times the scale (B operand: 8 dims of row ln) ----
   V8 qf[kSteps], ql[EXACT ? kSteps : 1];
@@ -256,9 +261,9 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   const int tr_row = 4 * lh + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
-    v_at[d] = lds_base + (uint32_t)(2 * kTileBytes + tr_row * kRowBytes + 16 * chunk_value_slot<D>(tr_row, 4 * d + tr_chunk) + 8 * (lane & 1));
+    v_at[d] = lds_base + (uint32_t)(kTileBytes + tr_row * kRowBytes + 16 * chunk_value_slot<D>(tr_row, 4 * d + tr_chunk) + 8 * (lane & 1));
   auto value_operand = [&](int d, int st, int buf) -> V8 {
-    const uint32_t at = v_at[d] + (uint32_t)(buf * kTileBytes + 16 * st * kRowBytes);
+    const uint32_t at = v_at[d] + (uint32_t)(2 * buf * kTileBytes + 16 * st * kRowBytes);
     const V4 lo = lds_read_tr<V4>(at), hi = lds_read_tr<V4>(at + 8 * kRowBytes);
     return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
@@ -269,7 +274,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
       sc[kb] = shift;
 #pragma unroll
       for (int c = 0; c < kSteps; ++c) {
-        const V8 ka = *(lds_v8*)(size_t)(k_at[c] + (uint32_t)(buf * kTileBytes + 32 * kb * kRowBytes));
+        const V8 ka = *(lds_v8*)(size_t)(k_at[c] + (uint32_t)(2 * buf * kTileBytes + 32 * kb * kRowBytes));
         sc[kb] = mfma32<DT>(ka, qf[c], sc[kb]);
         if constexpr (EXACT) sc[kb] = mfma32<DT>(ka, ql[c], sc[kb]);
       }
@@ -317,35 +322,31 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     }
     l += (t4[0] + t4[1]) + (t4[2] + t4[3]);
   };
-  auto wave_full = [&](int32_t e0) {
-    return e0 + kChunkTile - 1 <= wfirst && (e0 > wlast - a.window || e0 + kChunkTile <= a.sinks);
-  };
   const bool unit = a.scale2 == 1.f;
 
   bool found = false;  // an infinite or NaN value in a masked tile
   auto clean = [&](int buf) {
     for (int at = 16 * tid; at < kTileBytes; at += 16 * 64 * kChunkWaves) {
-      uint4v* w = (uint4v*)(lds + (2 + buf) * kTileBytes + at);
+      uint4v* w = (uint4v*)(lds + (2 * buf + 1) * kTileBytes + at);
       *w = finite_halves<DT>(*w, &found);
     }
-    meet();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
   auto step = [&](int32_t i, auto parity) {
     constexpr int buf = decltype(parity)::value;
-    const int32_t e0 = entry_of(i);
+    const int32_t is = __builtin_amdgcn_readlane(what, i - run0);
     meet();
-    if (!block_full(e0)) clean(buf);
-    load_keys(i + 1, buf ^ 1);
-    load_values(i + 1, buf ^ 1);
-    if (!wave_sees(e0)) return;
+    load_stage(i + 1, buf ^ 1);
+    if (!(is & kBlockFull)) clean(buf);
+    if (!(is & kWaveSees)) return;
     float16v sc[2];
     scores(buf, sc);
     JKV_SG(0x100, kSteps);
     for (int x = 0; x < kSteps; ++x) { JKV_SG(0x8, EXACT ? 2 : 1); JKV_SG(0x100, 1); }
     JKV_SG(0x8, EXACT ? 2 * kSteps : kSteps);
-    if (!unit || !wave_full(e0)) {
+    if (!unit || !(is & kWaveFull)) {
       for (int kb = 0; kb < 2; ++kb) sc[kb] *= a.scale2;
-      hide(e0, sc);
+      hide(entry_of(i), sc);
     }
     V8 va[2][kDims];
 #pragma unroll
@@ -378,10 +379,10 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   if (__syncthreads_or(found)) {
     for (int32_t i = tile0; i < tile1; ++i) {
       const int32_t e0 = entry_of(i);
-      if (block_full(e0)) continue;
-      run0 = i - 64;  // the tile's page anew
-      meet();
+      run0 = i - 64;  // the tile's place anew
       look_up(i);
+      if (__builtin_amdgcn_readlane(what, 0) & kBlockFull) continue;
+      meet();
       load_values(i, 0);
       meet();
       V8 seen[4];
@@ -445,30 +446,32 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
 }
 
 // The weights of chunks.  A wave holds 32 entries' keys in registers, walks the
-// rows that may see them in tiles of 32 (their rotated queries in two parts
-// through LDS, shared by the workgroup's waves) and adds exp2(score - lse) up:
-// S^T[entry][row] leaves 16 entries of one row with a lane, the sum over the
-// rows' lanes comes last.  Every sum has one order.
-static const int kWeightEntries = 128;  // a workgroup's: four waves of 32
+// rows that may see them (their rotated queries in two parts) and adds
+// exp2(score - lse) up: S^T[entry][row] leaves 16 entries of one row with a
+// lane, the sum over the rows' lanes comes last.  A workgroup of eight waves
+// takes 128 entries and 64 rows a stage, half of the waves each half of the
+// rows; three stages are on their way into LDS behind the one worked on (with
+// one, loads took 1.5 us a tile where the products take 0.25).  Every sum has
+// one order.
+static const int kWeightEntries = 128, kWeightRows = 64, kWeightStages = 4;
 
 template <int DT, int D>
-__global__ __launch_bounds__(256, 2) void paged_chunk_weights_kernel(PagedAttnArgs a, int32_t blocks) {
+__global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnArgs a, int32_t blocks) {
   typedef typename Half16<DT>::V8 V8;
-  constexpr int kSteps = D / 16, kRowBytes = 4 * D, kChunks = kRowBytes / 16;
-  constexpr int kLoads = 32 * kRowBytes / (256 * 16);
-  __shared__ __align__(16) uint8_t q_lds[2][32 * kRowBytes];
+  constexpr int kSteps = D / 16, kRowBytes = 4 * D, kChunks = kRowBytes / 16, kRowsPerLoad = 1024 / kRowBytes;
+  constexpr int kLoads = kWeightRows / kRowsPerLoad / 8, kStageBytes = kWeightRows * kRowBytes;
+  __shared__ __align__(1024) uint8_t q_lds[kWeightStages * kStageBytes];
+  __shared__ __align__(16) float norm_lds[kWeightStages][8][64];  // each wave its own
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, lh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  uint32_t bid = xcd_remap(blockIdx.x, gridDim.x);
-  const int32_t blk = (int32_t)(bid % (uint32_t)blocks);
-  bid /= (uint32_t)blocks;
-  const int32_t b = (int32_t)(bid / (uint32_t)a.KVH), kvh = (int32_t)(bid % (uint32_t)a.KVH);
-  if (b >= a.c.B) return;
+  const uint32_t at_block = blockIdx.x / (uint32_t)a.KVH;  // (kv heads fastest, as above)
+  const int32_t kvh = (int32_t)(blockIdx.x - at_block * (uint32_t)a.KVH);
+  const int32_t b = (int32_t)(at_block / (uint32_t)blocks), blk = (int32_t)(at_block - (uint32_t)b * (uint32_t)blocks);
   const PagedSeq s = paged_seq(a.c, b);
   const int32_t j0 = blk * kWeightEntries;
   if (j0 >= s.length) return;
   const int32_t tokens = s.tokens < a.max_new ? s.tokens : a.max_new, before = s.length - s.tokens;
-  const int32_t wj0 = j0 + 32 * wave;
+  const int32_t wj0 = j0 + 32 * (wave & 3);
 
   // the wave's keys (A operand: 8 dims of entry ln)
   V8 kf[kSteps];
@@ -484,6 +487,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_weights_kernel(PagedAttnAr
       kf[c] = V8{};
       if (ok) kf[c] = *(const V8*)(kp + 32 * c);
     }
+#pragma unroll
+    for (int c = 0; c < kSteps; ++c) asm volatile("" : "+v"(kf[c]));  // waited for here, not beside the loads below
   }
 
   // the rows that may see one of the workgroup's entries
@@ -499,72 +504,90 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_weights_kernel(PagedAttnAr
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = 0.f;
 
-  uint4v qs[kLoads];
-  auto fetch = [&](int32_t r) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int at = i * 256 + tid;
-      int32_t row = r + at / kChunks;
-      if (row >= r1) row = r1 - 1;
+  const uint32_t lds_base = lds_address(q_lds);
+  // rows at or behind r1 load the last one's; they take no part
+  auto load_stage = [&](int32_t r, int stage) {
+    if (r > r1 - 1) r = r1 - 1;
+    const int32_t tf = __builtin_amdgcn_readfirstlane((int32_t)((uint32_t)r / per));
+    const int64_t row_f = (int64_t)(s.row0 + tf) * a.QH + kvh * a.per;
+    const uint64_t at = (uint64_t)a.q_parts + (uint64_t)row_f * kRowBytes, norm_at = (uint64_t)(a.lse2 + row_f);
+    const uint4v rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
+    const uint4v norm_rsrc = {(uint32_t)norm_at, (uint32_t)(norm_at >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
+    auto row_at = [&](int32_t row) -> uint32_t {  // rows from row_f on
+      if (row > r1 - 1) row = r1 - 1;
       const int32_t t = (int32_t)((uint32_t)row / per);
-      qs[i] = *(const uint4v*)(a.q_parts + (int64_t)((s.row0 + t) * a.QH + kvh * a.per + (row - t * a.per)) * kRowBytes +
-                               16 * (at % kChunks));
-    }
-  };
-  auto stage = [&](int buf) {
+      return (uint32_t)((t - tf) * a.QH + (row - t * a.per));
+    };
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int at = i * 256 + tid, r = at / kChunks;
-      *(uint4v*)(q_lds[buf] + r * kRowBytes + 16 * ((at % kChunks) ^ (r & 15))) = qs[i];
+    for (int j = 0; j < kLoads; ++j) {
+      const int x = wave * kLoads + j, rr = x * kRowsPerLoad + lane / kChunks;
+      const uint32_t off = row_at(r + rr) * kRowBytes + 16u * (uint32_t)((lane % kChunks) ^ (rr & 15));
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(lds_base + (uint32_t)(stage * kStageBytes + 1024 * x)), "v"(off), "s"(rsrc) : "memory");
     }
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :: "s"(lds_address(norm_lds[stage][wave])), "v"(4u * row_at(r + lane)), "s"(norm_rsrc) : "memory");
   };
+  typedef __attribute__((address_space(3))) const V8 lds_v8;
+  uint32_t q_at[kSteps];
+#pragma unroll
+  for (int c = 0; c < kSteps; ++c)
+    q_at[c] = lds_base + (uint32_t)((32 * (wave >> 2) + ln) * kRowBytes + 16 * ((2 * c + lh) ^ (ln & 15)));
+
   if (r0 < r1) {
-    fetch(r0);
-    stage(0);
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int32_t r = r0; r < r1; r += 32, buf ^= 1) {
-    const bool more = r + 32 < r1;
-    if (more) fetch(r + 32);
-    const int32_t row = r + ln;
-    const bool row_ok = row < r1;
-    const int32_t t = row_ok ? (int32_t)((uint32_t)row / per) : 0, self = row_ok ? before + t : -1;
-    float norm = INFINITY;
-    if (row_ok) norm = a.lse2[(int64_t)(s.row0 + t) * a.QH + kvh * a.per + (row - t * a.per)];
-    if (norm == -INFINITY) norm = INFINITY;  // it saw nothing
-    const uint8_t* ql = q_lds[buf];
-    float16v sc = {};
 #pragma unroll
-    for (int c = 0; c < kSteps; ++c) {
-      const V8 hi = *(const V8*)(ql + ln * kRowBytes + 16 * ((2 * c + lh) ^ (ln & 15)));
-      const V8 lo = *(const V8*)(ql + ln * kRowBytes + 16 * ((kChunks / 2 + 2 * c + lh) ^ (ln & 15)));
-      sc = mfma32<DT>(kf[c], hi, sc);
-      sc = mfma32<DT>(kf[c], lo, sc);
-    }
-    const int32_t tf = before + (int32_t)((uint32_t)r / per);
-    const int32_t tl = before + (int32_t)((uint32_t)(r + 31 < r1 ? r + 31 : r1 - 1) / per);
-    const bool full = r + 32 <= r1 && wj0 + 31 <= tf && (wj0 > tl - a.window || wj0 + 32 <= a.sinks);
-    if (!full) {
+    for (int st = 0; st < kWeightStages - 1; ++st) load_stage(r0 + kWeightRows * st, st);
+    int stage = 0;
+    for (int32_t rs = r0; rs < r1; rs += kWeightRows, stage = (stage + 1) % kWeightStages) {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((kWeightStages - 2) * (kLoads + 1)) : "memory");
+      load_stage(rs + kWeightRows * (kWeightStages - 1), (stage + kWeightStages - 1) % kWeightStages);
+      const int32_t r = rs + 32 * (wave >> 2);
+      if (r >= r1) continue;
+      const int32_t row = r + ln;
+      const bool row_ok = row < r1;
+      float norm = norm_lds[stage][wave][32 * (wave >> 2) + ln];
+      if (!row_ok || norm == -INFINITY) norm = INFINITY;  // (it saw nothing)
+      float16v sc = {};
+      V8 part[2 * kSteps];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int32_t j = wj0 + 8 * (e >> 2) + 4 * lh + (e & 3);
-        const bool seen = j <= self && (j > self - a.window || j < a.sinks);
-        sc[e] = seen ? sc[e] : -INFINITY;
+      for (int c = 0; c < kSteps; ++c) {
+        part[c] = *(lds_v8*)(size_t)(q_at[c] + (uint32_t)(stage * kStageBytes));
+        part[kSteps + c] = *(lds_v8*)(size_t)((q_at[c] + (uint32_t)(stage * kStageBytes)) ^ (uint32_t)(2 * D));
       }
-    }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] += __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -norm));
-    if (more) stage(buf ^ 1);
-    __syncthreads();
+      for (int c = 0; c < 2 * kSteps; ++c) sc = mfma32<DT>(kf[c % kSteps], part[c], sc);
+      const int32_t tf = before + (int32_t)((uint32_t)r / per);
+      const int32_t tl = before + (int32_t)((uint32_t)(r + 31 < r1 ? r + 31 : r1 - 1) / per);
+      const bool full = wj0 + 31 <= tf && (wj0 > tl - a.window || wj0 + 32 <= a.sinks);
+      if (!full) {
+        const int32_t self = row_ok ? before + (int32_t)((uint32_t)row / per) : -1;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int32_t j = wj0 + 8 * (e >> 2) + 4 * lh + (e & 3);
+          const bool seen = j <= self && (j > self - a.window || j < a.sinks);
+          sc[e] = seen ? sc[e] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] += __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -norm));
+    }
   }
+  // the last loads land before their room is used for the halves' sums
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  float* sums = (float*)q_lds;  // [4][32]: the second half's
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    float v = acc[e];
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    const int32_t j = wj0 + 8 * (e >> 2) + 4 * lh + (e & 3);
+    for (int off = 16; off >= 1; off >>= 1) acc[e] += __shfl_xor(acc[e], off, 64);
+    if (wave >= 4 && ln == e) sums[32 * (wave & 3) + 8 * (e >> 2) + 4 * lh + (e & 3)] = acc[e];
+  }
+  __syncthreads();
+  if (wave >= 4) return;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int32_t at = 8 * (e >> 2) + 4 * lh + (e & 3), j = wj0 + at;
     if (ln == e && j < s.length) {
+      const float v = acc[e] + sums[32 * wave + at];
       float* w = a.weights + b * a.wsb + kvh * a.wsh + j;
       *w = a.accumulate ? *w + v : v;
     }
@@ -573,19 +596,20 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_weights_kernel(PagedAttnAr
 
 template <int DT, int D>
 static int launch_chunk(const PagedAttnArgs& a, hipStream_t stream) {
-  const int64_t blocks = ceil_div((int64_t)a.items * a.KVH * a.splits, 8) * 8;
+  const int64_t blocks = (int64_t)a.items * a.KVH * a.splits;
   JKV_CHECK_ARG(blocks < ((int64_t)1 << 31), "paged attention grid too large");
   const dim3 grid((uint32_t)blocks), block(64 * kChunkWaves);
-  if (a.lse != nullptr || a.lse2 != nullptr) hipLaunchKernelGGL((paged_chunk_kernel<DT, D, true>), grid, block, 0, stream, a);
+  const bool exact = a.lse != nullptr || a.lse2 != nullptr;
+  if (exact) hipLaunchKernelGGL((paged_chunk_kernel<DT, D, true>), grid, block, 0, stream, a);
   else hipLaunchKernelGGL((paged_chunk_kernel<DT, D, false>), grid, block, 0, stream, a);
   if (a.splits > 1) {
     const int rc = paged_launch_join(a, DT, D, stream);
     if (rc != JKV_OK) return rc;
   }
   if (a.weights != nullptr && a.c.top > 0) {
-    const int64_t each = ceil_div(a.c.top, kWeightEntries), all = ceil_div(each * a.c.B * a.KVH, 8) * 8;
+    const int64_t each = ceil_div(a.c.top, kWeightEntries), all = each * a.c.B * a.KVH;
     JKV_CHECK_ARG(all < ((int64_t)1 << 31), "paged weights grid too large");
-    hipLaunchKernelGGL((paged_chunk_weights_kernel<DT, D>), dim3((uint32_t)all), dim3(256), 0, stream, a, (int32_t)each);
+    hipLaunchKernelGGL((paged_chunk_weights_kernel<DT, D>), dim3((uint32_t)all), dim3(512), 0, stream, a, (int32_t)each);
   }
   JKV_CHECK_LAUNCH();
   return JKV_OK;

@@ -112,16 +112,24 @@ struct PagedAttnArgs {
   // that a rotated fp16 query (up to sqrt 2 of its size) cannot overflow.
   float q_mul, scale2;
   int32_t items;  // chunks: an upper bound of all sequences' row blocks
+  int32_t fold;   // chunks: the item from which the order runs backwards
   // splits of the entries, joined by paged_join_kernel (one split: none)
   int32_t splits, split_tiles;
   int32_t waves;  // few rows: 1, or more waves a workgroup that join in LDS
   float2* part_ml;  // [splits][N*QH] reference maximum (base 2) and sum
   float* part_o;    // [splits][N*QH][D]
-  float* lse2;      // [N,QH] base-2 log-sum-exp for the weights, or null
+  float* lse2;      // [KVH][N][per] base-2 log-sum-exps for the weights, or null
   float* scores;    // few rows with weights: [B,KVH,max_new*per,score_width] base-2 scores, or null
   int64_t score_width;
-  uint8_t* q_parts;  // chunks with weights: [N,QH] rotated queries, D of their leading and D of their trailing parts
+  uint8_t* q_parts;  // chunks with weights: [KVH][N][per] rotated queries, D of their leading and D of their trailing parts
 };
+
+// where lse2 holds row n * QH + head
+__device__ __forceinline__ int64_t paged_lse2_at(int32_t N, int32_t per, int64_t row, int32_t QH) {
+  const int32_t n = (int32_t)((uint32_t)row / (uint32_t)QH), head = (int32_t)(row - (int64_t)n * QH);
+  const int32_t kvh = (int32_t)((uint32_t)head / (uint32_t)per);
+  return ((int64_t)kvh * N + n) * per + (head - kvh * per);
+}
 
 static const int32_t kPagedMost = 0x3fffffff;  // entries of a sequence: sums of two of them stay in 32 bits
 

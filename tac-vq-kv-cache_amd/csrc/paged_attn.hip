@@ -76,7 +76,15 @@ static PagedPlan paged_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64
     const int64_t bound = ceil_div(window + std::min<int64_t>(max_new, kChunkRows / per + 1), 64) + 1 + ceil_div(sinks, 64);
     if (bound < tiles) tiles = bound;
     if (tiles < 1) tiles = 1;
-    p.splits = std::max<int64_t>(1, std::min<int64_t>(512 / (p.items * KVH), tiles / 8));
+    // Splits save (1 - 1/s) of a block's tiles, about 1 us each at 128 dims, and
+    // cost a join of 6 us and its parts' way through memory, N QH D 8 bytes each
+    // at 4 TB/s: the best s is the root of the two's ratio.  us with two splits
+    // and without, 32/8 heads: 1 x 1,000 tokens 44 and 36; with four and
+    // without, 1 x 512 over 4,096 entries 59 and 75.
+    const double save = (double)tiles * (D == 128 ? 1.0 : 0.6), part = (double)(N * QH) * (double)D * 8.0 / 4.0e6;
+    const int64_t most = std::min<int64_t>(512 / (p.items * KVH), tiles / 4);
+    const int64_t best = std::min<int64_t>(most, (int64_t)(sqrt(save / part) + 0.5));
+    p.splits = best > 1 && save * (1.0 - 1.0 / (double)best) > 6.0 + part * (double)best ? best : 1;
     if (p.splits > 1) {
       p.ml_at = take(p.splits * N * QH * 8);
       p.o_at = take(p.splits * N * QH * D * 4);
@@ -155,6 +163,8 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   }
   a.splits = (int32_t)p.splits; a.split_tiles = (int32_t)p.split_tiles;
   a.items = (int32_t)p.items;
+  const bool resident = p.splits == 1 && p.items * KVH > 256 && p.items * KVH <= 512;
+  a.fold = resident ? (int32_t)(256 / KVH) : 0x7fffffff;
   a.waves = (int32_t)p.waves;
   a.part_ml = (float2*)(ws + p.ml_at);
   a.part_o = (float*)(ws + p.o_at);

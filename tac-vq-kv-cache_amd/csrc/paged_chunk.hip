@@ -52,28 +52,36 @@ template <int D> __device__ __forceinline__ int chunk_value_slot(int r, int j) {
 }
 
 // The sequence and row block of an item: items are the row blocks of all
-// sequences in turn, a sequence's last one first (it sees most).
-__device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int32_t item, int32_t* b, int32_t* block) {
+// sequences in turn, a sequence's last one first (it sees most).  From item
+// `fold` on the order runs backwards, so that where all workgroups are resident
+// at once, two a CU, one that sees much shares a CU with one that sees little.
+__device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int32_t item, int32_t fold, int32_t* b, int32_t* block) {
   const int lane = threadIdx.x & 63;
-  int32_t before = 0;
-  for (int32_t b0 = 0; b0 < a.c.B; b0 += 64) {
-    int32_t n = 0;
+  auto blocks_upto = [&](int32_t b0) -> int32_t {  // of sequences b0 to b0 + lane
+    int32_t upto = 0;
     if (b0 + lane < a.c.B) {
       int32_t row0, tokens;
       paged_rows(a.c, b0 + lane, &row0, &tokens);
       if (tokens > a.max_new) tokens = a.max_new;
-      n = (tokens * a.per + kChunkRows - 1) / kChunkRows;
+      upto = (tokens * a.per + kChunkRows - 1) / kChunkRows;
     }
-    int32_t upto = n;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const int32_t up = __shfl_up(upto, off, 64);
       if (lane >= off) upto += up;
     }
-    const int32_t all = __builtin_amdgcn_readlane(upto, 63);
+    return upto;
+  };
+  if (item >= fold) {
+    int32_t total = 0;
+    for (int32_t b0 = 0; b0 < a.c.B; b0 += 64) total += __builtin_amdgcn_readlane(blocks_upto(b0), 63);
+    if (item < total) item = fold + (total - 1 - item);
+  }
+  int32_t before = 0;
+  for (int32_t b0 = 0; b0 < a.c.B; b0 += 64) {
+    const int32_t upto = blocks_upto(b0), all = __builtin_amdgcn_readlane(upto, 63);
     if (item < before + all) {
-      const uint64_t hit = __ballot(item < before + upto);
-      const int at = __builtin_ctzll(hit);
+      const int at = __builtin_ctzll(__ballot(item < before + upto));
       *b = b0 + at;
       *block = before + __builtin_amdgcn_readlane(upto, at) - 1 - item;
       return true;
@@ -102,7 +110,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   const int32_t kvh = (int32_t)(bid - at_item * (uint32_t)a.KVH);
   const int32_t item = (int32_t)(at_item / (uint32_t)a.splits), split = (int32_t)(at_item - (uint32_t)item * (uint32_t)a.splits);
   int32_t b, block;
-  if (!paged_item(a, item, &b, &block)) return;
+  if (!paged_item(a, item, a.fold, &b, &block)) return;
   b = __builtin_amdgcn_readfirstlane(b);
   block = __builtin_amdgcn_readfirstlane(block);
   const PagedSeq s = paged_seq(a.c, b);
@@ -235,7 +243,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   }
   if constexpr (EXACT) {
     if (a.q_parts != nullptr && split == 0 && row_ok) {
-      uint8_t* to = a.q_parts + ((int64_t)(s.row0 + row_t) * a.QH + head) * (4 * D) + 16 * lh;
+      uint8_t* to = a.q_parts + (((int64_t)kvh * a.c.N + s.row0) * a.per + wr0 + ln) * (4 * D) + 16 * lh;
 #pragma unroll
       for (int c = 0; c < kSteps; ++c) {
         *(V8*)(to + 32 * c) = qf[c];
@@ -430,7 +438,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   if (lh == 0) {
     const float l2 = none ? -INFINITY : log2f(lt) - shift[0] * a.scale2;
     if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
-    if (a.lse2 != nullptr) a.lse2[row] = l2;
+    if (a.lse2 != nullptr) a.lse2[((int64_t)kvh * a.c.N + s.row0) * a.per + wr0 + ln] = l2;
   }
   const float inv = 1.0f / lt;
   uint8_t* op = a.out + n * a.ost + (int64_t)head * a.osh;
@@ -449,16 +457,17 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
 // rows that may see them (their rotated queries in two parts) and adds
 // exp2(score - lse) up: S^T[entry][row] leaves 16 entries of one row with a
 // lane, the sum over the rows' lanes comes last.  A workgroup of eight waves
-// takes 128 entries and 64 rows a stage, half of the waves each half of the
-// rows; three stages are on their way into LDS behind the one worked on (with
-// one, loads took 1.5 us a tile where the products take 0.25).  Every sum has
-// one order.
-static const int kWeightEntries = 128, kWeightRows = 64, kWeightStages = 4;
+// takes 64 entries and 128 rows a stage (two waves' entries, four waves' rows),
+// the next stage on its way into LDS.  A kv head's rows of a
+// sequence lie one behind another, so a stage is one stretch of memory.  Every
+// sum has one order.
+static const int kWeightEntries = 64, kWeightRows = 128;
 
 template <int DT, int D>
 __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnArgs a, int32_t blocks) {
   typedef typename Half16<DT>::V8 V8;
   constexpr int kSteps = D / 16, kRowBytes = 4 * D, kChunks = kRowBytes / 16, kRowsPerLoad = 1024 / kRowBytes;
+  constexpr int kWeightStages = 2;
   constexpr int kLoads = kWeightRows / kRowsPerLoad / 8, kStageBytes = kWeightRows * kRowBytes;
   __shared__ __align__(1024) uint8_t q_lds[kWeightStages * kStageBytes];
   __shared__ __align__(16) float norm_lds[kWeightStages][8][64];  // each wave its own
@@ -471,7 +480,7 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
   const int32_t j0 = blk * kWeightEntries;
   if (j0 >= s.length) return;
   const int32_t tokens = s.tokens < a.max_new ? s.tokens : a.max_new, before = s.length - s.tokens;
-  const int32_t wj0 = j0 + 32 * (wave & 3);
+  const int32_t wj0 = j0 + 32 * (wave & 1);
 
   // the wave's keys (A operand: 8 dims of entry ln)
   V8 kf[kSteps];
@@ -499,40 +508,39 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
     if (end < t1) t1 = end;
   }
   const uint32_t per = (uint32_t)a.per;
-  const int32_t r0 = t0 * a.per, r1 = t1 * a.per;  // (rows fit 31 bits: host-checked)
+  // (rows fit 31 bits: host-checked)
+  const int32_t r0 = __builtin_amdgcn_readfirstlane(t0 * a.per), r1 = __builtin_amdgcn_readfirstlane(t1 * a.per);
   float acc[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = 0.f;
 
   const uint32_t lds_base = lds_address(q_lds);
-  // rows at or behind r1 load the last one's; they take no part
-  auto load_stage = [&](int32_t r, int stage) {
-    if (r > r1 - 1) r = r1 - 1;
-    const int32_t tf = __builtin_amdgcn_readfirstlane((int32_t)((uint32_t)r / per));
-    const int64_t row_f = (int64_t)(s.row0 + tf) * a.QH + kvh * a.per;
-    const uint64_t at = (uint64_t)a.q_parts + (uint64_t)row_f * kRowBytes, norm_at = (uint64_t)(a.lse2 + row_f);
-    const uint4v rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
-    const uint4v norm_rsrc = {(uint32_t)norm_at, (uint32_t)(norm_at >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
-    auto row_at = [&](int32_t row) -> uint32_t {  // rows from row_f on
-      if (row > r1 - 1) row = r1 - 1;
-      const int32_t t = (int32_t)((uint32_t)row / per);
-      return (uint32_t)((t - tf) * a.QH + (row - t * a.per));
-    };
+  // (rows at or behind r1 land as zeros and take no part)
+  const int64_t row_base = ((int64_t)kvh * a.c.N + __builtin_amdgcn_readfirstlane(s.row0)) * a.per;
+  uint32_t off[kLoads];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int x = wave * kLoads + j, rr = x * kRowsPerLoad + lane / kChunks;
-      const uint32_t off = row_at(r + rr) * kRowBytes + 16u * (uint32_t)((lane % kChunks) ^ (rr & 15));
+  for (int j = 0; j < kLoads; ++j) {
+    const int rr = (wave * kLoads + j) * kRowsPerLoad + lane / kChunks;
+    off[j] = (uint32_t)(rr * kRowBytes + 16 * ((lane % kChunks) ^ (rr & 15)));
+  }
+  auto load_stage = [&](int32_t r, int stage) {
+    const int32_t some = r1 - r < 0 ? 0 : (r1 - r < 2 * kWeightRows ? r1 - r : 2 * kWeightRows);
+    const int32_t left = __builtin_amdgcn_readfirstlane(some);  // (the compiler takes the minimum in a vector register)
+    const uint64_t at = (uint64_t)a.q_parts + (uint64_t)(row_base + r) * kRowBytes, norm_at = (uint64_t)(a.lse2 + row_base + r);
+    const uint4v rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, (uint32_t)(left * kRowBytes), 0x00020000u};
+    const uint4v norm_rsrc = {(uint32_t)norm_at, (uint32_t)(norm_at >> 32) & 0xffffu, 4u * (uint32_t)left, 0x00020000u};
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(lds_base + (uint32_t)(stage * kStageBytes + 1024 * x)), "v"(off), "s"(rsrc) : "memory");
-    }
+                   :: "s"(lds_base + (uint32_t)(stage * kStageBytes + 1024 * (wave * kLoads + j))), "v"(off[j]), "s"(rsrc) : "memory");
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                 :: "s"(lds_address(norm_lds[stage][wave])), "v"(4u * row_at(r + lane)), "s"(norm_rsrc) : "memory");
+                 :: "s"(lds_address(norm_lds[stage][wave])), "v"(4u * (uint32_t)(32 * (wave >> 1) + lane)), "s"(norm_rsrc) : "memory");
   };
   typedef __attribute__((address_space(3))) const V8 lds_v8;
   uint32_t q_at[kSteps];
 #pragma unroll
   for (int c = 0; c < kSteps; ++c)
-    q_at[c] = lds_base + (uint32_t)((32 * (wave >> 2) + ln) * kRowBytes + 16 * ((2 * c + lh) ^ (ln & 15)));
+    q_at[c] = lds_base + (uint32_t)((32 * (wave >> 1) + ln) * kRowBytes + 16 * ((2 * c + lh) ^ (ln & 15)));
 
   if (r0 < r1) {
 #pragma unroll
@@ -541,11 +549,11 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
     for (int32_t rs = r0; rs < r1; rs += kWeightRows, stage = (stage + 1) % kWeightStages) {
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((kWeightStages - 2) * (kLoads + 1)) : "memory");
       load_stage(rs + kWeightRows * (kWeightStages - 1), (stage + kWeightStages - 1) % kWeightStages);
-      const int32_t r = rs + 32 * (wave >> 2);
+      const int32_t r = rs + 32 * (wave >> 1);
       if (r >= r1) continue;
       const int32_t row = r + ln;
       const bool row_ok = row < r1;
-      float norm = norm_lds[stage][wave][32 * (wave >> 2) + ln];
+      float norm = norm_lds[stage][wave][ln];
       if (!row_ok || norm == -INFINITY) norm = INFINITY;  // (it saw nothing)
       float16v sc = {};
       V8 part[2 * kSteps];
@@ -572,25 +580,21 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
       for (int e = 0; e < 16; ++e) acc[e] += __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -norm));
     }
   }
-  // the last loads land before their room is used for the halves' sums
+  // the last loads land before their room is used for the row groups' sums
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  float* sums = (float*)q_lds;  // [4][32]: the second half's
+  float* sums = (float*)q_lds;  // [4 row groups][64]
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) acc[e] += __shfl_xor(acc[e], off, 64);
-    if (wave >= 4 && ln == e) sums[32 * (wave & 3) + 8 * (e >> 2) + 4 * lh + (e & 3)] = acc[e];
+    for (int off2 = 16; off2 >= 1; off2 >>= 1) acc[e] += __shfl_xor(acc[e], off2, 64);
+    if (ln == e) sums[64 * (wave >> 1) + 32 * (wave & 1) + 8 * (e >> 2) + 4 * lh + (e & 3)] = acc[e];
   }
   __syncthreads();
-  if (wave >= 4) return;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int32_t at = 8 * (e >> 2) + 4 * lh + (e & 3), j = wj0 + at;
-    if (ln == e && j < s.length) {
-      const float v = acc[e] + sums[32 * wave + at];
-      float* w = a.weights + b * a.wsb + kvh * a.wsh + j;
-      *w = a.accumulate ? *w + v : v;
-    }
+  const int32_t j = j0 + tid;
+  if (tid < kWeightEntries && j < s.length) {
+    const float v = (sums[tid] + sums[64 + tid]) + (sums[128 + tid] + sums[192 + tid]);
+    float* w = a.weights + b * a.wsb + kvh * a.wsh + j;
+    *w = a.accumulate ? *w + v : v;
   }
 }
 

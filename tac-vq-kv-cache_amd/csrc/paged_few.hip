@@ -368,7 +368,7 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
       if (part == 0) {
         const float l2 = none ? -INFINITY : (top == -INFINITY ? 0.f : top) + log2f(lt);
         if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
-        if (a.lse2 != nullptr) a.lse2[row] = l2;
+        if (a.lse2 != nullptr) a.lse2[paged_lse2_at(a.c.N, a.per, row, a.QH)] = l2;
       }
       V4 h;
 #pragma unroll
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
     if (lg == 0) {
       const float l2 = none ? -INFINITY : (m[g] == -INFINITY ? 0.f : m[g] - 10.f) + log2f(lt);
       if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
-      if (a.lse2 != nullptr) a.lse2[row] = l2;
+      if (a.lse2 != nullptr) a.lse2[paged_lse2_at(a.c.N, a.per, row, a.QH)] = l2;
     }
     const float inv = 1.0f / lt;
     uint8_t* op = a.out + (int64_t)(s.row0 + row_t[g]) * a.ost + (row - (int64_t)(s.row0 + row_t[g]) * a.QH) * a.osh;
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256) void paged_few_weights_kernel(PagedAttnArgs a)
   for (int32_t t = 0; t < tokens; ++t) {
     const int32_t self = first + t;
     if (!(j <= self && (j > self - a.window || j < a.sinks))) continue;
-    const float* norm = a.lse2 + (int64_t)(s.row0 + t) * a.QH + kvh * a.per;
+    const float* norm = a.lse2 + ((int64_t)kvh * a.c.N + s.row0 + t) * a.per;
     for (int32_t g = 0; g < a.per; ++g)
       sum += __builtin_amdgcn_exp2f(sc[(int64_t)(t * a.per + g) * a.score_width] - norm[g]);
   }
@@ -442,7 +442,7 @@ struct JoinArgs {
   uint8_t* out;
   int64_t ost, osh;
   float *lse, *lse2;
-  int32_t N, B, QH, splits;
+  int32_t N, B, QH, per, splits;
 };
 
 template <int DT, int D, int GROUPS>
@@ -518,7 +518,7 @@ __global__ __launch_bounds__(8 * D) void paged_join_kernel(JoinArgs a) {
   if (part == 0) {
     const float l2 = none ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
     if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
-    if (a.lse2 != nullptr) a.lse2[row] = l2;
+    if (a.lse2 != nullptr) a.lse2[paged_lse2_at(a.N, a.per, row, a.QH)] = l2;
   }
   V4 h;
 #pragma unroll
@@ -528,7 +528,7 @@ __global__ __launch_bounds__(8 * D) void paged_join_kernel(JoinArgs a) {
 
 template <int DT, int D>
 static void launch_join(const PagedAttnArgs& x, hipStream_t stream) {
-  const JoinArgs a = {x.part_ml, x.part_o, x.c.starts, x.out, x.ost, x.osh, x.lse, x.lse2, x.c.N, x.c.B, x.QH, x.splits};
+  const JoinArgs a = {x.part_ml, x.part_o, x.c.starts, x.out, x.ost, x.osh, x.lse, x.lse2, x.c.N, x.c.B, x.QH, x.per, x.splits};
   const int64_t rows = (int64_t)a.N * a.QH;
   const dim3 block(8 * D);
   if (a.splits > 8)

@@ -104,14 +104,16 @@ __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(SelectArgs
           const int32_t i = round * kRound + 1024 * k + tid;
           const bool in = i >= first && i < last && (pass == 0 || (u[k] >> (shift + bits)) == prefix);
           const uint32_t digit = (u[k] >> shift) & ((1u << bits) - 1u);
-          // lanes that share the first one's digit count once (many weights are
-          // equal, or close); the others one by one
+          // equal weights meet in one digit: a wave that shares one counts once (64
+          // adds to one word took 16,384 equal weights from 16 to 51 us)
           const uint64_t on = __ballot(in);
           if (on == 0) continue;
           const uint32_t lead = __builtin_amdgcn_readlane(digit, __builtin_ctzll(on));
-          const uint64_t same = __ballot(in && digit == lead);
-          if (in && digit != lead) atomicAdd(&hist[digit], 1u);
-          if (lane == __builtin_ctzll(on)) atomicAdd(&hist[lead], (uint32_t)__builtin_popcountll(same));
+          if (__ballot(in && digit == lead) == on) {
+            if (lane == __builtin_ctzll(on)) atomicAdd(&hist[lead], (uint32_t)__builtin_popcountll(on));
+          } else if (in) {
+            atomicAdd(&hist[digit], 1u);
+          }
         }
       }
       __syncthreads();

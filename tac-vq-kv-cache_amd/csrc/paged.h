@@ -112,6 +112,7 @@ struct PagedAttnArgs {
   // that a rotated fp16 query (up to sqrt 2 of its size) cannot overflow.
   float q_mul, scale2;
   int32_t items;  // chunks: an upper bound of all sequences' row blocks
+  int32_t item_rows;  // chunks: packed (token, head) rows of a block, 128 or 256
   int32_t fold;   // chunks: the item from which the order runs backwards
   // splits of the entries, joined by paged_join_kernel (one split: none)
   int32_t splits, split_tiles;
@@ -137,7 +138,6 @@ static const int32_t kPagedMost = 0x3fffffff;  // entries of a sequence: sums of
 int paged_launch_few(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
 int paged_launch_chunk(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
 int paged_launch_join(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
-static const int kChunkRows = 128;  // packed (token, head) rows of a chunk kernel's workgroup
 
 // The tiles of `size` entries that rows at entries first..last may see: `lead`
 // tiles from entry 0 on that hold sinks, then those from tile `main` on.

@@ -19,7 +19,7 @@ namespace jkv {
 // How a call's work is divided and what of the workspace it takes.
 struct PagedPlan {
   bool few;  // at most 32 rows a sequence and kv head
-  int64_t items, waves, splits, split_tiles, score_width;
+  int64_t items, item_rows, waves, splits, split_tiles, score_width;
   int64_t ml_at, o_at, lse2_at, scores_at, q_at, bytes;
 };
 
@@ -71,9 +71,19 @@ static PagedPlan paged_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64
       p.scores_at = take(B * KVH * max_new * per * p.score_width * 4);
     }
   } else {
-    p.items = std::min<int64_t>(B * ceil_div(max_new * per, kChunkRows), N * per / kChunkRows + B);
+    // Eight-wave blocks of 256 rows where one a CU goes round: their tiles serve
+    // twice the rows.  Where most of what is seen is the chunk itself, blocks
+    // differ in length, and it takes two a CU to even them out.  us with four and
+    // with eight waves, 32/8 heads of 128: 2 x 2,048 tokens over 16,384 entries
+    // 917 and 852, 2 x 1,024 over 4,096 135 and 129; prompts of 1 x 2,000 57 and
+    // 63, 16 x 2,048 the same; at 64 dims, where three workgroups share a CU, 4 x
+    // 1,024 over 4,096 150 and 168.
+    auto blocks_of = [&](int64_t rows) { return std::min<int64_t>(B * ceil_div(max_new * per, rows), N * per / rows + B); };
+    const int64_t rounds = blocks_of(256) * KVH / 256;
+    p.item_rows = D == 128 && rounds >= (max_length >= 2 * max_new ? 1 : 2) ? 256 : 128;
+    p.items = blocks_of(p.item_rows);
     int64_t tiles = ceil_div(max_length, 64);
-    const int64_t bound = ceil_div(window + std::min<int64_t>(max_new, kChunkRows / per + 1), 64) + 1 + ceil_div(sinks, 64);
+    const int64_t bound = ceil_div(window + std::min<int64_t>(max_new, p.item_rows / per + 1), 64) + 1 + ceil_div(sinks, 64);
     if (bound < tiles) tiles = bound;
     if (tiles < 1) tiles = 1;
     // Splits save (1 - 1/s) of a block's tiles, about 1 us each at 128 dims, and
@@ -163,7 +173,8 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   }
   a.splits = (int32_t)p.splits; a.split_tiles = (int32_t)p.split_tiles;
   a.items = (int32_t)p.items;
-  const bool resident = p.splits == 1 && p.items * KVH > 256 && p.items * KVH <= 512;
+  a.item_rows = (int32_t)p.item_rows;
+  const bool resident = p.item_rows == 128 && p.splits == 1 && p.items * KVH > 256 && p.items * KVH <= 512;
   a.fold = resident ? (int32_t)(256 / KVH) : 0x7fffffff;
   a.waves = (int32_t)p.waves;
   a.part_ml = (float2*)(ws + p.ml_at);

@@ -1,8 +1,8 @@
 // Attention of chunks of new tokens over a paged K/V cache.
 //
 // The matrix products bound it.  The packed (token, query head) rows of a
-// sequence and kv head go 128 to a workgroup of four waves, 32 rows a wave, so
-// any number of heads shares the keys and values of its group.  Tiles of 64
+// sequence and kv head go 128 or 256 to a workgroup, 32 rows a wave, so any
+// number of heads shares the keys and values of its group.  Tiles of 64
 // entries lie twice in LDS (keys and values 4 x 64 x D x 2 bytes), loaded
 // there directly a tile ahead.
 //
@@ -24,7 +24,6 @@ namespace jkv {
 #define JKV_SG(what, n) __builtin_amdgcn_sched_group_barrier(what, n, 0)
 
 static const int kChunkTile = 64;
-static const int kChunkWaves = kChunkRows / 32;
 
 template <int DT>
 __device__ __forceinline__ float16v mfma32(typename Half16<DT>::V8 a, typename Half16<DT>::V8 b, float16v c) {
@@ -63,7 +62,7 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int32_t item,
       int32_t row0, tokens;
       paged_rows(a.c, b0 + lane, &row0, &tokens);
       if (tokens > a.max_new) tokens = a.max_new;
-      upto = (tokens * a.per + kChunkRows - 1) / kChunkRows;
+      upto = (tokens * a.per + a.item_rows - 1) / a.item_rows;
     }
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -91,12 +90,12 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int32_t item,
   return false;
 }
 
-template <int DT, int D, bool EXACT>
+template <int DT, int D, bool EXACT, int kChunkWaves>
 __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedAttnArgs a) {
   typedef typename Half16<DT>::T T;
   typedef typename Half16<DT>::V8 V8;
   typedef typename Half16<DT>::V4 V4;
-  constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D;
+  constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D, kChunkRows = 32 * kChunkWaves;
   constexpr int kTileBytes = kChunkTile * kRowBytes;
   constexpr int kRowsPerLoad = 1024 / kRowBytes, kWaveRows = kChunkTile / kChunkWaves, kLoads = kWaveRows / kRowsPerLoad;
   __shared__ __align__(1024) uint8_t lds[4 * kTileBytes];  // twice a tile of keys, one of values
@@ -139,7 +138,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     tile1 = tile0 + each < pt.count ? tile0 + each : pt.count;
   }
 
-  // ---- tile loader: a wave's 16 entries lie in one page, and go from global
+  // ---- tile loader: a wave's 8 or 16 entries lie in one page, and go from global
   // memory into LDS directly.  A page outside the pool and the entries at or
   // behind the length lie beyond the resource's bound and land as zeros.  (The
   // loads are asm: for the builtin the compiler holds every LDS read back until
@@ -155,13 +154,13 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   uint32_t k_off[kLoads], v_off[kLoads];
 #pragma unroll
   for (int j = 0; j < kLoads; ++j) {
-    const int r = j * kRowsPerLoad + lrow;  // (a wave's first row is a multiple of 16: it does not change the slot)
-    k_off[j] = (uint32_t)r * (uint32_t)a.c.slot_bytes + 16u * (uint32_t)chunk_key_slot<D>(r, lslot);
-    v_off[j] = (uint32_t)r * (uint32_t)a.c.slot_bytes + 16u * (uint32_t)chunk_value_slot<D>(r, lslot);
+    const int r = j * kRowsPerLoad + lrow, tile_r = kWaveRows * wave + r;
+    k_off[j] = (uint32_t)r * (uint32_t)a.c.slot_bytes + 16u * (uint32_t)chunk_key_slot<D>(tile_r, lslot);
+    v_off[j] = (uint32_t)r * (uint32_t)a.c.slot_bytes + 16u * (uint32_t)chunk_value_slot<D>(tile_r, lslot);
   }
   auto entry_of = [&](int32_t i) { return (i < pt.lead ? i : pt.main + i - pt.lead) * kChunkTile; };
   // What a tile needs is found 64 tiles at a time, a lane each, and read from
-  // there: the place of this wave's 16 entries in the pools, the bytes that may
+  // there: the place of this wave's entries in the pools, the bytes that may
   // be read there (none past the last tile), and
   enum { kBlockFull = 1 << 28, kWaveFull = 2 << 28, kWaveSees = 4 << 28, kBytes = kBlockFull - 1 };
   // all rows of the workgroup, or of the wave, see the whole tile; some row of
@@ -602,10 +601,18 @@ template <int DT, int D>
 static int launch_chunk(const PagedAttnArgs& a, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.items * a.KVH * a.splits;
   JKV_CHECK_ARG(blocks < ((int64_t)1 << 31), "paged attention grid too large");
-  const dim3 grid((uint32_t)blocks), block(64 * kChunkWaves);
+  const dim3 grid((uint32_t)blocks), block((uint32_t)(2 * a.item_rows));
   const bool exact = a.lse != nullptr || a.lse2 != nullptr;
-  if (exact) hipLaunchKernelGGL((paged_chunk_kernel<DT, D, true>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((paged_chunk_kernel<DT, D, false>), grid, block, 0, stream, a);
+  if constexpr (D == 128) {
+    if (a.item_rows == 256) {
+      if (exact) hipLaunchKernelGGL((paged_chunk_kernel<DT, D, true, 8>), grid, block, 0, stream, a);
+      else hipLaunchKernelGGL((paged_chunk_kernel<DT, D, false, 8>), grid, block, 0, stream, a);
+    }
+  }
+  if (a.item_rows == 128) {
+    if (exact) hipLaunchKernelGGL((paged_chunk_kernel<DT, D, true, 4>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((paged_chunk_kernel<DT, D, false, 4>), grid, block, 0, stream, a);
+  }
   if (a.splits > 1) {
     const int rc = paged_launch_join(a, DT, D, stream);
     if (rc != JKV_OK) return rc;

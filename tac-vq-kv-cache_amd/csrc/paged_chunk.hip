@@ -455,18 +455,18 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
 // The weights of chunks.  A wave holds 32 entries' keys in registers, walks the
 // rows that may see them (their rotated queries in two parts) and adds
 // exp2(score - lse) up: S^T[entry][row] leaves 16 entries of one row with a
-// lane, the sum over the rows' lanes comes last.  A workgroup of eight waves
-// takes 64 entries and 128 rows a stage (two waves' entries, four waves' rows),
-// the next stage on its way into LDS.  A kv head's rows of a
-// sequence lie one behind another, so a stage is one stretch of memory.  Every
-// sum has one order.
-static const int kWeightEntries = 64, kWeightRows = 128;
-
-template <int DT, int D>
+// lane, the sum over the rows' lanes comes last.  Eight waves a workgroup are
+// ENTRIES times ROWS of 32, and STAGES of the rows lie in LDS or are on their
+// way: a stage's products are over before its successor's loads have come, so
+// with few entries a workgroup (rows are read once by each) four stages count.
+// A kv head's rows of a sequence lie one behind another, so a stage is one
+// stretch of memory.  Every sum has one order.
+template <int DT, int D, int ENTRIES, int ROWS, int STAGES>
 __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnArgs a, int32_t blocks) {
   typedef typename Half16<DT>::V8 V8;
   constexpr int kSteps = D / 16, kRowBytes = 4 * D, kChunks = kRowBytes / 16, kRowsPerLoad = 1024 / kRowBytes;
-  constexpr int kWeightStages = 2;
+  constexpr int kWeightEntries = 32 * ENTRIES, kWeightRows = 32 * ROWS, kWeightStages = STAGES;
+  static_assert(ENTRIES * ROWS == 8, "eight waves");
   constexpr int kLoads = kWeightRows / kRowsPerLoad / 8, kStageBytes = kWeightRows * kRowBytes;
   __shared__ __align__(1024) uint8_t q_lds[kWeightStages * kStageBytes];
   __shared__ __align__(16) float norm_lds[kWeightStages][8][64];  // each wave its own
@@ -479,7 +479,7 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
   const int32_t j0 = blk * kWeightEntries;
   if (j0 >= s.length) return;
   const int32_t tokens = s.tokens < a.max_new ? s.tokens : a.max_new, before = s.length - s.tokens;
-  const int32_t wj0 = j0 + 32 * (wave & 1);
+  const int32_t wj0 = j0 + 32 * (wave % ENTRIES);
 
   // the wave's keys (A operand: 8 dims of entry ln)
   V8 kf[kSteps];
@@ -533,13 +533,13 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                    :: "s"(lds_base + (uint32_t)(stage * kStageBytes + 1024 * (wave * kLoads + j))), "v"(off[j]), "s"(rsrc) : "memory");
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                 :: "s"(lds_address(norm_lds[stage][wave])), "v"(4u * (uint32_t)(32 * (wave >> 1) + lane)), "s"(norm_rsrc) : "memory");
+                 :: "s"(lds_address(norm_lds[stage][wave])), "v"(4u * (uint32_t)(32 * (wave / ENTRIES) + lane)), "s"(norm_rsrc) : "memory");
   };
   typedef __attribute__((address_space(3))) const V8 lds_v8;
   uint32_t q_at[kSteps];
 #pragma unroll
   for (int c = 0; c < kSteps; ++c)
-    q_at[c] = lds_base + (uint32_t)((32 * (wave >> 1) + ln) * kRowBytes + 16 * ((2 * c + lh) ^ (ln & 15)));
+    q_at[c] = lds_base + (uint32_t)((32 * (wave / ENTRIES) + ln) * kRowBytes + 16 * ((2 * c + lh) ^ (ln & 15)));
 
   if (r0 < r1) {
 #pragma unroll
@@ -548,7 +548,7 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
     for (int32_t rs = r0; rs < r1; rs += kWeightRows, stage = (stage + 1) % kWeightStages) {
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((kWeightStages - 2) * (kLoads + 1)) : "memory");
       load_stage(rs + kWeightRows * (kWeightStages - 1), (stage + kWeightStages - 1) % kWeightStages);
-      const int32_t r = rs + 32 * (wave >> 1);
+      const int32_t r = rs + 32 * (wave / ENTRIES);
       if (r >= r1) continue;
       const int32_t row = r + ln;
       const bool row_ok = row < r1;
@@ -581,17 +581,19 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
   }
   // the last loads land before their room is used for the row groups' sums
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  float* sums = (float*)q_lds;  // [4 row groups][64]
+  float* sums = (float*)q_lds;  // [ROWS][32 ENTRIES]
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
 #pragma unroll
     for (int off2 = 16; off2 >= 1; off2 >>= 1) acc[e] += __shfl_xor(acc[e], off2, 64);
-    if (ln == e) sums[64 * (wave >> 1) + 32 * (wave & 1) + 8 * (e >> 2) + 4 * lh + (e & 3)] = acc[e];
+    if (ln == e) sums[kWeightEntries * (wave / ENTRIES) + 32 * (wave % ENTRIES) + 8 * (e >> 2) + 4 * lh + (e & 3)] = acc[e];
   }
   __syncthreads();
   const int32_t j = j0 + tid;
   if (tid < kWeightEntries && j < s.length) {
-    const float v = (sums[tid] + sums[64 + tid]) + (sums[128 + tid] + sums[192 + tid]);
+    float v = 0.f;
+#pragma unroll
+    for (int g = 0; g < ROWS; ++g) v += sums[kWeightEntries * g + tid];
     float* w = a.weights + b * a.wsb + kvh * a.wsh + j;
     *w = a.accumulate ? *w + v : v;
   }
@@ -618,9 +620,17 @@ static int launch_chunk(const PagedAttnArgs& a, hipStream_t stream) {
     if (rc != JKV_OK) return rc;
   }
   if (a.weights != nullptr && a.c.top > 0) {
-    const int64_t each = ceil_div(a.c.top, kWeightEntries), all = each * a.c.B * a.KVH;
-    JKV_CHECK_ARG(all < ((int64_t)1 << 31), "paged weights grid too large");
-    hipLaunchKernelGGL((paged_chunk_weights_kernel<DT, D>), dim3((uint32_t)all), dim3(512), 0, stream, a, (int32_t)each);
+    // 128 entries a workgroup where that fills the CUs, 64 elsewhere.  us of the
+    // attention and its weights with 64 and with 128, 32/8 heads of 128: 2 x 1,024
+    // tokens over 4,096 entries 386 and 343, 1 x 256 over 8,000 143 and 126, 1 x
+    // 2,000 161 and 204 (128 workgroups).
+    const int64_t each = ceil_div(a.c.top, 128), all = each * a.c.B * a.KVH;
+    JKV_CHECK_ARG(2 * all < ((int64_t)1 << 31), "paged weights grid too large");
+    if (all >= 256)
+      hipLaunchKernelGGL((paged_chunk_weights_kernel<DT, D, 4, 2, 4>), dim3((uint32_t)all), dim3(512), 0, stream, a, (int32_t)each);
+    else
+      hipLaunchKernelGGL((paged_chunk_weights_kernel<DT, D, 2, 4, 2>), dim3((uint32_t)(2 * all)), dim3(512), 0, stream, a,
+                         (int32_t)(2 * each));
   }
   JKV_CHECK_LAUNCH();
   return JKV_OK;

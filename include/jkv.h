@@ -690,7 +690,7 @@ int jkv_paged_append(const void* key, int64_t key_stride_t, int64_t key_stride_h
  *                added to what is there with `accumulate`, stored without
  *   max_new, max_length  the caller's bounds of a sequence's new tokens and
  *                entries (weight_width >= max_length).  Entries past max_length
- *                take no part; rows past max_new may be left out.
+ *                take no part; rows past max_new hold anything.
  * A token whose entry would lie before the first sees nothing: output 0, lse
  * -inf.
  */

@@ -205,6 +205,10 @@ __device__ __forceinline__ float marked(float o, float up, float down) {
   return o + (up > 0.f ? INFINITY : 0.f) + (down > 0.f ? -INFINITY : 0.f);
 }
 
+// A launch's threads along x have to fit 32 bits.
+#define JKV_CHECK_GRID(blocks, threads) \
+  JKV_CHECK_ARG((int64_t)(blocks) * (threads) < ((int64_t)1 << 32), "paged cache grid too large")
+
 // host side: fills c and the rates, or says what is wrong with them
 int paged_cache_args(PagedCache* c, const void* k, const void* v, int64_t page_stride, int64_t head_stride,
                      int64_t slot_stride, int64_t n_pages, int64_t page_size, const int32_t* tables,

@@ -26,6 +26,7 @@ int paged_cache_args(PagedCache* c, const void* k, const void* v, int64_t page_s
                 "the page size must be a power of two from 16 to 4096, got %lld", (long long)page_size);
   JKV_CHECK_ARG(n_pages >= 0 && n_pages < ((int64_t)1 << 31), "invalid page count");
   JKV_CHECK_ARG(table_width >= 0 && table_width < ((int64_t)1 << 27), "invalid block table");
+  JKV_CHECK_ARG(page_stride >= 0 && head_stride >= 0, "page strides must not be negative");
   JKV_CHECK_ARG(page_stride % 8 == 0 && head_stride % 8 == 0 && slot_stride % 8 == 0 && slot_stride >= D &&
                     slot_stride < ((int64_t)1 << 22),
                 "page strides must be multiples of 8 elements, slots at least a row apart");
@@ -148,8 +149,9 @@ int jkv_paged_append(const void* key, int64_t key_stride_t, int64_t key_stride_h
   a.key = (const uint8_t*)key; a.kst = 2 * key_stride_t; a.ksh = 2 * key_stride_h;
   a.value = (const uint8_t*)value; a.vst = 2 * value_stride_t; a.vsh = 2 * value_stride_h;
   a.KVH = (int32_t)KVH;
+  JKV_CHECK_ARG(KVH < ((int64_t)1 << 20), "too many kv heads");
   const int64_t blocks = ceil_div(N * KVH * (D / 16), 256);
-  JKV_CHECK_ARG(KVH < ((int64_t)1 << 20) && blocks < ((int64_t)1 << 31), "append grid too large");
+  JKV_CHECK_GRID(blocks, 256);
   const dim3 grid((uint32_t)blocks), block(256);
   if (dtype == JKV_F16 && D == 128) hipLaunchKernelGGL((paged_append_kernel<JKV_F16, 128>), grid, block, 0, stream, a);
   else if (dtype == JKV_F16) hipLaunchKernelGGL((paged_append_kernel<JKV_F16, 64>), grid, block, 0, stream, a);

@@ -5,6 +5,7 @@
 // Token t of a sequence with T new tokens and L entries sits at entry
 // i = L - T + t and sees the entries j <= i with j > i - window or j < sinks:
 //   o_t = sum_j p_tj v_j,  p_tj = softmax_j(scale q_t k_j),  w_j = sum_t,h p_tj
+// A row that sees nothing (or only scores of -infinity) gives 0.
 // Here: a call's checks, the division of its work and its workspace.  Sequences
 // of few rows (paged_few.hip) and chunks (paged_chunk.hip) have kernels of
 // their own.

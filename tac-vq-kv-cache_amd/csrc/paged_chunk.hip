@@ -457,9 +457,8 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
 // exp2(score - lse) up: S^T[entry][row] leaves 16 entries of one row with a
 // lane, the sum over the rows' lanes comes last.  Eight waves a workgroup are
 // ENTRIES times ROWS of 32, and STAGES of the rows lie in LDS or are on their
-// way: a stage's products are over before its successor's loads have come, so
-// with few entries a workgroup (rows are read once by each) four stages count.
-// A kv head's rows of a sequence lie one behind another, so a stage is one
+// way: a stage's products (0.5 us) are over before its successor's loads have
+// come, so what LDS holds goes into stages.  A kv head's rows of a sequence lie one behind another, so a stage is one
 // stretch of memory.  Every sum has one order.
 template <int DT, int D, int ENTRIES, int ROWS, int STAGES>
 __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnArgs a, int32_t blocks) {
@@ -602,7 +601,7 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
 template <int DT, int D>
 static int launch_chunk(const PagedAttnArgs& a, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.items * a.KVH * a.splits;
-  JKV_CHECK_ARG(blocks < ((int64_t)1 << 31), "paged attention grid too large");
+  JKV_CHECK_GRID(blocks, 2 * a.item_rows);
   const dim3 grid((uint32_t)blocks), block((uint32_t)(2 * a.item_rows));
   const bool exact = a.lse != nullptr || a.lse2 != nullptr;
   if constexpr (D == 128) {
@@ -625,7 +624,7 @@ static int launch_chunk(const PagedAttnArgs& a, hipStream_t stream) {
     // tokens over 4,096 entries 386 and 343, 1 x 256 over 8,000 143 and 126, 1 x
     // 2,000 161 and 204 (128 workgroups).
     const int64_t each = ceil_div(a.c.top, 128), all = each * a.c.B * a.KVH;
-    JKV_CHECK_ARG(2 * all < ((int64_t)1 << 31), "paged weights grid too large");
+    JKV_CHECK_GRID(2 * all, 512);
     if (all >= 256)
       hipLaunchKernelGGL((paged_chunk_weights_kernel<DT, D, 4, 2, 4>), dim3((uint32_t)all), dim3(512), 0, stream, a, (int32_t)each);
     else

@@ -538,6 +538,7 @@ static void launch_join(const PagedAttnArgs& x, hipStream_t stream) {
 }
 
 int paged_launch_join(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream) {
+  JKV_CHECK_GRID(ceil_div((int64_t)a.c.N * a.QH, a.splits > 8 ? 4 : 32), 1024);
   if (dtype == JKV_F16) D == 128 ? launch_join<JKV_F16, 128>(a, stream) : launch_join<JKV_F16, 64>(a, stream);
   else D == 128 ? launch_join<JKV_BF16, 128>(a, stream) : launch_join<JKV_BF16, 64>(a, stream);
   JKV_CHECK_LAUNCH();
@@ -547,7 +548,7 @@ int paged_launch_join(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStrea
 template <int DT, int D>
 static int launch_few(const PagedAttnArgs& a, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.c.B * a.KVH * a.splits;
-  JKV_CHECK_ARG(blocks < ((int64_t)1 << 31), "paged attention grid too large");
+  JKV_CHECK_GRID(blocks, 64 * a.waves);
   const dim3 grid((uint32_t)blocks);
   constexpr int W2 = D == 128 ? 4 : 8;
   if (a.max_new * a.per <= 16) {

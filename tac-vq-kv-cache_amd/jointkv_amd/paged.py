@@ -60,6 +60,19 @@ def _rows(tensor: torch.Tensor) -> torch.Tensor:
     return tensor
 
 
+def _overlaps(tensor: torch.Tensor) -> bool:
+    """Whether two elements of ``tensor`` share memory (strides that nest)."""
+
+    if tensor.is_contiguous():
+        return False
+    span = 1
+    for stride, extent in sorted(zip(tensor.stride(), tensor.shape)):
+        if extent > 1 and stride < span:
+            return True
+        span = max(span, stride * extent)
+    return False
+
+
 def _pool_args(key_pages: torch.Tensor, value_pages: torch.Tensor, written: bool) -> tuple:
     if key_pages.ndim != 4 or key_pages.shape != value_pages.shape:
         raise ValueError("key and value pages must be two [pages,KVH,page_size,D] tensors of one shape")
@@ -71,13 +84,8 @@ def _pool_args(key_pages: torch.Tensor, value_pages: torch.Tensor, written: bool
     if strides[3] != 1:
         raise ValueError("page rows must be contiguous")
     pages, heads, size, dim = key_pages.shape
-    if written and not key_pages.is_contiguous():
-        # slots that share memory would be written by more than one entry
-        span = 1
-        for stride, extent in sorted(zip(strides, (pages, heads, size, dim))):
-            if extent > 1 and stride < span:
-                raise ValueError("pages that are written must not overlap")
-            span = max(span, stride * extent)
+    if written and (_overlaps(key_pages) or _overlaps(value_pages)):
+        raise ValueError("pages that are written must not overlap")
     return (strides[0], strides[1], strides[2], pages, size), heads, dim
 
 
@@ -181,7 +189,8 @@ def paged_attention(
     whole number of query heads shares a kv head.  ``max_new`` and
     ``max_length`` bound a sequence's new tokens and entries (defaults: all
     packed rows, the table's room); closer bounds make for a better division
-    of the work, and entries past ``max_length`` take no part.
+    of the work.  They are promises: entries past ``max_length`` take no part,
+    and rows past ``max_new`` hold anything.
 
     ``weights`` (fp32 ``[B,KVH,C]``, C at least ``max_length``): entry j below
     ``lengths[b]`` receives the sum of its softmax weights over the sequence's
@@ -192,7 +201,13 @@ def paged_attention(
     Returns ``[N,QH,D]`` (``out``, if given).  Rows that no sequence owns are
     left as they were; a token with no entry to see (a length below the number
     of new tokens) gets zeros and an ``lse`` of ``-inf``; a page number outside
-    the pool reads as zeros.  A call repeats bit for bit.
+    the pool reads as zeros.  A call repeats bit for bit; how the work is
+    divided follows from the sizes and bounds, so a row may differ in its last
+    bits between calls of other ones.  Single tokens and small chunks (tokens
+    times heads of a group at most 32) keep 32-bit scores and weights; larger
+    chunks round the rotated queries and the weights once to the pages' type
+    before the matrix products, the queries not where ``weights`` or ``lse``
+    are asked for.
     """
 
     device = _lib.require_device(query, key_pages, value_pages, block_tables, lengths, starts, positions, weights,
@@ -221,8 +236,7 @@ def paged_attention(
             max_length = min(room, width)
         elif min(max_length, room) > width:
             raise ValueError("weights have fewer entries than max_length")
-        if (heads > 1 and per_head < width) or (batch > 1 and per_batch < (heads - 1) * per_head + width and (
-                per_batch < width or (heads > 1 and per_head < (batch - 1) * per_batch + width))):
+        if _overlaps(weights):
             raise ValueError("weights that are written must not overlap")
         weight_args = (weights.data_ptr(), per_batch, per_head, width)
     max_length = room if max_length is None else min(int(max_length), room)
@@ -234,6 +248,8 @@ def paged_attention(
     elif out.dtype != query.dtype or out.shape != query.shape or out.stride(2) != 1 or out.stride(0) % 8 or (
             out.stride(1) % 8 or out.data_ptr() % 16):
         raise ValueError("out must match the queries, with contiguous 16-byte aligned rows")
+    elif _overlaps(out):
+        raise ValueError("an out that is written must not overlap")
     query = _rows(query)
     span = 0 if window is None else min(int(window), 0x7fffffff)
     sinks = min(int(sinks), 0x7fffffff)
@@ -334,7 +350,7 @@ def compact_pages(
 @dataclass(frozen=True)
 class PagedStep:
     """One step's sequences as the kernels take them: every layer of the step
-    appends and attends with it."""
+    appends and attends with it (until the next eviction or release)."""
 
     block_tables: torch.Tensor
     lengths: torch.Tensor
@@ -412,9 +428,12 @@ class PagedKVCache:
         host = torch.tensor(values, dtype=torch.int32, pin_memory=True)
         return host.to(self.key.device, non_blocking=True)
 
-    def _tables(self) -> torch.Tensor:
+    def _upload(self, rows: list[list[int]]) -> None:
+        """The block tables on the device, in their place (steps and captured
+        graphs hold the tensor)."""
+
         width = self.block_tables.shape[1]
-        return self._on_device([row + [-1] * (width - len(row)) for row in self._pages])
+        self.block_tables.copy_(self._on_device([row + [-1] * (width - len(row)) for row in rows]))
 
     def begin(self, new_tokens: Sequence[int]) -> PagedStep:
         """Take pages for ``new_tokens[b]`` more entries of every sequence b
@@ -430,9 +449,11 @@ class PagedKVCache:
         if sum(more) > len(self._free):
             raise ValueError(f"the step needs {sum(more)} pages, {len(self._free)} are free")
         if sum(more):
-            for row, n in zip(self._pages, more):
-                row.extend(self._free.pop() for _ in range(n))
-            self.block_tables = self._tables()
+            free = iter(reversed(self._free))
+            pages = [row + [next(free) for _ in range(n)] for row, n in zip(self._pages, more)]
+            self._upload(pages)
+            self._pages = pages
+            del self._free[-sum(more) :]
         starts = [0]
         for n in new:
             starts.append(starts[-1] + n)
@@ -483,18 +504,27 @@ class PagedKVCache:
         each = -(-budget // self.page_size)
         if each * len(over) > len(self._free):
             raise ValueError(f"the eviction needs {each * len(over)} pages, {len(self._free)} are free")
-        old_tables, old_pages = self.block_tables, list(self._pages)
-        lengths = self._on_device(self._lengths)
+        taken = self._free[-each * len(over) :]
+        pages = list(self._pages)
+        for n, b in enumerate(over):
+            pages[b] = taken[n * each : (n + 1) * each]
+        lengths, old_tables = self._on_device(self._lengths), self.block_tables.clone()
+        try:
+            self._upload(pages)
+            moved = []
+            for layer, weights in enumerate(self.weights):
+                kept, _ = select_entries(weights, lengths, budget, sinks=sinks, recent=recent)
+                moved.append(compact_pages(self.key[layer], self.value[layer], old_tables, kept, self.block_tables,
+                                           weights=weights))
+        except BaseException:
+            self.block_tables.copy_(old_tables)  # nothing is taken: the old pages are as they were
+            raise
+        self.weights = moved
+        del self._free[-each * len(over) :]
         for b in over:
-            self._pages[b] = [self._free.pop() for _ in range(each)]
+            self._free.extend(reversed(self._pages[b]))
             self._lengths[b] = budget
-        self.block_tables = self._tables()
-        for layer, weights in enumerate(self.weights):
-            kept, _ = select_entries(weights, lengths, budget, sinks=sinks, recent=recent)
-            self.weights[layer] = compact_pages(self.key[layer], self.value[layer], old_tables, kept,
-                                                self.block_tables, weights=weights)
-        for b in over:
-            self._free.extend(reversed(old_pages[b]))
+        self._pages = pages
 
     def release(self, sequence: int) -> None:
         """Drop a sequence: its pages are free and its slot empty."""
@@ -502,7 +532,7 @@ class PagedKVCache:
         self._free.extend(reversed(self._pages[sequence]))
         self._pages[sequence] = []
         self._lengths[sequence] = self._positions[sequence] = 0
-        self.block_tables = self._tables()
+        self._upload(self._pages)
         if self.weights is not None:
             for weights in self.weights:
                 weights[sequence].zero_()

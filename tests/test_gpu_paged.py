@@ -562,6 +562,101 @@ def test_streams_devices_and_graphs(device):
                 assert torch.equal(w[b, :, :length], eager[i][1][b, :, :length])
 
 
+def test_pages_beyond_four_gigabytes(device):
+    """Offsets that pass 32 bits: the sequence lies at the end of a large pool."""
+
+    page, kvh, dim = 64, 8, 128
+    pages = (1 << 32) // (page * kvh * dim * 2) + 40
+    print(f"pool of {pages} pages, {2 * pages * page * kvh * dim * 2 >> 30} GiB", flush=True)
+    pools = [torch.empty(pages, kvh, page, dim, dtype=torch.float16, device=device) for _ in range(2)]
+    length = 300
+    for new in (1, 30):
+        batch = Batch(31, [length], [new], qh=16, kvh=kvh, dim=dim, page=page)
+        count = -(-length // page)
+        tables = torch.tensor([[pages - 1 - 7 * i for i in range(count)]], dtype=torch.int32, device=device)
+        for pool in pools:
+            pool[tables[0].long()] = float("nan")
+        lengths = torch.tensor([length], dtype=torch.int32, device=device)
+        starts = torch.tensor([0, length], dtype=torch.int32, device=device)
+        jkv.paged_append(batch.keys[0].to(device), batch.values[0].to(device), *pools, tables, lengths, starts=starts,
+                         rope_theta=None)
+        starts = torch.tensor([0, new], dtype=torch.int32, device=device)
+        weights = torch.zeros(1, kvh, length, device=device)
+        out = jkv.paged_attention(batch.query.to(device), *pools, tables, lengths, starts=starts, window=None,
+                                  weights=weights)
+        expect = batch.expect(None, 0)
+        check_out(out, expect, torch.float16)
+        check_weights(weights, expect, [length])
+        # and their compaction to other pages there
+        kept, _ = jkv.select_entries(weights, lengths, 100)
+        moved = torch.tensor([[pages - 3, pages - 4]], dtype=torch.int32, device=device)
+        jkv.compact_pages(*pools, tables, kept, moved)
+        stay = kept[0, 5].long().cpu()
+        got = pools[1][moved[0].long()][:, 5].reshape(-1, dim)[:100].cpu()
+        assert torch.equal(got, batch.values[0][stay, 5])
+
+
+def test_two_calls_at_once(device):
+    """Two streams with calls in flight over the same pages: each has its own
+    workspace."""
+
+    one = Batch(41, [900, 300], [1, 1], qh=8, kvh=2, dim=128)
+    two = Batch(42, [500, 90], [60, 9], qh=8, kvh=2, dim=64)
+    args = [one.on(device), two.on(device)]
+    args[0]["starts"] = None
+    queries = [one.query.to(device), two.query.to(device)]
+    widths = [torch.zeros(2, 2, 1024, device=device), torch.zeros(2, 2, 1024, device=device)]
+    alone = [jkv.paged_attention(q, **a, weights=w).clone() for q, a, w in zip(queries, args, widths)]
+    kept = [w.clone() for w in widths]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [[], []]
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                outs[i].append(jkv.paged_attention(queries[i], **args[i], weights=widths[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
+        assert torch.equal(widths[i], kept[i])
+
+
+def test_an_output_may_be_the_query(device):
+    for lengths, new in (([900, 300], [1, 1]), ([700, 90], [200, 60])):
+        batch = Batch(43, lengths, new, qh=8, kvh=2, dim=128)
+        args = batch.on(device)
+        query = batch.query.to(device)
+        want = jkv.paged_attention(query, **args)
+        jkv.paged_attention(query, **args, out=query)
+        assert torch.equal(query, want)
+
+
+def test_bounds_are_kept_where_lengths_are_not(device):
+    """Lengths past the table's room or the caller's bound count as that."""
+
+    batch = Batch(44, [96], [1], qh=4, kvh=2, dim=64)
+    args = batch.on(device)
+    args["starts"] = None
+    query = batch.query.to(device)
+    want = jkv.paged_attention(query, **args)
+    for length in (97, 10 ** 9, 2 ** 31 - 1):
+        args["lengths"] = torch.tensor([length], dtype=torch.int32, device=device)
+        weights = torch.zeros(1, 2, 96, device=device)
+        assert torch.equal(jkv.paged_attention(query, **args, weights=weights), want)
+    args["lengths"] = torch.tensor([-5], dtype=torch.int32, device=device)
+    assert bool((jkv.paged_attention(query, **args) == 0).all())
+    # starts that run past the rows, or backwards, stay inside them
+    for starts in ([0, 99], [-7, 1], [1, 0]):
+        args["starts"] = torch.tensor(starts, dtype=torch.int32, device=device)
+        out = torch.full_like(query, 5.0)
+        jkv.paged_attention(query, **args, out=out)
+        key = torch.ones(1, 2, 64, dtype=torch.float16, device=device)
+        before = args["key_pages"].clone()
+        jkv.paged_append(key, key, args["key_pages"], args["value_pages"], args["block_tables"], args["lengths"],
+                         starts=args["starts"])
+        assert torch.equal(before.view(torch.int16), args["key_pages"].view(torch.int16))
+
+
 def test_refusals(device):
     batch = Batch(2, [20, 30], [1, 1], qh=4, kvh=2, dim=64)
     args = batch.on(device)
@@ -594,6 +689,7 @@ def test_refusals(device):
     refused("must not overlap", weights=torch.zeros(1, 1, 32, device=device).expand(2, 2, 32))
     refused("lse must be", lse=torch.zeros(2, 2, device=device))
     refused("out must match", out=torch.zeros(2, 4, 64, device=device))
+    refused("must not overlap", out=torch.zeros(1, 4, 64, dtype=torch.float16, device=device).expand(2, 4, 64))
     page8 = torch.zeros(4, 2, 8, 64, dtype=torch.float16, device=device)
     refused("power of two", key_pages=page8, value_pages=page8.clone())
     page24 = torch.zeros(4, 2, 24, 64, dtype=torch.float16, device=device)

@@ -57,8 +57,12 @@ static PagedPlan paged_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64
       p.waves = many;
       p.split_tiles = tiles;
     } else {
-      // two waves a SIMD of every CU
-      const int64_t want = std::max<int64_t>(1, 2048 / std::max<int64_t>(1, bh));
+      // a wave a SIMD of every CU, two at 64 dims: 64 KiB of loads in flight a CU
+      // carry the memory's rate, and more splits are more to join.  us with 1,024
+      // waves and with 2,048: 4 ragged sequences to 65,536 entries 122 and 133, 1
+      // x 60,000 59 and 65, 16 x 4,096 60 and 62; at 64 dims 24 windows of 4,096
+      // 29 and 27.
+      const int64_t want = std::max<int64_t>(1, 1024 * (128 / D) / std::max<int64_t>(1, bh));
       p.split_tiles = std::max<int64_t>(2, ceil_div(tiles, want));
     }
     p.splits = ceil_div(tiles, p.split_tiles);

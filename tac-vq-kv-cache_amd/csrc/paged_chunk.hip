@@ -11,8 +11,19 @@
 // sum take one swap.  O^T[dim][row] += V^T P^T takes P from those registers,
 // 4 entries of each of two groups of 8 a lane, and V^T by transposing reads of
 // the row-major tile in the same order.  Online softmax in 32 bits; p and the
-// rotated, scaled q enter the products rounded once to the cache's type, except
-// that with EXACT (weights or log-sum-exps are asked for) q is a sum of two parts.
+// rotated, scaled q enter the products rounded once to the cache's type (that is
+// 2^-9 of a bf16 weight and up to as much of a score: the output is 0.3 % off
+// where its own rounding alone is 0.17 %; two parts of each would double the
+// products), except that with EXACT (weights or log-sum-exps are asked for) q is
+// a sum of two parts.
+//
+// 2 x 2,048 bf16 tokens over 16,384 entries, 32/8 heads of 128: 852 us, 1.21
+// PFLOP/s (a large matrix product reaches 1.30).  Per tile and wave 32 products
+// (1,024 cycles of its SIMD) stand beside about 210 vector instructions (1,000)
+// and 32 KiB of LDS reads; two waves a SIMD overlap a third of them.  Measured
+// without gain: three and four stages of tiles, wave priorities around the
+// products, the next tile's loads behind the scores (1,720 us: they take a whole
+// tile's time to come).
 #include <math.h>
 
 #include <type_traits>

@@ -73,6 +73,10 @@ static PagedPlan paged_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64
     if (weights) {
       p.lse2_at = take(N * QH * 4);
       p.score_width = ceil_div(max_length, 32) * 32;
+      if ((double)(B * KVH) * (double)(max_new * per) * (double)p.score_width > 1e14) {  // no memory holds them
+        p.bytes = INT64_MAX;
+        return p;
+      }
       p.scores_at = take(B * KVH * max_new * per * p.score_width * 4);
     }
   } else {

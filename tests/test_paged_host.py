@@ -55,7 +55,7 @@ def _attention_call(**overrides):
 @pytest.mark.parametrize("change,message", [
     (dict(dtype=2), b"fp16 or bf16"), (dict(D=96), b"head_dim"), (dict(QH=3), b"multiple"), (dict(B=-1), b"geometry"),
     (dict(N=3), b"one new token"), (dict(page_size=8), b"power of two"), (dict(page_size=48), b"power of two"),
-    (dict(page=4097), b"strides"), (dict(slot=64), b"strides"), (dict(k=8), b"aligned"), (dict(window=-1), b"negative"),
+    (dict(page=4097), b"strides"), (dict(page=-4096), b"negative"), (dict(head=-2048), b"negative"), (dict(slot=64), b"strides"), (dict(k=8), b"aligned"), (dict(window=-1), b"negative"),
     (dict(max_new=-1), b"negative"), (dict(sinks=-1), b"negative"), (dict(theta=-2.0), b"rotary"),
     (dict(theta=float("nan")), b"rotary"), (dict(scale=float("nan")), b"scale"), (dict(qst=12), b"multiples of 8"),
     (dict(out=8), b"aligned"), (dict(weights=16, width=10), b"fewer entries"), (dict(lengths=None), b"null"),
@@ -65,6 +65,15 @@ def test_attention_refuses_before_the_device_is_touched(change, message):
     # only calls that fail their checks: one that passes would launch
     assert _attention_call(**change) == _lib.JKV_EINVAL
     assert message in _lib.load().jkv_last_error(), _lib.load().jkv_last_error()
+
+
+def test_workspaces_that_no_memory_holds_are_refused():
+    # scores of 2^24 sequences of 2^29 entries: their bytes would wrap
+    batch = (1 << 24) - 1
+    sizes = dict(N=batch, B=batch, max_length=1 << 29, twidth=1 << 20, page_size=1024,
+                 page=1 << 20, head=1 << 17, tstride=0, weights=16, width=1 << 29, wsb=1 << 30, wsh=1 << 29)
+    assert _attention_call(**sizes) == _lib.JKV_EINVAL
+    assert b"workspace" in _lib.load().jkv_last_error()
 
 
 def test_empty_calls_are_no_ops():

@@ -681,7 +681,7 @@ int jkv_paged_append(const void* key, int64_t key_stride_t, int64_t key_stride_h
  * Attention of the new tokens over their sequences' entries.  A token at entry
  * i sees the entries j <= i with j > i - window (window 0: all) or j < sinks.
  *   q, out       [N,QH,D] of the cache's type, element strides (multiples of 8)
- *   scale        of the scores (1/sqrt(D) for plain attention)
+ *   scale        of the scores (1/sqrt(D) for plain attention), below 1e30
  *   lse          fp32 [N,QH] contiguous or NULL: natural log of each row's sum
  *                of exponentials
  *   weights      fp32 [B,KVH,weight_width] (rows contiguous) or NULL: entry j <

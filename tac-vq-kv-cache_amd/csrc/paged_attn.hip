@@ -150,7 +150,8 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   rc = paged_rope_args(&a.rope, rope_theta, D);
   if (rc != JKV_OK) return rc;
   JKV_CHECK_ARG(window >= 0 && sinks >= 0, "window and sinks must not be negative");
-  JKV_CHECK_ARG(isfinite(scale), "the softmax scale must be finite");
+  // (its powers of two have to fit 32 bits below)
+  JKV_CHECK_ARG(fabsf(scale) < 1e30f, "the softmax scale must be finite and below 1e30");
   const int64_t strides[4] = {q_stride_t, q_stride_h, out_stride_t, out_stride_h};
   for (int i = 0; i < 4; ++i)
     JKV_CHECK_ARG(strides[i] % 8 == 0, "token and head strides must be multiples of 8 elements");

@@ -76,6 +76,12 @@ def test_workspaces_that_no_memory_holds_are_refused():
     assert b"workspace" in _lib.load().jkv_last_error()
 
 
+@pytest.mark.parametrize("scale", [3e38, -3e38, 1e30, float("inf")])
+def test_scales_whose_base_2_form_overflows_are_refused(scale):
+    assert _attention_call(scale=scale) == _lib.JKV_EINVAL
+    assert b"scale" in _lib.load().jkv_last_error()
+
+
 def test_empty_calls_are_no_ops():
     assert _attention_call(N=0, B=0) == _lib.JKV_OK
     lib = _lib.load()

@@ -711,7 +711,8 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                         int32_t accumulate, void* workspace,
                         int64_t workspace_bytes, jkv_stream_t stream);
 
-/* Workspace of jkv_paged_attention for these sizes (bytes). */
+/* Workspace of jkv_paged_attention for these sizes (bytes; 0 for sizes that it
+ * refuses). */
 int64_t jkv_paged_attention_workspace_bytes(int64_t N, int64_t B, int64_t QH,
                                             int64_t KVH, int64_t D,
                                             int64_t max_new, int64_t max_length,

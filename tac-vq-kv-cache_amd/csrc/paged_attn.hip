@@ -124,6 +124,10 @@ extern "C" {
 int64_t jkv_paged_attention_workspace_bytes(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t max_new,
                                             int64_t max_length, int64_t window, int64_t sinks, int32_t with_weights) {
   if (N <= 0 || B <= 0 || QH <= 0 || KVH <= 0 || QH % KVH != 0) return 0;
+  // sizes that the call refuses need none
+  if ((D != 64 && D != 128) || N >= ((int64_t)1 << 30) || B >= ((int64_t)1 << 24) || QH >= 65536 || max_length < 0 ||
+      window < 0 || sinks < 0)
+    return 0;
   const int64_t most = jkv::kPagedMost;
   return jkv::paged_plan(N, B, QH, KVH, D, std::max<int64_t>(1, std::min(max_new, N)), std::min(max_length, most),
                          window > 0 && window < most ? window : most, std::min(sinks, most), with_weights != 0).bytes;

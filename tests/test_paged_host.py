@@ -82,6 +82,15 @@ def test_scales_whose_base_2_form_overflows_are_refused(scale):
     assert b"scale" in _lib.load().jkv_last_error()
 
 
+@pytest.mark.parametrize("change", [dict(D=0), dict(D=-64), dict(D=256), dict(N=1 << 62), dict(B=1 << 62),
+                                    dict(QH=1 << 20), dict(max_length=-1), dict(window=-1), dict(sinks=-1)])
+def test_workspaces_of_refused_sizes_are_none(change):
+    sizes = dict(N=2, B=2, QH=4, KVH=2, D=128, max_new=1, max_length=4096, window=0, sinks=0, weights=1)
+    query = _lib.load().jkv_paged_attention_workspace_bytes
+    assert query(*sizes.values()) > 0
+    assert query(*{**sizes, **change}.values()) == 0
+
+
 def test_empty_calls_are_no_ops():
     assert _attention_call(N=0, B=0) == _lib.JKV_OK
     lib = _lib.load()

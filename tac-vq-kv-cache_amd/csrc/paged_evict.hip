@@ -280,6 +280,7 @@ int jkv_paged_compact(void* key_pages, void* value_pages, int32_t dtype, int64_t
   a.kept = kept; a.budget = (int32_t)budget; a.KVH = (int32_t)KVH;
   a.to_tables = new_tables; a.to_stride = new_table_stride; a.to_width = new_table_width;
   a.weights = weights; a.w_sb = weight_stride_b; a.w_sh = weight_stride_h; a.moved = moved; a.width = (int32_t)width;
+  JKV_CHECK_GRID(ceil_div(rows, 64), 256);
   const dim3 grid((uint32_t)ceil_div(rows, 64), (uint32_t)KVH, (uint32_t)B), block(256);
   if (D == 128) hipLaunchKernelGGL((paged_compact_kernel<128>), grid, block, 0, (hipStream_t)stream_, a);
   else hipLaunchKernelGGL((paged_compact_kernel<64>), grid, block, 0, (hipStream_t)stream_, a);

@@ -116,6 +116,12 @@ def test_other_entries_refuse_before_the_device_is_touched():
                                  None, None) == _lib.JKV_EINVAL
 
 
+def test_copies_that_pass_32_bits_of_threads_are_refused():
+    assert _lib.load().jkv_paged_compact(16, 16, 0, 4096, 2048, 128, 4, 16, 1, 4, 4, 1, (1 << 30) - 1, 1, 4, 4, 1, 2, 128,
+                                         None, 0, 0, 0, None, None) == _lib.JKV_EINVAL
+    assert b"grid" in _lib.load().jkv_last_error()
+
+
 def test_operators_refuse_cpu_tensors():
     pages = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
     ints = torch.zeros(2, 4, dtype=torch.int32)

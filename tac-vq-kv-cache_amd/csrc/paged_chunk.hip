@@ -513,8 +513,10 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
   int32_t t0 = j0 - before, t1 = tokens;
   if (t0 < 0) t0 = 0;
   if (j0 >= a.sinks) {
-    const int32_t end = j0 + kWeightEntries - 1 + a.window - before;  // the last entry's window ends here
-    if (end < t1) t1 = end;
+    // the last entry's window ends here: far before the new tokens (or 2^31 on),
+    // whose product with the heads below would wrap
+    const int64_t end = (int64_t)j0 + kWeightEntries - 1 + a.window - before;
+    if (end < t1) t1 = end > 0 ? (int32_t)end : 0;
   }
   const uint32_t per = (uint32_t)a.per;
   // (rows fit 31 bits: host-checked)

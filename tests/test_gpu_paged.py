@@ -596,6 +596,29 @@ def test_pages_beyond_four_gigabytes(device):
         assert torch.equal(got, batch.values[0][stay, 5])
 
 
+def test_weights_where_heads_times_entries_pass_31_bits(device):
+    """2.2 million entries (the same four pages over and over) and 1,024 heads:
+    most entries lie far before the window of the new token."""
+
+    length, page, qh, dim, seen = 2_200_000, 4096, 1024, 64, 64
+    gen = torch.Generator().manual_seed(41)
+    pools = [torch.randn(4, 1, page, dim, generator=gen).to(torch.float16) for _ in range(2)]
+    query = torch.randn(1, qh, dim, generator=gen).to(torch.float16)
+    width = -(-length // page)
+    tables = (torch.arange(width, dtype=torch.int32) % 4)[None]
+    at = torch.arange(length - seen, length)
+    k, v = (p[at // page % 4, 0, at % page][:, None].double().numpy() for p in pools)
+    expect = [ref.attend(query.double().numpy(), k, v, 0, window=seen, sinks=0, theta=None)]
+    weights = torch.full((1, 1, length + 3), 7.0, device=device)
+    print(f"{length} entries, {qh} heads", flush=True)
+    out = jkv.paged_attention(query.to(device), *(p.to(device) for p in pools), tables.to(device),
+                              torch.tensor([length], dtype=torch.int32, device=device), window=seen, rope_theta=None,
+                              max_length=length, weights=weights)
+    check_out(out, expect, torch.float16)
+    check_weights(weights[:, :, length - seen :], expect, [seen])
+    assert (weights[:, :, : length - seen] == 0).all() and (weights[:, :, length:] == 7.0).all()
+
+
 def test_two_calls_at_once(device):
     """Two streams with calls in flight over the same pages: each has its own
     workspace."""

@@ -218,7 +218,7 @@ def paged_attention(
     rows, qheads, query_dim = query.shape
     if query_dim != dim:
         raise ValueError("queries must be [N,QH,D] of the pages' type and dims")
-    if qheads == 0 or qheads % heads:
+    if heads == 0 or qheads == 0 or qheads % heads:
         raise ValueError("query heads must be a multiple of kv heads")
     batch, table, (lengths, starts, positions) = _batch_args(block_tables, lengths, starts, positions, rows)
     room = table[2] * strides[4]

@@ -736,3 +736,11 @@ def test_refusals(device):
     with pytest.raises(ValueError, match="kept entries"):
         jkv.compact_pages(args["key_pages"], args["value_pages"], args["block_tables"],
                           torch.zeros(2, 1, 4, dtype=torch.int32, device=device), args["block_tables"])
+
+
+def test_pools_without_heads_are_refused(device):
+    pages = torch.zeros(4, 0, 16, 64, dtype=torch.float16, device=device)
+    with pytest.raises(ValueError, match="multiple of kv heads"):
+        jkv.paged_attention(torch.zeros(2, 4, 64, dtype=torch.float16, device=device), pages, pages.clone(),
+                            torch.zeros(2, 4, dtype=torch.int32, device=device),
+                            torch.ones(2, dtype=torch.int32, device=device))

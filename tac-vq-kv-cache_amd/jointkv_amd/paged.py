@@ -350,7 +350,12 @@ def compact_pages(
 @dataclass(frozen=True)
 class PagedStep:
     """One step's sequences as the kernels take them: every layer of the step
-    appends and attends with it (until the next eviction or release)."""
+    appends and attends with it (until the next eviction or release).
+
+    A captured step is replayed with ``lengths`` and ``positions`` (and
+    ``starts``) refilled from a later ``begin``; give it the cache's
+    ``max_length`` first (``dataclasses.replace``), as entries past the bound
+    take no part."""
 
     block_tables: torch.Tensor
     lengths: torch.Tensor
@@ -519,7 +524,7 @@ class PagedKVCache:
         except BaseException:
             self.block_tables.copy_(old_tables)  # nothing is taken: the old pages are as they were
             raise
-        self.weights = moved
+        torch._foreach_copy_(self.weights, moved)  # in their place: captured graphs hold them
         del self._free[-each * len(over) :]
         for b in over:
             self._free.extend(reversed(self._pages[b]))

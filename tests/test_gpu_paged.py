@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import dataclasses
+
 import numpy as np
 import pytest
 import torch
@@ -497,6 +499,54 @@ def test_cache_serves_two_layers_evicts_and_goes_on(device):
         cache.begin([200, 0, 0])
     with pytest.raises(ValueError, match="are free"):
         cache.begin([105, 140, 94])
+
+
+def test_captured_steps_outlive_an_eviction(device):
+    """A step captured once and replayed, its tensors refilled, before and after
+    an eviction, against a second cache that is stepped eagerly."""
+
+    kvh, qh, dim = 2, 4, 64
+    gen = torch.Generator().manual_seed(43)
+
+    def new_cache():
+        return jkv.PagedKVCache(1, 2, 20, kvh, max_length=128, page_size=16, head_dim=dim, track_weights=True,
+                                device=device)
+
+    def randn(n, heads):
+        return torch.randn(n, heads, dim, generator=gen).half().to(device)
+
+    def run(cache, step, k, v, q):
+        cache.append(0, step, k, v)
+        return cache.attention(0, step, q, window=50, sinks=2)
+
+    caches = [new_cache(), new_cache()]
+    prompt = randn(120, kvh), randn(120, kvh), randn(120, qh)
+    for cache in caches:
+        run(cache, cache.begin([70, 50]), *prompt)
+    # replays of longer sequences than now: the bound is the cache's
+    held = dataclasses.replace(caches[0].begin([1, 1]), max_length=128)
+    k, v, q = randn(2, kvh), randn(2, kvh), randn(2, qh)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(caches[0], held, k, v, q)
+    for turn in range(4):
+        if turn == 2:
+            for cache in caches:
+                cache.evict(32, sinks=2, recent=8)
+        if turn > 0:
+            step = caches[0].begin([1, 1])
+            held.lengths.copy_(step.lengths)
+            held.positions.copy_(step.positions)
+            for t, heads in ((k, kvh), (v, kvh), (q, qh)):
+                t.copy_(randn(2, heads))
+        want = run(caches[1], caches[1].begin([1, 1]), k, v, q)
+        other = torch.full((2, kvh, 128), -1.0, device=device)  # takes what memory is free
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.allclose(out.float(), want.float(), rtol=2 * half_step(torch.float16), atol=2.0 ** -20)
+        assert torch.allclose(caches[0].weights[0], caches[1].weights[0], rtol=2.0 ** -18, atol=0)
+        assert (other == -1.0).all()
+    assert caches[0].lengths == (34, 34)
 
 
 def test_codec_reconstructions_through_pages_match_the_prefill(device):

@@ -104,6 +104,14 @@ static PagedPlan paged_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64
     const int64_t most = std::min<int64_t>(512 / (p.items * KVH), tiles / 4);
     const int64_t best = std::min<int64_t>(most, (int64_t)(sqrt(save / part) + 0.5));
     p.splits = best > 1 && save * (1.0 - 1.0 / (double)best) > 6.0 + part * (double)best ? best : 1;
+    // Between one and two workgroups a CU some CUs have two and the others wait
+    // for them: two splits even that out where long chains pay for the join.  us
+    // with two and without: 1 x 1,200 tokens over 16,384 entries 392 and 404, 1 x
+    // 1,500 over 32,000 765 and 812, four ragged of 500 over 16,384 273 and 309,
+    // 1 x 1,500 over 16,384 at 64 dims 240 and 275; below the line 1 x 1,100 over
+    // 6,000 156 and 146, 1 x 1,600 over 16,384 480 and 445.
+    const int64_t groups = p.items * KVH;
+    if (groups > 256 && groups < 512 && 0.45 * (double)tiles * (1.0 - (double)groups / 512.0) > 6.0 + 2.0 * part) p.splits = 2;
     if (p.splits > 1) {
       p.ml_at = take(p.splits * N * QH * 8);
       p.o_at = take(p.splits * N * QH * D * 4);

@@ -374,6 +374,25 @@ def test_long_cache_is_split_and_joined(device):
         check_out(out, batch.expect(5000, 130), dtype)
 
 
+def test_blocks_between_one_and_two_a_cu_are_split(device):
+    """520 tokens of 64 heads over 4,900 entries: 264 blocks of rows with chains
+    long enough to be split in two."""
+
+    batch = Batch(45, [4900], [520], qh=64, kvh=8, dim=64, page=64)
+    weights = torch.full((1, 8, 4900), -1.0, device=device)
+    query, args = batch.query.to(device), batch.on(device)
+    plain = jkv.paged_attention(query, **args, window=None, max_length=4900, max_new=520)
+    exact = jkv.paged_attention(query, **args, window=None, max_length=4900, max_new=520, weights=weights)
+    for h in (0, 7):
+        heads = slice(8 * h, 8 * h + 8)
+        expect = [ref.attend(batch.queries[0][:, heads].double().numpy(), batch.keys[0][:, h : h + 1].double().numpy(),
+                             batch.values[0][:, h : h + 1].double().numpy(), batch.positions[0], window=None, sinks=0,
+                             theta=THETA)]
+        check_out(plain[:, heads], expect, torch.float16)
+        check_out(exact[:, heads], expect, torch.float16)
+        check_weights(weights[:, h : h + 1], expect, [4900])
+
+
 @pytest.mark.parametrize("length,budget,sinks,recent", [
     (10, 20, 0, 0), (20, 20, 2, 3), (21, 20, 0, 0), (100, 20, 4, 16), (100, 20, 20, 0), (100, 20, 0, 20),
     (5000, 1024, 4, 256), (4097, 4096, 0, 0), (12345, 1, 0, 0), (9000, 8000, 1, 1),

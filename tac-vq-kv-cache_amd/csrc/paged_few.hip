@@ -16,7 +16,9 @@
 // P's accumulator layout, 4 entries of each of two groups of 16 a lane).  The
 // matrix cores have time to spare here, so neither q nor p is rounded to 16
 // bits: both enter as a sum of two (q = hi + lo, p = hi + lo), which leaves
-// 32-bit scores and sums and the output's own rounding.
+// 32-bit scores and sums and the output's own rounding.  (Two bf16 parts hold a
+// query to 2^-17: the weights are 2e-6 off, 7e-7 in fp16.  A third part took 1 to
+// 3 % longer.)
 #include <math.h>
 
 #include <type_traits>

@@ -26,8 +26,6 @@ from pathlib import Path
 import numpy as np
 import torch
 
-sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "tac-vq-kv-cache_amd"))
-
 own = False
 
 THETA = 10000.0
@@ -333,9 +331,17 @@ def _plain_evict(state):
     return [kept, new_lengths.to(torch.int32), state["key_pages"], state["value_pages"], moved]
 
 
-def _own(state):
-    import jointkv_amd as jkv
+def _framework():
+    path = str(Path(__file__).resolve().parent.parent / "tac-vq-kv-cache_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import jointkv_amd
 
+    return jointkv_amd
+
+
+def _own(state):
+    jkv = _framework()
     case = state["case"]
     if case["op"] == "append":
         starts = None if state["single"] else state["starts"]

@@ -430,8 +430,10 @@ __global__ __launch_bounds__(256) void paged_few_weights_kernel(PagedAttnArgs a)
     const int32_t self = first + t;
     if (!(j <= self && (j > self - a.window || j < a.sinks))) continue;
     const float* norm = a.lse2 + ((int64_t)kvh * a.c.N + s.row0 + t) * a.per;
-    for (int32_t g = 0; g < a.per; ++g)
-      sum += __builtin_amdgcn_exp2f(sc[(int64_t)(t * a.per + g) * a.score_width] - norm[g]);
+    for (int32_t g = 0; g < a.per; ++g) {
+      const float p = __builtin_amdgcn_exp2f(sc[(int64_t)(t * a.per + g) * a.score_width] - norm[g]);
+      sum += norm[g] == -INFINITY ? 0.f : p;  // (a row of only -infinities saw nothing)
+    }
   }
   float* w = a.weights + b * a.wsb + kvh * a.wsh + j;
   *w = a.accumulate ? *w + sum : sum;

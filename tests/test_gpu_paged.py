@@ -813,3 +813,19 @@ def test_pools_without_heads_are_refused(device):
         jkv.paged_attention(torch.zeros(2, 4, 64, dtype=torch.float16, device=device), pages, pages.clone(),
                             torch.zeros(2, 4, dtype=torch.int32, device=device),
                             torch.ones(2, dtype=torch.int32, device=device))
+
+
+def test_weights_of_scores_that_pass_32_bits(device):
+    """Finite keys whose scaled scores pass the largest fp32 number: a row of
+    only such scores sees nothing, and its entries' tracked weights stay."""
+
+    for new, length in ((1, 1), (1, 70), (90, 90)):
+        batch = Batch(7, [length], [new], qh=4, kvh=2, dim=64, dtype=torch.bfloat16, theta=None)
+        batch.query.copy_(batch.query.abs() + 1e5)
+        batch.keys[0] = -batch.keys[0].abs() - 1e5
+        batch.write(0, batch.keys[0], batch.values[0])
+        args = batch.on(device)
+        weights = torch.full((1, 2, batch.width * 16), 3.0, device=device)
+        out = jkv.paged_attention(batch.query.to(device), **args, window=None, rope_theta=None, scale=1e29,
+                                  weights=weights, accumulate=True)
+        assert bool((out == 0).all()) and bool((weights == 3.0).all())

@@ -136,6 +136,7 @@ static const int32_t kPagedMost = 0x3fffffff;  // entries of a sequence: sums of
 
 // launches; what they need of the workspace is in the arguments already
 int paged_launch_few(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
+int paged_launch_few_weights(const PagedAttnArgs& a, hipStream_t stream);
 int paged_launch_chunk(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
 int paged_launch_join(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
 

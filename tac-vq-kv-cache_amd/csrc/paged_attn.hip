@@ -170,7 +170,14 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   JKV_CHECK_ARG(((uintptr_t)q | (uintptr_t)out) % 16 == 0, "queries and outputs must be 16-byte aligned");
   max_length = a.c.top;
   JKV_CHECK_ARG(weights == nullptr || weight_width >= max_length, "weights have fewer entries than max_length");
-  if (N == 0 || B == 0) return JKV_OK;
+  if (B == 0) return JKV_OK;
+  a.QH = (int32_t)QH; a.KVH = (int32_t)KVH; a.per = (int32_t)(QH / KVH);
+  a.weights = weights; a.wsb = weight_stride_b; a.wsh = weight_stride_h; a.accumulate = accumulate;
+  if (N == 0) {  // nobody attends: the entries received nothing
+    if (weights == nullptr || accumulate) return JKV_OK;
+    JKV_CHECK_ARG(lengths, "null buffer");
+    return paged_launch_few_weights(a, stream);
+  }
   JKV_CHECK_ARG(q && out, "null buffer");
   JKV_CHECK_ARG(N * QH < ((int64_t)1 << 31) - 256, "too many rows");
   max_new = std::max<int64_t>(1, std::min(max_new, N));
@@ -184,8 +191,6 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   a.q = (const uint8_t*)q; a.qst = 2 * q_stride_t; a.qsh = 2 * q_stride_h;
   a.out = (uint8_t*)out; a.ost = 2 * out_stride_t; a.osh = 2 * out_stride_h;
   a.lse = lse;
-  a.weights = weights; a.wsb = weight_stride_b; a.wsh = weight_stride_h; a.accumulate = accumulate;
-  a.QH = (int32_t)QH; a.KVH = (int32_t)KVH; a.per = (int32_t)(QH / KVH);
   a.max_new = (int32_t)max_new;
   a.q_mul = scale * 1.4426950408889634f;
   a.scale2 = 1.f;

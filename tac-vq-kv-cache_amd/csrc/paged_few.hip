@@ -552,6 +552,15 @@ int paged_launch_join(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStrea
   return JKV_OK;
 }
 
+int paged_launch_few_weights(const PagedAttnArgs& a, hipStream_t stream) {
+  const int64_t bh = (int64_t)a.c.B * a.KVH;
+  if (a.c.top > 0)
+    hipLaunchKernelGGL(paged_few_weights_kernel, dim3((uint32_t)ceil_div(a.c.top, 256), (uint32_t)(bh < 32768 ? bh : 32768),
+                       (uint32_t)ceil_div(bh, 32768)), dim3(256), 0, stream, a);
+  JKV_CHECK_LAUNCH();
+  return JKV_OK;
+}
+
 template <int DT, int D>
 static int launch_few(const PagedAttnArgs& a, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.c.B * a.KVH * a.splits;
@@ -569,11 +578,7 @@ static int launch_few(const PagedAttnArgs& a, hipStream_t stream) {
     const int rc = paged_launch_join(a, DT, D, stream);
     if (rc != JKV_OK) return rc;
   }
-  if (a.weights != nullptr && a.c.top > 0) {
-    const int64_t bh = (int64_t)a.c.B * a.KVH;
-    hipLaunchKernelGGL(paged_few_weights_kernel, dim3((uint32_t)ceil_div(a.c.top, 256), (uint32_t)(bh < 32768 ? bh : 32768),
-                       (uint32_t)ceil_div(bh, 32768)), dim3(256), 0, stream, a);
-  }
+  if (a.weights != nullptr) return paged_launch_few_weights(a, stream);
   JKV_CHECK_LAUNCH();
   return JKV_OK;
 }

@@ -829,3 +829,17 @@ def test_weights_of_scores_that_pass_32_bits(device):
         out = jkv.paged_attention(batch.query.to(device), **args, window=None, rope_theta=None, scale=1e29,
                                   weights=weights, accumulate=True)
         assert bool((out == 0).all()) and bool((weights == 3.0).all())
+
+
+def test_a_step_without_new_tokens_stores_zero_weights(device):
+    """Entries below the lengths receive nothing: 0 is stored, or added."""
+
+    batch = Batch(6, [40, 0, 17], [0, 0, 0], qh=4, kvh=2, dim=64)
+    args = batch.on(device)
+    query = torch.zeros(0, 4, 64, dtype=torch.float16, device=device)
+    weights = torch.full((3, 2, 48), 7.0, device=device)
+    out = jkv.paged_attention(query, **args, weights=weights, accumulate=True)
+    assert out.shape == (0, 4, 64) and bool((weights == 7.0).all())
+    jkv.paged_attention(query, **args, weights=weights)
+    for b, length in enumerate(batch.lengths):
+        assert bool((weights[b, :, :length] == 0).all()) and bool((weights[b, :, length:] == 7.0).all())

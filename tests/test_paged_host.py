@@ -173,3 +173,11 @@ def test_cache_refuses_geometry(change):
     args.update(change)
     with pytest.raises(ValueError):
         jkv.PagedKVCache(**args)
+
+
+def test_a_call_without_tokens_checks_what_it_reads():
+    # it stores zero weights below the lengths
+    assert _attention_call(N=0, starts=1, lengths=None, weights=16, wsb=128, wsh=64, width=64) == _lib.JKV_EINVAL
+    assert b"null" in _lib.load().jkv_last_error()
+    assert _attention_call(N=0, starts=1, lengths=None) == _lib.JKV_OK
+    assert _attention_call(N=0, starts=1, lengths=None, weights=16, wsb=128, wsh=64, width=64, accumulate=1) == _lib.JKV_OK

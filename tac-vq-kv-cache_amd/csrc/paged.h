@@ -188,6 +188,12 @@ __device__ __forceinline__ uint4v finite_halves(uint4v w, bool* found) {
   }
   return w;
 }
+// v with the infinite and NaN elements 0
+template <int DT, typename V8>
+__device__ __forceinline__ V8 finite_part(V8 v) {
+  bool found = false;
+  return __builtin_bit_cast(V8, finite_halves<DT>(__builtin_bit_cast(uint4v, v), &found));
+}
 // `up`: 1 where v is +infinity or NaN; `down`: 1 where it is -infinity or NaN.
 // Their products with the rows' visibility say which sums they belong to (both: NaN).
 template <int DT, typename V8>

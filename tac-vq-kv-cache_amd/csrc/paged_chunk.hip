@@ -231,7 +231,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     auto put = [&](int c, int e, float v) {
       v = row_ok ? v * a.q_mul : 0.f;
       qf[c][e] = (T)v;
-      if constexpr (EXACT) ql[c][e] = (T)(v - (float)(T)v);
+      if constexpr (EXACT) ql[c][e] = __builtin_isfinite((float)(T)v) ? (T)(v - (float)(T)v) : (T)0.f;
     };
     if (a.rope.on) {
 #pragma unroll
@@ -286,7 +286,9 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
   typedef __attribute__((address_space(3))) const V8 lds_v8;
-  auto scores = [&](int buf, float16v (&sc)[2]) {
+  // AGAIN: infinite keys meet the queries' leading part alone
+  auto scores = [&](int buf, float16v (&sc)[2], auto again) {
+    constexpr bool AGAIN = decltype(again)::value;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       sc[kb] = shift;
@@ -294,7 +296,8 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
       for (int c = 0; c < kSteps; ++c) {
         const V8 ka = *(lds_v8*)(size_t)(k_at[c] + (uint32_t)(2 * buf * kTileBytes + 32 * kb * kRowBytes));
         sc[kb] = mfma32<DT>(ka, qf[c], sc[kb]);
-        if constexpr (EXACT) sc[kb] = mfma32<DT>(ka, ql[c], sc[kb]);
+        if constexpr (EXACT && AGAIN) sc[kb] = mfma32<DT>(finite_part<DT>(ka), ql[c], sc[kb]);
+        else if constexpr (EXACT) sc[kb] = mfma32<DT>(ka, ql[c], sc[kb]);
       }
     }
   };
@@ -350,15 +353,10 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
-  auto step = [&](int32_t i, auto parity) {
+  auto work = [&](int32_t i, int32_t is, auto parity, auto again) {
     constexpr int buf = decltype(parity)::value;
-    const int32_t is = __builtin_amdgcn_readlane(what, i - run0);
-    meet();
-    load_stage(i + 1, buf ^ 1);
-    if (!(is & kBlockFull)) clean(buf);
-    if (!(is & kWaveSees)) return;
     float16v sc[2];
-    scores(buf, sc);
+    scores(buf, sc, again);
     JKV_SG(0x100, kSteps);
     for (int x = 0; x < kSteps; ++x) { JKV_SG(0x8, EXACT ? 2 : 1); JKV_SG(0x100, 1); }
     JKV_SG(0x8, EXACT ? 2 * kSteps : kSteps);
@@ -389,9 +387,39 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     for (int x = 0; x < 2 * kDims; ++x) { JKV_SG(0x8, 1); JKV_SG(0x100, 2); JKV_SG(0x2, 40 / (2 * kDims)); }
     JKV_SG(0x8, 2 * kDims);
   };
+  auto step = [&](int32_t i, auto parity) {
+    constexpr int buf = decltype(parity)::value;
+    const int32_t is = __builtin_amdgcn_readlane(what, i - run0);
+    meet();
+    load_stage(i + 1, buf ^ 1);
+    if (!(is & kBlockFull)) clean(buf);
+    if (is & kWaveSees) work(i, is, parity, std::false_type());
+  };
   for (int32_t i = tile0; i < tile1; i += 2) {
     step(i, std::integral_constant<int, 0>());
     if (i + 1 < tile1) step(i + 1, std::integral_constant<int, 1>());
+  }
+
+  if constexpr (EXACT) {
+    // An infinite key's product with a query's trailing part is 0 times infinity
+    // or the other infinity: NaN where the leading part's alone says which one.
+    // Whatever it went into is NaN, so finite sums need no second look.
+    if (__syncthreads_or(l != l)) {
+      shift = float16v{};
+      l = 0.f;
+      limit = -INFINITY;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) o[d] = float16v{};
+      run0 = tile0 - 64;
+      for (int32_t i = tile0; i < tile1; ++i) {
+        meet();
+        load_stage(i, 0);
+        const int32_t is = __builtin_amdgcn_readlane(what, i - run0);
+        meet();
+        if (!(is & kBlockFull)) clean(0);
+        if (is & kWaveSees) work(i, is, std::integral_constant<int, 0>(), std::true_type());
+      }
+    }
   }
 
   if (__syncthreads_or(found)) {
@@ -508,6 +536,10 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
 #pragma unroll
     for (int c = 0; c < kSteps; ++c) asm volatile("" : "+v"(kf[c]));  // waited for here, not beside the loads below
   }
+  // (infinite keys meet the queries' leading part alone, as in the attention)
+  V8 kl[kSteps];
+#pragma unroll
+  for (int c = 0; c < kSteps; ++c) kl[c] = finite_part<DT>(kf[c]);
 
   // the rows that may see one of the workgroup's entries
   int32_t t0 = j0 - before, t1 = tokens;
@@ -574,10 +606,11 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
         part[kSteps + c] = *(lds_v8*)(size_t)((q_at[c] + (uint32_t)(stage * kStageBytes)) ^ (uint32_t)(2 * D));
       }
 #pragma unroll
-      for (int c = 0; c < 2 * kSteps; ++c) sc = mfma32<DT>(kf[c % kSteps], part[c], sc);
+      for (int c = 0; c < 2 * kSteps; ++c) sc = mfma32<DT>(c < kSteps ? kf[c] : kl[c - kSteps], part[c], sc);
       const int32_t tf = before + (int32_t)((uint32_t)r / per);
       const int32_t tl = before + (int32_t)((uint32_t)(r + 31 < r1 ? r + 31 : r1 - 1) / per);
-      const bool full = wj0 + 31 <= tf && (wj0 > tl - a.window || wj0 + 32 <= a.sinks);
+      // (rows behind the last are zeros, which an infinite key turns into NaN)
+      const bool full = r + 31 < r1 && wj0 + 31 <= tf && (wj0 > tl - a.window || wj0 + 32 <= a.sinks);
       if (!full) {
         const int32_t self = row_ok ? before + (int32_t)((uint32_t)row / per) : -1;
 #pragma unroll

@@ -224,13 +224,9 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
       const V4 lo = lds_read_tr<V4>(at), hi = lds_read_tr<V4>(at + 16u * kRowBytes);
       return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
-    for (int32_t i = tile0; i < tile1; ++i) {
-      const int32_t e0 = entry_of(i);
-      const bool full = is_full(e0);
-      stage(full);
-      if (i + 1 < tile1) fetch(i + 1);
-
-      float4v sc[RG][2];
+    // TRAILING_FINITE: infinite keys meet the queries' leading part alone
+    auto scores = [&](float4v (&sc)[RG][2], auto trailing_finite) {
+      constexpr bool TRAILING_FINITE = decltype(trailing_finite)::value;
 #pragma unroll
       for (int kg = 0; kg < 2; ++kg) {
 #pragma unroll
@@ -239,68 +235,102 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
         for (int c = 0; c < kSteps; ++c) {
           const int r = 16 * kg + ln;
           const V8 ka = *(const V8*)(k_lds + r * kRowBytes + 16 * key_slot<D>(r, 4 * c + lg));
+          V8 kl = ka;
+          if constexpr (TRAILING_FINITE) kl = finite_part<DT>(ka);
 #pragma unroll
           for (int g = 0; g < RG; ++g) {
             sc[g][kg] = mfma16<DT>(ka, qh[g][c], sc[g][kg]);
-            sc[g][kg] = mfma16<DT>(ka, ql[g][c], sc[g][kg]);
+            sc[g][kg] = mfma16<DT>(kl, ql[g][c], sc[g][kg]);
           }
         }
       }
-      V8 ph[RG], pl[RG];
+    };
+    for (bool again = false;; again = true) {
+      for (int32_t i = tile0; i < tile1; ++i) {
+        const int32_t e0 = entry_of(i);
+        const bool full = is_full(e0);
+        stage(full);
+        if (i + 1 < tile1) fetch(i + 1);
+
+        float4v sc[RG][2];
+        scores(sc, std::false_type());
+        if (again) scores(sc, std::true_type());
+        V8 ph[RG], pl[RG];
 #pragma unroll
-      for (int g = 0; g < RG; ++g) {
-        if (!full) {
+        for (int g = 0; g < RG; ++g) {
+          if (!full) {
+#pragma unroll
+            for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int32_t j = e0 + 16 * kg + 4 * lg + e;
+                const bool seen = j <= self[g] && (j > self[g] - a.window || j < a.sinks);
+                sc[g][kg][e] = seen ? sc[g][kg][e] : -INFINITY;
+              }
+          }
+          if (a.scores != nullptr && row_ok[g]) {
+            float* to = a.scores + (((int64_t)b * a.KVH + kvh) * (a.max_new * a.per) + 16 * g + ln) * a.score_width + e0 + 4 * lg;
+#pragma unroll
+            for (int kg = 0; kg < 2; ++kg) *(float4v*)(to + 16 * kg) = sc[g][kg] * a.scale2;
+          }
+          float mx = -INFINITY;
 #pragma unroll
           for (int kg = 0; kg < 2; ++kg)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int32_t j = e0 + 16 * kg + 4 * lg + e;
-              const bool seen = j <= self[g] && (j > self[g] - a.window || j < a.sinks);
-              sc[g][kg][e] = seen ? sc[g][kg][e] : -INFINITY;
-            }
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[g][kg][e]);
+          mx = lanes4_max(mx) * a.scale2;
+          // the reference moves only when the maximum passes it by more than 4;
+          // p is 2^10 times its weight against the reference, at most 2^14, so
+          // that fp16 holds weights of 2^-34
+          const float mn = mx > m[g] + 4.f ? mx : m[g], mu = mn == -INFINITY ? 0.f : mn - 10.f;
+          const float alpha = m[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[g] - mn);
+          if (__any(mn != m[g])) {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) o[g][d] *= alpha;
+            l[g] *= alpha;
+          }
+          m[g] = mn;
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[g][e >> 2][e & 3], a.scale2, -mu));
+            sum += p;
+            const T hi = (T)p;
+            ph[g][e] = hi;
+            pl[g][e] = (T)(p - (float)hi);
+          }
+          l[g] += sum;
         }
-        if (a.scores != nullptr && row_ok[g]) {
-          float* to = a.scores + (((int64_t)b * a.KVH + kvh) * (a.max_new * a.per) + 16 * g + ln) * a.score_width + e0 + 4 * lg;
 #pragma unroll
-          for (int kg = 0; kg < 2; ++kg) *(float4v*)(to + 16 * kg) = sc[g][kg] * a.scale2;
-        }
-        float mx = -INFINITY;
+        for (int d = 0; d < kDims; ++d) {
+          const V8 va = value_operand(d);
 #pragma unroll
-        for (int kg = 0; kg < 2; ++kg)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[g][kg][e]);
-        mx = lanes4_max(mx) * a.scale2;
-        // the reference moves only when the maximum passes it by more than 4;
-        // p is 2^10 times its weight against the reference, at most 2^14, so
-        // that fp16 holds weights of 2^-34
-        const float mn = mx > m[g] + 4.f ? mx : m[g], mu = mn == -INFINITY ? 0.f : mn - 10.f;
-        const float alpha = m[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[g] - mn);
-        if (__any(mn != m[g])) {
-#pragma unroll
-          for (int d = 0; d < kDims; ++d) o[g][d] *= alpha;
-          l[g] *= alpha;
-        }
-        m[g] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(sc[g][e >> 2][e & 3], a.scale2, -mu));
-          sum += p;
-          const T hi = (T)p;
-          ph[g][e] = hi;
-          pl[g][e] = (T)(p - (float)hi);
-        }
-        l[g] += sum;
-      }
-#pragma unroll
-      for (int d = 0; d < kDims; ++d) {
-        const V8 va = value_operand(d);
-#pragma unroll
-        for (int g = 0; g < RG; ++g) {
-          o[g][d] = mfma16<DT>(va, ph[g], o[g][d]);
-          o[g][d] = mfma16<DT>(va, pl[g], o[g][d]);
+          for (int g = 0; g < RG; ++g) {
+            o[g][d] = mfma16<DT>(va, ph[g], o[g][d]);
+            o[g][d] = mfma16<DT>(va, pl[g], o[g][d]);
+          }
         }
       }
+      // An infinite key's product with a query's trailing part is 0 times infinity
+      // or the other infinity: NaN where the leading part's alone says which one.
+      // Whatever it goes into is NaN, so finite sums need no second walk.
+      bool odd = false;
+#pragma unroll
+      for (int g = 0; g < RG; ++g) odd = odd || l[g] != l[g];
+      if (again || !__any(odd)) break;
+#pragma unroll
+      for (int g = 0; g < RG; ++g) {
+        m[g] = -INFINITY;
+        l[g] = 0.f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) o[g][d] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)  // (infinite queries have no trailing part)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ql[g][c][e] = __builtin_isfinite((float)qh[g][c][e]) ? ql[g][c][e] : (T)0.f;
+      }
+      look_up(tile0);
+      fetch(tile0);
     }
     if (__any(found)) {
       for (int32_t i = tile0; i < tile1; ++i) {

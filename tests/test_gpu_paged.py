@@ -843,3 +843,80 @@ def test_a_step_without_new_tokens_stores_zero_weights(device):
     jkv.paged_attention(query, **args, weights=weights)
     for b, length in enumerate(batch.lengths):
         assert bool((weights[b, :, :length] == 0).all()) and bool((weights[b, :, length:] == 7.0).all())
+
+
+# ---- infinite and NaN keys and values that rows do see ----
+
+REACHED = [
+    # length, new tokens, heads, dims: which kernel and division of the entries
+    pytest.param(100, 1, 8, 2, 128, id="one-wave"),
+    pytest.param(200, 1, 8, 2, 64, id="waves"),
+    pytest.param(200, 5, 8, 2, 128, id="waves-two-groups"),
+    pytest.param(900, 1, 4, 2, 128, id="splits"),
+    pytest.param(900, 6, 8, 2, 64, id="splits-two-groups"),
+    pytest.param(400, 90, 4, 2, 128, id="chunk"),
+    pytest.param(5000, 64, 4, 1, 64, id="chunk-splits"),
+]
+
+
+def odd_call(batch, device, exact, **more):
+    """Output and weights (where ``exact`` asks for them) of ``batch``, all entries visible."""
+
+    args = batch.on(device)
+    weights = torch.zeros(len(batch.lengths), batch.kvh, batch.width * batch.page, device=device) if exact else None
+    out = jkv.paged_attention(batch.query.to(device), **args, window=None, rope_theta=batch.theta, weights=weights,
+                              max_new=max(batch.new), max_length=max(batch.lengths), **more)
+    return out, weights
+
+
+@pytest.mark.parametrize("exact", [False, True], ids=["out", "weights"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("length,new,qh,kvh,dim", REACHED)
+def test_keys_whose_scores_are_minus_infinity_weigh_nothing(device, length, new, qh, kvh, dim, dtype, exact):
+    """An entry whose key makes a score of -infinity gets weight 0 and leaves
+    the row finite; one that makes +infinity makes it NaN."""
+
+    batch = Batch(length + dim + 1, [length], [new], qh=qh, kvh=kvh, dim=dim, dtype=dtype, theta=None)
+    batch.query[:, :, 6] = batch.query[:, :, 6].abs() + 0.25
+    batch.query[:, :, 21] = -batch.query[:, :, 21].abs() - 0.25
+    batch.queries = [batch.query]
+    hidden = [1, 33, 39, 64]  # (all before the new tokens)
+    kept = [j for j in range(length) if j not in hidden]
+    expect = [ref.attend(batch.query.double().numpy(), batch.keys[0][kept].double().numpy(),
+                         batch.values[0][kept].double().numpy(), batch.positions[0], window=None, sinks=0, theta=None)]
+    keys = batch.keys[0]
+    keys[hidden[:2], :, 6] = float("-inf")
+    keys[hidden[2:], :, 21] = float("inf")
+    batch.write(0, keys, batch.values[0])
+    out, weights = odd_call(batch, device, exact)
+    check_out(out, expect, dtype)
+    if exact:
+        assert bool((weights[0][:, hidden] == 0).all())
+        check_weights(weights[:, :, kept], expect, [len(kept)])
+    keys[37, kvh - 1, 6] = float("inf")
+    batch.write(0, keys, batch.values[0])
+    again, _weights = odd_call(batch, device, exact)
+    per = qh // kvh
+    assert bool(again[:, qh - per :].isnan().all())
+    if kvh > 1:
+        assert torch.equal(again[:, : qh - per], out[:, : qh - per])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("length,new,dim", [(1, 1, 64), (50, 1, 128), (200, 1, 128), (900, 1, 64), (40, 5, 128),
+                                            (80, 80, 64), (400, 90, 128)])
+def test_rows_whose_scores_are_all_minus_infinity(device, length, new, dim, dtype):
+    """They give 0, a log-sum-exp of -infinity, and no weight to any entry,
+    whether the keys or the queries are infinite."""
+
+    for infinite in ("keys", "queries"):
+        batch = Batch(length, [length], [new], qh=8, kvh=2, dim=dim, dtype=dtype, theta=None)
+        batch.query[:, :, 6] = batch.query[:, :, 6].abs() + 0.25
+        batch.keys[0][:, :, 6] = -batch.keys[0][:, :, 6].abs() - 0.25
+        (batch.keys[0] if infinite == "keys" else batch.query)[:, :, 6] *= float("inf")
+        batch.write(0, batch.keys[0], batch.values[0])
+        lse = torch.full((new, 8), 9.0, device=device)
+        out, weights = odd_call(batch, device, True, lse=lse)
+        assert bool((out == 0).all()) and bool((lse == float("-inf")).all()) and bool((weights == 0).all())
+        out, _weights = odd_call(batch, device, False)
+        assert bool((out == 0).all())

@@ -174,7 +174,9 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 
 // A masked weight is 0, but 0 times an infinite or NaN value is not.  Tiles with
 // masked entries are therefore staged with such values as 0, and where one was
-// met a second walk over those tiles adds it to the rows that do see it.
+// met a second walk over those tiles adds it to the rows that do see it.  So are
+// all tiles once a walk has ended in sums that are not finite: a visible weight
+// is above 0 even where its 16 bits are not.
 
 // w with the infinite and NaN halves 0; sets *found if there were any
 template <int DT>

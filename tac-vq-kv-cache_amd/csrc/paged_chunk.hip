@@ -345,7 +345,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   };
   const bool unit = a.scale2 == 1.f;
 
-  bool found = false;  // an infinite or NaN value in a masked tile
+  bool found = false;  // an infinite or NaN value in a tile that was cleaned of them
   auto clean = [&](int buf) {
     for (int at = 16 * tid; at < kTileBytes; at += 16 * 64 * kChunkWaves) {
       uint4v* w = (uint4v*)(lds + (2 * buf + 1) * kTileBytes + at);
@@ -400,25 +400,30 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     if (i + 1 < tile1) step(i + 1, std::integral_constant<int, 1>());
   }
 
-  if constexpr (EXACT) {
-    // An infinite key's product with a query's trailing part is 0 times infinity
-    // or the other infinity: NaN where the leading part's alone says which one.
-    // Whatever it went into is NaN, so finite sums need no second look.
-    if (__syncthreads_or(l != l)) {
-      shift = float16v{};
-      l = 0.f;
-      limit = -INFINITY;
+  // An infinite value times a weight that rounds to 0, an infinite key times a
+  // query's trailing part: 0 times infinity or the other infinity, NaN where
+  // there is a result.  What these go into is not finite, so a walk that ends in
+  // finite sums needs no second.
+  float odd = l * 0.f;
 #pragma unroll
-      for (int d = 0; d < kDims; ++d) o[d] = float16v{};
-      run0 = tile0 - 64;
-      for (int32_t i = tile0; i < tile1; ++i) {
-        meet();
-        load_stage(i, 0);
-        const int32_t is = __builtin_amdgcn_readlane(what, i - run0);
-        meet();
-        if (!(is & kBlockFull)) clean(0);
-        if (is & kWaveSees) work(i, is, std::integral_constant<int, 0>(), std::true_type());
-      }
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) odd = fmaf(o[d][e], 0.f, odd);
+  const bool again = __syncthreads_or(odd != 0.f);
+  if (again) {
+    shift = float16v{};
+    l = 0.f;
+    limit = -INFINITY;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) o[d] = float16v{};
+    run0 = tile0 - 64;
+    for (int32_t i = tile0; i < tile1; ++i) {
+      meet();
+      load_stage(i, 0);
+      const int32_t is = __builtin_amdgcn_readlane(what, i - run0);
+      meet();
+      clean(0);
+      if (is & kWaveSees) work(i, is, std::integral_constant<int, 0>(), std::true_type());
     }
   }
 
@@ -427,7 +432,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
       const int32_t e0 = entry_of(i);
       run0 = i - 64;  // the tile's place anew
       look_up(i);
-      if (__builtin_amdgcn_readlane(what, 0) & kBlockFull) continue;
+      if ((__builtin_amdgcn_readlane(what, 0) & kBlockFull) && !again) continue;
       meet();
       load_values(i, 0);
       meet();

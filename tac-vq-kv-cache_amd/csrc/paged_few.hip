@@ -49,6 +49,10 @@ __device__ __forceinline__ float lanes4_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// A part's factor against the largest maximum.  Never 0: a part may hold an
+// infinite value (to finite sums 2^-126 of them adds nothing).
+__device__ __forceinline__ float part_factor(float m, float top) { return fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-126f); }
+
 // Slot of 16-byte chunk j of row r in a tile: keys so that 16 rows' equal
 // chunks, values so that 8 rows' equal chunk pairs, fall on distinct banks.
 template <int D> __device__ __forceinline__ int key_slot(int r, int j) {
@@ -174,7 +178,7 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
     auto is_full = [&](int32_t e0) {
       return e0 + kFewTile - 1 <= first && (e0 > last - a.window || e0 + kFewTile <= a.sinks);
     };
-    bool found = false;  // an infinite or NaN value in a masked tile
+    bool found = false;  // an infinite or NaN value in a tile that was staged without them
     auto stage = [&](bool full) {
       if (!full) {
 #pragma unroll
@@ -245,11 +249,12 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
         }
       }
     };
-    for (bool again = false;; again = true) {
+    bool again = false;
+    for (;; again = true) {
       for (int32_t i = tile0; i < tile1; ++i) {
         const int32_t e0 = entry_of(i);
         const bool full = is_full(e0);
-        stage(full);
+        stage(full && !again);
         if (i + 1 < tile1) fetch(i + 1);
 
         float4v sc[RG][2];
@@ -311,13 +316,20 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
           }
         }
       }
-      // An infinite key's product with a query's trailing part is 0 times infinity
-      // or the other infinity: NaN where the leading part's alone says which one.
-      // Whatever it goes into is NaN, so finite sums need no second walk.
-      bool odd = false;
+      // An infinite value times a weight's trailing part, or one that rounds to 0,
+      // an infinite key times a query's trailing part: 0 times infinity or the other
+      // infinity, NaN where there is a result.  What these go into is not finite, so
+      // a walk that ends in finite sums needs no second.
+      float odd = 0.f;
 #pragma unroll
-      for (int g = 0; g < RG; ++g) odd = odd || l[g] != l[g];
-      if (again || !__any(odd)) break;
+      for (int g = 0; g < RG; ++g) {
+        odd = fmaf(l[g], 0.f, odd);
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd = fmaf(o[g][d][e], 0.f, odd);
+      }
+      if (again || !__any(odd != 0.f)) break;
 #pragma unroll
       for (int g = 0; g < RG; ++g) {
         m[g] = -INFINITY;
@@ -335,7 +347,7 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
     if (__any(found)) {
       for (int32_t i = tile0; i < tile1; ++i) {
         const int32_t e0 = entry_of(i);
-        if (is_full(e0)) continue;
+        if (is_full(e0) && !again) continue;
         look_up(i);
         fetch(i);
         stage(true);  // as they are
@@ -385,7 +397,7 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
       for (int w = 0; w < W; ++w) {
         const float2 ml = ml_lds[w][r];
         if (ml.y == 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(ml.x - top);
+        const float f = part_factor(ml.x, top);
         lt = fmaf(ml.y, f, lt);
         const float4v p = *(const float4v*)(lds[w] + (r * D + 4 * part) * 4);
 #pragma unroll
@@ -514,14 +526,14 @@ __global__ __launch_bounds__(8 * D) void paged_join_kernel(JoinArgs a) {
         if (i0 + j * GROUPS >= a.splits) ml[j] = float2{-INFINITY, 0.f};
         top = fmaxf(top, ml[j].x);
       }
-      const float f0 = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+      const float f0 = m == top ? 1.f : part_factor(m, top);
       l *= f0;
       o *= f0;
       m = top;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (ml[j].y != 0.f) {  // a split that saw nothing may have written no sums
-          const float f = __builtin_amdgcn_exp2f(ml[j].x - top);
+          const float f = part_factor(ml[j].x, top);
           l = fmaf(ml[j].y, f, l);
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] = fmaf(p[j][e], f, o[e]);
@@ -542,7 +554,7 @@ __global__ __launch_bounds__(8 * D) void paged_join_kernel(JoinArgs a) {
     for (int j = 0; j < GROUPS; ++j) {
       const float2 ml = ml_lds[j][r];
       if (ml.y == 0.f) continue;
-      const float f = __builtin_amdgcn_exp2f(ml.x - top);
+      const float f = part_factor(ml.x, top);
       l = fmaf(ml.y, f, l);
       const float4v p = *(const float4v*)&o_lds[j][r][4 * part];
 #pragma unroll

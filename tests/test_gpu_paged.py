@@ -920,3 +920,53 @@ def test_rows_whose_scores_are_all_minus_infinity(device, length, new, dim, dtyp
         assert bool((out == 0).all()) and bool((lse == float("-inf")).all()) and bool((weights == 0).all())
         out, _weights = odd_call(batch, device, False)
         assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("exact", [False, True], ids=["out", "weights"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("length,new,qh,kvh,dim", REACHED)
+def test_non_finite_values_in_tiles_that_every_row_sees(device, length, new, qh, kvh, dim, dtype, exact):
+    """An infinite value that a row sees makes that dim infinite, two of unlike
+    sign or a NaN make it NaN, wherever in its tile the entry lies; the other
+    dims keep their results."""
+
+    batch = Batch(length + dim, [length], [new], qh=qh, kvh=kvh, dim=dim, dtype=dtype)
+    expect = batch.expect(None, 0)
+    values = batch.values[0]
+    for j in (3, 37, 38, 66):  # (all before the new tokens)
+        values[j, 0, 5] = float("inf")
+        values[j + 1, 0, 7] = float("-inf")
+    values[40, 0, 9] = float("nan")
+    values[2, 0, 11], values[70, 0, 11] = float("inf"), float("-inf")
+    batch.write(0, batch.keys[0], values)
+    out, weights = odd_call(batch, device, exact)
+    per, odd = qh // kvh, out[:, : qh // kvh]
+    assert bool((odd[:, :, 5] == float("inf")).all()) and bool((odd[:, :, 7] == float("-inf")).all())
+    assert bool(odd[:, :, (9, 11)].isnan().all())
+    plain = out.clone()
+    for d in (5, 7, 9, 11):
+        want = torch.from_numpy(expect[0]["out"][:, :per, d])
+        plain[:, :per, d] = want.to(device=device, dtype=dtype)
+    check_out(plain, expect, dtype)
+    if exact:
+        check_weights(weights, expect, [length])
+
+
+@pytest.mark.parametrize("length,new", [(90, 1), (250, 1), (3000, 1), (400, 60), (3000, 60)])
+def test_infinite_values_of_entries_that_hardly_count(device, length, new):
+    """A weight below what 32 bits hold is still no zero: the infinite value
+    that it weighs makes the sum infinite, in one tile as over many."""
+
+    for dtype in (torch.float16, torch.bfloat16):
+        batch = Batch(length, [length], [new], qh=2, kvh=1, dim=128, dtype=dtype, theta=None)
+        batch.query[:, :, 6] = 8.0
+        # scores of the first entries (a whole split, where there are some) lie about 300 below the others'
+        batch.keys[0][:, :, 6] = 0.0
+        batch.keys[0][: 300 if length > 2000 else 40, :, 6] = -425.0
+        batch.values[0][20, 0, 5] = float("inf")
+        batch.values[0][21, 0, 7] = float("-inf")
+        batch.write(0, batch.keys[0], batch.values[0])
+        out, _weights = odd_call(batch, device, False)
+        assert bool((out[:, :, 5] == float("inf")).all()) and bool((out[:, :, 7] == float("-inf")).all())
+        rest = [d for d in range(128) if d not in (5, 7)]
+        assert bool(out[:, :, rest].isfinite().all())

@@ -377,7 +377,7 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
 
   // ---- out, or this split's part of it ----
   if constexpr (W > 1) {
-    // the waves' sums meet in LDS, in the waves' order
+    // the waves' sums meet in LDS, in the waves' order (such sequences are not split)
 #pragma unroll
     for (int g = 0; g < RG; ++g) {
       const float lt = lanes4_sum(l[g]);
@@ -405,12 +405,6 @@ __global__ __launch_bounds__(64 * W, RG == 2 && D == 128 ? 1 : 2) void paged_few
       }
       const int32_t t = (int32_t)((uint32_t)r / (uint32_t)a.per), head = kvh * a.per + (r - t * a.per);
       const int64_t row = (int64_t)(s.row0 + t) * a.QH + head;
-      if (a.splits > 1) {
-        const int64_t at = (int64_t)split * a.c.N * a.QH + row;
-        if (part == 0) a.part_ml[at] = float2{top, lt};
-        *(float4v*)(a.part_o + at * D + 4 * part) = acc;
-        continue;
-      }
       const bool none = lt == 0.f;  // sees nothing
       if (part == 0) {
         const float l2 = none ? -INFINITY : (top == -INFINITY ? 0.f : top) + log2f(lt);

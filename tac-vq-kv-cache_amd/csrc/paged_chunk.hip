@@ -52,6 +52,23 @@ __device__ __forceinline__ float lanes2_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// BYTES a lane from the resource's `off` into LDS at `to` and on, lane after lane.
+// (Asm: for the builtin the compiler holds every LDS read back until all loads
+// have landed.  There are no result registers, and the callers' waits count these
+// loads.  M0 holds their place in LDS; a register that the compiler reserves
+// cannot be declared as changed, so it is left as it was.)
+template <int BYTES>
+__device__ __forceinline__ void load_to_lds(uint32_t to, uint32_t off, uint4v rsrc) {
+  static_assert(BYTES == 4 || BYTES == 16, "one or four words a lane");
+  uint32_t m0;
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "s"(to), "v"(off), "s"(rsrc) : "memory");
+  else
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "s"(to), "v"(off), "s"(rsrc) : "memory");
+}
+
 // Slot of 16-byte chunk j of row r in a tile: keys so that 16 rows' equal
 // chunks, values so that 4 rows' 64-byte groups, fall on distinct banks.
 template <int D> __device__ __forceinline__ int chunk_key_slot(int r, int j) {
@@ -151,11 +168,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
 
   // ---- tile loader: a wave's 8 or 16 entries lie in one page, and go from global
   // memory into LDS directly.  A page outside the pool and the entries at or
-  // behind the length lie beyond the resource's bound and land as zeros.  (The
-  // loads are asm: for the builtin the compiler holds every LDS read back until
-  // all of them have landed.  They have no result registers, and the waits below
-  // count them.  M0, their place in LDS, is set beside each: nothing else here
-  // uses it.) ----
+  // behind the length lie beyond the resource's bound and land as zeros. ----
   const int32_t* table = a.c.tables + b * a.c.table_stride;
   const int32_t mask = (1 << a.c.page_shift) - 1;
   const int lrow = lane / (64 / kRowsPerLoad), lslot = lane % (64 / kRowsPerLoad);
@@ -203,9 +216,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   auto load_tile = [&](uint4v rsrc, const uint32_t (&off)[kLoads], uint32_t to) {
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(to + (uint32_t)(kWaveRows * kRowBytes) * (uint32_t)wave + 1024u * j), "v"(off[j]), "s"(rsrc)
-                   : "memory");
+      load_to_lds<16>(to + (uint32_t)(kWaveRows * kRowBytes) * (uint32_t)wave + 1024u * j, off[j], rsrc);
   };
   auto load_values = [&](int32_t i, int stage) {
     load_tile(resource(i, v_head), v_off, lds_base + (2 * stage + 1) * kTileBytes);
@@ -579,10 +590,8 @@ __global__ __launch_bounds__(512, 2) void paged_chunk_weights_kernel(PagedAttnAr
     const uint4v norm_rsrc = {(uint32_t)norm_at, (uint32_t)(norm_at >> 32) & 0xffffu, 4u * (uint32_t)left, 0x00020000u};
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(lds_base + (uint32_t)(stage * kStageBytes + 1024 * (wave * kLoads + j))), "v"(off[j]), "s"(rsrc) : "memory");
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                 :: "s"(lds_address(norm_lds[stage][wave])), "v"(4u * (uint32_t)(32 * (wave / ENTRIES) + lane)), "s"(norm_rsrc) : "memory");
+      load_to_lds<16>(lds_base + (uint32_t)(stage * kStageBytes + 1024 * (wave * kLoads + j)), off[j], rsrc);
+    load_to_lds<4>(lds_address(norm_lds[stage][wave]), 4u * (uint32_t)(32 * (wave / ENTRIES) + lane), norm_rsrc);
   };
   typedef __attribute__((address_space(3))) const V8 lds_v8;
   uint32_t q_at[kSteps];

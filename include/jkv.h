@@ -736,10 +736,10 @@ int jkv_paged_select(const float* weights, int64_t weight_stride_b,
 
 /*
  * Copies row kept[b][h][j] of a sequence's key and value pages to entry j of
- * its new pages, which must not be pages that are read (an entry copied onto
- * itself is fine); negative entries copy nothing.  With `weights`, moved[b][h]
- * (contiguous [B,KVH,width]) receives their weights in the new order and 0
- * behind them.
+ * its new pages, which must not be pages that are read (an entry that stays
+ * where it is is neither read nor written); negative entries copy nothing.
+ * With `weights`, moved[b][h] (contiguous [B,KVH,width]) receives their weights
+ * in the new order and 0 behind them.
  */
 int jkv_paged_compact(void* key_pages, void* value_pages, int32_t dtype,
                       int64_t page_stride, int64_t head_stride,

@@ -315,7 +315,7 @@ def compact_pages(
     Entry ``kept[b,h,j]`` (int32 ``[B,KVH,budget]``, negative: nothing) of a
     sequence's pages becomes entry j of its ``new_tables`` row.  The new pages
     must be none that are read, of this or another sequence (other sequences
-    may share the old ones); an entry may be copied onto itself.  With
+    may share the old ones); an entry that stays where it is costs nothing.  With
     ``weights`` ``[B,KVH,C]`` returns those of the entries that stay, in their
     new order, zeros behind.
     """

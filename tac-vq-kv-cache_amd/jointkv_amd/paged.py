@@ -497,34 +497,46 @@ class PagedKVCache:
         all layers: the first ``sinks``, the last ``recent`` and those between
         that received most stay.  They move to free pages (what else reads the
         old ones, a shared prompt, is not disturbed) and the old pages are
-        freed."""
+        freed.  The pages of one sequence's ``budget`` have to be free; where
+        those of all do not fit, sequences follow one another into the pages
+        that the ones before left."""
 
         if self.weights is None:
             raise ValueError("the cache does not track weights")
         if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
             raise ValueError("the budget must be positive and hold the first and the last entries that stay")
         over = [b for b, length in enumerate(self._lengths) if length > budget]
-        if not over:
-            return
         each = -(-budget // self.page_size)
-        if each * len(over) > len(self._free):
-            raise ValueError(f"the eviction needs {each * len(over)} pages, {len(self._free)} are free")
+        if over and each > len(self._free):
+            raise ValueError(f"the eviction needs {each} pages, {len(self._free)} are free")
+        while over:  # (what a round frees is at least what it takes)
+            now = over[: len(self._free) // each]
+            self._evict(now, each, budget, sinks, recent)
+            over = over[len(now) :]
+
+    def _evict(self, over: list[int], each: int, budget: int, sinks: int, recent: int) -> None:
         taken = self._free[-each * len(over) :]
         pages = list(self._pages)
         for n, b in enumerate(over):
             pages[b] = taken[n * each : (n + 1) * each]
-        lengths, old_tables = self._on_device(self._lengths), self.block_tables.clone()
+        lengths = self._on_device([self._lengths[b] for b in over])
+        rows = self._on_device(over)
+        old_tables = self.block_tables.clone()
         try:
             self._upload(pages)
+            tables = [t.index_select(0, rows) for t in (old_tables, self.block_tables)]
             moved = []
             for layer, weights in enumerate(self.weights):
-                kept, _ = select_entries(weights, lengths, budget, sinks=sinks, recent=recent)
-                moved.append(compact_pages(self.key[layer], self.value[layer], old_tables, kept, self.block_tables,
-                                           weights=weights))
+                received = weights.index_select(0, rows)
+                kept, _ = select_entries(received, lengths, budget, sinks=sinks, recent=recent)
+                moved.append(compact_pages(self.key[layer], self.value[layer], tables[0], kept, tables[1],
+                                           weights=received))
+            rows = rows.long()
         except BaseException:
             self.block_tables.copy_(old_tables)  # nothing is taken: the old pages are as they were
             raise
-        torch._foreach_copy_(self.weights, moved)  # in their place: captured graphs hold them
+        for weights, left in zip(self.weights, moved):
+            weights.index_copy_(0, rows, left)  # in their place: captured graphs hold them
         del self._free[-each * len(over) :]
         for b in over:
             self._free.extend(reversed(self._pages[b]))

@@ -970,3 +970,35 @@ def test_infinite_values_of_entries_that_hardly_count(device, length, new):
         assert bool((out[:, :, 5] == float("inf")).all()) and bool((out[:, :, 7] == float("-inf")).all())
         rest = [d for d in range(128) if d not in (5, 7)]
         assert bool(out[:, :, rest].isfinite().all())
+
+
+def test_eviction_of_an_almost_full_pool_goes_round_by_round(device):
+    """Pages for one sequence's budget are free: three sequences follow one
+    another into them, with the same results as in a pool that takes all."""
+
+    kvh, qh, dim = 2, 4, 64
+    gen = torch.Generator().manual_seed(44)
+    caches = [jkv.PagedKVCache(2, 4, pages, kvh, max_length=128, page_size=16, head_dim=dim, track_weights=True,
+                               device=device) for pages in (7 + 4 + 5 + 1 + 2, 40)]
+    lengths = [100, 60, 70, 9]
+    prompt = [[torch.randn(sum(lengths), heads, dim, generator=gen).half().to(device) for heads in (kvh, kvh, qh)]
+              for _ in range(2)]
+    single = [[torch.randn(4, heads, dim, generator=gen).half().to(device) for heads in (kvh, kvh, qh)]
+              for _ in range(2)]
+    outs = []
+    for cache in caches:
+        step = cache.begin(lengths)
+        for layer, (k, v, q) in enumerate(prompt):
+            cache.append(layer, step, k, v)
+            cache.attention(layer, step, q)
+        cache.evict(32, sinks=2, recent=8)
+        assert cache.lengths == (32, 32, 32, 9) and cache.positions == (100, 60, 70, 9)
+        assert cache.free_pages == cache.key.shape[1] - 7
+        cache.release(0)  # (the next entries need pages)
+        step = cache.begin([1, 1, 1, 1])
+        for layer, (k, v, q) in enumerate(single):
+            cache.append(layer, step, k, v)
+            outs.append(cache.attention(layer, step, q))
+    assert torch.equal(torch.stack(outs[:2]), torch.stack(outs[2:]))
+    for few, many in zip(*(c.weights for c in caches)):
+        assert torch.equal(few, many)

@@ -166,6 +166,122 @@ def test_page_accounting():
     assert cache.lengths == (0, 2, 1) and cache.free_pages == 8 and cache.positions == (0, 2, 1)
 
 
+def _plain_eviction(monkeypatch, seen):
+    """Selection and compaction in plain form (the oracle's choice), for caches
+    on the host; ``seen`` collects the rows of each call."""
+
+    def select_entries(weights, lengths, budget, *, sinks, recent):
+        kept = torch.full((*weights.shape[:2], budget), -1, dtype=torch.int32)
+        for b, length in enumerate(lengths.tolist()):
+            for h in range(weights.shape[1]):
+                stay = ref.select(weights[b, h, :length].numpy(), budget, sinks, recent)
+                kept[b, h, : len(stay)] = torch.from_numpy(stay).int()
+        return kept, lengths.clamp(max=budget)
+
+    def compact_pages(key, value, tables, kept, new_tables, *, weights):
+        seen.append(tables.shape[0])
+        size, moved = key.shape[2], torch.zeros_like(weights)
+        for pool in (key, value):
+            before = pool.clone()
+            for b, h, j in (kept >= 0).nonzero().tolist():
+                e = int(kept[b, h, j])
+                pool[new_tables[b, j // size], h, j % size] = before[tables[b, e // size], h, e % size]
+                moved[b, h, j] = weights[b, h, e]
+        return moved
+
+    monkeypatch.setattr(jkv.paged, "select_entries", select_entries)
+    monkeypatch.setattr(jkv.paged, "compact_pages", compact_pages)
+
+
+def _filled(pages, lengths):
+    """A cache on the host whose entries hold their sequence and index."""
+
+    cache = _HostCache(2, len(lengths), pages, 2, max_length=100, page_size=16, head_dim=64, track_weights=True,
+                       device="cpu")
+    cache.key.zero_()
+    cache.value.zero_()
+    cache.begin(lengths)
+    gen = torch.Generator().manual_seed(len(lengths))
+    for layer in range(2):
+        for b, length in enumerate(lengths):
+            cache.weights[layer][b, :, :length] = torch.rand(2, length, generator=gen)
+            for j in range(length):
+                page = cache.block_tables[b, j // 16]
+                cache.key[layer][page, :, j % 16] = 1000 * b + j
+                cache.value[layer][page, :, j % 16] = -1000 * b - j
+    return cache
+
+
+def _entries(cache, layer, b):
+    """Keys, values and weights of a sequence: [KVH, length] each (one dim stands for all)."""
+
+    length = cache.lengths[b]
+    pages = cache.block_tables[b, : -(-length // 16)].long()
+    k, v = (pool[layer][pages].transpose(0, 1).reshape(2, -1, 64)[:, :length, 0] for pool in (cache.key, cache.value))
+    return k, v, cache.weights[layer][b, :, :length].clone()
+
+
+@pytest.mark.parametrize("spare", [2, 3, 4, 20])
+def test_eviction_touches_only_sequences_over_the_budget_and_reuses_pages(monkeypatch, spare):
+    """With pages for one sequence's budget free, or more: the same entries
+    stay, the others' pages and weights are not passed on at all."""
+
+    seen = []
+    _plain_eviction(monkeypatch, seen)
+    lengths = [70, 20, 33, 97, 0]
+    cache = _filled(5 + 2 + 3 + 7 + spare, lengths)
+    before = [[_entries(cache, layer, b) for b in range(5)] for layer in range(2)]
+    pages = cache.block_tables.clone()
+    cache.evict(30, sinks=2, recent=8)
+    assert cache.lengths == (30, 20, 30, 30, 0) and cache.positions == tuple(lengths)
+    assert cache.free_pages == 5 + 2 + 3 + 7 + spare - 4 * 2
+    assert sum(seen) == 2 * 3, "rows of sequences within the budget were passed on"
+    table = cache.block_tables.tolist()
+    used = [p for row in table for p in row if p >= 0]
+    assert len(set(used)) == len(used) == 8 and not set(used) & set(cache._free)
+    assert torch.equal(cache.block_tables[1], pages[1])
+    for layer in range(2):
+        for b, length in enumerate(lengths):
+            for h in range(2):
+                k, v, w = (x[h] for x in before[layer][b])
+                stay = torch.from_numpy(ref.select(w.numpy(), 30, 2, 8))
+                for got, want in zip(_entries(cache, layer, b), (k, v, w)):
+                    assert torch.equal(got[h], want[stay])
+                assert bool((cache.weights[layer][b, h, len(stay) :] == 0).all())
+
+
+def test_eviction_without_pages_for_one_budget_is_refused(monkeypatch):
+    _plain_eviction(monkeypatch, [])
+    cache = _filled(5 + 7 + 1, [70, 97])
+    before, weights = cache.block_tables.clone(), cache.weights[0].clone()
+    with pytest.raises(ValueError, match="needs 2 pages, 1 are free"):
+        cache.evict(30)
+    assert cache.lengths == (70, 97) and cache.free_pages == 1
+    assert torch.equal(cache.block_tables, before) and torch.equal(cache.weights[0], weights)
+
+
+def test_an_eviction_that_fails_leaves_the_cache_as_it_was(monkeypatch):
+    _plain_eviction(monkeypatch, [])
+    cache = _filled(5 + 7 + 4, [70, 97])
+    before, weights = cache.block_tables.clone(), [w.clone() for w in cache.weights]
+    entries = [_entries(cache, 1, b) for b in range(2)]
+    plain, calls = jkv.paged.select_entries, []
+
+    def failing(*args, **kwargs):
+        calls.append(1)
+        if len(calls) == 2:
+            raise RuntimeError("second layer")
+        return plain(*args, **kwargs)
+
+    monkeypatch.setattr(jkv.paged, "select_entries", failing)
+    with pytest.raises(RuntimeError, match="second layer"):
+        cache.evict(30)
+    assert cache.lengths == (70, 97) and cache.free_pages == 4 and torch.equal(cache.block_tables, before)
+    assert all(torch.equal(a, b) for a, b in zip(cache.weights, weights))
+    for b in range(2):
+        assert all(torch.equal(x, y) for x, y in zip(entries[b], _entries(cache, 1, b)))
+
+
 @pytest.mark.parametrize("change", [dict(layers=0), dict(head_dim=32), dict(page_size=24), dict(page_size=8),
                                     dict(dtype=torch.float32), dict(max_length=0)])
 def test_cache_refuses_geometry(change):

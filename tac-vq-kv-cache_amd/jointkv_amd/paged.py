@@ -411,6 +411,7 @@ class PagedKVCache:
         self._pages: list[list[int]] = [[] for _ in range(sequences)]
         self._lengths = [0] * sequences
         self._positions = [0] * sequences
+        self._begun: tuple | None = None  # the latest step's lengths tensor, and what it is taken back to
 
     @property
     def lengths(self) -> tuple[int, ...]:
@@ -442,7 +443,8 @@ class PagedKVCache:
 
     def begin(self, new_tokens: Sequence[int]) -> PagedStep:
         """Take pages for ``new_tokens[b]`` more entries of every sequence b
-        (0: none this step)."""
+        (0: none this step).  The entries count from here on: a step whose
+        appends or attention fail is taken back with :meth:`cancel`."""
 
         new = [int(n) for n in new_tokens]
         if len(new) != len(self._lengths) or any(n < 0 for n in new):
@@ -453,6 +455,7 @@ class PagedKVCache:
         more = [-(-a // self.page_size) - len(row) for a, row in zip(after, self._pages)]
         if sum(more) > len(self._free):
             raise ValueError(f"the step needs {sum(more)} pages, {len(self._free)} are free")
+        before = self._lengths, self._positions, self._pages
         if sum(more):
             free = iter(reversed(self._free))
             pages = [row + [next(free) for _ in range(n)] for row, n in zip(self._pages, more)]
@@ -467,8 +470,30 @@ class PagedKVCache:
         single = all(n == 1 for n in new)
         self._lengths = after
         self._positions = [p + n for p, n in zip(self._positions, new)]
-        return PagedStep(self.block_tables, ints[:batch], None if single else ints[2 * batch :],
+        step = PagedStep(self.block_tables, ints[:batch], None if single else ints[2 * batch :],
                          ints[batch : 2 * batch], starts[-1], max(new), max(after))
+        self._begun = (step.lengths, *before)
+        return step
+
+    def cancel(self, step: PagedStep) -> None:
+        """Take back ``step``, the latest one, before an eviction or release:
+        lengths, positions and pages are again those before it, and its own
+        entries' weights 0.  What its attention added to the weights of earlier
+        entries stays."""
+
+        if self._begun is None or step.lengths is not self._begun[0]:
+            raise ValueError("only the latest step can be taken back, before an eviction or release")
+        lengths, positions, pages = self._begun[1:]
+        taken = [page for old, now in zip(pages, self._pages) for page in now[len(old) :]]
+        if taken:
+            self._upload(pages)
+        if self.weights is not None:
+            for weights in self.weights:
+                for b, (old, now) in enumerate(zip(lengths, self._lengths)):
+                    if now > old:
+                        weights[b, :, old:now].zero_()
+        self._free.extend(reversed(taken))
+        self._lengths, self._positions, self._pages, self._begun = lengths, positions, pages, None
 
     def append(self, layer: int, step: PagedStep, key: torch.Tensor, value: torch.Tensor, *,
                rope_theta: float | None = MISTRAL_ROPE_THETA) -> None:
@@ -535,6 +560,7 @@ class PagedKVCache:
         except BaseException:
             self.block_tables.copy_(old_tables)  # nothing is taken: the old pages are as they were
             raise
+        self._begun = None
         for weights, left in zip(self.weights, moved):
             weights.index_copy_(0, rows, left)  # in their place: captured graphs hold them
         del self._free[-each * len(over) :]
@@ -546,6 +572,7 @@ class PagedKVCache:
     def release(self, sequence: int) -> None:
         """Drop a sequence: its pages are free and its slot empty."""
 
+        self._begun = None
         self._free.extend(reversed(self._pages[sequence]))
         self._pages[sequence] = []
         self._lengths[sequence] = self._positions[sequence] = 0

@@ -3,6 +3,8 @@ the host's page accounting, and what the C entry points refuse."""
 
 from __future__ import annotations
 
+import dataclasses
+
 import numpy as np
 import pytest
 import torch
@@ -280,6 +282,38 @@ def test_an_eviction_that_fails_leaves_the_cache_as_it_was(monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(cache.weights, weights))
     for b in range(2):
         assert all(torch.equal(x, y) for x, y in zip(entries[b], _entries(cache, 1, b)))
+
+
+def test_a_step_that_failed_is_taken_back(monkeypatch):
+    _plain_eviction(monkeypatch, [])
+    cache = _filled(20, [40, 16, 0])
+    tables, weights = cache.block_tables.clone(), [w.clone() for w in cache.weights]
+    state = cache.lengths, cache.positions, cache.free_pages, list(cache._free)
+    step = cache.begin([30, 1, 2])
+    assert cache.lengths == (70, 17, 2) and cache.free_pages == 20 - 5 - 2 - 1
+    with pytest.raises(ValueError, match="33 new tokens"):
+        cache.append(0, step, torch.zeros(32, 2, 64), torch.zeros(32, 2, 64))
+    for w in cache.weights:  # a layer's attention before the failure
+        w[0, :, 40:70] = 3.0
+    cache.cancel(step)
+    assert (cache.lengths, cache.positions, cache.free_pages, cache._free) == state
+    assert torch.equal(cache.block_tables, tables)
+    assert all(torch.equal(a, b) for a, b in zip(cache.weights, weights))
+    with pytest.raises(ValueError, match="latest step"):
+        cache.cancel(step)
+    # the same step again finds what the first one found
+    again = cache.begin([30, 1, 2])
+    for name in ("block_tables", "lengths", "starts", "positions"):
+        assert torch.equal(getattr(again, name), getattr(step, name))
+    with pytest.raises(ValueError, match="latest step"):
+        cache.cancel(step)
+    cache.cancel(dataclasses.replace(again, max_length=100))
+    assert (cache.lengths, cache.positions, cache.free_pages, cache._free) == state
+    for end in (lambda: cache.release(1), lambda: cache.evict(30)):
+        step = cache.begin([1, 0, 0])
+        end()
+        with pytest.raises(ValueError, match="before an eviction or release"):
+            cache.cancel(step)
 
 
 @pytest.mark.parametrize("change", [dict(layers=0), dict(head_dim=32), dict(page_size=24), dict(page_size=8),

@@ -56,7 +56,7 @@ def _rows(tensor: torch.Tensor) -> torch.Tensor:
 
     t, h, d = tensor.stride()
     if d != 1 or t % 8 or h % 8 or tensor.data_ptr() % 16:
-        return tensor.contiguous()
+        return tensor.clone(memory_format=torch.contiguous_format)  # (contiguous ones may be misaligned)
     return tensor
 
 

@@ -139,6 +139,18 @@ def test_operators_refuse_cpu_tensors():
         jkv.compact_pages(pages, pages, ints, torch.zeros(2, 2, 4, dtype=torch.int32), ints)
 
 
+@pytest.mark.parametrize("make", [
+    lambda: torch.arange(2 * 3 * 64 + 1).half()[1:].view(2, 3, 64), lambda: torch.zeros(2, 3, 65).half()[:, :, 1:],
+    lambda: torch.zeros(3, 2, 64).half().transpose(0, 1), lambda: torch.zeros(2, 64, 3).half().transpose(1, 2),
+    lambda: torch.zeros(2, 3, 68).half()[:, :, :64], lambda: torch.zeros(1, 64).half().expand(2, 3, 64)])
+def test_rows_are_aligned_or_copied(make):
+    rows = make()
+    got = jkv.paged._rows(rows)
+    t, h, d = got.stride()
+    assert got.data_ptr() % 16 == 0 and d == 1 and t % 8 == 0 and h % 8 == 0
+    assert torch.equal(got, rows)
+
+
 class _HostCache(jkv.PagedKVCache):
     def _on_device(self, values):
         return torch.tensor(values, dtype=torch.int32)

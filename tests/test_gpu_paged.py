@@ -1002,3 +1002,125 @@ def test_eviction_of_an_almost_full_pool_goes_round_by_round(device):
     assert torch.equal(torch.stack(outs[:2]), torch.stack(outs[2:]))
     for few, many in zip(*(c.weights for c in caches)):
         assert torch.equal(few, many)
+
+
+# ---- how exact the few-row and the weighing kernels are, and the kernels of larger calls ----
+
+
+def check_parts(out, expect, dtype, p_parts):
+    """As :func:`check_out` for a q in two 16-bit parts, and a p in ``p_parts``
+    of them.  Two parts hold a number to h^2 of itself: 2^-16 in bf16; in fp16
+    2^-22, or 2^-25 for parts that are subnormal, which the rotation's sine and
+    cosine (2^-20) and these queries' sizes keep under 2^-18.  The outputs' own
+    rounding is off by h / sqrt(3) of a number's power of two, 0.39 h of its size
+    where mantissas spread evenly over their logarithm; a p of one part would
+    bring as much again, 0.55 h in all."""
+
+    h, slack = half_step(dtype), 2.0 ** -20
+    part = 2.0 ** -16 if dtype == torch.bfloat16 else 2.0 ** -18
+    got = out.detach().double().cpu().numpy()
+    want = np.concatenate([e["out"] for e in expect])
+    spread = np.concatenate([e["spread"] for e in expect])
+    reach = np.concatenate([e["reach"] for e in expect])[..., None]
+    p_error = h if p_parts == 1 else part
+    tol = h * np.abs(want) + spread * (p_error + np.expm1(2 * (part + slack) * reach) + slack) * (1 + h)
+    err = np.abs(got - want)
+    worst = np.unravel_index(np.argmax(err - tol), err.shape)
+    assert (err <= tol + float(torch.finfo(dtype).tiny)).all(), f"error {err[worst]} over {tol[worst]} at {worst}"
+    rel = np.linalg.norm(err) / np.linalg.norm(want)
+    assert rel <= (0.45 if p_parts == 2 else 0.65) * h, f"relative error {rel / h} h"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("length,new,qh,window,sinks", [
+    (100, 1, 32, None, 0), (200, 1, 32, None, 0), (900, 1, 32, None, 0), (9000, 1, 32, None, 0), (900, 1, 32, 300, 40),
+    (100, 5, 8, None, 0), (200, 5, 8, None, 0), (900, 5, 8, None, 0), (9000, 8, 8, 5000, 3)])
+def test_few_rows_keep_queries_and_weights_in_two_parts(device, length, new, qh, dim, window, sinks, dtype):
+    """In one wave, in waves that join, in splits, in one and two groups of rows:
+    what is left is the output's rounding."""
+
+    batch = Batch(length + new, [length], [new], qh=qh, kvh=2, dim=dim, page=64, dtype=dtype)
+    out = jkv.paged_attention(batch.query.to(device), **batch.on(device), window=window, sinks=sinks, max_new=new,
+                              max_length=length)
+    check_parts(out, batch.expect(window, sinks), dtype, 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("length,new,dim", [(400, 90, 128), (300, 300, 64), (5000, 64, 64)])
+def test_chunks_that_weigh_keep_queries_in_two_parts(device, length, new, dim, dtype):
+    batch = Batch(length + new, [length], [new], qh=4, kvh=2, dim=dim, page=64, dtype=dtype)
+    expect = batch.expect(None, 0)
+    query, args = batch.query.to(device), batch.on(device)
+    lse = torch.empty(new, 4, device=device)
+    weights = torch.empty(1, 2, length, device=device)
+    for more in (dict(lse=lse), dict(weights=weights)):
+        out = jkv.paged_attention(query, **args, window=None, max_new=new, max_length=length, **more)
+        check_parts(out, expect, dtype, 1)
+
+
+def check_some_heads(device, batch, groups, window, sinks):
+    """Output, weights and log-sum-exps of a larger call, with weights and
+    without, for the kv heads ``groups`` (the oracle takes a row at a time)."""
+
+    per, length = batch.qh // batch.kvh, max(batch.lengths)
+    query, args = batch.query.to(device), batch.on(device)
+    weights = torch.full((len(batch.lengths), batch.kvh, length), 7.0, device=device)
+    lse = torch.empty(len(query), batch.qh, device=device)
+    bounds = dict(window=window, sinks=sinks, max_new=max(batch.new), max_length=length)
+    plain = jkv.paged_attention(query, **args, **bounds)
+    exact = jkv.paged_attention(query, **args, **bounds, weights=weights, lse=lse)
+    for g in groups:
+        heads = slice(per * g, per * g + per)
+        expect = [ref.attend(q[:, heads].double().numpy(), k[:, g : g + 1].double().numpy(),
+                             v[:, g : g + 1].double().numpy(), p, window=window, sinks=sinks, theta=batch.theta)
+                  for q, k, v, p in zip(batch.queries, batch.keys, batch.values, batch.positions)]
+        check_out(plain[:, heads], expect, batch.dtype)
+        check_parts(exact[:, heads], expect, batch.dtype, 1)
+        check_weights(weights[:, g : g + 1], expect, batch.lengths)
+        want = np.concatenate([e["lse"] for e in expect])
+        reach = np.concatenate([e["reach"] for e in expect])
+        got = lse[:, heads].double().cpu().numpy()
+        assert (np.abs(got - want) <= 2.0 ** -17 * reach + 2.0 ** -19 * (1 + np.abs(want))).all()
+    for b, n in enumerate(batch.lengths):
+        assert bool((weights[b, :, n:] == 7.0).all()), "weights behind the last entry were written"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (700, 20)])
+def test_blocks_of_eight_waves(device, window, sinks, dtype):
+    """Two ragged chunks of 32 groups of two heads: 256 blocks of 256 rows, one
+    a CU, whose last ones hold 232 and 132 rows; weights of 128 entries a
+    workgroup, whose last ones hold 76 and 4."""
+
+    batch = Batch(61, [1100, 900], [500, 450], qh=64, kvh=32, dim=128, page=64, dtype=dtype)
+    check_some_heads(device, batch, (0, 13, 31), window, sinks)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_blocks_that_are_resident_at_once_run_in_folded_order(device, dim):
+    """Prompts of unlike lengths, one of them idle, in blocks of 128 rows: between
+    one and two workgroups a CU, and more row blocks than the order keeps from
+    the front."""
+
+    batch = Batch(62, [300, 17, 9, 257], [300, 17, 0, 257], qh=64, kvh=64, dim=dim, page=16)
+    check_some_heads(device, batch, (0, 40, 63), None, 0)
+
+
+def test_the_second_walk_of_eight_waves_changes_only_what_is_infinite(device):
+    """An infinite value in blocks of 256 rows: the dim that holds it becomes
+    infinite, the others keep every bit."""
+
+    batch = Batch(61, [1100, 900], [500, 450], qh=64, kvh=32, dim=128, page=64)
+    query = batch.query.to(device)
+    weights = [torch.zeros(2, 32, 1100, device=device) for _ in range(2)]
+    bounds = dict(window=None, max_new=500, max_length=1100)
+    clean = [jkv.paged_attention(query, **batch.on(device), **bounds, weights=w) for w in (None, weights[0])]
+    batch.values[0][100, 4, 77] = float("-inf")
+    batch.write(0, batch.keys[0][:101], batch.values[0][:101])
+    odd = [jkv.paged_attention(query, **batch.on(device), **bounds, weights=w) for w in (None, weights[1])]
+    for was, now in zip(clean, odd):
+        assert bool((now[:500, 8:10, 77] == float("-inf")).all())
+        now[:500, 8:10, 77] = was[:500, 8:10, 77]
+        assert torch.equal(was, now)
+    assert torch.equal(*weights)

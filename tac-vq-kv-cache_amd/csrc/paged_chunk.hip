@@ -11,16 +11,18 @@
 // sum take one swap.  O^T[dim][row] += V^T P^T takes P from those registers,
 // 4 entries of each of two groups of 8 a lane, and V^T by transposing reads of
 // the row-major tile in the same order.  Online softmax in 32 bits; p and the
-// rotated, scaled q enter the products rounded once to the cache's type (that is
-// 2^-9 of a bf16 weight and up to as much of a score: the output is 0.3 % off
-// where its own rounding alone is 0.17 %; two parts of each would double the
-// products), except that with EXACT (weights or log-sum-exps are asked for) q is
-// a sum of two parts.
+// rotated, scaled q enter the products rounded once to the cache's type: up to
+// 2^-8 of a bf16 weight and of a score's terms.  The output is 0.30 % off where
+// its own rounding alone is 0.17 % (fp16 0.041 and 0.021).  A second part of q
+// would bring 0.23 % for half as many products again: 2 x 2,048 bf16 tokens over
+// 16,384 entries 894 -> 1,200 us, ragged fp16 chunks of 777 62 -> 72; one of p
+// too, the output's own rounding for twice the products.  With EXACT, where weights
+// or log-sum-exps are asked for (they would show it), q is a sum of two parts.
 //
-// 2 x 2,048 bf16 tokens over 16,384 entries, 32/8 heads of 128: 852 us, 1.21
-// PFLOP/s (a large matrix product reaches 1.30).  Per tile and wave 32 products
-// (1,024 cycles of its SIMD) stand beside about 210 vector instructions (1,000)
-// and 32 KiB of LDS reads; two waves a SIMD overlap a third of them.  Measured
+// 2 x 2,048 bf16 tokens over 16,384 entries, 32/8 heads of 128: 852 to 892 us on
+// different cards, 1.15 to 1.21 PFLOP/s (a large matrix product reaches 1.26 to
+// 1.30).  Of its cycles the products fill 61 %, vector instructions 46 %, both at
+// once 22 %, and the products' power holds the clock at 1.76 GHz.  Measured
 // without gain: three and four stages of tiles, wave priorities around the
 // products, the next tile's loads behind the scores (1,720 us: they take a whole
 // tile's time to come).

@@ -201,12 +201,16 @@ def paged_attention(
     Returns ``[N,QH,D]`` (``out``, if given).  Rows that no sequence owns are
     left as they were; a token with no entry to see (a length below the number
     of new tokens) gets zeros and an ``lse`` of ``-inf``; a page number outside
-    the pool reads as zeros.  A call repeats bit for bit; how the work is
+    the pool reads as zeros.  Infinite and NaN keys and values count for the rows
+    that see them alone: a score of -infinity weighs nothing, an infinite value
+    makes its dim infinite.  A call repeats bit for bit; how the work is
     divided follows from the sizes and bounds, so a row may differ in its last
-    bits between calls of other ones.  Single tokens and small chunks (tokens
-    times heads of a group at most 32) keep 32-bit scores and weights; larger
-    chunks round the rotated queries and the weights once to the pages' type
-    before the matrix products, the queries not where ``weights`` or ``lse``
+    bits between calls of other ones.  Calls whose ``max_new`` times the heads of
+    a group is at most 32 (steps of single tokens, small chunks) keep queries and
+    weights in two 16-bit parts before the matrix products, 2^-17 of each or
+    better.  All sequences of other calls, single tokens among them, have both
+    rounded once to the pages' type; ask for ``lse`` to keep the queries in two
+    parts there (a sixth to a third slower), as they are where ``weights``
     are asked for.
     """
 

@@ -50,8 +50,8 @@ __device__ __forceinline__ float lanes4_sum(float v) {
 }
 
 // A part's factor against the largest maximum.  Never 0: a part may hold an
-// infinite value (to finite sums 2^-126 of them adds nothing).
-__device__ __forceinline__ float part_factor(float m, float top) { return fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-126f); }
+// infinite value (2^-149 of the largest finite one is 5e-7).
+__device__ __forceinline__ float part_factor(float m, float top) { return fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-149f); }
 
 // Slot of 16-byte chunk j of row r in a tile: keys so that 16 rows' equal
 // chunks, values so that 8 rows' equal chunk pairs, fall on distinct banks.

@@ -1124,3 +1124,23 @@ def test_the_second_walk_of_eight_waves_changes_only_what_is_infinite(device):
         now[:500, 8:10, 77] = was[:500, 8:10, 77]
         assert torch.equal(was, now)
     assert torch.equal(*weights)
+
+
+@pytest.mark.parametrize("length", [250, 3000])
+def test_parts_that_hardly_count_add_nothing(device, length):
+    """Huge finite values in splits whose weights 32 bits do not hold."""
+
+    batch = Batch(length, [length], [1], qh=2, kvh=1, dim=128, dtype=torch.bfloat16, theta=None)
+    batch.query[:, :, 6] = 8.0
+    batch.queries = [batch.query]
+    low = 300 if length > 2000 else 40
+    batch.keys[0][:, :, 6] = 0.0
+    batch.keys[0][:low, :, 6] = -425.0
+    # (a split's sums hold up to 2^14 weights' worth of them)
+    batch.values[0][:low, :, 9] = 2.0 ** 100
+    batch.write(0, batch.keys[0], batch.values[0])
+    expect = batch.expect(None, 0)
+    for e in expect:  # what is left of them in 64 bits is below 1e-90
+        assert np.abs(e["out"]).max() < 10
+    out, _weights = odd_call(batch, device, False)
+    check_out(out, expect, torch.bfloat16)

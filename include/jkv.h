@@ -711,6 +711,74 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                         int32_t accumulate, void* workspace,
                         int64_t workspace_bytes, jkv_stream_t stream);
 
+/*
+ * The same with shaped scores.  Score s (scale included) of a token at entry i
+ * and entry j becomes softcap * tanh(s / softcap) (softcap 0.001 to 1024, within
+ * 2e-7 of it; 0: as it is), then slopes[head] * |i - j| is taken off (fp32 [QH];
+ * NULL: none), and the first prefixes[b] entries (int32 [B]; NULL: none) are
+ * visible to all new tokens of sequence b, also to those before them.
+ * Workspace: jkv_paged_attention_workspace_bytes().
+ */
+int jkv_paged_attention_shaped(const void* q, int64_t q_stride_t,
+                        int64_t q_stride_h, int32_t dtype, const void* key_pages,
+                        const void* value_pages, int64_t page_stride,
+                        int64_t head_stride, int64_t slot_stride,
+                        int64_t n_pages, int64_t page_size,
+                        const int32_t* block_tables, int64_t table_stride,
+                        int64_t table_width, const int32_t* lengths,
+                        const int32_t* starts, const int32_t* positions,
+                        int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D,
+                        int64_t max_new, int64_t max_length, int64_t window,
+                        int64_t sinks, double rope_theta, float scale, void* out,
+                        int64_t out_stride_t, int64_t out_stride_h, float* lse,
+                        float* weights, int64_t weight_stride_b,
+                        int64_t weight_stride_h, int64_t weight_width,
+                        int32_t accumulate, float softcap, const float* slopes,
+                        const int32_t* prefixes, void* workspace,
+                        int64_t workspace_bytes, jkv_stream_t stream);
+
+/*
+ * Attention inside sequences packed one behind another, without a cache: row i
+ * of sequence b (rows [starts[b], starts[b+1])) sees its rows j with j <= i or j <
+ * prefixes[b], and j > i - window (window 0: all) or j < sinks.  Scores as in
+ * jkv_paged_attention_shaped.  Rows that no sequence owns get zeros and an lse
+ * of -inf.
+ *   q, out       [N,QH,D], k, v [N,KVH,D] of JKV_F16 or JKV_BF16, D 64 or 128,
+ *                element strides of token and head (multiples of 8, a token's
+ *                below 2^22), 16-byte aligned; queries and keys turned already
+ *   starts       int32 [B+1] device, not decreasing
+ *   lse          fp32 [N,QH] contiguous or NULL: natural log of each row's sum
+ */
+int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                         const void* k, int64_t k_stride_t, int64_t k_stride_h,
+                         const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                         int32_t dtype, const int32_t* starts,
+                         const int32_t* prefixes, int64_t N, int64_t B,
+                         int64_t QH, int64_t KVH, int64_t D, int64_t window,
+                         int64_t sinks, float scale, float softcap,
+                         const float* slopes, void* out, int64_t out_stride_t,
+                         int64_t out_stride_h, float* lse, jkv_stream_t stream);
+
+/*
+ * Its gradients: d_q [N,QH,D], d_k and d_v [N,KVH,D], contiguous, of the inputs'
+ * type (fp32 sums, one rounding), each NULL if not wanted.  o and lse are the
+ * forward's, d_out the gradient of o.  Rows that no sequence owns get 0.  Every
+ * sum has one order.
+ *   workspace    jkv_packed_backward_workspace_bytes() bytes, 16-byte aligned
+ */
+int jkv_packed_attention_backward(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+    int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+    int64_t v_stride_h, const void* o, int64_t o_stride_t, int64_t o_stride_h,
+    const void* d_out, int64_t d_stride_t, int64_t d_stride_h, const float* lse,
+    int32_t dtype, const int32_t* starts, const int32_t* prefixes, int64_t N,
+    int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t window, int64_t sinks,
+    float scale, float softcap, const float* slopes, void* d_q, void* d_k,
+    void* d_v, void* workspace, int64_t workspace_bytes, jkv_stream_t stream);
+
+/* Workspace of jkv_packed_attention_backward (bytes). */
+int64_t jkv_packed_backward_workspace_bytes(int64_t N, int64_t QH);
+
 /* Workspace of jkv_paged_attention for these sizes (bytes; 0 for sizes that it
  * refuses). */
 int64_t jkv_paged_attention_workspace_bytes(int64_t N, int64_t B, int64_t QH,
@@ -751,6 +819,46 @@ int jkv_paged_compact(void* key_pages, void* value_pages, int32_t dtype,
                       const float* weights, int64_t weight_stride_b,
                       int64_t weight_stride_h, int64_t width, float* moved,
                       jkv_stream_t stream);
+
+/*
+ * Copies rows [0, entries[i]) (all heads; entries NULL: whole pages) of page
+ * sources[i] to page targets[i], keys and values, in every layer: what a forked
+ * sequence needs before it writes to a page that it shares.  Targets must all
+ * be different and none a source.  Page numbers outside the pool copy nothing;
+ * a page onto itself is left as it is.
+ *   pages        pools as above, layers of them layer_stride elements apart
+ *   sources, targets, entries  int32 [pairs], device
+ */
+int jkv_paged_copy(void* key_pages, void* value_pages, int32_t dtype,
+                   int64_t layers, int64_t layer_stride, int64_t page_stride,
+                   int64_t head_stride, int64_t slot_stride, int64_t n_pages,
+                   int64_t page_size, int64_t KVH, int64_t D,
+                   const int32_t* sources, const int32_t* targets,
+                   const int32_t* entries, int64_t pairs, jkv_stream_t stream);
+
+/*
+ * Queries and keys turned at their positions (rotary embedding), one launch.
+ * Pair i of a head's first `dims` dims, (i, i + dims/2) or with side_by_side
+ * (2i, 2i + 1), turns by position * rates[i] radians (64-bit products), times
+ * `magnitude`; with `inverse` by the negative angle, which is the gradient.
+ * The other dims are copied.  Products in fp32, one rounding.
+ *   q, q_out     [N,QH,D], k, k_out [N,KVH,D] of dtype JKV_F16, JKV_BF16 or
+ *                JKV_F32, D even and at most 256, element strides of token and
+ *                head; an output may be its input.  QH or KVH may be 0.
+ *   rates        host, dims/2 doubles
+ *   starts       int32 [B+1] device, not decreasing, or NULL: rows [starts[b],
+ *                starts[b+1]) are sequence b, its first at position positions[b]
+ *                (NULL: 0).  Rows that no sequence owns are copied.
+ *   positions    without starts: int32 [N], each row's (NULL: its number)
+ */
+int jkv_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, void* q_out,
+               int64_t q_out_stride_t, int64_t q_out_stride_h, int64_t QH,
+               const void* k, int64_t k_stride_t, int64_t k_stride_h, void* k_out,
+               int64_t k_out_stride_t, int64_t k_out_stride_h, int64_t KVH,
+               int32_t dtype, int64_t N, int64_t D, int64_t dims,
+               int32_t side_by_side, const double* rates, double magnitude,
+               int32_t inverse, const int32_t* starts, int64_t B,
+               const int32_t* positions, jkv_stream_t stream);
 
 /* fp32 -> fp16 copy (the deploy round trip tables.half()), n elements. */
 int jkv_f32_to_f16(const float* src, void* dst, int64_t n, jkv_stream_t stream);

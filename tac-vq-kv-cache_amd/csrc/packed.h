@@ -1,0 +1,33 @@
+// What the kernels over packed sequences without pages share.
+#pragma once
+
+#include "paged.h"
+
+namespace jkv {
+
+// What the kernels of the attention's gradients share.  Strides in bytes; dq, dk
+// and dv are contiguous.
+struct PackedGradArgs {
+  const uint8_t *q, *k, *v, *o, *d;
+  int64_t qst, qsh, kst, ksh, vst, vsh, ost, osh, dst, dsh;
+  uint8_t *dq, *dk, *dv;  // null: not wanted
+  const int32_t *starts, *prefixes;
+  const float* lse;
+  int32_t N, B, QH, KVH, per, window, sinks;
+  float scale, scale2, cap_mul, cap2;
+  const float* slopes;
+  float2* stats;   // [QH][N]: base-2 log-sum-exp less 10, rowsum(do o)
+  float2* maxima;  // [kGradBlocks]: largest finite |do| and |v| (fp16)
+  int32_t items;   // row blocks of all sequences at most
+};
+static const int kGradBlocks = 512;  // workgroups of the rows' pass
+
+// launches of the gradients: the rows' sums, then dk and dv, then dq
+int packed_grad_launch_f16(const PackedGradArgs& a, int form, int64_t D, hipStream_t stream);
+int packed_grad_launch_bf16(const PackedGradArgs& a, int form, int64_t D, hipStream_t stream);
+
+// launches of the attention; all but the type is in the arguments
+void packed_launch_f16(const PagedAttnArgs& a, int form, int64_t D, hipStream_t stream);
+void packed_launch_bf16(const PagedAttnArgs& a, int form, int64_t D, hipStream_t stream);
+
+}  // namespace jkv

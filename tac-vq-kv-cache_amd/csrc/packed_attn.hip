@@ -1,0 +1,142 @@
+// Attention inside sequences that lie packed one behind another, keys and values
+// beside the queries: prompts without a cache, and training.
+//
+// Sequence b owns rows starts[b] to starts[b+1]; its row i sees its row j where
+// (j <= i or j < prefix) and (j > i - window or j < sinks):
+//   x_ij = cap tanh(scale q_i k_j / cap) - slope |i - j|,  p = softmax_j(x),  o_i = sum_j p_ij v_j
+// Here: a call's checks and the division of its work.  The kernel is the paged
+// chunks' one (chunk_attn.h) over rows in place of pages.
+#include <math.h>
+
+#include <algorithm>
+
+#include "packed.h"
+
+namespace jkv {
+
+static int packed_checks(int32_t dtype, int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t window, int64_t sinks,
+                         float scale) {
+  JKV_CHECK_ARG(dtype == JKV_F16 || dtype == JKV_BF16, "packed attention takes fp16 or bf16, got dtype %d", dtype);
+  JKV_CHECK_ARG(D == 64 || D == 128, "packed attention supports head_dim 64 and 128, got %lld", (long long)D);
+  JKV_CHECK_ARG(QH > 0 && KVH > 0 && QH % KVH == 0 && QH < 65536, "query heads must be a multiple of kv heads");
+  JKV_CHECK_ARG(N >= 0 && N < ((int64_t)1 << 30) && B >= 0 && B < ((int64_t)1 << 24), "too many rows or sequences");
+  JKV_CHECK_ARG(N * QH < ((int64_t)1 << 31) - 256, "too many rows");
+  JKV_CHECK_ARG(window >= 0 && sinks >= 0, "window and sinks must not be negative");
+  JKV_CHECK_ARG(fabsf(scale) < 1e30f, "the softmax scale must be finite and below 1e30");
+  return JKV_OK;
+}
+
+// token and head strides of 16-bit rows
+static int packed_strides(const int64_t* strides, int count) {
+  for (int i = 0; i < count; ++i)
+    JKV_CHECK_ARG(strides[i] % 8 == 0 && strides[i] >= 0 && strides[i] < (i % 2 ? (int64_t)1 << 40 : (int64_t)1 << 22),
+                  "token and head strides must be multiples of 8 elements, a token's below 2^22");
+  return JKV_OK;
+}
+
+}  // namespace jkv
+
+extern "C" {
+
+int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                         int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, int32_t dtype,
+                         const int32_t* starts, const int32_t* prefixes, int64_t N, int64_t B, int64_t QH, int64_t KVH,
+                         int64_t D, int64_t window, int64_t sinks, float scale, float softcap, const float* slopes,
+                         void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse, jkv_stream_t stream_) {
+  using namespace jkv;
+  int rc = packed_checks(dtype, N, B, QH, KVH, D, window, sinks, scale);
+  if (rc != JKV_OK) return rc;
+  const int64_t strides[8] = {q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, out_stride_t, out_stride_h};
+  rc = packed_strides(strides, 8);
+  if (rc != JKV_OK) return rc;
+  PagedAttnArgs a = {};
+  int form;
+  rc = paged_form_args(&a, &form, scale, softcap, slopes, prefixes);
+  if (rc != JKV_OK) return rc;
+  if (form == kFormPlain) {
+    form = kFormShaped;
+    a.q_mul = 1.f;
+    a.scale2 = scale * 1.4426950408889634f;
+  }
+  if (N == 0) return JKV_OK;
+  JKV_CHECK_ARG(q && k && v && out && starts, "null buffer");
+  JKV_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 == 0, "packed rows must be 16-byte aligned");
+  a.c.k = (uint8_t*)k; a.c.v = (uint8_t*)v;
+  a.c.head_bytes = 2 * k_stride_h; a.c.slot_bytes = 2 * k_stride_t;
+  a.v_head_bytes = 2 * v_stride_h; a.v_slot_bytes = 2 * v_stride_t;
+  a.c.starts = starts;
+  a.c.N = (int32_t)N; a.c.B = (int32_t)B;
+  a.q = (const uint8_t*)q; a.qst = 2 * q_stride_t; a.qsh = 2 * q_stride_h;
+  a.out = (uint8_t*)out; a.ost = 2 * out_stride_t; a.osh = 2 * out_stride_h;
+  a.lse = lse;
+  a.QH = (int32_t)QH; a.KVH = (int32_t)KVH; a.per = (int32_t)(QH / KVH);
+  a.window = (int32_t)(window > 0 && window < kPagedMost ? window : kPagedMost);
+  a.sinks = (int32_t)(sinks < kPagedMost ? sinks : kPagedMost);
+  a.max_new = (int32_t)N;
+  a.splits = 1;
+  // blocks of all sequences at most, and one that clears unowned rows
+  auto blocks_of = [&](int64_t rows) { return std::min<int64_t>(B * ceil_div(N * a.per, rows), N * a.per / rows + B) + 1; };
+  a.item_rows = D == 128 && blocks_of(256) * KVH / 256 >= 2 ? 256 : 128;
+  const int64_t items = blocks_of(a.item_rows);
+  JKV_CHECK_GRID(items * KVH, 2 * a.item_rows);
+  a.items = (int32_t)items;
+  // (where all blocks are resident at once, two a CU, long ones share a CU with short ones)
+  a.fold = a.item_rows == 128 && items * KVH > 256 && items * KVH <= 512 ? (int32_t)(256 / KVH) : 0x7fffffff;
+  hipStream_t stream = (hipStream_t)stream_;
+  if (dtype == JKV_F16) packed_launch_f16(a, form, D, stream);
+  else packed_launch_bf16(a, form, D, stream);
+  JKV_CHECK_LAUNCH();
+  return JKV_OK;
+}
+
+int64_t jkv_packed_backward_workspace_bytes(int64_t N, int64_t QH) {
+  if (N <= 0 || QH <= 0 || N * QH >= ((int64_t)1 << 31)) return 0;
+  return jkv::ceil_div(N * QH * 8, 256) * 256 + jkv::kGradBlocks * 8;
+}
+
+int jkv_packed_attention_backward(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                                  int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                                  const void* o, int64_t o_stride_t, int64_t o_stride_h, const void* d_out,
+                                  int64_t d_stride_t, int64_t d_stride_h, const float* lse, int32_t dtype,
+                                  const int32_t* starts, const int32_t* prefixes, int64_t N, int64_t B, int64_t QH,
+                                  int64_t KVH, int64_t D, int64_t window, int64_t sinks, float scale, float softcap,
+                                  const float* slopes, void* d_q, void* d_k, void* d_v, void* workspace,
+                                  int64_t workspace_bytes, jkv_stream_t stream_) {
+  using namespace jkv;
+  int rc = packed_checks(dtype, N, B, QH, KVH, D, window, sinks, scale);
+  if (rc != JKV_OK) return rc;
+  const int64_t strides[10] = {q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t,
+                               v_stride_h, o_stride_t, o_stride_h, d_stride_t, d_stride_h};
+  rc = packed_strides(strides, 10);
+  if (rc != JKV_OK) return rc;
+  PagedAttnArgs shape = {};
+  int form;
+  rc = paged_form_args(&shape, &form, scale, softcap, slopes, prefixes);
+  if (rc != JKV_OK) return rc;
+  if (N == 0) return JKV_OK;
+  JKV_CHECK_ARG(q && k && v && o && d_out && lse && starts, "null buffer");
+  JKV_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)d_out | (uintptr_t)d_q | (uintptr_t)d_k |
+                 (uintptr_t)d_v) % 16 == 0, "packed rows must be 16-byte aligned");
+  const int64_t need = jkv_packed_backward_workspace_bytes(N, QH);
+  JKV_CHECK_ARG(workspace != nullptr && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need,
+                "packed gradients need an aligned workspace of %lld bytes, got %lld", (long long)need, (long long)workspace_bytes);
+  PackedGradArgs a = {};
+  a.q = (const uint8_t*)q; a.k = (const uint8_t*)k; a.v = (const uint8_t*)v; a.o = (const uint8_t*)o; a.d = (const uint8_t*)d_out;
+  a.qst = 2 * q_stride_t; a.qsh = 2 * q_stride_h; a.kst = 2 * k_stride_t; a.ksh = 2 * k_stride_h;
+  a.vst = 2 * v_stride_t; a.vsh = 2 * v_stride_h; a.ost = 2 * o_stride_t; a.osh = 2 * o_stride_h;
+  a.dst = 2 * d_stride_t; a.dsh = 2 * d_stride_h;
+  a.dq = (uint8_t*)d_q; a.dk = (uint8_t*)d_k; a.dv = (uint8_t*)d_v;
+  a.starts = starts; a.prefixes = prefixes; a.lse = lse;
+  a.N = (int32_t)N; a.B = (int32_t)B; a.QH = (int32_t)QH; a.KVH = (int32_t)KVH; a.per = (int32_t)(QH / KVH);
+  a.window = (int32_t)(window > 0 && window < kPagedMost ? window : kPagedMost);
+  a.sinks = (int32_t)(sinks < kPagedMost ? sinks : kPagedMost);
+  a.scale = scale; a.scale2 = scale * 1.4426950408889634f;
+  a.cap_mul = shape.cap_mul; a.cap2 = shape.cap2; a.slopes = slopes;
+  a.stats = (float2*)workspace;
+  a.maxima = (float2*)((uint8_t*)workspace + ceil_div(N * QH * 8, 256) * 256);
+  if (form == kFormPlain) form = kFormShaped;
+  return dtype == JKV_F16 ? packed_grad_launch_f16(a, form, D, (hipStream_t)stream_)
+                          : packed_grad_launch_bf16(a, form, D, (hipStream_t)stream_);
+}
+
+}  // extern "C"

@@ -1,0 +1,32 @@
+// Attention of packed sequences without pages, bf16.  The kernel is in chunk_attn.h.
+#include "chunk_attn.h"
+#include "packed.h"
+
+namespace jkv {
+
+template <int D, int FORM>
+static void launch_packed(const PagedAttnArgs& a, hipStream_t stream) {
+  const dim3 grid((uint32_t)((int64_t)a.items * a.KVH)), block((uint32_t)(2 * a.item_rows));
+  if constexpr (D == 128) {
+    if (a.item_rows == 256) {
+      hipLaunchKernelGGL((paged_chunk_kernel<JKV_BF16, D, false, 8, FORM, true>), grid, block, 0, stream, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((paged_chunk_kernel<JKV_BF16, D, false, 4, FORM, true>), grid, block, 0, stream, a);
+}
+
+void packed_launch_bf16(const PagedAttnArgs& a, int form, int64_t D, hipStream_t stream) {
+  switch (form) {
+    case kFormShaped: return D == 128 ? launch_packed<128, kFormShaped>(a, stream) : launch_packed<64, kFormShaped>(a, stream);
+    case kFormShaped | kFormCap:
+      return D == 128 ? launch_packed<128, kFormShaped | kFormCap>(a, stream) : launch_packed<64, kFormShaped | kFormCap>(a, stream);
+    case kFormShaped | kFormBias:
+      return D == 128 ? launch_packed<128, kFormShaped | kFormBias>(a, stream) : launch_packed<64, kFormShaped | kFormBias>(a, stream);
+    default:
+      return D == 128 ? launch_packed<128, kFormShaped | kFormCap | kFormBias>(a, stream)
+                      : launch_packed<64, kFormShaped | kFormCap | kFormBias>(a, stream);
+  }
+}
+
+}  // namespace jkv

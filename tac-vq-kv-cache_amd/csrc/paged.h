@@ -122,8 +122,46 @@ struct PagedAttnArgs {
   float* lse2;      // [KVH][N][per] base-2 log-sum-exps for the weights, or null
   float* scores;    // few rows with weights: [B,KVH,max_new*per,score_width] base-2 scores, or null
   int64_t score_width;
+  // what becomes of a score before its softmax (see ScoreShape), base 2
+  float cap_mul, cap2;      // 2 scale log2(e) / cap and cap log2(e), or 0
+  const float* slopes;      // [QH] a unit of distance, or null
+  const int32_t* prefixes;  // [B] first entries that all of a sequence's rows see, or null
+  int64_t v_head_bytes, v_slot_bytes;  // of values that lie without pages
   uint8_t* q_parts;  // chunks with weights: [KVH][N][per] rotated queries, D of their leading and D of their trailing parts
 };
+
+// A score's form (a bit each; plain: the kernels without any of these).
+enum { kFormPlain = 0, kFormShaped = 1, kFormCap = 2, kFormBias = 4 };
+
+// A shaped score is cap * tanh(scale q k / cap) - slope * distance, in base 2.
+// With E = exp(2x), tanh x = 1 - 2 / (1 + E): two transcendental instructions of
+// 7 cycles each and three others, where a rational function of x^2 as exact
+// would take eleven of 2 and a reciprocal.  Of a cap c it is within 2e-7 c, and
+// right at infinite scores.
+struct ScoreShape {
+  float mul, cap2, twice, slope2;
+};
+template <int FORM, typename Args> __device__ __forceinline__ ScoreShape score_shape(const Args& a, int32_t head) {
+  ScoreShape s = {};
+  if constexpr (FORM != kFormPlain) {
+    s.mul = FORM & kFormCap ? a.cap_mul : a.scale2;
+    s.cap2 = a.cap2;
+    s.twice = -2.f * a.cap2;
+    if constexpr (FORM & kFormBias) s.slope2 = a.slopes[head] * 1.4426950408889634f;
+  }
+  return s;
+}
+template <int FORM> __device__ __forceinline__ float shape_score(const ScoreShape& s, float x, float distance) {
+  x *= s.mul;
+  if constexpr (FORM & kFormCap) x = fmaf(s.twice, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x)), s.cap2);
+  if constexpr (FORM & kFormBias) x = fmaf(-s.slope2, fabsf(distance), x);
+  return x;
+}
+
+// the first entries that all rows of a sequence see
+__device__ __forceinline__ int32_t paged_prefix(const int32_t* prefixes, int32_t b, int32_t length) {
+  return prefixes != nullptr ? clamp_i32(prefixes[b], 0, length) : 0;
+}
 
 // where lse2 holds row n * QH + head
 __device__ __forceinline__ int64_t paged_lse2_at(int32_t N, int32_t per, int64_t row, int32_t QH) {
@@ -138,6 +176,8 @@ static const int32_t kPagedMost = 0x3fffffff;  // entries of a sequence: sums of
 int paged_launch_few(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
 int paged_launch_few_weights(const PagedAttnArgs& a, hipStream_t stream);
 int paged_launch_chunk(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
+int paged_launch_form_f16(const PagedAttnArgs& a, int form, bool few, int64_t D, hipStream_t stream);
+int paged_launch_form_bf16(const PagedAttnArgs& a, int form, bool few, int64_t D, hipStream_t stream);
 int paged_launch_join(const PagedAttnArgs& a, int32_t dtype, int64_t D, hipStream_t stream);
 
 // The tiles of `size` entries that rows at entries first..last may see: `lead`
@@ -225,5 +265,6 @@ int paged_cache_args(PagedCache* c, const void* k, const void* v, int64_t page_s
                      const int32_t* positions, int64_t N, int64_t B, int64_t KVH, int64_t D, int64_t max_length,
                      int32_t dtype);
 int paged_rope_args(RopeRates* r, double theta, int64_t D);
+int paged_form_args(PagedAttnArgs* a, int* form, float scale, float softcap, const float* slopes, const int32_t* prefixes);
 
 }  // namespace jkv

@@ -125,6 +125,25 @@ static PagedPlan paged_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64
   return p;
 }
 
+// what becomes of a score: the form's bits and what its kernels take
+int paged_form_args(PagedAttnArgs* a, int* form, float scale, float softcap, const float* slopes, const int32_t* prefixes) {
+  *form = kFormPlain;
+  // (a capped score is within 2e-7 of the cap)
+  JKV_CHECK_ARG(softcap == 0.f || (softcap >= 1e-3f && softcap <= 1024.f), "a cap must be from 0.001 to 1024, or 0 for none");
+  if (softcap == 0.f && slopes == nullptr && prefixes == nullptr) return JKV_OK;
+  *form = kFormShaped | (softcap > 0.f ? kFormCap : 0) | (slopes != nullptr ? kFormBias : 0);
+  a->slopes = slopes;
+  a->prefixes = prefixes;
+  // a rotated fp16 query reaches sqrt 2 of its size
+  a->q_mul = a->rope.on ? 0.5f : 1.f;
+  a->scale2 = scale * 1.4426950408889634f / a->q_mul;
+  if (softcap > 0.f) {
+    a->cap_mul = 2.f * a->scale2 / softcap;
+    a->cap2 = softcap * 1.4426950408889634f;
+  }
+  return JKV_OK;
+}
+
 }  // namespace jkv
 
 extern "C" {
@@ -141,15 +160,16 @@ int64_t jkv_paged_attention_workspace_bytes(int64_t N, int64_t B, int64_t QH, in
                          window > 0 && window < most ? window : most, std::min(sinks, most), with_weights != 0).bytes;
 }
 
-int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, int32_t dtype, const void* key_pages,
+int jkv_paged_attention_shaped(const void* q, int64_t q_stride_t, int64_t q_stride_h, int32_t dtype, const void* key_pages,
                         const void* value_pages, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
                         int64_t n_pages, int64_t page_size, const int32_t* block_tables, int64_t table_stride,
                         int64_t table_width, const int32_t* lengths, const int32_t* starts, const int32_t* positions,
                         int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t max_new, int64_t max_length,
                         int64_t window, int64_t sinks, double rope_theta, float scale, void* out, int64_t out_stride_t,
                         int64_t out_stride_h, float* lse, float* weights, int64_t weight_stride_b,
-                        int64_t weight_stride_h, int64_t weight_width, int32_t accumulate, void* workspace,
-                        int64_t workspace_bytes, jkv_stream_t stream_) {
+                        int64_t weight_stride_h, int64_t weight_width, int32_t accumulate, float softcap,
+                        const float* slopes, const int32_t* prefixes, void* workspace, int64_t workspace_bytes,
+                        jkv_stream_t stream_) {
   using namespace jkv;
   hipStream_t stream = (hipStream_t)stream_;
   PagedAttnArgs a = {};
@@ -170,6 +190,9 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   JKV_CHECK_ARG(((uintptr_t)q | (uintptr_t)out) % 16 == 0, "queries and outputs must be 16-byte aligned");
   max_length = a.c.top;
   JKV_CHECK_ARG(weights == nullptr || weight_width >= max_length, "weights have fewer entries than max_length");
+  int form;
+  rc = paged_form_args(&a, &form, scale, softcap, slopes, prefixes);
+  if (rc != JKV_OK) return rc;
   if (B == 0) return JKV_OK;
   a.QH = (int32_t)QH; a.KVH = (int32_t)KVH; a.per = (int32_t)(QH / KVH);
   a.weights = weights; a.wsb = weight_stride_b; a.wsh = weight_stride_h; a.accumulate = accumulate;
@@ -192,11 +215,13 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   a.out = (uint8_t*)out; a.ost = 2 * out_stride_t; a.osh = 2 * out_stride_h;
   a.lse = lse;
   a.max_new = (int32_t)max_new;
-  a.q_mul = scale * 1.4426950408889634f;
-  a.scale2 = 1.f;
-  while (fabsf(a.q_mul) > 0.5f) {
-    a.q_mul *= 0.5f;
-    a.scale2 *= 2.f;
+  if (form == kFormPlain) {
+    a.q_mul = scale * 1.4426950408889634f;
+    a.scale2 = 1.f;
+    while (fabsf(a.q_mul) > 0.5f) {
+      a.q_mul *= 0.5f;
+      a.scale2 *= 2.f;
+    }
   }
   a.splits = (int32_t)p.splits; a.split_tiles = (int32_t)p.split_tiles;
   a.items = (int32_t)p.items;
@@ -212,7 +237,26 @@ int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, i
     if (p.few) a.scores = (float*)(ws + p.scores_at);
     else a.q_parts = ws + p.q_at;
   }
+  if (form != kFormPlain)
+    return dtype == JKV_F16 ? paged_launch_form_f16(a, form, p.few, D, stream) : paged_launch_form_bf16(a, form, p.few, D, stream);
   return p.few ? paged_launch_few(a, dtype, D, stream) : paged_launch_chunk(a, dtype, D, stream);
+}
+
+int jkv_paged_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, int32_t dtype, const void* key_pages,
+                        const void* value_pages, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                        int64_t n_pages, int64_t page_size, const int32_t* block_tables, int64_t table_stride,
+                        int64_t table_width, const int32_t* lengths, const int32_t* starts, const int32_t* positions,
+                        int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t max_new, int64_t max_length,
+                        int64_t window, int64_t sinks, double rope_theta, float scale, void* out, int64_t out_stride_t,
+                        int64_t out_stride_h, float* lse, float* weights, int64_t weight_stride_b,
+                        int64_t weight_stride_h, int64_t weight_width, int32_t accumulate, void* workspace,
+                        int64_t workspace_bytes, jkv_stream_t stream) {
+  return jkv_paged_attention_shaped(q, q_stride_t, q_stride_h, dtype, key_pages, value_pages, page_stride, head_stride,
+                                    slot_stride, n_pages, page_size, block_tables, table_stride, table_width, lengths,
+                                    starts, positions, N, B, QH, KVH, D, max_new, max_length, window, sinks, rope_theta,
+                                    scale, out, out_stride_t, out_stride_h, lse, weights, weight_stride_b,
+                                    weight_stride_h, weight_width, accumulate, 0.f, nullptr, nullptr, workspace,
+                                    workspace_bytes, stream);
 }
 
 }  // extern "C"

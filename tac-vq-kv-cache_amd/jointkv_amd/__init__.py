@@ -37,6 +37,7 @@ from .closed_loop_vq import (
 )
 from .cq_tac import ClosedLoopGroupedCQ, hard_grouped_cq
 from .gain_shape import fit_residual_stages
+from .packed import packed_attention
 from .packed_nested import (
     PackedLayoutLedger,
     PackedNestedKVCache,
@@ -51,7 +52,8 @@ from .packed_nested import (
     unpack_paired_progressive_indices,
     validate_packed_nested_cache,
 )
-from .paged import PagedKVCache, PagedStep, compact_pages, paged_append, paged_attention, select_entries
+from .paged import PagedKVCache, PagedStep, compact_pages, copy_pages, paged_append, paged_attention, select_entries
+from .rotary_rule import RotaryRule, rotary
 from .uniform_depth_tac import ClosedLoopUniformResidualVQ
 from .v_only import ClosedLoopRunContext, DecoderStack, causal_loss, run_loss, v_only_step
 
@@ -75,10 +77,12 @@ __all__ = [
     "PagedKVCache",
     "PagedStep",
     "QuantizedKV",
+    "RotaryRule",
     "StorageLedger",
     "clip_codebook_gradients",
     "closed_loop_attention",
     "compact_pages",
+    "copy_pages",
     "decode_attention",
     "decode_attention_window",
     "deploy_tables",
@@ -92,6 +96,7 @@ __all__ = [
     "hard_residual_vq_exits",
     "pack_fixed_width",
     "pack_paired_progressive_indices",
+    "packed_attention",
     "paged_append",
     "paged_attention",
     "prefill_attention",
@@ -100,6 +105,7 @@ __all__ = [
     "prefix_index_bits",
     "relative_trajectory_attention_mse",
     "residual_vq_ledger",
+    "rotary",
     "run_loss",
     "select_entries",
     "sgd_step",

@@ -148,6 +148,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f64, _f32, _vp, _i64, _i64, _vp,
          _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp],
     ),
+    "jkv_paged_attention_shaped": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+         _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f64, _f32, _vp, _i64, _i64, _vp,
+         _vp, _i64, _i64, _i64, _i32, _f32, _vp, _vp, _vp, _i64, _vp],
+    ),
+    "jkv_packed_attention": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _f32, _f32, _vp, _vp, _i64, _i64, _vp, _vp],
+    ),
+    "jkv_packed_attention_backward": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _vp,
+         _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    ),
+    "jkv_packed_backward_workspace_bytes": (_i64, [_i64, _i64]),
     "jkv_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32]),
     "jkv_paged_select": (
         ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
@@ -155,6 +172,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64,
          _vp, _i64, _i64, _i64, _vp, _vp],
+    ),
+    "jkv_paged_copy": (
+        ctypes.c_int,
+        [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp],
+    ),
+    "jkv_rotary": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _i64, _i64,
+         _i64, _i32, _vp, _f64, _i32, _vp, _i64, _vp, _vp],
     ),
 }
 

@@ -7,6 +7,7 @@ on the current HIP stream.  Nothing here computes on the CPU.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from typing import Sequence
@@ -32,6 +33,30 @@ def _plain(like: torch.Tensor):
     if type(like) is torch.Tensor:
         return like.new_empty
     return functools.partial(torch.empty, dtype=like.dtype, device=like.device)
+
+
+_NO_CHANGE = contextlib.nullcontext()
+
+
+def _current(device: torch.device):
+    """The device's own context where another device is current."""
+
+    if torch._C._cuda_getDevice() == device.index:
+        return _NO_CHANGE
+    return torch.cuda.device(device)
+
+
+def _overlaps(tensor: torch.Tensor) -> bool:
+    """Whether two elements of ``tensor`` share memory (strides that nest)."""
+
+    if tensor.is_contiguous():
+        return False
+    span = 1
+    for stride, extent in sorted(zip(tensor.stride(), tensor.shape)):
+        if extent > 1 and stride < span:
+            return True
+        span = max(span, stride * extent)
+    return False
 
 
 def rvq_encode(

@@ -11,6 +11,8 @@ many sequences share one pool of pages:
   visible, and can sum up the softmax weight that every entry received;
 * :func:`select_entries` and :func:`compact_pages` drop the entries that
   received least;
+* :func:`copy_pages` copies pages in all layers, what a forked sequence needs
+  before it writes to one that it shares;
 * :class:`PagedKVCache` keeps the pages, tables and lengths of a model's
   layers.
 
@@ -27,28 +29,17 @@ through :func:`jointkv_amd.prefill_attention`).
 
 from __future__ import annotations
 
-import contextlib
 from dataclasses import dataclass
 from typing import Sequence
 
 import torch
 
 from . import _lib
-from ._ops import _plain
+from ._ops import _current, _overlaps, _plain
 from .attention import MISTRAL_ROPE_THETA, MISTRAL_WINDOW
+from .rotary_rule import RotaryRule, rotary
 
 PAGE_TYPES = (torch.float16, torch.bfloat16)
-
-
-_NO_CHANGE = contextlib.nullcontext()
-
-
-def _current(device: torch.device):
-    """The device's own context where another device is current."""
-
-    if torch._C._cuda_getDevice() == device.index:
-        return _NO_CHANGE
-    return torch.cuda.device(device)
 
 
 def _rows(tensor: torch.Tensor) -> torch.Tensor:
@@ -58,19 +49,6 @@ def _rows(tensor: torch.Tensor) -> torch.Tensor:
     if d != 1 or t % 8 or h % 8 or tensor.data_ptr() % 16:
         return tensor.clone(memory_format=torch.contiguous_format)  # (contiguous ones may be misaligned)
     return tensor
-
-
-def _overlaps(tensor: torch.Tensor) -> bool:
-    """Whether two elements of ``tensor`` share memory (strides that nest)."""
-
-    if tensor.is_contiguous():
-        return False
-    span = 1
-    for stride, extent in sorted(zip(tensor.stride(), tensor.shape)):
-        if extent > 1 and stride < span:
-            return True
-        span = max(span, stride * extent)
-    return False
 
 
 def _pool_args(key_pages: torch.Tensor, value_pages: torch.Tensor, written: bool) -> tuple:
@@ -118,6 +96,24 @@ def _theta(rope_theta: float | None) -> float:
     if not rope_theta > 0.0:
         raise ValueError("the rotary base must be positive")
     return float(rope_theta)
+
+
+def _shape_args(softcap, slopes, prefixes, heads: int, batch: int) -> tuple:
+    """What becomes of scores, checked: (cap or 0, slopes, prefixes)."""
+
+    if softcap is not None and not 1e-3 <= softcap <= 1024.0:
+        raise ValueError("a cap must be from 0.001 to 1024")
+    if slopes is not None:
+        if slopes.dtype != torch.float32 or slopes.shape != (heads,):
+            raise ValueError("slopes must be fp32 [QH]")
+        if slopes.requires_grad:
+            raise ValueError("slopes have no gradient")
+        slopes = slopes.contiguous()
+    if prefixes is not None:
+        if prefixes.dtype != torch.int32 or prefixes.shape != (batch,):
+            raise ValueError("prefixes must be int32 [B]")
+        prefixes = prefixes.contiguous()
+    return 0.0 if softcap is None else float(softcap), slopes, prefixes
 
 
 def paged_append(
@@ -180,6 +176,9 @@ def paged_attention(
     accumulate: bool = False,
     lse: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
+    softcap: float | None = None,
+    slopes: torch.Tensor | None = None,
+    prefixes: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Attention of new tokens over the cached entries of their sequences.
 
@@ -198,6 +197,15 @@ def paged_attention(
     ``accumulate``, stored without; entries behind are left as they were.
     ``lse`` (fp32 ``[N,QH]``) receives each row's log-sum-exp.
 
+    ``softcap`` c (0.001 to 1024) bends a score s, scale included, to
+    ``c tanh(s / c)`` (within 2e-7 c).  ``slopes`` (fp32 ``[QH]``) then takes
+    ``slopes[h] |i - j|`` off it, the distance counted in entries, so not of
+    sequences that had entries evicted.  ``prefixes`` (int32 ``[B]``): the first
+    ``prefixes[b]`` entries are visible to all new tokens of sequence b, also to
+    those before them (what a window hides stays hidden).  With any of the
+    three, scores are scaled in 32 bits behind the product, so queries that come
+    rotated (``rope_theta=None``) enter it as they are.
+
     Returns ``[N,QH,D]`` (``out``, if given).  Rows that no sequence owns are
     left as they were; a token with no entry to see (a length below the number
     of new tokens) gets zeros and an ``lse`` of ``-inf``; a page number outside
@@ -215,7 +223,7 @@ def paged_attention(
     """
 
     device = _lib.require_device(query, key_pages, value_pages, block_tables, lengths, starts, positions, weights,
-                                 lse, out)
+                                 lse, out, slopes, prefixes)
     strides, heads, dim = _pool_args(key_pages, value_pages, written=False)
     if query.ndim != 3 or query.dtype != key_pages.dtype:
         raise ValueError("queries must be [N,QH,D] of the pages' type and dims")
@@ -254,6 +262,10 @@ def paged_attention(
         raise ValueError("out must match the queries, with contiguous 16-byte aligned rows")
     elif _overlaps(out):
         raise ValueError("an out that is written must not overlap")
+    shaped = softcap is not None or slopes is not None or prefixes is not None
+    if shaped:
+        softcap, slopes, prefixes = _shape_args(softcap, slopes, prefixes, qheads, batch)
+        shape_args = (softcap, _lib.ptr(slopes), _lib.ptr(prefixes))
     query = _rows(query)
     span = 0 if window is None else min(int(window), 0x7fffffff)
     sinks = min(int(sinks), 0x7fffffff)
@@ -261,12 +273,14 @@ def paged_attention(
         ws_bytes = _lib.workspace_bytes("jkv_paged_attention_workspace_bytes", rows, batch, qheads, heads, dim, max_new,
                                         max_length, span, sinks, int(weights is not None))
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
-        _lib.check(_lib.load().jkv_paged_attention(
+        lib = _lib.load()
+        _lib.check((lib.jkv_paged_attention_shaped if shaped else lib.jkv_paged_attention)(
             query.data_ptr(), query.stride(0), query.stride(1), _lib.dtype_code(query.dtype), key_pages.data_ptr(),
             value_pages.data_ptr(), *strides, *table, lengths.data_ptr(), _lib.ptr(starts), _lib.ptr(positions), rows,
             batch, qheads, heads, dim, max_new, max_length, span, sinks, _theta(rope_theta),
             dim ** -0.5 if scale is None else float(scale), out.data_ptr(), out.stride(0), out.stride(1),
-            _lib.ptr(lse), *weight_args, int(accumulate), _lib.ptr(workspace), ws_bytes, _lib.stream_handle(device)))
+            _lib.ptr(lse), *weight_args, int(accumulate), *(shape_args if shaped else ()), _lib.ptr(workspace), ws_bytes,
+            _lib.stream_handle(device)))
     return out
 
 
@@ -351,6 +365,48 @@ def compact_pages(
     return moved
 
 
+def copy_pages(
+    key_pages: torch.Tensor,
+    value_pages: torch.Tensor,
+    sources: torch.Tensor,
+    targets: torch.Tensor,
+    *,
+    entries: torch.Tensor | None = None,
+) -> None:
+    """Copy pages ``sources`` (int32 ``[P]``) to pages ``targets`` of the same
+    pools, keys and values.
+
+    ``key_pages``/``value_pages`` ``[pages,KVH,page_size,D]`` or, for all layers
+    in one call, ``[layers,pages,KVH,page_size,D]``.  ``entries`` (int32 ``[P]``)
+    counts the slots of each page that hold something; the others are not
+    copied.  The targets must all be different and none a source.  A page
+    number outside the pool copies nothing.
+    """
+
+    device = _lib.require_device(key_pages, value_pages, sources, targets, entries)
+    layers, layer_stride = 1, 0
+    if key_pages.ndim == 5:
+        if key_pages.shape != value_pages.shape or key_pages.stride() != value_pages.stride():
+            raise ValueError("key and value pages must be of one shape, with identical strides")
+        if _overlaps(key_pages) or _overlaps(value_pages):
+            raise ValueError("pages that are written must not overlap")
+        layers, layer_stride = key_pages.shape[0], key_pages.stride(0)
+        if layers == 0:
+            return
+        key_pages, value_pages = key_pages[0], value_pages[0]
+    strides, heads, dim = _pool_args(key_pages, value_pages, written=True)
+    for t in (sources, targets, entries):
+        if t is not None and (t.dtype != torch.int32 or t.ndim != 1 or t.shape != sources.shape):
+            raise ValueError("sources, targets and entries must be int32 [P]")
+    sources, targets = sources.contiguous(), targets.contiguous()
+    entries = None if entries is None else entries.contiguous()
+    with _current(device):
+        _lib.check(_lib.load().jkv_paged_copy(
+            key_pages.data_ptr(), value_pages.data_ptr(), _lib.dtype_code(key_pages.dtype), layers, layer_stride,
+            *strides, heads, dim, sources.data_ptr(), targets.data_ptr(), _lib.ptr(entries), sources.shape[0],
+            _lib.stream_handle(device)))
+
+
 @dataclass(frozen=True)
 class PagedStep:
     """One step's sequences as the kernels take them: every layer of the step
@@ -370,6 +426,13 @@ class PagedStep:
     max_length: int
 
 
+def _turned(tensor: torch.Tensor, rule: RotaryRule, step: PagedStep) -> torch.Tensor:
+    """A step's keys or queries at their positions."""
+
+    with torch.no_grad():
+        return rotary(tensor, rule=rule, starts=step.starts, positions=step.positions)
+
+
 class PagedKVCache:
     """Pages, tables and lengths of a model's layers for up to ``sequences``
     sequences at once.
@@ -380,6 +443,8 @@ class PagedKVCache:
     ``begin([new tokens of each sequence])``, then per layer ``append`` and
     ``attention``.  With ``track_weights`` attention adds up what every entry
     receives, and :meth:`evict` brings sequences down to a budget by it.
+    :meth:`fork` lets a sequence go on from another's entries, in pages that
+    both share until one of them writes.
     """
 
     def __init__(
@@ -412,6 +477,7 @@ class PagedKVCache:
         self.weights = ([torch.zeros(sequences, kv_heads, max_length, dtype=torch.float32, device=device)
                          for _ in range(layers)] if track_weights else None)
         self._free = list(range(pages - 1, -1, -1))
+        self._uses = [0] * pages  # sequences that list a page
         self._pages: list[list[int]] = [[] for _ in range(sequences)]
         self._lengths = [0] * sequences
         self._positions = [0] * sequences
@@ -445,10 +511,20 @@ class PagedKVCache:
         width = self.block_tables.shape[1]
         self.block_tables.copy_(self._on_device([row + [-1] * (width - len(row)) for row in rows]))
 
+    def _drop(self, row: list[int]) -> None:
+        """A sequence lists these pages no more: those that none lists are free."""
+
+        for page in reversed(row):
+            self._uses[page] -= 1
+            if not self._uses[page]:
+                self._free.append(page)
+
     def begin(self, new_tokens: Sequence[int]) -> PagedStep:
         """Take pages for ``new_tokens[b]`` more entries of every sequence b
         (0: none this step).  The entries count from here on: a step whose
-        appends or attention fail is taken back with :meth:`cancel`."""
+        appends or attention fail is taken back with :meth:`cancel`.  A
+        sequence that would write to a page that others share gets a copy of it
+        first, in every layer (a page more than its entries need)."""
 
         new = [int(n) for n in new_tokens]
         if len(new) != len(self._lengths) or any(n < 0 for n in new):
@@ -457,15 +533,38 @@ class PagedKVCache:
         if max(after) > self.max_length:
             raise ValueError(f"a sequence would have {max(after)} entries, the cache holds {self.max_length}")
         more = [-(-a // self.page_size) - len(row) for a, row in zip(after, self._pages)]
-        if sum(more) > len(self._free):
-            raise ValueError(f"the step needs {sum(more)} pages, {len(self._free)} are free")
+        # half-written last pages that another sequence still reads: whoever
+        # writes first, until one is left, takes a copy
+        uses, copied = {}, []
+        for b, (length, n, row) in enumerate(zip(self._lengths, new, self._pages)):
+            if n and length % self.page_size:
+                page = row[-1]
+                count = uses.get(page, self._uses[page])
+                if count > 1:
+                    uses[page] = count - 1
+                    copied.append(b)
+        if sum(more) + len(copied) > len(self._free):
+            raise ValueError(f"the step needs {sum(more) + len(copied)} pages, {len(self._free)} are free")
         before = self._lengths, self._positions, self._pages
-        if sum(more):
-            free = iter(reversed(self._free))
-            pages = [row + [next(free) for _ in range(n)] for row, n in zip(self._pages, more)]
+        left = [self._pages[b][-1] for b in copied]
+        taken = self._free[: -sum(more) - len(copied) - 1 : -1]
+        if taken:
+            free = iter(taken)
+            pages = list(self._pages)
+            for b in copied:
+                pages[b] = pages[b][:-1] + [next(free)]
+            pages = [row + [next(free) for _ in range(n)] for row, n in zip(pages, more)]
+            if copied:
+                held = [self._lengths[b] % self.page_size for b in copied]
+                ints = self._on_device(left + taken[: len(copied)] + held).view(3, -1)
+                copy_pages(self.key, self.value, ints[0], ints[1], entries=ints[2])
             self._upload(pages)
             self._pages = pages
-            del self._free[-sum(more) :]
+            del self._free[-len(taken) :]
+            for page in left:
+                self._uses[page] -= 1
+            for page in taken:
+                self._uses[page] = 1
         starts = [0]
         for n in new:
             starts.append(starts[-1] + n)
@@ -476,7 +575,7 @@ class PagedKVCache:
         self._positions = [p + n for p, n in zip(self._positions, new)]
         step = PagedStep(self.block_tables, ints[:batch], None if single else ints[2 * batch :],
                          ints[batch : 2 * batch], starts[-1], max(new), max(after))
-        self._begun = (step.lengths, *before)
+        self._begun = (step.lengths, *before, taken, left)
         return step
 
     def cancel(self, step: PagedStep) -> None:
@@ -487,8 +586,7 @@ class PagedKVCache:
 
         if self._begun is None or step.lengths is not self._begun[0]:
             raise ValueError("only the latest step can be taken back, before an eviction or release")
-        lengths, positions, pages = self._begun[1:]
-        taken = [page for old, now in zip(pages, self._pages) for page in now[len(old) :]]
+        lengths, positions, pages, taken, left = self._begun[1:]
         if taken:
             self._upload(pages)
         if self.weights is not None:
@@ -497,29 +595,44 @@ class PagedKVCache:
                     if now > old:
                         weights[b, :, old:now].zero_()
         self._free.extend(reversed(taken))
+        for page in taken:
+            self._uses[page] = 0
+        for page in left:
+            self._uses[page] += 1
         self._lengths, self._positions, self._pages, self._begun = lengths, positions, pages, None
 
     def append(self, layer: int, step: PagedStep, key: torch.Tensor, value: torch.Tensor, *,
-               rope_theta: float | None = MISTRAL_ROPE_THETA) -> None:
-        """The step's packed ``[tokens,KVH,D]`` keys and values into ``layer``'s pages."""
+               rope_theta: float | None = MISTRAL_ROPE_THETA, rule: RotaryRule | None = None) -> None:
+        """The step's packed ``[tokens,KVH,D]`` keys and values into ``layer``'s
+        pages.  With a ``rule`` the keys turn by it (:func:`jointkv_amd.rotary`)
+        in place of ``rope_theta``."""
 
         if key.shape[0] != step.tokens:
             raise ValueError(f"the step has {step.tokens} new tokens, got {key.shape[0]}")
+        if rule is not None:
+            key, rope_theta = _turned(key, rule, step), None
         paged_append(key, value, self.key[layer], self.value[layer], step.block_tables, step.lengths,
                      starts=step.starts, positions=step.positions, rope_theta=rope_theta)
 
     def attention(self, layer: int, step: PagedStep, query: torch.Tensor, *, window: int | None = MISTRAL_WINDOW,
                   sinks: int = 0, rope_theta: float | None = MISTRAL_ROPE_THETA,
-                  scale: float | None = None) -> torch.Tensor:
+                  scale: float | None = None, rule: RotaryRule | None = None, softcap: float | None = None,
+                  slopes: torch.Tensor | None = None, prefixes: torch.Tensor | None = None) -> torch.Tensor:
         """:func:`paged_attention` of the step's packed queries over ``layer``,
-        adding to its weights if the cache tracks them."""
+        adding to its weights if the cache tracks them.  With a ``rule`` the
+        queries turn by it in place of ``rope_theta``."""
 
         if query.shape[0] != step.tokens:
             raise ValueError(f"the step has {step.tokens} new tokens, got {query.shape[0]}")
+        if (slopes is not None or prefixes is not None) and self._lengths != self._positions:
+            raise ValueError("distances and prefixes count entries: not of sequences that had some evicted")
+        if rule is not None:
+            query, rope_theta = _turned(query, rule, step), None
         return paged_attention(query, self.key[layer], self.value[layer], step.block_tables, step.lengths,
                                starts=step.starts, positions=step.positions, window=window, sinks=sinks,
                                rope_theta=rope_theta, scale=scale, max_new=step.max_new, max_length=step.max_length,
-                               weights=None if self.weights is None else self.weights[layer], accumulate=True)
+                               weights=None if self.weights is None else self.weights[layer], accumulate=True,
+                               softcap=softcap, slopes=slopes, prefixes=prefixes)
 
     def evict(self, budget: int, *, sinks: int = 0, recent: int = 0) -> None:
         """Bring every sequence of more than ``budget`` entries down to it, in
@@ -536,12 +649,21 @@ class PagedKVCache:
             raise ValueError("the budget must be positive and hold the first and the last entries that stay")
         over = [b for b, length in enumerate(self._lengths) if length > budget]
         each = -(-budget // self.page_size)
-        if over and each > len(self._free):
-            raise ValueError(f"the eviction needs {each} pages, {len(self._free)} are free")
-        while over:  # (what a round frees is at least what it takes)
-            now = over[: len(self._free) // each]
-            self._evict(now, each, budget, sinks, recent)
+        # (a round frees what it takes and more, but for pages that others list)
+        rounds, free, uses = [], len(self._free), {}
+        while over:
+            now = over[: free // each]
+            if not now:
+                raise ValueError(f"the eviction needs {each} pages, {free} are free")
+            free -= each * len(now)
+            for b in now:
+                for page in self._pages[b]:
+                    uses[page] = uses.get(page, self._uses[page]) - 1
+                    free += not uses[page]
+            rounds.append(now)
             over = over[len(now) :]
+        for now in rounds:
+            self._evict(now, each, budget, sinks, recent)
 
     def _evict(self, over: list[int], each: int, budget: int, sinks: int, recent: int) -> None:
         taken = self._free[-each * len(over) :]
@@ -568,16 +690,50 @@ class PagedKVCache:
         for weights, left in zip(self.weights, moved):
             weights.index_copy_(0, rows, left)  # in their place: captured graphs hold them
         del self._free[-each * len(over) :]
+        for page in taken:
+            self._uses[page] = 1
         for b in over:
-            self._free.extend(reversed(self._pages[b]))
+            self._drop(self._pages[b])
             self._lengths[b] = budget
         self._pages = pages
 
+    def fork(self, source: int, target: int, length: int | None = None) -> None:
+        """Let the empty sequence ``target`` go on from ``source``'s entries, or
+        its first ``length`` (a prompt that several share), without copying
+        them: both list the same pages, and :meth:`begin` copies a half-written
+        one before either writes to it.  The weights that the entries received
+        are taken over.  Only sequences without evicted entries have a first
+        ``length``."""
+
+        have = self._lengths[source]
+        length = have if length is None else int(length)
+        if source == target or self._lengths[target] or self._pages[target]:
+            raise ValueError("a fork goes into an empty sequence")
+        if not 0 <= length <= have:
+            raise ValueError(f"a fork takes up to {have} entries, got {length}")
+        if length < have and self._positions[source] != have:
+            raise ValueError("a sequence with evicted entries is forked as a whole")
+        pages = list(self._pages)
+        pages[target] = pages[source][: -(-length // self.page_size)]
+        self._upload(pages)
+        self._begun = None
+        self._pages = pages
+        for page in pages[target]:
+            self._uses[page] += 1
+        self._lengths = list(self._lengths)
+        self._positions = list(self._positions)
+        self._lengths[target] = length
+        self._positions[target] = self._positions[source] if length == have else length
+        if self.weights is not None:
+            for weights in self.weights:
+                weights[target, :, :length] = weights[source, :, :length]
+
     def release(self, sequence: int) -> None:
-        """Drop a sequence: its pages are free and its slot empty."""
+        """Drop a sequence: its slot is empty, and those of its pages that no
+        other lists are free."""
 
         self._begun = None
-        self._free.extend(reversed(self._pages[sequence]))
+        self._drop(self._pages[sequence])
         self._pages[sequence] = []
         self._lengths[sequence] = self._positions[sequence] = 0
         self._upload(self._pages)

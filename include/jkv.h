@@ -748,6 +748,8 @@ int jkv_paged_attention_shaped(const void* q, int64_t q_stride_t,
  *                below 2^22), 16-byte aligned; queries and keys turned already
  *   starts       int32 [B+1] device, not decreasing
  *   lse          fp32 [N,QH] contiguous or NULL: natural log of each row's sum
+ *   rest         [N,QH,D] of the output's type, contiguous, or NULL: what the
+ *                output's rounding took off, for the gradients
  */
 int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                          const void* k, int64_t k_stride_t, int64_t k_stride_h,
@@ -757,11 +759,13 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                          int64_t QH, int64_t KVH, int64_t D, int64_t window,
                          int64_t sinks, float scale, float softcap,
                          const float* slopes, void* out, int64_t out_stride_t,
-                         int64_t out_stride_h, float* lse, jkv_stream_t stream);
+                         int64_t out_stride_h, float* lse, void* rest,
+                         jkv_stream_t stream);
 
 /*
  * Its gradients: d_q [N,QH,D], d_k and d_v [N,KVH,D], contiguous, of the inputs'
- * type (fp32 sums, one rounding), each NULL if not wanted.  o and lse are the
+ * type (fp32 sums, one rounding), each NULL if not wanted.  o, lse and
+ * rest (or NULL: gradients of bf16 rows are half as far off again) are the
  * forward's, d_out the gradient of o.  Rows that no sequence owns get 0.  Every
  * sum has one order.
  *   workspace    jkv_packed_backward_workspace_bytes() bytes, 16-byte aligned
@@ -770,7 +774,7 @@ int jkv_packed_attention_backward(
     const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
     int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
     int64_t v_stride_h, const void* o, int64_t o_stride_t, int64_t o_stride_h,
-    const void* d_out, int64_t d_stride_t, int64_t d_stride_h, const float* lse,
+    const void* rest, const void* d_out, int64_t d_stride_t, int64_t d_stride_h, const float* lse,
     int32_t dtype, const int32_t* starts, const int32_t* prefixes, int64_t N,
     int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t window, int64_t sinks,
     float scale, float softcap, const float* slopes, void* d_q, void* d_k,

@@ -603,6 +603,14 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
 #pragma unroll
       for (int e = 0; e < 4; ++e) h[e] = (T)(none ? 0.f : o[d][4 * q4 + e] * inv);
       *(V4*)(op + 2 * (32 * d + 8 * q4 + 4 * lh)) = h;
+      if constexpr (LINEAR) {
+        if (a.rest != nullptr) {  // what the rounding took off
+          V4 r;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[e] = (T)(none ? 0.f : o[d][4 * q4 + e] * inv - (float)h[e]);
+          *(V4*)(a.rest + row * (2 * D) + 2 * (32 * d + 8 * q4 + 4 * lh)) = r;
+        }
+      }
     }
 }
 

@@ -8,7 +8,7 @@ namespace jkv {
 // What the kernels of the attention's gradients share.  Strides in bytes; dq, dk
 // and dv are contiguous.
 struct PackedGradArgs {
-  const uint8_t *q, *k, *v, *o, *d;
+  const uint8_t *q, *k, *v, *o, *d, *rest;  // rest: what o's rounding took off, contiguous, or null
   int64_t qst, qsh, kst, ksh, vst, vsh, ost, osh, dst, dsh;
   uint8_t *dq, *dk, *dv;  // null: not wanted
   const int32_t *starts, *prefixes;
@@ -16,7 +16,7 @@ struct PackedGradArgs {
   int32_t N, B, QH, KVH, per, window, sinks;
   float scale, scale2, cap_mul, cap2;
   const float* slopes;
-  float2* stats;   // [QH][N]: base-2 log-sum-exp less 10, rowsum(do o)
+  float *lse2, *minus_delta;  // [QH][N]: base-2 log-sum-exp less 10, -rowsum(do o)
   float2* maxima;  // [kGradBlocks]: largest finite |do| and |v| (fp16)
   int32_t items;   // row blocks of all sequences at most
 };

@@ -42,7 +42,8 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
                          int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, int32_t dtype,
                          const int32_t* starts, const int32_t* prefixes, int64_t N, int64_t B, int64_t QH, int64_t KVH,
                          int64_t D, int64_t window, int64_t sinks, float scale, float softcap, const float* slopes,
-                         void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse, jkv_stream_t stream_) {
+                         void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse, void* rest,
+                         jkv_stream_t stream_) {
   using namespace jkv;
   int rc = packed_checks(dtype, N, B, QH, KVH, D, window, sinks, scale);
   if (rc != JKV_OK) return rc;
@@ -60,7 +61,7 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   }
   if (N == 0) return JKV_OK;
   JKV_CHECK_ARG(q && k && v && out && starts, "null buffer");
-  JKV_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 == 0, "packed rows must be 16-byte aligned");
+  JKV_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)rest) % 16 == 0, "packed rows must be 16-byte aligned");
   a.c.k = (uint8_t*)k; a.c.v = (uint8_t*)v;
   a.c.head_bytes = 2 * k_stride_h; a.c.slot_bytes = 2 * k_stride_t;
   a.v_head_bytes = 2 * v_stride_h; a.v_slot_bytes = 2 * v_stride_t;
@@ -68,7 +69,7 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   a.c.N = (int32_t)N; a.c.B = (int32_t)B;
   a.q = (const uint8_t*)q; a.qst = 2 * q_stride_t; a.qsh = 2 * q_stride_h;
   a.out = (uint8_t*)out; a.ost = 2 * out_stride_t; a.osh = 2 * out_stride_h;
-  a.lse = lse;
+  a.lse = lse; a.rest = (uint8_t*)rest;
   a.QH = (int32_t)QH; a.KVH = (int32_t)KVH; a.per = (int32_t)(QH / KVH);
   a.window = (int32_t)(window > 0 && window < kPagedMost ? window : kPagedMost);
   a.sinks = (int32_t)(sinks < kPagedMost ? sinks : kPagedMost);
@@ -91,13 +92,13 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
 
 int64_t jkv_packed_backward_workspace_bytes(int64_t N, int64_t QH) {
   if (N <= 0 || QH <= 0 || N * QH >= ((int64_t)1 << 31)) return 0;
-  return jkv::ceil_div(N * QH * 8, 256) * 256 + jkv::kGradBlocks * 8;
+  return 2 * jkv::ceil_div(N * QH * 4, 256) * 256 + jkv::kGradBlocks * 8;
 }
 
 int jkv_packed_attention_backward(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
                                   int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
-                                  const void* o, int64_t o_stride_t, int64_t o_stride_h, const void* d_out,
-                                  int64_t d_stride_t, int64_t d_stride_h, const float* lse, int32_t dtype,
+                                  const void* o, int64_t o_stride_t, int64_t o_stride_h, const void* rest,
+                                  const void* d_out, int64_t d_stride_t, int64_t d_stride_h, const float* lse, int32_t dtype,
                                   const int32_t* starts, const int32_t* prefixes, int64_t N, int64_t B, int64_t QH,
                                   int64_t KVH, int64_t D, int64_t window, int64_t sinks, float scale, float softcap,
                                   const float* slopes, void* d_q, void* d_k, void* d_v, void* workspace,
@@ -115,13 +116,14 @@ int jkv_packed_attention_backward(const void* q, int64_t q_stride_t, int64_t q_s
   if (rc != JKV_OK) return rc;
   if (N == 0) return JKV_OK;
   JKV_CHECK_ARG(q && k && v && o && d_out && lse && starts, "null buffer");
-  JKV_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)d_out | (uintptr_t)d_q | (uintptr_t)d_k |
+  JKV_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)rest | (uintptr_t)d_out | (uintptr_t)d_q | (uintptr_t)d_k |
                  (uintptr_t)d_v) % 16 == 0, "packed rows must be 16-byte aligned");
   const int64_t need = jkv_packed_backward_workspace_bytes(N, QH);
   JKV_CHECK_ARG(workspace != nullptr && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need,
                 "packed gradients need an aligned workspace of %lld bytes, got %lld", (long long)need, (long long)workspace_bytes);
   PackedGradArgs a = {};
   a.q = (const uint8_t*)q; a.k = (const uint8_t*)k; a.v = (const uint8_t*)v; a.o = (const uint8_t*)o; a.d = (const uint8_t*)d_out;
+  a.rest = (const uint8_t*)rest;
   a.qst = 2 * q_stride_t; a.qsh = 2 * q_stride_h; a.kst = 2 * k_stride_t; a.ksh = 2 * k_stride_h;
   a.vst = 2 * v_stride_t; a.vsh = 2 * v_stride_h; a.ost = 2 * o_stride_t; a.osh = 2 * o_stride_h;
   a.dst = 2 * d_stride_t; a.dsh = 2 * d_stride_h;
@@ -132,8 +134,10 @@ int jkv_packed_attention_backward(const void* q, int64_t q_stride_t, int64_t q_s
   a.sinks = (int32_t)(sinks < kPagedMost ? sinks : kPagedMost);
   a.scale = scale; a.scale2 = scale * 1.4426950408889634f;
   a.cap_mul = shape.cap_mul; a.cap2 = shape.cap2; a.slopes = slopes;
-  a.stats = (float2*)workspace;
-  a.maxima = (float2*)((uint8_t*)workspace + ceil_div(N * QH * 8, 256) * 256);
+  const int64_t each = ceil_div(N * QH * 4, 256) * 256;
+  a.lse2 = (float*)workspace;
+  a.minus_delta = (float*)((uint8_t*)workspace + each);
+  a.maxima = (float2*)((uint8_t*)workspace + 2 * each);
   if (form == kFormPlain) form = kFormShaped;
   return dtype == JKV_F16 ? packed_grad_launch_f16(a, form, D, (hipStream_t)stream_)
                           : packed_grad_launch_bf16(a, form, D, (hipStream_t)stream_);

@@ -57,13 +57,22 @@ __global__ __launch_bounds__(256) void packed_rows_kernel(PackedGradArgs a) {
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum = fmaf((float)d[e], (float)o[e], sum);
+    // (where one place holds most of a row's weight, do v and delta are near each
+    // other: without the rest the gradients of bf16 rows are 3.6e-3 off, with it 2.5e-3)
+    if (a.rest != nullptr) {
+      const V8 rest = *(const V8*)(a.rest + row * (2 * D) + 16 * part);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf((float)d[e], (float)rest[e], sum);
+    }
     if constexpr (DT == JKV_F16) most_d = largest_finite<DT>(dw, most_d);
 #pragma unroll
     for (int off = kLanes / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
     if (part == 0) {
       const float lse = a.lse[row];
       // (a row that saw nothing weighs nothing)
-      a.stats[(int64_t)head * a.N + n] = float2{lse == -INFINITY ? INFINITY : fmaf(lse, 1.4426950408889634f, -10.f), sum};
+      const int64_t at = (int64_t)head * a.N + n;
+      a.lse2[at] = lse == -INFINITY ? INFINITY : fmaf(lse, 1.4426950408889634f, -10.f);
+      a.minus_delta[at] = -sum;
     }
   }
   const int64_t kv_rows = (int64_t)a.N * a.KVH;
@@ -187,7 +196,7 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
   typedef typename Half16<DT>::V4 V4;
   typedef __attribute__((address_space(3))) const V8 lds_v8;
   typedef __attribute__((address_space(3))) const float4v lds_f4;
-  constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D, kTile = 32 * kRowBytes, kStage = 2 * kTile + 256;
+  constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D, kTile = 32 * kRowBytes, kStage = 2 * kTile + 512;
   __shared__ __align__(1024) uint8_t lds[4 * kTile + 2 * kStage];  // values; twice rows of q, rows of do, their stats
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, lh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -233,12 +242,12 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
     const uint32_t to = lds_base + 4 * kTile + stage * kStage;
     load_rows32<D>(a.q + n * a.qst + (int64_t)head * a.qsh, left, (uint32_t)a.qst, to, wave, lane);
     load_rows32<D>(a.d + n * a.dst + (int64_t)head * a.dsh, left, (uint32_t)a.dst, to + kTile, wave, lane);
-    if (wave == 0) {
-      const uint64_t at = (uint64_t)(a.stats + (int64_t)head * a.N + n);
-      const int32_t bytes = 8 * (left < 32 ? (left > 0 ? left : 0) : 32);
+    if (wave < 2) {
+      const uint64_t at = (uint64_t)((wave == 0 ? a.lse2 : a.minus_delta) + (int64_t)head * a.N + n);
+      const int32_t bytes = 4 * (left < 32 ? (left > 0 ? left : 0) : 32);
       const uint4v rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)(at >> 32)) & 0xffffu,
                            (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
-      load_to_lds<4>(to + 2 * kTile, 4u * (uint32_t)lane, rsrc);
+      load_to_lds<4>(to + 2 * kTile + 256 * wave, 4u * (uint32_t)lane, rsrc);
     }
   };
   float16v dk[kDims], dv[kDims];
@@ -248,66 +257,79 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
     dv[d] = float16v{};
   }
   // LDS addresses: rows as A operand (8 dims of row ln), transposed (4 of each of
-  // two groups of 8 rows, dim ln)
-  uint32_t row_at[kSteps], tr_at[kDims];
+  // two groups of 8 rows, dim ln); the rest are offsets known at compile time
+  uint32_t row_at[kSteps], lo_at[kDims], hi_at[kDims];
 #pragma unroll
   for (int c = 0; c < kSteps; ++c) row_at[c] = lds_base + (uint32_t)(ln * kRowBytes + 16 * chunk_both_slot<D>(ln, 2 * c + lh));
+  const uint32_t v_wave = (uint32_t)(wave * kTile);
   const int tr_row = 4 * lh + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  auto transposed = [&](int d, int st, uint32_t tile) -> V8 {
-    // (rows 16 on share a slot pattern, 8 on do not)
-    const uint32_t lo_at = lds_base + tile + (uint32_t)((16 * st + tr_row) * kRowBytes + 16 * chunk_both_slot<D>(tr_row, 4 * d + tr_chunk) + 8 * (lane & 1));
-    const uint32_t hi_at = lds_base + tile + (uint32_t)((16 * st + tr_row + 8) * kRowBytes + 16 * chunk_both_slot<D>(tr_row + 8, 4 * d + tr_chunk) + 8 * (lane & 1));
-    const V4 lo = lds_read_tr<V4>(lo_at), hi = lds_read_tr<V4>(hi_at);
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) {
+    lo_at[d] = lds_base + (uint32_t)(tr_row * kRowBytes + 16 * chunk_both_slot<D>(tr_row, 4 * d + tr_chunk) + 8 * (lane & 1));
+    hi_at[d] = lds_base + (uint32_t)((tr_row + 8) * kRowBytes + 16 * chunk_both_slot<D>(tr_row + 8, 4 * d + tr_chunk) + 8 * (lane & 1));
+  }
+  auto transposed = [&](int d, uint32_t off) -> V8 {
+    const V4 lo = lds_read_tr<V4>(lo_at[d] + off), hi = lds_read_tr<V4>(hi_at[d] + off);
     return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
   const int32_t key = wj0 + ln;
-  (void)tr_at;
 
-  auto work = [&](int32_t tile, int32_t g, uint32_t stage_at, auto masked) {
+  auto work = [&](int32_t tile, int32_t g, auto stage, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
+    const uint32_t stage_at = 4 * kTile + (uint32_t)(stage * kStage);
     const int32_t head = kvh * a.per + g, t0 = 32 * tile;
     const ScoreShape shape = score_shape<FORM>(a, head);
-    float16v sc = {}, dp = {};
+    // row 8 q4 + 4 lh + e's statistics: of 16 rows a lane
+    const uint32_t stats_at = lds_base + 16u * (uint32_t)lh + stage_at + 2 * kTile;
+    float16v sc = {}, dp;  // dp starts from -delta
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const float4v d = *(lds_f4*)(size_t)(stats_at + 256 + 32 * q4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = d[e];
+    }
 #pragma unroll
     for (int c = 0; c < kSteps; ++c) sc = mfma32<DT>(*(lds_v8*)(size_t)(row_at[c] + stage_at), kf[c], sc);
 #pragma unroll
     for (int c = 0; c < kSteps; ++c)
-      dp = mfma32<DT>(*(lds_v8*)(size_t)(row_at[c] + stage_at + kTile), *(lds_v8*)(size_t)(row_at[c] + (uint32_t)(wave * kTile)), dp);
+      dp = mfma32<DT>(*(lds_v8*)(size_t)(row_at[c] + stage_at + kTile), *(lds_v8*)(size_t)(row_at[c] + v_wave), dp);
+    __builtin_amdgcn_sched_barrier(0);
     V8 pf[2], df[2];
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) {
-      // {lse, delta} of rows 8 q4 + 4 lh + 0..3
-      const uint32_t at = lds_base + stage_at + 2 * kTile + (uint32_t)(64 * q4 + 32 * lh);
-      const float4v s01 = *(lds_f4*)(size_t)at, s23 = *(lds_f4*)(size_t)(at + 16);
+      const float4v lse = *(lds_f4*)(size_t)(stats_at + 32 * q4);
+      float4v poison;
+      if constexpr (MASKED) poison = *(lds_f4*)(size_t)(stats_at + 256 + 32 * q4) * 0.f;
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
         const int e = 4 * q4 + e4;
-        const float lse = e4 < 2 ? s01[2 * e4] : s23[2 * e4 - 4], delta = e4 < 2 ? s01[2 * e4 + 1] : s23[2 * e4 - 3];
         const int32_t i = t0 + 8 * q4 + 4 * lh + e4;
         float slant = 1.f;
-        float x = shape_and_slant<FORM>(shape, sc[e], (float)(i - key), &slant) - lse;
+        float x = shape_and_slant<FORM>(shape, sc[e], (float)(i - key), &slant) - lse[e4];
         bool seen = true;
         if constexpr (MASKED) {
           seen = (key <= i || key < prefix) && (key > i - a.window || key < a.sinks) && i < T0;
           x = seen ? x : -INFINITY;
         }
         float p = __builtin_amdgcn_exp2f(x);
-        float ds = p * (dp[e] - delta);
+        float ds = p * dp[e];
         if constexpr (FORM & kFormCap) ds *= slant;
         if constexpr (DT == JKV_F16) ds *= factor;
         if constexpr (MASKED) {
           ds = seen ? ds : 0.f;
-          p = seen ? fmaf(delta, 0.f, p) : 0.f;  // (NaN where do is not finite)
+          p = seen ? p + poison[e4] : 0.f;  // (NaN where do is not finite)
         }
         pf[e >> 3][e & 7] = (T)p;
         df[e >> 3][e & 7] = (T)ds;
       }
+      if (q4 == 1) __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int st = 0; st < 2; ++st)
 #pragma unroll
       for (int d = 0; d < kDims; ++d) {
-        V8 dot = transposed(d, st, stage_at + kTile), qt = transposed(d, st, stage_at);
+        V8 dot = transposed(d, stage_at + kTile + 16 * st * kRowBytes), qt = transposed(d, stage_at + 16 * st * kRowBytes);
         if constexpr (MASKED) {
           dot = finite_part<DT>(dot);
           qt = finite_part<DT>(qt);
@@ -315,32 +337,66 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
         dv[d] = mfma32<DT>(pf[st], dot, dv[d]);
         dk[d] = mfma32<DT>(df[st], qt, dk[d]);
       }
+    JKV_SG(0x100, 4);
+    for (int x = 0; x < 2 * kDims - 1; ++x) { JKV_SG(0x100, 4); JKV_SG(0x8, 2); }
+    JKV_SG(0x8, 2);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  const int32_t steps = tile1 > tile0 ? (tile1 - tile0) * a.per : 0;
-  int32_t tile = tile0, g = 0, next_tile = tile0, next_g = 0;
-  auto advance = [&](int32_t& t, int32_t& h) {
-    if (++h == a.per) {
-      h = 0;
-      ++t;
+  // Row tiles that all of the block's keys are seen by, [full0, full1), come last and
+  // have code without masks (in one loop with the masked tiles' code, the compiler
+  // keeps the sums in two places: 214 registers spilled).
+  int32_t full0 = j0 + 128 <= prefix ? tile0 : j0 / 32 + 4, full1 = T0 / 32;
+  if (j0 + 128 > a.sinks && (j0 + a.window) / 32 < full1) full1 = (j0 + a.window) / 32;
+  if (full0 < tile0) full0 = tile0;
+  if (full1 > tile1) full1 = tile1;
+  if (j0 + 128 > T0 || full1 <= full0) full0 = full1 = tile1;
+  const int32_t plain = (full1 - full0) * a.per, edge = tile1 > tile0 ? (tile1 - tile0) * a.per - plain : 0;
+  struct Step { int32_t tile, g; };
+  Step now = {tile0 == full0 ? full1 : tile0, 0};
+  if (now.tile >= tile1) now.tile = full0;
+  Step next = now;
+  // heads of a tile in turn; tiles before the full ones, behind them, then those
+  auto advance = [&](Step& s) {
+    if (++s.g < a.per) return;
+    s.g = 0;
+    const bool in_full = s.tile >= full0 && s.tile < full1;
+    ++s.tile;
+    if (in_full) return;
+    if (s.tile == full0) s.tile = full1;
+    if (s.tile >= tile1) s.tile = full0;
+  };
+  int32_t left = edge + plain;  // steps not yet loaded
+  // the step ahead into the other stage, once every load has landed and every LDS
+  // access of the step before is done, in all waves
+  auto turn_over = [&](int other) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (left > 0) {
+      load_step(next.tile, next.g, other);
+      advance(next);
+      --left;
     }
   };
-  if (steps > 0) load_step(next_tile, next_g, 0);
-  advance(next_tile, next_g);
-  for (int32_t step = 0; step < steps; ++step) {
-    // every load has landed and every LDS access of the step before is done, in all waves
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (step + 1 < steps) load_step(next_tile, next_g, (step + 1) & 1);
-    advance(next_tile, next_g);
-    const int32_t t0 = 32 * tile, last = t0 + 31;
-    const uint32_t stage_at = (uint32_t)(4 * kTile + (step & 1) * kStage);
-    const bool some = wj0 < T0 && (wj0 <= last || wj0 < prefix) && (wj0 + 31 > t0 - a.window || wj0 < a.sinks);
-    if (some) {
-      const bool full = last < T0 && wj0 + 31 < T0 && (wj0 + 31 <= t0 || wj0 + 32 <= prefix) && (wj0 > last - a.window || wj0 + 32 <= a.sinks);
-      if (full) work(tile, g, stage_at, std::false_type());
-      else work(tile, g, stage_at, std::true_type());
-    }
-    advance(tile, g);
+  if (left > 0) {
+    load_step(next.tile, next.g, edge & 1);  // (so that the full tiles start in stage 0)
+    advance(next);
+    --left;
+  }
+  for (int32_t n = edge; n > 0; --n) {
+    turn_over((n & 1) ^ 1);
+    const int32_t t0 = 32 * now.tile;
+    if (wj0 < T0 && (wj0 <= t0 + 31 || wj0 < prefix) && (wj0 + 31 > t0 - a.window || wj0 < a.sinks))
+      work(now.tile, now.g, n & 1, std::true_type());
+    advance(now);
+  }
+  for (int32_t n = 0; n < plain; n += 2) {
+    turn_over(1);
+    work(now.tile, now.g, std::integral_constant<int, 0>(), std::false_type());
+    advance(now);
+    if (n + 1 >= plain) break;
+    turn_over(0);
+    work(now.tile, now.g, std::integral_constant<int, 1>(), std::false_type());
+    advance(now);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
@@ -402,7 +458,6 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
     load_rows32<D>(a.k + n * a.kst + (int64_t)kvh * a.ksh, T0 - e0, (uint32_t)a.kst, lds_base + 2 * stage * kTile, wave, lane);
     load_rows32<D>(a.v + n * a.vst + (int64_t)kvh * a.vsh, T0 - e0, (uint32_t)a.vst, lds_base + (2 * stage + 1) * kTile, wave, lane);
   };
-  if (pt.count > 0) load_step(0, 0);
 
   // the wave's queries and output gradients (B operands: 8 dims of row ln)
   V8 qf[kSteps], dof[kSteps];
@@ -415,26 +470,29 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
       dof[c] = *(const V8*)(dp + 32 * c);
     }
   }
-  const float2 stat = a.stats[(int64_t)head * a.N + row0 + self];
-  const float lse = stat.x, delta = stat.y;
+  const float lse = a.lse2[(int64_t)head * a.N + row0 + self], minus_delta = a.minus_delta[(int64_t)head * a.N + row0 + self];
   const float factor = ds_factor<DT, D>(a);
   const ScoreShape shape = score_shape<FORM>(a, head);
 
   float16v dq[kDims];
 #pragma unroll
   for (int d = 0; d < kDims; ++d) dq[d] = float16v{};
-  uint32_t row_at[kSteps];
+  uint32_t row_at[kSteps], lo_at[kDims], hi_at[kDims];
 #pragma unroll
   for (int c = 0; c < kSteps; ++c) row_at[c] = lds_base + (uint32_t)(ln * kRowBytes + 16 * chunk_both_slot<D>(ln, 2 * c + lh));
   const int tr_row = 4 * lh + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  auto transposed = [&](int d, int st, uint32_t tile) -> V8 {
-    const uint32_t lo_at = lds_base + tile + (uint32_t)((16 * st + tr_row) * kRowBytes + 16 * chunk_both_slot<D>(tr_row, 4 * d + tr_chunk) + 8 * (lane & 1));
-    const uint32_t hi_at = lds_base + tile + (uint32_t)((16 * st + tr_row + 8) * kRowBytes + 16 * chunk_both_slot<D>(tr_row + 8, 4 * d + tr_chunk) + 8 * (lane & 1));
-    const V4 lo = lds_read_tr<V4>(lo_at), hi = lds_read_tr<V4>(hi_at);
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) {
+    lo_at[d] = lds_base + (uint32_t)(tr_row * kRowBytes + 16 * chunk_both_slot<D>(tr_row, 4 * d + tr_chunk) + 8 * (lane & 1));
+    hi_at[d] = lds_base + (uint32_t)((tr_row + 8) * kRowBytes + 16 * chunk_both_slot<D>(tr_row + 8, 4 * d + tr_chunk) + 8 * (lane & 1));
+  }
+  auto transposed = [&](int d, uint32_t off) -> V8 {
+    const V4 lo = lds_read_tr<V4>(lo_at[d] + off), hi = lds_read_tr<V4>(hi_at[d] + off);
     return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-  auto work = [&](int32_t e0, uint32_t stage_at, auto masked) {
+  auto work = [&](int32_t e0, auto stage, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
+    const uint32_t stage_at = (uint32_t)(stage * 2 * kTile);
     float16v sc = {}, dp = {};
 #pragma unroll
     for (int c = 0; c < kSteps; ++c) sc = mfma32<DT>(*(lds_v8*)(size_t)(row_at[c] + stage_at), qf[c], sc);
@@ -452,7 +510,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
         seen = j <= reach && (j > self - a.window || j < a.sinks);
         x = seen ? x : -INFINITY;
       }
-      float ds = __builtin_amdgcn_exp2f(x) * (dp[e] - delta);
+      float ds = __builtin_amdgcn_exp2f(x) * (dp[e] + minus_delta);
       if constexpr (FORM & kFormCap) ds *= slant;
       if constexpr (DT == JKV_F16) ds *= factor;
       if constexpr (MASKED) ds = seen ? ds : 0.f;
@@ -462,22 +520,54 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
     for (int st = 0; st < 2; ++st)
 #pragma unroll
       for (int d = 0; d < kDims; ++d) {
-        V8 kt = transposed(d, st, stage_at);
+        V8 kt = transposed(d, stage_at + 16 * st * kRowBytes);
         if constexpr (MASKED) kt = finite_part<DT>(kt);
         dq[d] = mfma32<DT>(kt, df[st], dq[d]);
       }
   };
-  for (int32_t i = 0; i < pt.count; ++i) {
+  // as above: the tiles that all rows see, [full0, full1), come last
+  int32_t full1 = pt.lead + (row_reach<FORM>(first, prefix) + 1) / 32 - pt.main, full0 = pt.lead;
+  if (last >= a.window && (last - a.window) / 32 + 1 > pt.main) full0 += (last - a.window) / 32 + 1 - pt.main;
+  if (full1 > pt.count) full1 = pt.count;
+  if (full1 <= full0) full0 = full1 = pt.count;
+  const int32_t plain = full1 - full0, edge = pt.count - plain;
+  int32_t now = full0 == 0 ? full1 : 0;
+  if (now >= pt.count) now = full0;
+  int32_t next = now, left = pt.count;
+  auto advance = [&](int32_t& i) {
+    const bool in_full = i >= full0 && i < full1;
+    ++i;
+    if (in_full) return;
+    if (i == full0) i = full1;
+    if (i >= pt.count) i = full0;
+  };
+  auto turn_over = [&](int other) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (i + 1 < pt.count) load_step(i + 1, (i + 1) & 1);
-    const int32_t e0 = entry_of(i);
-    const uint32_t stage_at = (uint32_t)(2 * (i & 1) * kTile);
-    const bool some = e0 <= row_reach<FORM>(wlast, prefix) && (e0 + 31 > wfirst - a.window || e0 < a.sinks);
-    if (some) {
-      const bool full = e0 + 31 <= row_reach<FORM>(wfirst, prefix) && (e0 > wlast - a.window || e0 + 32 <= a.sinks);
-      if (full) work(e0, stage_at, std::false_type());
-      else work(e0, stage_at, std::true_type());
+    if (left > 0) {
+      load_step(next, other);
+      advance(next);
+      --left;
     }
+  };
+  if (left > 0) {
+    load_step(next, edge & 1);
+    advance(next);
+    --left;
+  }
+  for (int32_t n = edge; n > 0; --n) {
+    turn_over((n & 1) ^ 1);
+    const int32_t e0 = entry_of(now);
+    if (e0 <= row_reach<FORM>(wlast, prefix) && (e0 + 31 > wfirst - a.window || e0 < a.sinks)) work(e0, n & 1, std::true_type());
+    advance(now);
+  }
+  for (int32_t n = 0; n < plain; n += 2) {
+    turn_over(1);
+    work(entry_of(now), std::integral_constant<int, 0>(), std::false_type());
+    advance(now);
+    if (n + 1 >= plain) break;
+    turn_over(0);
+    work(entry_of(now), std::integral_constant<int, 1>(), std::false_type());
+    advance(now);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   if (!row_ok) return;

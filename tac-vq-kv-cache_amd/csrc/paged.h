@@ -127,6 +127,7 @@ struct PagedAttnArgs {
   const float* slopes;      // [QH] a unit of distance, or null
   const int32_t* prefixes;  // [B] first entries that all of a sequence's rows see, or null
   int64_t v_head_bytes, v_slot_bytes;  // of values that lie without pages
+  uint8_t* rest;  // [N,QH,D] of the output's type: what its rounding took off, or null
   uint8_t* q_parts;  // chunks with weights: [KVH][N][per] rotated queries, D of their leading and D of their trailing parts
 };
 

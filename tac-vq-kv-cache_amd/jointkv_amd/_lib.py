@@ -157,11 +157,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "jkv_packed_attention": (
         ctypes.c_int,
         [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
-         _f32, _f32, _vp, _vp, _i64, _i64, _vp, _vp],
+         _f32, _f32, _vp, _vp, _i64, _i64, _vp, _vp, _vp],
     ),
     "jkv_packed_attention_backward": (
         ctypes.c_int,
-        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _vp,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp,
+         _vp,
          _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     ),
     "jkv_packed_backward_workspace_bytes": (_i64, [_i64, _i64]),

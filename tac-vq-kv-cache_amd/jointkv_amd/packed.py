@@ -38,7 +38,7 @@ def _span(window: int | None, sinks: int) -> tuple[int, int]:
     return 0 if window is None else min(int(window), 0x7fffffff), min(int(sinks), 0x7fffffff)
 
 
-def _forward(query, key, value, starts, prefixes, slopes, softcap, window, sinks, scale, lse, out):
+def _forward(query, key, value, starts, prefixes, slopes, softcap, window, sinks, scale, lse, out, rest=None):
     device = _lib.require_device(query, key, value, starts, prefixes, slopes, lse, out)
     rows, qheads, dim = query.shape
     if out is None:
@@ -49,27 +49,28 @@ def _forward(query, key, value, starts, prefixes, slopes, softcap, window, sinks
             *q_at, *k_at, *v_at, _lib.dtype_code(query.dtype), starts.data_ptr(), _lib.ptr(prefixes), rows,
             starts.shape[0] - 1, qheads, key.shape[1], dim, *_span(window, sinks), scale, softcap, _lib.ptr(slopes),
             out.data_ptr(), out.stride(0) if rows > 1 else 0, out.stride(1) if qheads > 1 else 0, _lib.ptr(lse),
-            _lib.stream_handle(device)))
+            _lib.ptr(rest), _lib.stream_handle(device)))
     return out
 
 
 class _PackedAttention(torch.autograd.Function):
-    """The forward keeps each row's log-sum-exp; the backward forms the weights
-    anew from it."""
+    """The forward keeps each row's log-sum-exp and what the output's rounding took
+    off; the backward forms the weights anew from them."""
 
     @staticmethod
     def forward(ctx, query, key, value, starts, prefixes, slopes, softcap, window, sinks, scale, lse):
         if lse is None:
             lse = torch.empty(query.shape[:2], dtype=torch.float32, device=query.device)
-        out = _forward(query, key, value, starts, prefixes, slopes, softcap, window, sinks, scale, lse, None)
+        rest = _plain(query)(tuple(query.shape))
+        out = _forward(query, key, value, starts, prefixes, slopes, softcap, window, sinks, scale, lse, None, rest)
         ctx.params = (softcap, window, sinks, scale)
-        ctx.save_for_backward(query, key, value, out, lse, starts, prefixes, slopes)
+        ctx.save_for_backward(query, key, value, out, rest, lse, starts, prefixes, slopes)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        query, key, value, out, lse, starts, prefixes, slopes = ctx.saved_tensors
+        query, key, value, out, rest, lse, starts, prefixes, slopes = ctx.saved_tensors
         softcap, window, sinks, scale = ctx.params
         rows, qheads, dim = query.shape
         device = query.device
@@ -80,7 +81,7 @@ class _PackedAttention(torch.autograd.Function):
             ws_bytes = _lib.workspace_bytes("jkv_packed_backward_workspace_bytes", rows, qheads)
             workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
             _lib.check(_lib.load().jkv_packed_attention_backward(
-                *(x for _tensor, at in places for x in at), lse.data_ptr(), _lib.dtype_code(query.dtype),
+                *(x for _tensor, at in places[:4] for x in at), rest.data_ptr(), *places[4][1], lse.data_ptr(), _lib.dtype_code(query.dtype),
                 starts.data_ptr(), _lib.ptr(prefixes), rows, starts.shape[0] - 1, qheads, key.shape[1], dim,
                 *_span(window, sinks), scale, softcap, _lib.ptr(slopes), *map(_lib.ptr, grads), workspace.data_ptr(),
                 ws_bytes, _lib.stream_handle(device)))

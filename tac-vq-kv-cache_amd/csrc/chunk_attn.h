@@ -349,7 +349,13 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   // large scales need.)
   float16v shift = {}, o[kDims];
   float l = 0.f, limit = -INFINITY;
-  // Shaped scores are moved by `from` instead, the reference less 10.
+  // Shaped scores are moved by `from` instead, the reference less kHeld, which
+  // moves when a maximum passes it by kRoom: sharp heads move it often, and each
+  // time costs a rescaling (with 10 and 4, a quarter of the vector instructions of
+  // capped 8,192-token texts).  fp16 p stay below 2^15 and hold weights of 2^-30,
+  // bf16 ones below 2^34 (values past 2^93 over the number of entries can pass 32
+  // bits).
+  constexpr float kHeld = DT == JKV_F16 ? 6.f : 10.f, kRoom = DT == JKV_F16 ? 9.f : 24.f;
   float from = 0.f;
   const ScoreShape shape = score_shape<FORM>(a, head);
 #pragma unroll
@@ -394,14 +400,6 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
         sc[kb][e] = seen ? sc[kb][e] : -INFINITY;
       }
   };
-  auto shaped = [&](int32_t e0, float16v (&sc)[2]) {
-    const float at = (float)(e0 + 4 * lh - self);  // (distances below 2^24 are exact)
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        sc[kb][e] = shape_score<FORM>(shape, sc[kb][e], at + (float)(32 * kb + 8 * (e >> 2) + (e & 3)));
-  };
   auto largest = [&](const float16v (&sc)[2]) -> float {
     float mx = -INFINITY;
 #pragma unroll
@@ -412,20 +410,6 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   };
   auto move_reference = [&](float mx, float16v (&sc)[2]) {
     const bool need = mx > limit;
-    if constexpr (FORM != kFormPlain) {
-      if (__any(need)) {
-        const float to = need ? mx - 10.f : from;
-        const float alpha = limit == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(from - to);
-        limit = need ? mx + 4.f : limit;
-        from = to;
-        l *= alpha;
-#pragma unroll
-        for (int x = 0; x < kDims; ++x) o[x] *= alpha;
-      }
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) sc[kb] -= from;
-      return;
-    }
     if (!__any(need)) return;
     const float d = need ? mx - 10.f : 0.f, by = d / a.scale2;
     const float alpha = limit == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(-d);
@@ -465,10 +449,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     JKV_SG(0x100, kSteps);
     for (int x = 0; x < kSteps; ++x) { JKV_SG(0x8, EXACT ? 2 : 1); JKV_SG(0x100, 1); }
     JKV_SG(0x8, EXACT ? 2 * kSteps : kSteps);
-    if constexpr (FORM != kFormPlain) {
-      shaped(entry_of(i), sc);
-      if (!(is & kWaveFull)) hide(entry_of(i), sc);
-    } else if (!unit || !(is & kWaveFull)) {
+    if (!unit || !(is & kWaveFull)) {
       for (int kb = 0; kb < 2; ++kb) sc[kb] *= a.scale2;
       hide(entry_of(i), sc);
     }
@@ -495,13 +476,124 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     for (int x = 0; x < 2 * kDims; ++x) { JKV_SG(0x8, 1); JKV_SG(0x100, 2); JKV_SG(0x2, 40 / (2 * kDims)); }
     JKV_SG(0x8, 2 * kDims);
   };
+  // The same with shaped scores, whose vector instructions take longer than the
+  // products (13 and 1 a score, 64 cycles of issue and 32): a half's shaping goes
+  // beside the products of the other half's scores or of the values, a product
+  // and a few scores at a time, fenced, as the compiler else gathers each kind.
+  auto work_shaped = [&](int32_t i, int32_t is, auto parity, auto again) {
+    constexpr int buf = decltype(parity)::value;
+    constexpr bool AGAIN = decltype(again)::value;
+    constexpr int kEach = 16 / kSteps, kValues = 2 * kDims, kBeside = 16 / kValues;
+    const int32_t e0 = entry_of(i);
+    const float at = (float)(e0 + 4 * lh - self);  // (distances below 2^24 are exact)
+    float16v sc[2] = {};
+    V8 ring[3];
+    auto key_operand = [&](int n) -> V8 {
+      return *(lds_v8*)(size_t)(k_at[n % kSteps] + (uint32_t)(2 * buf * kTileBytes + 32 * (n / kSteps) * kRowBytes));
+    };
+    auto first = [&](int kb, int e) { sc[kb][e] = shape_first<FORM>(shape, sc[kb][e]); };
+    auto second = [&](int kb, int e) {
+      sc[kb][e] = shape_second<FORM>(shape, sc[kb][e], at + (float)(32 * kb + 8 * (e >> 2) + (e & 3)));
+    };
+    V8 pf[4];
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};
+    auto third = [&](int kb, int e) {
+      const float p = __builtin_amdgcn_exp2f(sc[kb][e] - from);
+      sums[e & 3] += p;
+      pf[2 * kb + (e >> 3)][e & 7] = (T)p;
+    };
+    auto reference = [&](int kb) {
+      if (!(is & kWaveFull)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int32_t j = e0 + 32 * kb + 8 * (e >> 2) + 4 * lh + (e & 3);
+          const bool seen = j <= reach && (j > self - a.window || j < a.sinks);
+          sc[kb][e] = seen ? sc[kb][e] : -INFINITY;
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, sc[kb][e]), sc[kb][e + 1]);
+      mx = lanes2_max(mx);
+      const bool need = mx > limit;
+      if (__any(need)) {
+        const float to = need ? mx - kHeld : from;
+        const float alpha = limit == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(from - to);
+        limit = need ? mx + kRoom : limit;
+        from = to;
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sums[t] *= alpha;
+#pragma unroll
+        for (int x = 0; x < kDims; ++x) o[x] *= alpha;
+      }
+    };
+    ring[0] = key_operand(0);
+    ring[1] = key_operand(1);
+#pragma unroll
+    for (int n = 0; n < 2 * kSteps; ++n) {
+      const int kb = n / kSteps, c = n % kSteps;
+      if (n + 2 < 2 * kSteps) ring[(n + 2) % 3] = key_operand(n + 2);
+      sc[kb] = mfma32<DT>(ring[n % 3], qf[c], sc[kb]);
+      if constexpr (EXACT) sc[kb] = mfma32<DT>(AGAIN ? finite_part<DT>(ring[n % 3]) : ring[n % 3], ql[c], sc[kb]);
+      if (kb == 1) {
+#pragma unroll
+        for (int e = c * kEach; e < (c + 1) * kEach; ++e) first(0, e);
+        if (c > 0)
+#pragma unroll
+          for (int e = (c - 1) * kEach; e < c * kEach; ++e) second(0, e);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    ring[0] = value_operand(0, 0, buf);
+    ring[1] = value_operand(1, 0, buf);
+#pragma unroll
+    for (int e = 16 - kEach; e < 16; ++e) second(0, e);
+    reference(0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) third(0, e);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int n = 0; n < kValues; ++n) {
+        if (n + 2 < kValues) ring[(n + 2) % 3] = value_operand((n + 2) % kDims, 2 * kb + (n + 2) / kDims, buf);
+        o[n % kDims] = mfma32<DT>(ring[n % 3], pf[2 * kb + n / kDims], o[n % kDims]);
+        if (n < kDims)
+#pragma unroll
+          for (int e = 8 + n * (8 / kDims); e < 8 + (n + 1) * (8 / kDims); ++e) third(kb, e);
+        if (kb == 0) {
+#pragma unroll
+          for (int e = n * kBeside; e < (n + 1) * kBeside; ++e) first(1, e);
+          if (n > 0)
+#pragma unroll
+            for (int e = (n - 1) * kBeside; e < n * kBeside; ++e) second(1, e);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (kb == 0) {
+        ring[0] = value_operand(0, 2, buf);
+        ring[1] = value_operand(1, 2, buf);
+#pragma unroll
+        for (int e = 16 - kBeside; e < 16; ++e) second(1, e);
+        reference(1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) third(1, e);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  };
   auto step = [&](int32_t i, auto parity) {
     constexpr int buf = decltype(parity)::value;
     const int32_t is = __builtin_amdgcn_readlane(what, i - run0);
     meet();
     load_stage(i + 1, buf ^ 1);
     if (!(is & kBlockFull)) clean(buf);
-    if (is & kWaveSees) work(i, is, parity, std::false_type());
+    if (is & kWaveSees) {
+      if constexpr (FORM == kFormPlain) work(i, is, parity, std::false_type());
+      else work_shaped(i, is, parity, std::false_type());
+    }
   };
   for (int32_t i = tile0; i < tile1; i += 2) {
     step(i, std::integral_constant<int, 0>());
@@ -532,7 +624,10 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
       const int32_t is = __builtin_amdgcn_readlane(what, i - run0);
       meet();
       clean(0);
-      if (is & kWaveSees) work(i, is, std::integral_constant<int, 0>(), std::true_type());
+      if (is & kWaveSees) {
+        if constexpr (FORM == kFormPlain) work(i, is, std::integral_constant<int, 0>(), std::true_type());
+        else work_shaped(i, is, std::integral_constant<int, 0>(), std::true_type());
+      }
     }
   }
 

@@ -19,10 +19,20 @@
 // are seen, p or delta are not finite and carry it.
 #pragma once
 
+#include <utility>
+
 #include "chunk_attn.h"
 #include "packed.h"
 
 namespace jkv {
+
+// f(0), f(1), .. f(N - 1), each with its number as a constant.
+template <typename F, int... I> __device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, typename F> __device__ __forceinline__ void each_to(F&& f) {
+  each_of(f, std::make_integer_sequence<int, N>());
+}
 
 // max of |x| over the finite halves of w, 0 if there are none
 template <int DT>
@@ -121,7 +131,7 @@ __device__ __forceinline__ float ds_factor(const PackedGradArgs& a) {
   }
   const float most = 2.f * D * most_d * most_v;
   if (!(most > 0.f)) return 1.f;
-  // (fp16 values: 2^-48 to 2^32 times 2^8)
+  // (fp16 values: 2^-48 to 2^32 times 2^8; with a cap, its slope's 4 comes last)
   int e;
   frexpf(most, &e);  // most < 2^e
   return __uint_as_float((uint32_t)(127 + 5 - e) << 23);
@@ -155,33 +165,68 @@ __device__ __forceinline__ bool packed_block(const PackedGradArgs& a, int32_t pe
   return false;
 }
 
-// A score's weight exponent and the cap's slope there.
+// Of what shape_first left of a score: its weight's exponent, and the cap's slope.
 template <int FORM>
 __device__ __forceinline__ float shape_and_slant(const ScoreShape& s, float x, float distance, float* slant) {
-  x *= s.mul;
   if constexpr (FORM & kFormCap) {
-    const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x));  // tanh = 1 - 2r
-    *slant = 4.f * fmaf(-r, r, r);
+    const float r = __builtin_amdgcn_rcpf(x);  // tanh = 1 - 2r
+    *slant = fmaf(-r, r, r);  // a quarter of it
     x = fmaf(s.twice, r, s.cap2);
   }
   if constexpr (FORM & kFormBias) x = fmaf(-s.slope2, fabsf(distance), x);
   return x;
 }
 
-// 32 rows of D elements into LDS, a wave's share of 8: row r's chunk j in slot
-// chunk_both_slot(r, j).  Rows at or behind `left` land as zeros.
+// 32 rows of D elements into LDS, row r's chunk j in slot chunk_both_slot(r, j),
+// 16 rows (D = 128) or 32 a load of the four waves.  Rows at or behind `left` land
+// as zeros.  Two groups of 16 rows share their slots, so one offset a lane serves
+// both.
 template <int D>
-__device__ __forceinline__ void load_rows32(const uint8_t* base, int32_t left, uint32_t stride, uint32_t to, int wave, int lane) {
-  constexpr int kRowBytes = 2 * D, kRowsPerLoad = 1024 / kRowBytes, kLoads = 8 / kRowsPerLoad;
-  const uint32_t bytes = left > 0 ? (uint32_t)((left < 32 ? left : 32) - 1) * stride + kRowBytes : 0u;
-  const uint64_t at = (uint64_t)base;
-  const uint4v rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)(at >> 32)) & 0xffffu,
-                       (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)bytes), 0x00020000u};
+__device__ __forceinline__ uint32_t rows32_offset(uint32_t stride, int wave, int lane) {
+  constexpr int kRowsPerLoad = 1024 / (2 * D);
+  const int r = kRowsPerLoad * wave + lane / (64 / kRowsPerLoad), slot = lane % (64 / kRowsPerLoad);
+  return (uint32_t)r * stride + 16u * (uint32_t)chunk_both_slot<D>(r, slot);
+}
+template <int D>
+__device__ __forceinline__ void load_rows32(const uint8_t* base, int32_t left, uint32_t stride, uint32_t offset, uint32_t to, int wave) {
+  constexpr int kRowBytes = 2 * D, kEach = 4096 / kRowBytes;
 #pragma unroll
-  for (int j = 0; j < kLoads; ++j) {
-    const int r = 8 * wave + j * kRowsPerLoad + lane / (64 / kRowsPerLoad), slot = lane % (64 / kRowsPerLoad);
-    load_to_lds<16>(to + (uint32_t)(8 * wave * kRowBytes) + 1024u * j, (uint32_t)r * stride + 16u * (uint32_t)chunk_both_slot<D>(r, slot), rsrc);
+  for (int j = 0; j < 32 / kEach; ++j) {
+    const int32_t rows = left - j * kEach;
+    const uint32_t bytes = rows > 0 ? (uint32_t)((rows < kEach ? rows : kEach) - 1) * stride + kRowBytes : 0u;
+    const uint64_t at = (uint64_t)base + (uint64_t)(j * kEach) * stride;
+    const uint4v rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)(at >> 32)) & 0xffffu,
+                         (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)bytes), 0x00020000u};
+    load_to_lds<16>(to + 4096u * j + 1024u * (uint32_t)wave, offset, rsrc);
   }
+}
+
+// A lane's LDS addresses in a tile of 32 rows.  Row ln's 16-byte chunk 2c + lh (an
+// operand's 8 contracted places) is at rows ^ 32c; 4 elements of each of two groups
+// of 8 rows, dim 32d + ln (transposing reads), at cols ^ 64d and, 8 rows on, at
+// (cols ^ 64d ^ 32) + 8 rows.  Two registers held in place of sixteen: the others
+// are made anew in every step.
+struct TileAt {
+  uint32_t rows, cols;
+};
+template <int D>
+__device__ __forceinline__ TileAt tile_at(uint32_t lds_base, int lane) {
+  constexpr int kRowBytes = 2 * D;
+  const int ln = lane & 31, lh = lane >> 5, r = 4 * lh + ((lane & 15) >> 2), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  return TileAt{lds_base + (uint32_t)(ln * kRowBytes + 16 * chunk_both_slot<D>(ln, lh)),
+                lds_base + (uint32_t)(r * kRowBytes + 16 * chunk_both_slot<D>(r, chunk) + 8 * (lane & 1))};
+}
+template <int DT, int D>
+__device__ __forceinline__ typename Half16<DT>::V8 read_rows(uint32_t rows, int c, uint32_t off) {
+  typedef __attribute__((address_space(3))) const typename Half16<DT>::V8 lds_v8;
+  return *(lds_v8*)(size_t)((rows ^ (uint32_t)(32 * c)) + off);
+}
+template <int DT, int D>
+__device__ __forceinline__ typename Half16<DT>::V8 read_cols(uint32_t cols, int d, uint32_t off) {
+  typedef typename Half16<DT>::V8 V8;
+  typedef typename Half16<DT>::V4 V4;
+  const V4 lo = lds_read_tr<V4>((cols ^ (uint32_t)(64 * d)) + off), hi = lds_read_tr<V4>((cols ^ (uint32_t)(64 * d + 32)) + (off + 16u * D));
+  return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
 // dk and dv of 128 keys: a wave's 32 are columns of S = Q K^T and dP = dO V^T
@@ -193,8 +238,6 @@ template <int DT, int D, int FORM>
 __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a) {
   typedef typename Half16<DT>::T T;
   typedef typename Half16<DT>::V8 V8;
-  typedef typename Half16<DT>::V4 V4;
-  typedef __attribute__((address_space(3))) const V8 lds_v8;
   typedef __attribute__((address_space(3))) const float4v lds_f4;
   constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D, kTile = 32 * kRowBytes, kStage = 2 * kTile + 512;
   __shared__ __align__(1024) uint8_t lds[4 * kTile + 2 * kStage];  // values; twice rows of q, rows of do, their stats
@@ -215,7 +258,7 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
 #pragma unroll
   for (int w = 0; w < 4; ++w)
     load_rows32<D>(a.v + (int64_t)(row0 + j0 + 32 * w) * a.vst + (int64_t)kvh * a.vsh, T0 - j0 - 32 * w, (uint32_t)a.vst,
-                   lds_base + w * kTile, wave, lane);
+                   rows32_offset<D>((uint32_t)a.vst, wave, lane), lds_base + w * kTile, wave);
   V8 kf[kSteps];
   {
     const bool ok = wj0 + ln < T0;
@@ -236,12 +279,13 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
   if (j0 >= a.sinks && (int64_t)j0 + 127 + a.window < i1) i1 = j0 + 127 + a.window;
   const int32_t tile0 = i0 / 32, tile1 = (i1 + 31) / 32;
   // steps: (row tile, head of the group), heads fastest
+  const uint32_t q_off = rows32_offset<D>((uint32_t)a.qst, wave, lane), d_off = rows32_offset<D>((uint32_t)a.dst, wave, lane);
   auto load_step = [&](int32_t tile, int32_t g, int stage) {
     const int32_t head = kvh * a.per + g, left = T0 - 32 * tile;
     const int64_t n = row0 + 32 * tile;
     const uint32_t to = lds_base + 4 * kTile + stage * kStage;
-    load_rows32<D>(a.q + n * a.qst + (int64_t)head * a.qsh, left, (uint32_t)a.qst, to, wave, lane);
-    load_rows32<D>(a.d + n * a.dst + (int64_t)head * a.dsh, left, (uint32_t)a.dst, to + kTile, wave, lane);
+    load_rows32<D>(a.q + n * a.qst + (int64_t)head * a.qsh, left, (uint32_t)a.qst, q_off, to, wave);
+    load_rows32<D>(a.d + n * a.dst + (int64_t)head * a.dsh, left, (uint32_t)a.dst, d_off, to + kTile, wave);
     if (wave < 2) {
       const uint64_t at = (uint64_t)((wave == 0 ? a.lse2 : a.minus_delta) + (int64_t)head * a.N + n);
       const int32_t bytes = 4 * (left < 32 ? (left > 0 ? left : 0) : 32);
@@ -256,91 +300,109 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
     dk[d] = float16v{};
     dv[d] = float16v{};
   }
-  // LDS addresses: rows as A operand (8 dims of row ln), transposed (4 of each of
-  // two groups of 8 rows, dim ln); the rest are offsets known at compile time
-  uint32_t row_at[kSteps], lo_at[kDims], hi_at[kDims];
-#pragma unroll
-  for (int c = 0; c < kSteps; ++c) row_at[c] = lds_base + (uint32_t)(ln * kRowBytes + 16 * chunk_both_slot<D>(ln, 2 * c + lh));
-  const uint32_t v_wave = (uint32_t)(wave * kTile);
-  const int tr_row = 4 * lh + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-#pragma unroll
-  for (int d = 0; d < kDims; ++d) {
-    lo_at[d] = lds_base + (uint32_t)(tr_row * kRowBytes + 16 * chunk_both_slot<D>(tr_row, 4 * d + tr_chunk) + 8 * (lane & 1));
-    hi_at[d] = lds_base + (uint32_t)((tr_row + 8) * kRowBytes + 16 * chunk_both_slot<D>(tr_row + 8, 4 * d + tr_chunk) + 8 * (lane & 1));
-  }
-  auto transposed = [&](int d, uint32_t off) -> V8 {
-    const V4 lo = lds_read_tr<V4>(lo_at[d] + off), hi = lds_read_tr<V4>(hi_at[d] + off);
-    return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  };
+  const TileAt tile_lane = tile_at<D>(lds_base, lane);
   const int32_t key = wj0 + ln;
 
+  // A step's products in turn: S, dP, dv, dk, and beside each a few places' vector
+  // instructions, fenced (the compiler else gathers each kind, and they overlap
+  // little).  Operands are read two products ahead.
   auto work = [&](int32_t tile, int32_t g, auto stage, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
+    constexpr int kOps = 2 * kSteps + 4 * kDims;
     const uint32_t stage_at = 4 * kTile + (uint32_t)(stage * kStage);
-    const int32_t head = kvh * a.per + g, t0 = 32 * tile;
-    const ScoreShape shape = score_shape<FORM>(a, head);
+    const int32_t t0 = 32 * tile;
+    const ScoreShape shape = score_shape<FORM>(a, kvh * a.per + g);
+    const float at = (float)(t0 + 4 * lh - key);  // (distances below 2^24 are exact)
+    uint32_t rows = tile_lane.rows, cols = tile_lane.cols;
+    asm volatile("" : "+v"(rows), "+v"(cols));  // (what is made from them is not kept)
+    const uint32_t v_rows = rows + (uint32_t)(wave * kTile);
     // row 8 q4 + 4 lh + e's statistics: of 16 rows a lane
     const uint32_t stats_at = lds_base + 16u * (uint32_t)lh + stage_at + 2 * kTile;
-    float16v sc = {}, dp;  // dp starts from -delta
+    float16v sc = {}, dp;
+    float4v lse[4];
+    V8 pf[2], df[2], ring[3], values[3];
+    auto read = [&](int n) {
+      if (n < kSteps) ring[n % 3] = read_rows<DT, D>(rows, n, stage_at);
+      else if (n < 2 * kSteps) {
+        ring[n % 3] = read_rows<DT, D>(rows, n - kSteps, stage_at + kTile);
+        values[n % 3] = read_rows<DT, D>(v_rows, n - kSteps, 0);
+      } else if (n < kOps) {
+        const int m = (n - 2 * kSteps) % (2 * kDims);
+        ring[n % 3] = read_cols<DT, D>(cols, m % kDims, stage_at + (n < 2 * kSteps + 2 * kDims ? kTile : 0) + 16 * (m / kDims) * kRowBytes);
+        if constexpr (MASKED) ring[n % 3] = finite_part<DT>(ring[n % 3]);
+      }
+    };
+    auto read_lse = [&](int q4) { lse[q4] = *(lds_f4*)(size_t)(stats_at + 32 * q4); };
+    auto first = [&](int e) { sc[e] = shape_first<FORM>(shape, sc[e]); };
+    // p, and what ds takes of it (in sc)
+    auto weigh = [&](int e) {
+      float slant = 1.f;
+      float x = shape_and_slant<FORM>(shape, sc[e], at + (float)(8 * (e >> 2) + (e & 3)), &slant) - lse[e >> 2][e & 3];
+      if constexpr (MASKED) {
+        const int32_t i = t0 + 8 * (e >> 2) + 4 * lh + (e & 3);
+        const bool seen = (key <= i || key < prefix) && (key > i - a.window || key < a.sinks) && i < T0;
+        const float minus_delta = *(__attribute__((address_space(3))) const float*)(size_t)(stats_at + 256 + 32 * (e >> 2) + 4 * (e & 3));
+        x = seen ? fmaf(minus_delta, 0.f, x) : -INFINITY;  // (NaN where do is not finite)
+      }
+      float p = __builtin_amdgcn_exp2f(x);
+      pf[e >> 3][e & 7] = (T)p;
+      if constexpr (FORM & kFormCap) p *= slant;
+      if constexpr (DT == JKV_F16) p *= factor;
+      sc[e] = p;
+    };
+    auto lean = [&](int e) {
+      float ds = sc[e] * dp[e];
+      if constexpr (MASKED) ds = sc[e] == 0.f ? 0.f : ds;
+      df[e >> 3][e & 7] = (T)ds;
+    };
+    read(0);
+    read(1);
 #pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
+    for (int q4 = 0; q4 < 4; ++q4) {  // dp starts from -delta
       const float4v d = *(lds_f4*)(size_t)(stats_at + 256 + 32 * q4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = d[e];
     }
+    each_to<kOps>([&](auto number) {
+      constexpr int n = decltype(number)::value;
+      read(n + 2);
+      if (n < kSteps) {
+        sc = mfma32<DT>(ring[n % 3], kf[n], sc);
+        if (n == kSteps - 2) { read_lse(0); read_lse(1); }
+      } else if (n < 2 * kSteps) {
+        constexpr int kFirst = 16 / kSteps, kWeigh = 8 / kSteps;
+        const int c = n - kSteps;
+        dp = mfma32<DT>(ring[n % 3], values[n % 3], dp);
 #pragma unroll
-    for (int c = 0; c < kSteps; ++c) sc = mfma32<DT>(*(lds_v8*)(size_t)(row_at[c] + stage_at), kf[c], sc);
+        for (int e = c * kFirst; e < (c + 1) * kFirst; ++e) first(e);
+        if (c > 0)
 #pragma unroll
-    for (int c = 0; c < kSteps; ++c)
-      dp = mfma32<DT>(*(lds_v8*)(size_t)(row_at[c] + stage_at + kTile), *(lds_v8*)(size_t)(row_at[c] + v_wave), dp);
-    __builtin_amdgcn_sched_barrier(0);
-    V8 pf[2], df[2];
+          for (int e = (c - 1) * kWeigh; e < c * kWeigh; ++e) weigh(e);
+        if (c == kSteps - 1) {
 #pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      const float4v lse = *(lds_f4*)(size_t)(stats_at + 32 * q4);
-      float4v poison;
-      if constexpr (MASKED) poison = *(lds_f4*)(size_t)(stats_at + 256 + 32 * q4) * 0.f;
-#pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        const int e = 4 * q4 + e4;
-        const int32_t i = t0 + 8 * q4 + 4 * lh + e4;
-        float slant = 1.f;
-        float x = shape_and_slant<FORM>(shape, sc[e], (float)(i - key), &slant) - lse[e4];
-        bool seen = true;
-        if constexpr (MASKED) {
-          seen = (key <= i || key < prefix) && (key > i - a.window || key < a.sinks) && i < T0;
-          x = seen ? x : -INFINITY;
+          for (int e = c * kWeigh; e < 8; ++e) weigh(e);
+          read_lse(2);
+          read_lse(3);
         }
-        float p = __builtin_amdgcn_exp2f(x);
-        float ds = p * dp[e];
-        if constexpr (FORM & kFormCap) ds *= slant;
-        if constexpr (DT == JKV_F16) ds *= factor;
-        if constexpr (MASKED) {
-          ds = seen ? ds : 0.f;
-          p = seen ? p + poison[e4] : 0.f;  // (NaN where do is not finite)
+      } else {
+        constexpr int kEach = 8 / kDims;
+        const int m = (n - 2 * kSteps) % (2 * kDims), d = m % kDims, st = m / kDims;
+        if (n < 2 * kSteps + 2 * kDims) {
+          dv[d] = mfma32<DT>(pf[st], ring[n % 3], dv[d]);
+#pragma unroll
+          for (int e = d * kEach; e < (d + 1) * kEach; ++e) {
+            if (st == 0) weigh(8 + e);
+            else lean(e);
+          }
+        } else {
+          dk[d] = mfma32<DT>(df[st], ring[n % 3], dk[d]);
+          if (st == 0)
+#pragma unroll
+            for (int e = d * kEach; e < (d + 1) * kEach; ++e) lean(8 + e);
         }
-        pf[e >> 3][e & 7] = (T)p;
-        df[e >> 3][e & 7] = (T)ds;
       }
-      if (q4 == 1) __builtin_amdgcn_sched_barrier(0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-      for (int d = 0; d < kDims; ++d) {
-        V8 dot = transposed(d, stage_at + kTile + 16 * st * kRowBytes), qt = transposed(d, stage_at + 16 * st * kRowBytes);
-        if constexpr (MASKED) {
-          dot = finite_part<DT>(dot);
-          qt = finite_part<DT>(qt);
-        }
-        dv[d] = mfma32<DT>(pf[st], dot, dv[d]);
-        dk[d] = mfma32<DT>(df[st], qt, dk[d]);
-      }
-    JKV_SG(0x100, 4);
-    for (int x = 0; x < 2 * kDims - 1; ++x) { JKV_SG(0x100, 4); JKV_SG(0x8, 2); }
-    JKV_SG(0x8, 2);
-    __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
 
   // Row tiles that all of the block's keys are seen by, [full0, full1), come last and
@@ -401,7 +463,7 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
   // lane holds dim 32d + ln of keys 8(e/4) + 4lh + e%4
-  const float dv_mul = 0x1p-10f, dk_mul = a.scale * 0x1p-10f / factor;
+  const float dv_mul = 0x1p-10f, dk_mul = a.scale * (FORM & kFormCap ? 4.f : 1.f) * 0x1p-10f / factor;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const int32_t j = wj0 + 8 * (e >> 2) + 4 * lh + (e & 3);
@@ -423,9 +485,8 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   typedef typename Half16<DT>::T T;
   typedef typename Half16<DT>::V8 V8;
   typedef typename Half16<DT>::V4 V4;
-  typedef __attribute__((address_space(3))) const V8 lds_v8;
-  constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D, kTile = 32 * kRowBytes;
-  __shared__ __align__(1024) uint8_t lds[4 * kTile];  // twice 32 keys and values
+  constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D, kTile = 64 * kRowBytes;
+  __shared__ __align__(1024) uint8_t lds[4 * kTile];  // twice 64 keys and values
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, lh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t at_item = blockIdx.x / (uint32_t)a.KVH;
@@ -450,13 +511,19 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   const int32_t reach = row_ok ? row_reach<FORM>(self, prefix) : -1;
   const uint32_t lds_base = lds_address(lds);
 
-  const PagedTiles pt = paged_tiles(first, row_reach<FORM>(last, prefix), a.window, a.sinks, 32);
-  auto entry_of = [&](int32_t i) { return (i < pt.lead ? i : pt.main + i - pt.lead) * 32; };
+  const PagedTiles pt = paged_tiles(first, row_reach<FORM>(last, prefix), a.window, a.sinks, 64);
+  auto entry_of = [&](int32_t i) { return (i < pt.lead ? i : pt.main + i - pt.lead) * 64; };
+  const uint32_t k_off = rows32_offset<D>((uint32_t)a.kst, wave, lane), v_off = rows32_offset<D>((uint32_t)a.vst, wave, lane);
   auto load_step = [&](int32_t i, int stage) {
     const int32_t e0 = entry_of(i);
     const int64_t n = row0 + e0;
-    load_rows32<D>(a.k + n * a.kst + (int64_t)kvh * a.ksh, T0 - e0, (uint32_t)a.kst, lds_base + 2 * stage * kTile, wave, lane);
-    load_rows32<D>(a.v + n * a.vst + (int64_t)kvh * a.vsh, T0 - e0, (uint32_t)a.vst, lds_base + (2 * stage + 1) * kTile, wave, lane);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int32_t rows = T0 - e0 - 32 * half;
+      const uint32_t to = lds_base + 2 * stage * kTile + half * (kTile / 2);
+      load_rows32<D>(a.k + (n + 32 * half) * a.kst + (int64_t)kvh * a.ksh, rows, (uint32_t)a.kst, k_off, to, wave);
+      load_rows32<D>(a.v + (n + 32 * half) * a.vst + (int64_t)kvh * a.vsh, rows, (uint32_t)a.vst, v_off, to + kTile, wave);
+    }
   };
 
   // the wave's queries and output gradients (B operands: 8 dims of row ln)
@@ -477,57 +544,77 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   float16v dq[kDims];
 #pragma unroll
   for (int d = 0; d < kDims; ++d) dq[d] = float16v{};
-  uint32_t row_at[kSteps], lo_at[kDims], hi_at[kDims];
-#pragma unroll
-  for (int c = 0; c < kSteps; ++c) row_at[c] = lds_base + (uint32_t)(ln * kRowBytes + 16 * chunk_both_slot<D>(ln, 2 * c + lh));
-  const int tr_row = 4 * lh + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-#pragma unroll
-  for (int d = 0; d < kDims; ++d) {
-    lo_at[d] = lds_base + (uint32_t)(tr_row * kRowBytes + 16 * chunk_both_slot<D>(tr_row, 4 * d + tr_chunk) + 8 * (lane & 1));
-    hi_at[d] = lds_base + (uint32_t)((tr_row + 8) * kRowBytes + 16 * chunk_both_slot<D>(tr_row + 8, 4 * d + tr_chunk) + 8 * (lane & 1));
-  }
-  auto transposed = [&](int d, uint32_t off) -> V8 {
-    const V4 lo = lds_read_tr<V4>(lo_at[d] + off), hi = lds_read_tr<V4>(hi_at[d] + off);
-    return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  };
+  const TileAt tile_lane = tile_at<D>(lds_base, lane);
   auto work = [&](int32_t e0, auto stage, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
     const uint32_t stage_at = (uint32_t)(stage * 2 * kTile);
-    float16v sc = {}, dp = {};
-#pragma unroll
-    for (int c = 0; c < kSteps; ++c) sc = mfma32<DT>(*(lds_v8*)(size_t)(row_at[c] + stage_at), qf[c], sc);
-#pragma unroll
-    for (int c = 0; c < kSteps; ++c) dp = mfma32<DT>(*(lds_v8*)(size_t)(row_at[c] + stage_at + kTile), dof[c], dp);
-    V8 df[2];
+    uint32_t rows = tile_lane.rows, cols = tile_lane.cols;
+    asm volatile("" : "+v"(rows), "+v"(cols));
+    // S^T and dP^T of each half of 32 entries, then its part of dq; fenced as above
+    constexpr int kOps = 4 * kSteps + 4 * kDims, kBoth = 2 * kSteps;
+    float16v sc[2] = {}, dp[2] = {};
+    V8 df[2][2], ring[3];
+    auto read = [&](int n) {
+      if (n < 4 * kSteps) {
+        const int half = n / kBoth, m = n % kBoth;
+        ring[n % 3] = read_rows<DT, D>(rows, m % kSteps, stage_at + half * (kTile / 2) + (m < kSteps ? 0 : kTile));
+      } else if (n < kOps) {
+        const int m = n - 4 * kSteps;
+        ring[n % 3] = read_cols<DT, D>(cols, m % kDims, stage_at + 16 * (m / kDims) * kRowBytes);
+        if constexpr (MASKED) ring[n % 3] = finite_part<DT>(ring[n % 3]);
+      }
+    };
     const float at = (float)(e0 + 4 * lh - self);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
+    auto first = [&](int half, int e) { sc[half][e] = shape_first<FORM>(shape, sc[half][e]); };
+    auto weigh = [&](int half, int e) {
       float slant = 1.f;
-      float x = shape_and_slant<FORM>(shape, sc[e], at + (float)(8 * (e >> 2) + (e & 3)), &slant) - lse;
-      bool seen = true;
+      float x = shape_and_slant<FORM>(shape, sc[half][e], at + (float)(32 * half + 8 * (e >> 2) + (e & 3)), &slant) - lse;
       if constexpr (MASKED) {
-        const int32_t j = e0 + 8 * (e >> 2) + 4 * lh + (e & 3);
-        seen = j <= reach && (j > self - a.window || j < a.sinks);
-        x = seen ? x : -INFINITY;
+        const int32_t j = e0 + 32 * half + 8 * (e >> 2) + 4 * lh + (e & 3);
+        x = j <= reach && (j > self - a.window || j < a.sinks) ? x : -INFINITY;
       }
-      float ds = __builtin_amdgcn_exp2f(x) * (dp[e] + minus_delta);
-      if constexpr (FORM & kFormCap) ds *= slant;
-      if constexpr (DT == JKV_F16) ds *= factor;
-      if constexpr (MASKED) ds = seen ? ds : 0.f;
-      df[e >> 3][e & 7] = (T)ds;
-    }
+      float p = __builtin_amdgcn_exp2f(x);
+      if constexpr (FORM & kFormCap) p *= slant;
+      if constexpr (DT == JKV_F16) p *= factor;
+      sc[half][e] = p;
+    };
+    auto lean = [&](int half, int e) {
+      float ds = sc[half][e] * (dp[half][e] + minus_delta);
+      if constexpr (MASKED) ds = sc[half][e] == 0.f ? 0.f : ds;
+      df[half][e >> 3][e & 7] = (T)ds;
+    };
+    read(0);
+    read(1);
+    each_to<kOps>([&](auto number) {
+      constexpr int n = decltype(number)::value;
+      constexpr int kEach = 16 / kSteps, kBeside = 8 / kDims;
+      read(n + 2);
+      if (n < 4 * kSteps) {
+        const int half = n / kBoth, m = n % kBoth, c = m % kSteps;
+        if (m < kSteps) sc[half] = mfma32<DT>(ring[n % 3], qf[c], sc[half]);
+        else dp[half] = mfma32<DT>(ring[n % 3], dof[c], dp[half]);
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
+        for (int e = c * kEach; e < (c + 1) * kEach; ++e) {
+          if (m >= kSteps) first(half, e);
+          if (half == 1 && m < kSteps) weigh(0, e);
+          if (half == 1 && m >= kSteps) lean(0, e);
+        }
+      } else {
+        const int m = n - 4 * kSteps, d = m % kDims, st = m / kDims;
+        dq[d] = mfma32<DT>(ring[n % 3], df[st / 2][st % 2], dq[d]);
 #pragma unroll
-      for (int d = 0; d < kDims; ++d) {
-        V8 kt = transposed(d, stage_at + 16 * st * kRowBytes);
-        if constexpr (MASKED) kt = finite_part<DT>(kt);
-        dq[d] = mfma32<DT>(kt, df[st], dq[d]);
+        for (int e = d * kBeside; e < (d + 1) * kBeside; ++e) {
+          if (st == 0) weigh(1, e);
+          if (st == 1) { weigh(1, 8 + e); lean(1, e); }
+          if (st == 2) lean(1, 8 + e);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
   // as above: the tiles that all rows see, [full0, full1), come last
-  int32_t full1 = pt.lead + (row_reach<FORM>(first, prefix) + 1) / 32 - pt.main, full0 = pt.lead;
-  if (last >= a.window && (last - a.window) / 32 + 1 > pt.main) full0 += (last - a.window) / 32 + 1 - pt.main;
+  int32_t full1 = pt.lead + (row_reach<FORM>(first, prefix) + 1) / 64 - pt.main, full0 = pt.lead;
+  if (last >= a.window && (last - a.window) / 64 + 1 > pt.main) full0 += (last - a.window) / 64 + 1 - pt.main;
   if (full1 > pt.count) full1 = pt.count;
   if (full1 <= full0) full0 = full1 = pt.count;
   const int32_t plain = full1 - full0, edge = pt.count - plain;
@@ -557,7 +644,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   for (int32_t n = edge; n > 0; --n) {
     turn_over((n & 1) ^ 1);
     const int32_t e0 = entry_of(now);
-    if (e0 <= row_reach<FORM>(wlast, prefix) && (e0 + 31 > wfirst - a.window || e0 < a.sinks)) work(e0, n & 1, std::true_type());
+    if (e0 <= row_reach<FORM>(wlast, prefix) && (e0 + 63 > wfirst - a.window || e0 < a.sinks)) work(e0, n & 1, std::true_type());
     advance(now);
   }
   for (int32_t n = 0; n < plain; n += 2) {
@@ -572,7 +659,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   if (!row_ok) return;
   // lane holds dims 32d + 8(e/4) + 4lh + e%4 of row ln
-  const float mul = a.scale * 0x1p-10f / factor;
+  const float mul = a.scale * (FORM & kFormCap ? 4.f : 1.f) * 0x1p-10f / factor;
   uint8_t* to = a.dq + ((int64_t)(row0 + self) * a.QH + head) * kRowBytes;
 #pragma unroll
   for (int d = 0; d < kDims; ++d)

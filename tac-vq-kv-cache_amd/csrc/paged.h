@@ -152,11 +152,19 @@ template <int FORM, typename Args> __device__ __forceinline__ ScoreShape score_s
   }
   return s;
 }
-template <int FORM> __device__ __forceinline__ float shape_score(const ScoreShape& s, float x, float distance) {
+// in two steps, so that a caller can put other work between them
+template <int FORM> __device__ __forceinline__ float shape_first(const ScoreShape& s, float x) {
   x *= s.mul;
-  if constexpr (FORM & kFormCap) x = fmaf(s.twice, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x)), s.cap2);
+  if constexpr (FORM & kFormCap) x = 1.f + __builtin_amdgcn_exp2f(x);
+  return x;
+}
+template <int FORM> __device__ __forceinline__ float shape_second(const ScoreShape& s, float x, float distance) {
+  if constexpr (FORM & kFormCap) x = fmaf(s.twice, __builtin_amdgcn_rcpf(x), s.cap2);
   if constexpr (FORM & kFormBias) x = fmaf(-s.slope2, fabsf(distance), x);
   return x;
+}
+template <int FORM> __device__ __forceinline__ float shape_score(const ScoreShape& s, float x, float distance) {
+  return shape_second<FORM>(s, shape_first<FORM>(s, x), distance);
 }
 
 // the first entries that all rows of a sequence see

@@ -77,7 +77,7 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   a.splits = 1;
   // blocks of all sequences at most, and one that clears unowned rows
   auto blocks_of = [&](int64_t rows) { return std::min<int64_t>(B * ceil_div(N * a.per, rows), N * a.per / rows + B) + 1; };
-  a.item_rows = D == 128 && blocks_of(256) * KVH / 256 >= 2 ? 256 : 128;
+  a.item_rows = 128;
   const int64_t items = blocks_of(a.item_rows);
   JKV_CHECK_GRID(items * KVH, 2 * a.item_rows);
   a.items = (int32_t)items;

@@ -14,9 +14,11 @@
 // itself (fp16 holds 2^-34 of it then), ds in fp16 times a power of two that keeps
 // the largest that inputs of their sizes could give below 2^15.
 //
-// A masked weight is 0, but 0 times an infinite or NaN row is not: in tiles with
-// masked places the second operands are read with such elements as 0.  Where they
-// are seen, p or delta are not finite and carry it.
+// A masked weight is 0, but 0 times an infinite or NaN row is not.  Such a row makes
+// its raw scores (or do's products) in a tile not finite, seen or not: in tiles with
+// masked places these are tested, and if one is odd the second operands are read
+// with such elements as 0.  Where they are seen, p or delta are not finite and
+// carry it.
 #pragma once
 
 #include <utility>
@@ -302,6 +304,10 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
   }
   const TileAt tile_lane = tile_at<D>(lds_base, lane);
   const int32_t key = wj0 + ln;
+  // rows [key_from, key_from + key_rows) see the lane's key
+  const int32_t key_from = key < prefix ? 0 : key;
+  int32_t key_upto = key >= a.sinks && key + a.window < T0 ? key + a.window : T0;
+  const uint32_t key_rows = key_upto > key_from ? (uint32_t)(key_upto - key_from) : 0u;
 
   // A step's products in turn: S, dP, dv, dk, and beside each a few places' vector
   // instructions, fenced (the compiler else gathers each kind, and they overlap
@@ -329,26 +335,43 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
       } else if (n < kOps) {
         const int m = (n - 2 * kSteps) % (2 * kDims);
         ring[n % 3] = read_cols<DT, D>(cols, m % kDims, stage_at + (n < 2 * kSteps + 2 * kDims ? kTile : 0) + 16 * (m / kDims) * kRowBytes);
-        if constexpr (MASKED) ring[n % 3] = finite_part<DT>(ring[n % 3]);
       }
     };
+    float odd = 0.f;
+    bool clean = false;
+    auto operand = [&](int n) -> V8 {
+      if (MASKED && clean) return finite_part<DT>(ring[n % 3]);
+      return ring[n % 3];
+    };
+    const uint32_t seen_at = (uint32_t)(t0 + 4 * lh - key_from);
     auto read_lse = [&](int q4) { lse[q4] = *(lds_f4*)(size_t)(stats_at + 32 * q4); };
-    auto first = [&](int e) { sc[e] = shape_first<FORM>(shape, sc[e]); };
+    auto first = [&](int e) {
+      if constexpr (MASKED) odd = fmaf(sc[e], 0.f, odd);
+      sc[e] = shape_first<FORM>(shape, sc[e]);
+    };
     // p, and what ds takes of it (in sc)
     auto weigh = [&](int e) {
       float slant = 1.f;
       float x = shape_and_slant<FORM>(shape, sc[e], at + (float)(8 * (e >> 2) + (e & 3)), &slant) - lse[e >> 2][e & 3];
-      if constexpr (MASKED) {
-        const int32_t i = t0 + 8 * (e >> 2) + 4 * lh + (e & 3);
-        const bool seen = (key <= i || key < prefix) && (key > i - a.window || key < a.sinks) && i < T0;
-        const float minus_delta = *(__attribute__((address_space(3))) const float*)(size_t)(stats_at + 256 + 32 * (e >> 2) + 4 * (e & 3));
-        x = seen ? fmaf(minus_delta, 0.f, x) : -INFINITY;  // (NaN where do is not finite)
-      }
       float p = __builtin_amdgcn_exp2f(x);
+      if constexpr (MASKED) {
+        const bool seen = seen_at + (uint32_t)(8 * (e >> 2) + (e & 3)) < key_rows;
+        p = seen ? p : 0.f;
+        if constexpr (FORM & kFormCap) slant = seen ? slant : 0.f;
+      }
       pf[e >> 3][e & 7] = (T)p;
       if constexpr (FORM & kFormCap) p *= slant;
       if constexpr (DT == JKV_F16) p *= factor;
       sc[e] = p;
+    };
+    // where do is not finite, delta is not, and what sees it takes a NaN
+    auto poison = [&](int e) {
+      const float minus_delta = *(__attribute__((address_space(3))) const float*)(size_t)(stats_at + 256 + 32 * (e >> 2) + 4 * (e & 3));
+      const bool seen = seen_at + (uint32_t)(8 * (e >> 2) + (e & 3)) < key_rows;
+      if (seen && !__builtin_isfinite(minus_delta)) {
+        pf[e >> 3][e & 7] = (T)NAN;
+        sc[e] = NAN;
+      }
     };
     auto lean = [&](int e) {
       float ds = sc[e] * dp[e];
@@ -383,19 +406,31 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
           for (int e = c * kWeigh; e < 8; ++e) weigh(e);
           read_lse(2);
           read_lse(3);
+          if constexpr (MASKED) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) odd = fmaf(dp[e], 0.f, odd);
+            clean = __any(odd != 0.f);
+            if (clean)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) poison(e);
+          }
         }
       } else {
         constexpr int kEach = 8 / kDims;
         const int m = (n - 2 * kSteps) % (2 * kDims), d = m % kDims, st = m / kDims;
         if (n < 2 * kSteps + 2 * kDims) {
-          dv[d] = mfma32<DT>(pf[st], ring[n % 3], dv[d]);
+          dv[d] = mfma32<DT>(pf[st], operand(n), dv[d]);
 #pragma unroll
           for (int e = d * kEach; e < (d + 1) * kEach; ++e) {
-            if (st == 0) weigh(8 + e);
-            else lean(e);
+            if (st == 0) {
+              weigh(8 + e);
+              if (MASKED && clean) poison(8 + e);
+            } else {
+              lean(e);
+            }
           }
         } else {
-          dk[d] = mfma32<DT>(df[st], ring[n % 3], dk[d]);
+          dk[d] = mfma32<DT>(df[st], operand(n), dk[d]);
           if (st == 0)
 #pragma unroll
             for (int e = d * kEach; e < (d + 1) * kEach; ++e) lean(8 + e);
@@ -541,6 +576,12 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   const float factor = ds_factor<DT, D>(a);
   const ScoreShape shape = score_shape<FORM>(a, head);
 
+  // entries [seen_from, seen_from + seen_count) are seen, and those before `sunk`
+  // more (counted from seen_from on)
+  const int32_t seen_from = self >= a.window ? self - a.window + 1 : 0;
+  const uint32_t seen_count = reach >= seen_from ? (uint32_t)(reach - seen_from + 1) : 0u;
+  const int32_t sunk = row_ok ? (a.sinks < seen_from ? a.sinks : seen_from) - seen_from : -kPagedMost - 1;
+
   float16v dq[kDims];
 #pragma unroll
   for (int d = 0; d < kDims; ++d) dq[d] = float16v{};
@@ -561,19 +602,27 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
       } else if (n < kOps) {
         const int m = n - 4 * kSteps;
         ring[n % 3] = read_cols<DT, D>(cols, m % kDims, stage_at + 16 * (m / kDims) * kRowBytes);
-        if constexpr (MASKED) ring[n % 3] = finite_part<DT>(ring[n % 3]);
       }
     };
+    float odd = 0.f;
+    bool clean = false;
+    const uint32_t seen_at = (uint32_t)(e0 + 4 * lh - seen_from);
     const float at = (float)(e0 + 4 * lh - self);
-    auto first = [&](int half, int e) { sc[half][e] = shape_first<FORM>(shape, sc[half][e]); };
+    auto first = [&](int half, int e) {
+      if constexpr (MASKED) odd = fmaf(sc[half][e], 0.f, odd);
+      sc[half][e] = shape_first<FORM>(shape, sc[half][e]);
+    };
     auto weigh = [&](int half, int e) {
       float slant = 1.f;
       float x = shape_and_slant<FORM>(shape, sc[half][e], at + (float)(32 * half + 8 * (e >> 2) + (e & 3)), &slant) - lse;
-      if constexpr (MASKED) {
-        const int32_t j = e0 + 32 * half + 8 * (e >> 2) + 4 * lh + (e & 3);
-        x = j <= reach && (j > self - a.window || j < a.sinks) ? x : -INFINITY;
-      }
       float p = __builtin_amdgcn_exp2f(x);
+      if constexpr (MASKED) {
+        const uint32_t from = seen_at + (uint32_t)(32 * half + 8 * (e >> 2) + (e & 3));
+        // (entries of the window, or first ones before it)
+        const bool seen = from < seen_count || (int32_t)from < sunk;
+        p = seen ? p : 0.f;
+        if constexpr (FORM & kFormCap) slant = seen ? slant : 0.f;
+      }
       if constexpr (FORM & kFormCap) p *= slant;
       if constexpr (DT == JKV_F16) p *= factor;
       sc[half][e] = p;
@@ -601,7 +650,8 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
         }
       } else {
         const int m = n - 4 * kSteps, d = m % kDims, st = m / kDims;
-        dq[d] = mfma32<DT>(ring[n % 3], df[st / 2][st % 2], dq[d]);
+        if (m == 0 && MASKED) clean = __any(odd != 0.f);
+        dq[d] = mfma32<DT>(MASKED && clean ? finite_part<DT>(ring[n % 3]) : ring[n % 3], df[st / 2][st % 2], dq[d]);
 #pragma unroll
         for (int e = d * kBeside; e < (d + 1) * kBeside; ++e) {
           if (st == 0) weigh(1, e);

@@ -182,3 +182,33 @@ def test_gradients(device, form, dtype, sizes, qh, kvh, dim, window, sinks):
     check_grads(texts, grads, results, want["cap"], want["slopes"])
     again = run_grads(texts, device, window=window, sinks=sinks, **call)[1]
     assert all(torch.equal(x, y) for x, y in zip(grads, again))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_gradients_beside_odd_rows(device, dtype, dim, bad):
+    """An infinite or NaN row reaches what sees it or is seen by it, and in its own
+    sequence nothing else: in tiles with masked places too."""
+
+    texts = Texts(9, [150, 200], 4, 2, dim, dtype)
+    args = dict(window=20, softcap=30.0)
+    _, clean = run_grads(texts, device, **args)
+    at = 150 + 90  # row 90 of the second sequence
+    near = slice(at - 19, at + 20)  # rows and places within its window, both ways
+    far = torch.ones(350, dtype=torch.bool, device=device)
+    far[near] = False
+    for name in ("q", "k", "v", "d"):
+        odd = Texts(9, [150, 200], 4, 2, dim, dtype)
+        getattr(odd, name)[at] = bad
+        _, grads = run_grads(odd, device, **args)
+        # a query or gradient row changes itself and the 20 places it sees; those that
+        # share a row with a changed one take it over: a key or value changes the 20
+        # rows that see it, and so what these see
+        reach = {"q": (at - 19, at + 1), "d": (at - 19, at + 1), "k": (at - 19, at + 20), "v": (at - 19, at + 20)}[name]
+        same = torch.ones(350, dtype=torch.bool, device=device)
+        same[reach[0] : reach[1]] = False
+        for got, want in zip(grads, clean):
+            assert torch.equal(got[same], want[same]), name
+        if name == "d" and bad != bad:
+            assert not torch.isfinite(grads[2][at].float()).any()

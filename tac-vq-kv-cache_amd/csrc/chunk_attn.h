@@ -875,7 +875,7 @@ static int launch_chunk(const PagedAttnArgs& a, hipStream_t stream) {
   JKV_CHECK_GRID(blocks, 2 * a.item_rows);
   const dim3 grid((uint32_t)blocks), block((uint32_t)(2 * a.item_rows));
   const bool exact = a.lse != nullptr || a.lse2 != nullptr;
-  if constexpr (D == 128) {
+  if constexpr (D == 128 && FORM == kFormPlain) {
     if (a.item_rows == 256) {
       if (exact) hipLaunchKernelGGL((paged_chunk_kernel<DT, D, true, 8, FORM>), grid, block, 0, stream, a);
       else hipLaunchKernelGGL((paged_chunk_kernel<DT, D, false, 8, FORM>), grid, block, 0, stream, a);

@@ -75,14 +75,17 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   a.sinks = (int32_t)(sinks < kPagedMost ? sinks : kPagedMost);
   a.max_new = (int32_t)N;
   a.splits = 1;
-  // blocks of all sequences at most, and one that clears unowned rows
-  auto blocks_of = [&](int64_t rows) { return std::min<int64_t>(B * ceil_div(N * a.per, rows), N * a.per / rows + B) + 1; };
+  // Blocks of 128 rows: vector instructions bound shaped scores, and two
+  // workgroups a CU, which meet apart, overlap them with products better than one
+  // of eight waves does (1.55 -> 1.46 ms for 21,760 bf16 tokens with a window of
+  // 4,096, 198 -> 180 us for four biased prompts).  At most those of all sequences,
+  // and one that clears unowned rows.
   a.item_rows = 128;
-  const int64_t items = blocks_of(a.item_rows);
+  const int64_t items = std::min<int64_t>(B * ceil_div(N * a.per, 128), N * a.per / 128 + B) + 1;
   JKV_CHECK_GRID(items * KVH, 2 * a.item_rows);
   a.items = (int32_t)items;
   // (where all blocks are resident at once, two a CU, long ones share a CU with short ones)
-  a.fold = a.item_rows == 128 && items * KVH > 256 && items * KVH <= 512 ? (int32_t)(256 / KVH) : 0x7fffffff;
+  a.fold = items * KVH > 256 && items * KVH <= 512 ? (int32_t)(256 / KVH) : 0x7fffffff;
   hipStream_t stream = (hipStream_t)stream_;
   if (dtype == JKV_F16) packed_launch_f16(a, form, D, stream);
   else packed_launch_bf16(a, form, D, stream);

@@ -6,14 +6,8 @@ namespace jkv {
 
 template <int D, int FORM>
 static void launch_packed(const PagedAttnArgs& a, hipStream_t stream) {
-  const dim3 grid((uint32_t)((int64_t)a.items * a.KVH)), block((uint32_t)(2 * a.item_rows));
-  if constexpr (D == 128) {
-    if (a.item_rows == 256) {
-      hipLaunchKernelGGL((paged_chunk_kernel<JKV_BF16, D, false, 8, FORM, true>), grid, block, 0, stream, a);
-      return;
-    }
-  }
-  hipLaunchKernelGGL((paged_chunk_kernel<JKV_BF16, D, false, 4, FORM, true>), grid, block, 0, stream, a);
+  const dim3 grid((uint32_t)((int64_t)a.items * a.KVH));
+  hipLaunchKernelGGL((paged_chunk_kernel<JKV_BF16, D, false, 4, FORM, true>), grid, dim3(256), 0, stream, a);
 }
 
 void packed_launch_bf16(const PagedAttnArgs& a, int form, int64_t D, hipStream_t stream) {

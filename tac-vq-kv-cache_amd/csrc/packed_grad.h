@@ -58,33 +58,47 @@ __global__ __launch_bounds__(256) void packed_rows_kernel(PackedGradArgs a) {
   if (from < lead) from = lead;
   float most_d = 0.f, most_v = 0.f;
   const int64_t rows = (int64_t)a.N * a.QH, stride = (int64_t)gridDim.x * kRows;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + r; row < rows; row += stride) {
-    const int32_t n = (int32_t)((uint32_t)row / (uint32_t)a.QH), head = (int32_t)(row - (int64_t)n * a.QH);
-    if (n < lead || n >= from) {
-      if (a.dq != nullptr) *(uint4v*)(a.dq + row * (2 * D) + 16 * part) = uint4v{0u, 0u, 0u, 0u};
-      continue;
+  // (four rows' loads in flight)
+  for (int64_t row0 = (int64_t)blockIdx.x * kRows + r; row0 < rows; row0 += 4 * stride) {
+    uint4v dw[4];
+    V8 o[4], rest[4];
+    int32_t n[4], head[4];
+    bool on[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = row0 + i * stride;
+      n[i] = (int32_t)((uint32_t)row / (uint32_t)a.QH);
+      head[i] = (int32_t)(row - (int64_t)n[i] * a.QH);
+      on[i] = row < rows && n[i] >= lead && n[i] < from;
+      if (row < rows && !on[i] && a.dq != nullptr) *(uint4v*)(a.dq + row * (2 * D) + 16 * part) = uint4v{0u, 0u, 0u, 0u};
+      dw[i] = uint4v{0u, 0u, 0u, 0u};
+      o[i] = V8{};
+      rest[i] = V8{};
+      if (!on[i]) continue;
+      dw[i] = *(const uint4v*)(a.d + n[i] * a.dst + head[i] * a.dsh + 16 * part);
+      o[i] = *(const V8*)(a.o + n[i] * a.ost + head[i] * a.osh + 16 * part);
+      if (a.rest != nullptr) rest[i] = *(const V8*)(a.rest + row * (2 * D) + 16 * part);
     }
-    const uint4v dw = *(const uint4v*)(a.d + n * a.dst + head * a.dsh + 16 * part);
-    const V8 d = __builtin_bit_cast(V8, dw), o = *(const V8*)(a.o + n * a.ost + head * a.osh + 16 * part);
-    float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fmaf((float)d[e], (float)o[e], sum);
-    // (where one place holds most of a row's weight, do v and delta are near each
-    // other: without the rest the gradients of bf16 rows are 3.6e-3 off, with it 2.5e-3)
-    if (a.rest != nullptr) {
-      const V8 rest = *(const V8*)(a.rest + row * (2 * D) + 16 * part);
+    for (int i = 0; i < 4; ++i) {
+      const V8 d = __builtin_bit_cast(V8, dw[i]);
+      // (where one place holds most of a row's weight, do v and delta are near each
+      // other: without the rest the gradients of bf16 rows are 3.6e-3 off, with it 2.5e-3)
+      float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf((float)d[e], (float)rest[e], sum);
-    }
-    if constexpr (DT == JKV_F16) most_d = largest_finite<DT>(dw, most_d);
+      for (int e = 0; e < 8; ++e) sum = fmaf((float)d[e], (float)o[i][e], sum);
 #pragma unroll
-    for (int off = kLanes / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    if (part == 0) {
-      const float lse = a.lse[row];
-      // (a row that saw nothing weighs nothing)
-      const int64_t at = (int64_t)head * a.N + n;
-      a.lse2[at] = lse == -INFINITY ? INFINITY : fmaf(lse, 1.4426950408889634f, -10.f);
-      a.minus_delta[at] = -sum;
+      for (int e = 0; e < 8; ++e) sum = fmaf((float)d[e], (float)rest[i][e], sum);
+      if constexpr (DT == JKV_F16) most_d = largest_finite<DT>(dw[i], most_d);
+#pragma unroll
+      for (int off = kLanes / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+      if (on[i] && part == 0) {
+        const float lse = a.lse[(int64_t)n[i] * a.QH + head[i]];
+        // (a row that saw nothing weighs nothing)
+        const int64_t at = (int64_t)head[i] * a.N + n[i];
+        a.lse2[at] = lse == -INFINITY ? INFINITY : fmaf(lse, 1.4426950408889634f, -10.f);
+        a.minus_delta[at] = -sum;
+      }
     }
   }
   const int64_t kv_rows = (int64_t)a.N * a.KVH;

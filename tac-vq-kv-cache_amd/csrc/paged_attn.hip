@@ -206,10 +206,18 @@ int jkv_paged_attention_shaped(const void* q, int64_t q_stride_t, int64_t q_stri
   max_new = std::max<int64_t>(1, std::min(max_new, N));
   a.window = (int32_t)(window > 0 && window < kPagedMost ? window : kPagedMost);
   a.sinks = (int32_t)(sinks < kPagedMost ? sinks : kPagedMost);
-  const PagedPlan p = paged_plan(N, B, QH, KVH, D, max_new, max_length, a.window, a.sinks, weights != nullptr);
+  PagedPlan p = paged_plan(N, B, QH, KVH, D, max_new, max_length, a.window, a.sinks, weights != nullptr);
   JKV_CHECK_ARG(workspace_bytes >= p.bytes && (p.bytes == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0)),
                 "paged attention needs an aligned workspace of %lld bytes, got %lld", (long long)p.bytes,
                 (long long)workspace_bytes);
+  if (form != kFormPlain && p.item_rows == 256) {
+    // Shaped scores are bound by vector instructions, and four-wave blocks, two a
+    // CU, overlap those with products better (2 x 2,048 capped bf16 tokens over 8,192
+    // entries 374 -> 343 us); they are enough to need no splits.
+    p.item_rows = 128;
+    p.items = std::min<int64_t>(B * ceil_div(max_new * (QH / KVH), 128), N * (QH / KVH) / 128 + B);
+    p.splits = 1;
+  }
   uint8_t* ws = (uint8_t*)workspace;
   a.q = (const uint8_t*)q; a.qst = 2 * q_stride_t; a.qsh = 2 * q_stride_h;
   a.out = (uint8_t*)out; a.ost = 2 * out_stride_t; a.osh = 2 * out_stride_h;

@@ -15,7 +15,7 @@ struct CopyArgs {
   PagedCache c;
   int64_t layer_bytes;
   const int32_t *sources, *targets, *entries;
-  int32_t KVH, pieces, runs;  // 16-byte pieces of a row, workgroups of a page
+  int32_t pieces, row_shift, runs;  // 16-byte pieces of a page, log2 of a row's, workgroups of a page
 };
 
 __global__ __launch_bounds__(kCopyThreads) void paged_copy_kernel(CopyArgs a) {
@@ -23,31 +23,27 @@ __global__ __launch_bounds__(kCopyThreads) void paged_copy_kernel(CopyArgs a) {
   const int32_t src = a.sources[pair], dst = a.targets[pair], size = 1 << a.c.page_shift;
   if ((uint32_t)src >= (uint32_t)a.c.n_pages || (uint32_t)dst >= (uint32_t)a.c.n_pages || src == dst) return;
   const int32_t count = a.entries != nullptr ? clamp_i32(a.entries[pair], 0, size) : size;
-  const int64_t layer = blockIdx.y;
-  const uint8_t* const pools[2] = {a.c.k, a.c.v};
-  const int64_t from = layer * a.layer_bytes + src * a.c.page_bytes, to = layer * a.layer_bytes + dst * a.c.page_bytes;
-  // a head's pieces of its first `count` rows, head after head
-  const uint32_t of_head = (uint32_t)count * (uint32_t)a.pieces, all = of_head * (uint32_t)a.KVH;
-  uint4 x[2][kCopyEach];
+  const int64_t layer = blockIdx.y * a.layer_bytes, from = layer + src * a.c.page_bytes, to = layer + dst * a.c.page_bytes;
+  uint4 k[kCopyEach], v[kCopyEach];
   int64_t off[kCopyEach];
-  for (uint32_t i0 = run * (kCopyThreads * kCopyEach) + threadIdx.x; i0 < all; i0 += (uint32_t)a.runs * (kCopyThreads * kCopyEach)) {
 #pragma unroll
-    for (int e = 0; e < kCopyEach; ++e) {
-      const uint32_t i = i0 + e * kCopyThreads;
-      off[e] = -1;
-      if (i >= all) continue;
-      const uint32_t h = i / of_head, in = i - h * of_head, slot = in / (uint32_t)a.pieces, part = in - slot * (uint32_t)a.pieces;
-      off[e] = h * a.c.head_bytes + slot * a.c.slot_bytes + 16 * part;
-#pragma unroll
-      for (int p = 0; p < 2; ++p) x[p][e] = *(const uint4*)(pools[p] + from + off[e]);
+  for (int e = 0; e < kCopyEach; ++e) {
+    // piece i of the page: head, slot, part
+    const int32_t i = (int32_t)((run * kCopyEach + e) * kCopyThreads + threadIdx.x);
+    const int32_t part = i & ((1 << a.row_shift) - 1), slot = (i >> a.row_shift) & (size - 1);
+    const bool on = i < a.pieces && slot < count;
+    off[e] = on ? (i >> (a.row_shift + a.c.page_shift)) * a.c.head_bytes + slot * a.c.slot_bytes + 16 * part : -1;
+    if (on) {
+      k[e] = *(const uint4*)(a.c.k + from + off[e]);
+      v[e] = *(const uint4*)(a.c.v + from + off[e]);
     }
-#pragma unroll
-    for (int e = 0; e < kCopyEach; ++e)
-      if (off[e] >= 0) {
-#pragma unroll
-        for (int p = 0; p < 2; ++p) *(uint4*)((uint8_t*)pools[p] + to + off[e]) = x[p][e];
-      }
   }
+#pragma unroll
+  for (int e = 0; e < kCopyEach; ++e)
+    if (off[e] >= 0) {
+      *(uint4*)(a.c.k + to + off[e]) = k[e];
+      *(uint4*)(a.c.v + to + off[e]) = v[e];
+    }
 }
 
 }  // namespace jkv
@@ -70,9 +66,10 @@ int jkv_paged_copy(void* key_pages, void* value_pages, int32_t dtype, int64_t la
   JKV_CHECK_ARG(key_pages && value_pages && sources && targets, "null buffer");
   a.layer_bytes = 2 * layer_stride;
   a.sources = sources; a.targets = targets; a.entries = entries;
-  a.KVH = (int32_t)KVH; a.pieces = (int32_t)(D / 8);
-  JKV_CHECK_ARG(page_size * a.pieces * KVH < ((int64_t)1 << 31), "pages too large");
-  a.runs = (int32_t)ceil_div(page_size * a.pieces * KVH, 2 * kCopyThreads * kCopyEach);
+  const int64_t pieces = page_size * (D / 8) * KVH;
+  JKV_CHECK_ARG(pieces < ((int64_t)1 << 30), "pages too large");
+  a.pieces = (int32_t)pieces; a.row_shift = D == 128 ? 4 : 3;
+  a.runs = (int32_t)ceil_div(pieces, kCopyThreads * kCopyEach);
   JKV_CHECK_GRID(pairs * a.runs, kCopyThreads);
   hipLaunchKernelGGL(paged_copy_kernel, dim3((uint32_t)(pairs * a.runs), (uint32_t)layers), dim3(kCopyThreads), 0,
                      (hipStream_t)stream_, a);

@@ -59,6 +59,15 @@ def _overlaps(tensor: torch.Tensor) -> bool:
     return False
 
 
+def _refuse_second_derivative(name: str) -> None:
+    """In a backward pass: gradients are recorded there if they are to be
+    differentiated again.  (A check of 0.1 us; ``once_differentiable`` costs a
+    backward of three tensors 20 us of host time.)"""
+
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name} has no second derivative")
+
+
 def rvq_encode(
     states: torch.Tensor,
     tables: torch.Tensor,

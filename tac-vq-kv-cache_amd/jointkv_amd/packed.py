@@ -13,10 +13,9 @@ and differentiable, what calibration needs.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._ops import _current, _overlaps, _plain
+from ._ops import _current, _overlaps, _plain, _refuse_second_derivative
 from .paged import _rows, _shape_args
 
 PACKED_TYPES = (torch.float16, torch.bfloat16)
@@ -68,8 +67,8 @@ class _PackedAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_out):
+        _refuse_second_derivative("packed_attention")
         query, key, value, out, rest, lse, starts, prefixes, slopes = ctx.saved_tensors
         softcap, window, sinks, scale = ctx.params
         rows, qheads, dim = query.shape

@@ -18,10 +18,9 @@ import math
 from dataclasses import dataclass
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._ops import _current, _overlaps, _plain
+from ._ops import _current, _overlaps, _plain, _refuse_second_derivative
 from .attention import MISTRAL_ROPE_THETA
 
 MOST_DIMS = 256
@@ -104,8 +103,9 @@ def _rates(rule: RotaryRule, head_dim: int) -> tuple[float, ...]:
 
 
 @functools.lru_cache(maxsize=64)
-def _rate_array(rule: RotaryRule, head_dim: int) -> ctypes.Array:
-    return _lib.ptr_array(ctypes.c_double, _rates(rule, head_dim))
+def _rate_array(rule: RotaryRule, head_dim: int) -> tuple[ctypes.Array, int, int]:
+    rates = _rates(rule, head_dim)
+    return _lib.ptr_array(ctypes.c_double, rates), len(rates), int(rule.layout == "interleaved")
 
 
 def _row_contiguous(tensor: torch.Tensor) -> torch.Tensor:
@@ -127,25 +127,23 @@ def _turn(query, key, rule, starts, positions, inverse, out=None, key_out=None):
 
     device = _lib.require_device(query, key, starts, positions, out, key_out)
     rows, heads, dim = query.shape
-    args = []
-    for tensor, to in ((query, out), (key, key_out)):
-        if tensor is None:
-            args += [None, 0, 0, None, 0, 0, 0]
-            continue
-        source, target = _row_contiguous(tensor), _target(tensor, to)
-        args += [source.data_ptr(), source.stride(0), source.stride(1), target.data_ptr(), target.stride(0),
-                 target.stride(1), tensor.shape[1]]
-        if tensor is query:
-            query_in, query_out = source, target
-        else:
-            key_in, key_result = source, target
-    rates = _rate_array(rule, dim)
+    source, target = _row_contiguous(query), _target(query, out)
+    t, h, _d = source.stride()
+    to_t, to_h, _d = target.stride()
+    if key is None:
+        key_args = (None, 0, 0, None, 0, 0, 0)
+    else:
+        key_source, key_target = _row_contiguous(key), _target(key, key_out)
+        kt, kh, _d = key_source.stride()
+        key_to_t, key_to_h, _d = key_target.stride()
+        key_args = (key_source.data_ptr(), kt, kh, key_target.data_ptr(), key_to_t, key_to_h, key.shape[1])
+    rates, pairs, interleaved = _rate_array(rule, dim)
     with _current(device):
         _lib.check(_lib.load().jkv_rotary(
-            *args, _lib.dtype_code(query.dtype), rows, dim, 2 * len(rates), int(rule.layout == "interleaved"), rates,
-            rule.magnitude, int(inverse), _lib.ptr(starts), 0 if starts is None else starts.shape[0] - 1,
-            _lib.ptr(positions), _lib.stream_handle(device)))
-    return query_out if key is None else (query_out, key_result)
+            source.data_ptr(), t, h, target.data_ptr(), to_t, to_h, heads, *key_args, _lib.dtype_code(query.dtype), rows,
+            dim, 2 * pairs, interleaved, rates, rule.magnitude, inverse, _lib.ptr(starts),
+            0 if starts is None else starts.shape[0] - 1, _lib.ptr(positions), _lib.stream_handle(device)))
+    return target if key is None else (target, key_target)
 
 
 class _Rotary(torch.autograd.Function):
@@ -160,8 +158,8 @@ class _Rotary(torch.autograd.Function):
         return _turn(query, key, rule, starts, positions, False)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_query, d_key=None):
+        _refuse_second_derivative("rotary")
         starts, positions = ctx.saved_tensors
         need = [ctx.needs_input_grad[0] and d_query is not None, ctx.needs_input_grad[1] and d_key is not None]
         if all(need):

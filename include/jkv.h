@@ -780,8 +780,11 @@ int jkv_packed_attention_backward(
     float scale, float softcap, const float* slopes, void* d_q, void* d_k,
     void* d_v, void* workspace, int64_t workspace_bytes, jkv_stream_t stream);
 
-/* Workspace of jkv_packed_attention_backward (bytes). */
-int64_t jkv_packed_backward_workspace_bytes(int64_t N, int64_t QH);
+/* Workspace of jkv_packed_attention_backward for these sizes (bytes; 0 for sizes
+ * that it refuses). */
+int64_t jkv_packed_backward_workspace_bytes(int64_t N, int64_t B, int64_t QH,
+                                            int64_t KVH, int64_t D,
+                                            int64_t window);
 
 /* Workspace of jkv_paged_attention for these sizes (bytes; 0 for sizes that it
  * refuses). */

@@ -18,9 +18,19 @@ struct PackedGradArgs {
   const float* slopes;
   float *lse2, *minus_delta;  // [QH][N]: base-2 log-sum-exp less 10, -rowsum(do o)
   float2* maxima;  // [kGradBlocks]: largest finite |do| and |v| (fp16)
-  int32_t items;   // row blocks of all sequences at most
+  // dk and dv: 32 keys a workgroup instead of 128; or the group's heads in splits
+  // of heads_each, whose sums a last launch adds up
+  int32_t alone, splits, heads_each;
+  float* part;  // [splits][dk, dv][N][KVH][D]
 };
 static const int kGradBlocks = 512;  // workgroups of the rows' pass
+
+// How dk and dv are divided.
+struct PackedGradPlan {
+  int32_t alone, splits, heads_each;
+  int64_t stats_bytes, part_at, bytes;
+};
+PackedGradPlan packed_grad_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t window);
 
 // launches of the gradients: the rows' sums, then dk and dv, then dq
 int packed_grad_launch_f16(const PackedGradArgs& a, int form, int64_t D, hipStream_t stream);

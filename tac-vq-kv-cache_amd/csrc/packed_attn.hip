@@ -34,6 +34,47 @@ static int packed_strides(const int64_t* strides, int count) {
   return JKV_OK;
 }
 
+// dk and dv: 128 keys a workgroup that walks all heads of the group (two a CU), the
+// same with the heads in splits whose sums are joined, or 32 keys a workgroup whose
+// waves share out the walk (one a CU at 128 dims, two at 64, and four times the rows'
+// traffic).  In steps of one head's 32 rows: the CUs' share of all walks, half the
+// longest walk for the end where not all CUs have one, and the join.  us of the
+// gradients of k and v with 1, 2 and 4 splits and with 32 keys, 32/8 heads of 128,
+// bf16: one sequence of 8,192 2,244, 2,027, 1,988 and 2,550; of 2,048 399, 256, 198
+// and 221; of 512 121, 85, 65 and 64; four of 2,048 740, 658, 657 and 792; eight of
+// 1,000 424, 429, 443 and 496; one of 4,096 with 8/8 heads 284 and (32 keys) 273; 48
+// texts of up to 511, 28/4 heads of 64, fp16, 286, 298, 300 and 249; 16/16 heads 190
+// and (32 keys) 250.
+PackedGradPlan packed_grad_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t window) {
+  PackedGradPlan p = {};
+  const int64_t per = QH / KVH;
+  const double mean = (double)N / (double)std::max<int64_t>(B, 1);  // rows of a sequence
+  const double seen = window > 0 ? std::min((double)window, mean) : mean;
+  const double walk = ceil(std::min(mean, seen + 128.0) / 32.0) * (double)per, all =
+      ((double)N / 128.0 + 0.5 * (double)B) * (double)KVH * walk * (1.0 - 0.5 * seen / mean);
+  const double step_us = D == 128 ? 2.4 : 1.5;
+  double least = 1e300;
+  for (int64_t each = per; each >= 1; each = each / 2) {
+    const int64_t splits = ceil_div(per, each);
+    const double join = splits > 1 ? 6.0 + 16.0 * (double)splits * (double)(N * KVH * D) / 4.5e6 : 0.0;
+    const double t = all / 512.0 + 0.5 * walk / (double)splits + join / step_us;
+    if (t < least) {
+      least = t;
+      p.heads_each = (int32_t)each;
+      p.splits = (int32_t)splits;
+    }
+  }
+  if ((D == 128 ? 2.0 : 1.2) * all / 512.0 + 0.125 * walk < least) {
+    p.alone = 1;
+    p.heads_each = (int32_t)per;
+    p.splits = 1;
+  }
+  p.stats_bytes = ceil_div(N * QH * 4, 256) * 256;
+  p.part_at = 2 * p.stats_bytes + kGradBlocks * 8;
+  p.bytes = p.part_at + (p.splits > 1 ? 2 * p.splits * N * KVH * D * 4 : 0);
+  return p;
+}
+
 }  // namespace jkv
 
 extern "C" {
@@ -93,9 +134,12 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   return JKV_OK;
 }
 
-int64_t jkv_packed_backward_workspace_bytes(int64_t N, int64_t QH) {
-  if (N <= 0 || QH <= 0 || N * QH >= ((int64_t)1 << 31)) return 0;
-  return 2 * jkv::ceil_div(N * QH * 4, 256) * 256 + jkv::kGradBlocks * 8;
+int64_t jkv_packed_backward_workspace_bytes(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t window) {
+  // sizes that the call refuses need none
+  if (N <= 0 || B < 0 || QH <= 0 || KVH <= 0 || QH % KVH || QH >= 65536 || N >= ((int64_t)1 << 30) || B >= ((int64_t)1 << 24) ||
+      N * QH >= ((int64_t)1 << 31) || (D != 64 && D != 128) || window < 0)
+    return 0;
+  return jkv::packed_grad_plan(N, B, QH, KVH, D, window).bytes;
 }
 
 int jkv_packed_attention_backward(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
@@ -121,7 +165,8 @@ int jkv_packed_attention_backward(const void* q, int64_t q_stride_t, int64_t q_s
   JKV_CHECK_ARG(q && k && v && o && d_out && lse && starts, "null buffer");
   JKV_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)rest | (uintptr_t)d_out | (uintptr_t)d_q | (uintptr_t)d_k |
                  (uintptr_t)d_v) % 16 == 0, "packed rows must be 16-byte aligned");
-  const int64_t need = jkv_packed_backward_workspace_bytes(N, QH);
+  const PackedGradPlan plan = packed_grad_plan(N, B, QH, KVH, D, window);
+  const int64_t need = plan.bytes;
   JKV_CHECK_ARG(workspace != nullptr && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need,
                 "packed gradients need an aligned workspace of %lld bytes, got %lld", (long long)need, (long long)workspace_bytes);
   PackedGradArgs a = {};
@@ -137,10 +182,11 @@ int jkv_packed_attention_backward(const void* q, int64_t q_stride_t, int64_t q_s
   a.sinks = (int32_t)(sinks < kPagedMost ? sinks : kPagedMost);
   a.scale = scale; a.scale2 = scale * 1.4426950408889634f;
   a.cap_mul = shape.cap_mul; a.cap2 = shape.cap2; a.slopes = slopes;
-  const int64_t each = ceil_div(N * QH * 4, 256) * 256;
   a.lse2 = (float*)workspace;
-  a.minus_delta = (float*)((uint8_t*)workspace + each);
-  a.maxima = (float2*)((uint8_t*)workspace + 2 * each);
+  a.minus_delta = (float*)((uint8_t*)workspace + plan.stats_bytes);
+  a.maxima = (float2*)((uint8_t*)workspace + 2 * plan.stats_bytes);
+  a.part = (float*)((uint8_t*)workspace + plan.part_at);
+  a.alone = plan.alone; a.splits = plan.splits; a.heads_each = plan.heads_each;
   if (form == kFormPlain) form = kFormShaped;
   return dtype == JKV_F16 ? packed_grad_launch_f16(a, form, D, (hipStream_t)stream_)
                           : packed_grad_launch_bf16(a, form, D, (hipStream_t)stream_);

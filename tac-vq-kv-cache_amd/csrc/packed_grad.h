@@ -217,6 +217,24 @@ __device__ __forceinline__ void load_rows32(const uint8_t* base, int32_t left, u
   }
 }
 
+// The same by one wave.
+template <int D>
+__device__ __forceinline__ void load_rows32_alone(const uint8_t* base, int32_t left, uint32_t stride, uint32_t to, int lane) {
+  constexpr int kRowBytes = 2 * D, kEach = 1024 / kRowBytes;
+  const int r = lane / (64 / kEach), slot = lane % (64 / kEach);
+  const uint32_t row = (uint32_t)r * stride, part = 16u * (uint32_t)chunk_both_slot<D>(r, slot);
+#pragma unroll
+  for (int j = 0; j < 32 / kEach; ++j) {
+    const int32_t rows = left - j * kEach;
+    const uint32_t bytes = rows > 0 ? (uint32_t)((rows < kEach ? rows : kEach) - 1) * stride + kRowBytes : 0u;
+    const uint64_t at = (uint64_t)base + (uint64_t)(j * kEach) * stride;
+    const uint4v rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)(at >> 32)) & 0xffffu,
+                         (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)bytes), 0x00020000u};
+    // (row r + 4 or 8's slots)
+    load_to_lds<16>(to + 1024u * j, row + (part ^ (D == 128 ? 16u * (j & 3) : 32u * (j & 1))), rsrc);
+  }
+}
+
 // A lane's LDS addresses in a tile of 32 rows.  Row ln's 16-byte chunk 2c + lh (an
 // operand's 8 contracted places) is at rows ^ 32c; 4 elements of each of two groups
 // of 8 rows, dim 32d + ln (transposing reads), at cols ^ 64d and, 8 rows on, at
@@ -250,29 +268,40 @@ __device__ __forceinline__ typename Half16<DT>::V8 read_cols(uint32_t cols, int 
 // dS^T Q, which take P and dS from those registers and dO and Q by transposing
 // reads in the same order.  Keys stay in registers, values in LDS, 32 rows of q and
 // do of one head come a step ahead.
-template <int DT, int D, int FORM>
-__global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a) {
+//
+// ALONE: 32 keys a workgroup, whose waves share out the steps, each with rows of
+// its own, and add their sums up in LDS in the waves' order: a quarter of the chain
+// where there are few keys or short texts.
+template <int DT, int D, int FORM, bool ALONE>
+__global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad_kernel(PackedGradArgs a) {
   typedef typename Half16<DT>::T T;
   typedef typename Half16<DT>::V8 V8;
   typedef __attribute__((address_space(3))) const float4v lds_f4;
   constexpr int kSteps = D / 16, kDims = D / 32, kRowBytes = 2 * D, kTile = 32 * kRowBytes, kStage = 2 * kTile + 512;
-  __shared__ __align__(1024) uint8_t lds[4 * kTile + 2 * kStage];  // values; twice rows of q, rows of do, their stats
+  constexpr int kKeys = ALONE ? 32 : 128, kValues = (kKeys / 32) * kTile, kStride = ALONE ? 4 : 1;
+  // values; (each wave's) twice rows of q, rows of do, their stats
+  __shared__ __align__(1024) uint8_t lds[kValues + (ALONE ? 4 : 1) * 2 * kStage];
+  static_assert(2 * kStage >= 2 * 32 * D * 4, "a wave's sums fit its rows' room");
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 31, lh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t at_item = blockIdx.x / (uint32_t)a.KVH;  // (kv heads fastest: each XCD has its own)
-  const int32_t kvh = (int32_t)(blockIdx.x - at_item * (uint32_t)a.KVH);
+  const uint32_t at_split = blockIdx.x / (uint32_t)a.KVH;  // (kv heads fastest: each XCD has its own)
+  const int32_t kvh = (int32_t)(blockIdx.x - at_split * (uint32_t)a.KVH);
+  const uint32_t at_item = ALONE ? at_split : at_split / (uint32_t)a.splits;
+  const int32_t split = ALONE ? 0 : (int32_t)(at_split - at_item * (uint32_t)a.splits);
+  // the heads of the group that it walks
+  const int32_t g0 = split * a.heads_each, heads = a.per - g0 < a.heads_each ? a.per - g0 : a.heads_each;
   int32_t b, block;
-  if (!packed_block(a, 1, 128, (int32_t)at_item, &b, &block)) return;
+  if (!packed_block(a, 1, kKeys, (int32_t)at_item, &b, &block)) return;
   b = __builtin_amdgcn_readfirstlane(b);
   block = __builtin_amdgcn_readfirstlane(block);
   const int32_t row0 = clamp_i32(a.starts[b], 0, a.N), T0 = clamp_i32(a.starts[b + 1], row0, a.N) - row0;
   const int32_t prefix = paged_prefix(a.prefixes, b, T0);
-  const int32_t j0 = 128 * block, wj0 = j0 + 32 * wave;
-  const uint32_t lds_base = lds_address(lds);
+  const int32_t j0 = kKeys * block, wj0 = ALONE ? j0 : j0 + 32 * wave;
+  const uint32_t lds_base = lds_address(lds), stages_at = kValues + (ALONE ? (uint32_t)(wave * 2 * kStage) : 0u);
 
   // values into LDS, the wave's keys into registers (B operand: 8 dims of key ln)
 #pragma unroll
-  for (int w = 0; w < 4; ++w)
+  for (int w = 0; w < kKeys / 32; ++w)
     load_rows32<D>(a.v + (int64_t)(row0 + j0 + 32 * w) * a.vst + (int64_t)kvh * a.vsh, T0 - j0 - 32 * w, (uint32_t)a.vst,
                    rows32_offset<D>((uint32_t)a.vst, wave, lane), lds_base + w * kTile, wave);
   V8 kf[kSteps];
@@ -292,23 +321,32 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
   // the rows that see some key of the block
   const int32_t i0 = prefix > j0 ? 0 : j0;
   int32_t i1 = T0;
-  if (j0 >= a.sinks && (int64_t)j0 + 127 + a.window < i1) i1 = j0 + 127 + a.window;
+  if (j0 >= a.sinks && (int64_t)j0 + kKeys - 1 + a.window < i1) i1 = j0 + kKeys - 1 + a.window;
   const int32_t tile0 = i0 / 32, tile1 = (i1 + 31) / 32;
   // steps: (row tile, head of the group), heads fastest
   const uint32_t q_off = rows32_offset<D>((uint32_t)a.qst, wave, lane), d_off = rows32_offset<D>((uint32_t)a.dst, wave, lane);
   auto load_step = [&](int32_t tile, int32_t g, int stage) {
-    const int32_t head = kvh * a.per + g, left = T0 - 32 * tile;
+    const int32_t head = kvh * a.per + g0 + g, left = T0 - 32 * tile;
     const int64_t n = row0 + 32 * tile;
-    const uint32_t to = lds_base + 4 * kTile + stage * kStage;
-    load_rows32<D>(a.q + n * a.qst + (int64_t)head * a.qsh, left, (uint32_t)a.qst, q_off, to, wave);
-    load_rows32<D>(a.d + n * a.dst + (int64_t)head * a.dsh, left, (uint32_t)a.dst, d_off, to + kTile, wave);
-    if (wave < 2) {
-      const uint64_t at = (uint64_t)((wave == 0 ? a.lse2 : a.minus_delta) + (int64_t)head * a.N + n);
-      const int32_t bytes = 4 * (left < 32 ? (left > 0 ? left : 0) : 32);
-      const uint4v rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)(at >> 32)) & 0xffffu,
-                           (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
-      load_to_lds<4>(to + 2 * kTile + 256 * wave, 4u * (uint32_t)lane, rsrc);
+    const uint32_t to = lds_base + stages_at + stage * kStage;
+    const uint8_t* q_at = a.q + n * a.qst + (int64_t)head * a.qsh;
+    const uint8_t* d_at = a.d + n * a.dst + (int64_t)head * a.dsh;
+    if constexpr (ALONE) {
+      load_rows32_alone<D>(q_at, left, (uint32_t)a.qst, to, lane);
+      load_rows32_alone<D>(d_at, left, (uint32_t)a.dst, to + kTile, lane);
+    } else {
+      load_rows32<D>(q_at, left, (uint32_t)a.qst, q_off, to, wave);
+      load_rows32<D>(d_at, left, (uint32_t)a.dst, d_off, to + kTile, wave);
     }
+    const uint32_t bytes = 4u * (uint32_t)(left < 32 ? (left > 0 ? left : 0) : 32);
+    auto load_stats = [&](const float* from, uint32_t at_to) {
+      const uint64_t at = (uint64_t)(from + (int64_t)head * a.N + n);
+      const uint4v rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)(at >> 32)) & 0xffffu,
+                           (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)bytes), 0x00020000u};
+      load_to_lds<4>(at_to, 4u * (uint32_t)lane, rsrc);
+    };
+    if (ALONE || wave == 0) load_stats(a.lse2, to + 2 * kTile);
+    if (ALONE || wave == 1) load_stats(a.minus_delta, to + 2 * kTile + 256);
   };
   float16v dk[kDims], dv[kDims];
 #pragma unroll
@@ -329,13 +367,13 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
   auto work = [&](int32_t tile, int32_t g, auto stage, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
     constexpr int kOps = 2 * kSteps + 4 * kDims;
-    const uint32_t stage_at = 4 * kTile + (uint32_t)(stage * kStage);
+    const uint32_t stage_at = stages_at + (uint32_t)(stage * kStage);
     const int32_t t0 = 32 * tile;
-    const ScoreShape shape = score_shape<FORM>(a, kvh * a.per + g);
+    const ScoreShape shape = score_shape<FORM>(a, kvh * a.per + g0 + g);
     const float at = (float)(t0 + 4 * lh - key);  // (distances below 2^24 are exact)
     uint32_t rows = tile_lane.rows, cols = tile_lane.cols;
     asm volatile("" : "+v"(rows), "+v"(cols));  // (what is made from them is not kept)
-    const uint32_t v_rows = rows + (uint32_t)(wave * kTile);
+    const uint32_t v_rows = ALONE ? rows : rows + (uint32_t)(wave * kTile);
     // row 8 q4 + 4 lh + e's statistics: of 16 rows a lane
     const uint32_t stats_at = lds_base + 16u * (uint32_t)lh + stage_at + 2 * kTile;
     float16v sc = {}, dp;
@@ -457,73 +495,140 @@ __global__ __launch_bounds__(256, 2) void packed_kv_grad_kernel(PackedGradArgs a
   // Row tiles that all of the block's keys are seen by, [full0, full1), come last and
   // have code without masks (in one loop with the masked tiles' code, the compiler
   // keeps the sums in two places: 214 registers spilled).
-  int32_t full0 = j0 + 128 <= prefix ? tile0 : j0 / 32 + 4, full1 = T0 / 32;
-  if (j0 + 128 > a.sinks && (j0 + a.window) / 32 < full1) full1 = (j0 + a.window) / 32;
+  int32_t full0 = j0 + kKeys <= prefix ? tile0 : (j0 + kKeys) / 32, full1 = T0 / 32;
+  if (j0 + kKeys > a.sinks && (j0 + a.window) / 32 < full1) full1 = (j0 + a.window) / 32;
   if (full0 < tile0) full0 = tile0;
   if (full1 > tile1) full1 = tile1;
-  if (j0 + 128 > T0 || full1 <= full0) full0 = full1 = tile1;
-  const int32_t plain = (full1 - full0) * a.per, edge = tile1 > tile0 ? (tile1 - tile0) * a.per - plain : 0;
+  if (j0 + kKeys > T0 || full1 <= full0) full0 = full1 = tile1;
+  int32_t plain = (full1 - full0) * heads, edge = tile1 > tile0 ? (tile1 - tile0) * heads - plain : 0;
   struct Step { int32_t tile, g; };
-  Step now = {tile0 == full0 ? full1 : tile0, 0};
-  if (now.tile >= tile1) now.tile = full0;
-  Step next = now;
-  // heads of a tile in turn; tiles before the full ones, behind them, then those
-  auto advance = [&](Step& s) {
-    if (++s.g < a.per) return;
-    s.g = 0;
-    const bool in_full = s.tile >= full0 && s.tile < full1;
-    ++s.tile;
-    if (in_full) return;
-    if (s.tile == full0) s.tile = full1;
-    if (s.tile >= tile1) s.tile = full0;
-  };
-  int32_t left = edge + plain;  // steps not yet loaded
-  // the step ahead into the other stage, once every load has landed and every LDS
-  // access of the step before is done, in all waves
-  auto turn_over = [&](int other) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (left > 0) {
-      load_step(next.tile, next.g, other);
-      advance(next);
-      --left;
+  // heads of a tile in turn; tiles before the full ones and those behind them; full
+  // ones from the last on, which all of a sequence's blocks see, so that they read
+  // it at about the same time (8,192 causal bf16 tokens in one sequence, 32/8 heads:
+  // 2,260 us from the first on)
+  auto advance = [&](Step& s, int32_t by) {
+    for (; by > 0; --by) {
+      if (++s.g < heads) continue;
+      s.g = 0;
+      if (++s.tile == full0) s.tile = full1;
     }
   };
-  if (left > 0) {
-    load_step(next.tile, next.g, edge & 1);  // (so that the full tiles start in stage 0)
-    advance(next);
-    --left;
+  auto go_back = [&](Step& s, int32_t by) {
+    for (; by > 0; --by) {
+      if (++s.g < heads) continue;
+      s.g = 0;
+      --s.tile;
+    }
+  };
+  Step now = {tile0 == full0 ? full1 : tile0, 0}, first_plain = {full1 - 1, 0};
+  if constexpr (ALONE) {  // a wave's share: every fourth
+    advance(now, wave);
+    go_back(first_plain, wave);
+    edge = (edge - wave + 3) / 4;
+    plain = (plain - wave + 3) / 4;
   }
+  Step next = now;
+  int32_t loaded = 0;
+  auto load_next = [&](int stage) {
+    if (loaded == edge + plain) return;
+    if (loaded == edge) next = first_plain;
+    load_step(next.tile, next.g, stage);
+    if (loaded < edge) advance(next, kStride);
+    else go_back(next, kStride);
+    ++loaded;
+  };
+  // the step ahead into the other stage, once every load has landed and every LDS
+  // access of the step before is done, in all waves (that share the rows)
+  auto turn_over = [&](int other) {
+    if constexpr (ALONE) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    load_next(other);
+  };
+  load_next(edge & 1);  // (so that the full tiles start in stage 0)
+  if constexpr (ALONE) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the values have landed
   for (int32_t n = edge; n > 0; --n) {
     turn_over((n & 1) ^ 1);
     const int32_t t0 = 32 * now.tile;
     if (wj0 < T0 && (wj0 <= t0 + 31 || wj0 < prefix) && (wj0 + 31 > t0 - a.window || wj0 < a.sinks))
       work(now.tile, now.g, n & 1, std::true_type());
-    advance(now);
+    advance(now, kStride);
   }
+  now = first_plain;
   for (int32_t n = 0; n < plain; n += 2) {
     turn_over(1);
     work(now.tile, now.g, std::integral_constant<int, 0>(), std::false_type());
-    advance(now);
+    go_back(now, kStride);
     if (n + 1 >= plain) break;
     turn_over(0);
     work(now.tile, now.g, std::integral_constant<int, 1>(), std::false_type());
-    advance(now);
+    go_back(now, kStride);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
   // lane holds dim 32d + ln of keys 8(e/4) + 4lh + e%4
   const float dv_mul = 0x1p-10f, dk_mul = a.scale * (FORM & kFormCap ? 4.f : 1.f) * 0x1p-10f / factor;
+  if constexpr (ALONE) {
+    __syncthreads();
+    float* sums = (float*)(lds + kValues);  // [wave][dk, dv][dims / 32][e][lane]
+    constexpr int kWave = 2 * kStage / 4;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        sums[wave * kWave + (16 * d + e) * 64 + lane] = dk[d][e];
+        sums[wave * kWave + (16 * (kDims + d) + e) * 64 + lane] = dv[d][e];
+      }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = wave; i < 32 * kDims; i += 4) {
+      const bool value = i >= 16 * kDims;
+      const int d = (i >> 4) % kDims, e = i & 15;
+      const int32_t j = j0 + 8 * (e >> 2) + 4 * lh + (e & 3);
+      const float* at = sums + i * 64 + lane;
+      const float sum = (at[0] + at[kWave]) + (at[2 * kWave] + at[3 * kWave]);
+      T* to = (T*)(value ? a.dv : a.dk);
+      if (j < T0 && to != nullptr) to[((int64_t)(row0 + j) * a.KVH + kvh) * D + 32 * d + ln] = (T)(sum * (value ? dv_mul : dk_mul));
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const int32_t j = wj0 + 8 * (e >> 2) + 4 * lh + (e & 3);
     if (j >= T0) continue;
     const int64_t at = ((int64_t)(row0 + j) * a.KVH + kvh) * D + ln;
+    if (a.splits > 1) {
+      const int64_t all = (int64_t)a.N * a.KVH * D;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) {
+        a.part[2 * split * all + at + 32 * d] = dk[d][e] * dk_mul;
+        a.part[(2 * split + 1) * all + at + 32 * d] = dv[d][e] * dv_mul;
+      }
+      continue;
+    }
 #pragma unroll
     for (int d = 0; d < kDims; ++d) {
       if (a.dk != nullptr) ((T*)a.dk)[at + 32 * d] = (T)(dk[d][e] * dk_mul);
       if (a.dv != nullptr) ((T*)a.dv)[at + 32 * d] = (T)(dv[d][e] * dv_mul);
     }
   }
+}
+
+// The splits' sums of dk (blockIdx.y 0) and dv added up, in their order.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedGradArgs a) {
+  typedef typename Half16<DT>::T T;
+  typedef typename Half16<DT>::V4 V4;
+  const int64_t all = (int64_t)a.N * a.KVH * D, i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  T* to = (T*)(blockIdx.y == 0 ? a.dk : a.dv);
+  if (i >= all || to == nullptr) return;
+  const int64_t n = i / ((int64_t)a.KVH * D);
+  if (n < a.starts[0] || n >= a.starts[a.B]) return;  // nobody's: 0 already
+  float4v sum = *(const float4v*)(a.part + blockIdx.y * all + i);
+  for (int s = 1; s < a.splits; ++s) sum += *(const float4v*)(a.part + (2 * s + blockIdx.y) * all + i);
+  V4 h;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) h[e] = (T)sum[e];
+  *(V4*)(to + i) = h;
 }
 
 // dq of 128 (token, head) rows of a sequence and kv head, 32 a wave, as in the
@@ -739,17 +844,25 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
 template <int DT, int D, int FORM>
 static int launch_grad(PackedGradArgs a, hipStream_t stream) {
   hipLaunchKernelGGL((packed_rows_kernel<DT, D>), dim3(kGradBlocks), dim3(256), 0, stream, a);
-  auto blocks_of = [&](int64_t per) -> int64_t {
-    const int64_t a1 = a.B * ceil_div((int64_t)a.N * per, 128), a2 = (int64_t)a.N * per / 128 + a.B;
+  auto blocks_of = [&](int64_t per, int64_t rows) -> int64_t {
+    const int64_t a1 = a.B * ceil_div((int64_t)a.N * per, rows), a2 = (int64_t)a.N * per / rows + a.B;
     return (a1 < a2 ? a1 : a2) * a.KVH;
   };
   if ((a.dk != nullptr || a.dv != nullptr) && a.B > 0) {
-    JKV_CHECK_GRID(blocks_of(1), 256);
-    hipLaunchKernelGGL((packed_kv_grad_kernel<DT, D, FORM>), dim3((uint32_t)blocks_of(1)), dim3(256), 0, stream, a);
+    const int64_t blocks = blocks_of(1, a.alone ? 32 : 128) * a.splits;
+    JKV_CHECK_GRID(blocks, 256);
+    const dim3 grid((uint32_t)blocks);
+    if (a.alone) hipLaunchKernelGGL((packed_kv_grad_kernel<DT, D, FORM, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((packed_kv_grad_kernel<DT, D, FORM, false>), grid, dim3(256), 0, stream, a);
+    if (a.splits > 1) {
+      const int64_t joins = ceil_div((int64_t)a.N * a.KVH * D, 1024);
+      JKV_CHECK_GRID(joins, 256);
+      hipLaunchKernelGGL((packed_join_kernel<DT, D>), dim3((uint32_t)joins, 2), dim3(256), 0, stream, a);
+    }
   }
   if (a.dq != nullptr && a.B > 0) {
-    JKV_CHECK_GRID(blocks_of(a.per), 256);
-    hipLaunchKernelGGL((packed_q_grad_kernel<DT, D, FORM>), dim3((uint32_t)blocks_of(a.per)), dim3(256), 0, stream, a);
+    JKV_CHECK_GRID(blocks_of(a.per, 128), 256);
+    hipLaunchKernelGGL((packed_q_grad_kernel<DT, D, FORM>), dim3((uint32_t)blocks_of(a.per, 128)), dim3(256), 0, stream, a);
   }
   JKV_CHECK_LAUNCH();
   return JKV_OK;

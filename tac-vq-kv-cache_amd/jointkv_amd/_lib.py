@@ -165,7 +165,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _vp,
          _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     ),
-    "jkv_packed_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "jkv_packed_backward_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "jkv_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32]),
     "jkv_paged_select": (
         ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),

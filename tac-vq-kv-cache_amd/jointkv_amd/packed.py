@@ -73,16 +73,17 @@ class _PackedAttention(torch.autograd.Function):
         softcap, window, sinks, scale = ctx.params
         rows, qheads, dim = query.shape
         device = query.device
+        span, sinks = _span(window, sinks)
         grads = [_plain(x)(tuple(x.shape)) if need else None
                  for x, need in zip((query, key, value), ctx.needs_input_grad)]
         places = [_place(x) for x in (query, key, value, out, d_out)]  # (copies live until the launches are queued)
         with _current(device):
-            ws_bytes = _lib.workspace_bytes("jkv_packed_backward_workspace_bytes", rows, qheads)
+            ws_bytes = getattr(_lib.load(), "jkv_packed_backward_workspace_bytes")(rows, starts.shape[0] - 1, qheads, key.shape[1], dim, span)
             workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
             _lib.check(_lib.load().jkv_packed_attention_backward(
                 *(x for _tensor, at in places[:4] for x in at), rest.data_ptr(), *places[4][1], lse.data_ptr(), _lib.dtype_code(query.dtype),
                 starts.data_ptr(), _lib.ptr(prefixes), rows, starts.shape[0] - 1, qheads, key.shape[1], dim,
-                *_span(window, sinks), scale, softcap, _lib.ptr(slopes), *map(_lib.ptr, grads), workspace.data_ptr(),
+                span, sinks, scale, softcap, _lib.ptr(slopes), *map(_lib.ptr, grads), workspace.data_ptr(),
                 ws_bytes, _lib.stream_handle(device)))
         return (*grads, *(None,) * 8)
 

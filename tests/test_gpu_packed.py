@@ -212,3 +212,159 @@ def test_gradients_beside_odd_rows(device, dtype, dim, bad):
             assert torch.equal(got[same], want[same]), name
         if name == "d" and bad != bad:
             assert not torch.isfinite(grads[2][at].float()).any()
+
+
+@pytest.mark.parametrize("dtype,form", [(torch.float16, 4), (torch.bfloat16, 1), (torch.bfloat16, 2)])
+@pytest.mark.parametrize("sizes,qh,kvh,dim,window,sinks", [
+    ([600], 16, 2, 128, None, 0),             # heads in splits, whose sums are joined
+    ([350, 90], 40, 2, 64, None, 0),
+    ([400], 6, 1, 128, 100, 4),
+    ([270, 150] * 8, 12, 12, 128, None, 0),   # 128 keys a workgroup, all heads
+    ([290, 220] * 16, 24, 24, 64, 120, 0),
+])
+def test_gradients_of_every_division(device, dtype, form, sizes, qh, kvh, dim, window, sinks):
+    texts = Texts(len(sizes), sizes, qh, kvh, dim, dtype, lead=1, tail=3, gain=1.5)
+    want, call = form_of(texts, FORMS[form], qh, device)
+    out, grads = run_grads(texts, device, window=window, sinks=sinks, **call)
+    results = texts.expect(window=window, sinks=sinks, grads=True, **want)
+    check_out(texts, out, results, want["cap"], want["slopes"])
+    check_grads(texts, grads, results, want["cap"], want["slopes"])
+    again = run_grads(texts, device, window=window, sinks=sinks, **call)[1]
+    assert all(torch.equal(x, y) for x, y in zip(grads, again))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-6, 1e4])
+def test_gradients_of_small_and_large_losses(device, dtype, size):
+    """fp16 gradients of a loss that was divided, or multiplied, by much: ds keeps
+    its digits (its scale follows the largest of do and v)."""
+
+    texts = Texts(12, [100, 60], 4, 2, 64, dtype)
+    texts.d = (texts.d.float() * (size if dtype == torch.bfloat16 or size > 1 else 1e-3)).to(dtype)
+    out, grads = run_grads(texts, device, softcap=20.0)
+    results = texts.expect(grads=True, cap=20.0)
+    h = half_step(dtype)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        want = torch.cat([r[name] for r in results])
+        size_of = torch.cat([r[name + "_size"] for r in results])
+        slack = torch.cat([r[name + "_slack"] for r in results])
+        # as in check_grads; fp16 results below 2^-14 are 2^-25 off
+        off = h * want.abs() + (h + 2.0**-22) * slack + 2.0**-12 * size_of + (2.0**-25 if dtype == torch.float16 else 1e-30)
+        got = got.cpu().double()
+        right = (got - want).abs() <= off
+        # (65,504 and half a step of 2^5 on, fp16 rounds to infinity)
+        right |= torch.isinf(got) & (got.sign() == want.sign()) & (want.abs() + off >= torch.finfo(dtype).max * (1 + h / 2))
+        assert int((~right).sum()) == 0, name
+
+
+def test_which_gradients_are_asked_for(device):
+    texts = Texts(13, [90, 40], 4, 2, 64, torch.bfloat16, tail=5)
+    _, all_of = run_grads(texts, device)
+    names = ("q", "k", "v")
+    for wanted in (("q",), ("k",), ("v",), ("q", "v")):
+        x = {n: getattr(texts, n).to(device).requires_grad_(n in wanted) for n in names}
+        out = jkv.packed_attention(x["q"], x["k"], x["v"], texts.starts.to(device))
+        grads = torch.autograd.grad(out, [x[n] for n in wanted], texts.d.to(device))
+        for n, g in zip(wanted, grads):
+            assert torch.equal(g, all_of[names.index(n)]), n
+    # leaves, strided inputs and a broadcast gradient
+    qkv = torch.cat((texts.q, texts.k, texts.v), 1).to(device).requires_grad_()
+    out = jkv.packed_attention(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], texts.starts.to(device))
+    out.sum().backward()
+    x = [getattr(texts, n).to(device).requires_grad_() for n in names]
+    whole = jkv.packed_attention(*x, texts.starts.to(device))
+    grads = torch.autograd.grad(whole, x, torch.ones_like(whole))
+    assert torch.equal(qkv.grad, torch.cat(grads, 1))
+    # one kv head seen as two: its gradient is their sum, rounded as they are
+    k1 = texts.k[:, :1].to(device).requires_grad_()
+    out = jkv.packed_attention(x[0].detach(), k1.expand(135, 2, 64), x[2].detach(), texts.starts.to(device))
+    g1 = torch.autograd.grad(out, k1, texts.d.to(device))[0]
+    k2 = texts.k[:, :1].repeat(1, 2, 1).to(device).requires_grad_()
+    out = jkv.packed_attention(x[0].detach(), k2, x[2].detach(), texts.starts.to(device))
+    g2 = torch.autograd.grad(out, k2, texts.d.to(device))[0]
+    assert torch.equal(g1, g2.sum(1, keepdim=True))
+
+
+def test_a_second_derivative_is_refused(device):
+    texts = Texts(14, [30], 2, 2, 64, torch.float16)
+    q = texts.q.to(device).requires_grad_()
+    out = jkv.packed_attention(q, texts.k.to(device), texts.v.to(device), texts.starts.to(device))
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(out.float().pow(2).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(jkv.rotary(q).float().pow(2).sum(), q, create_graph=True)
+
+
+def test_two_streams_and_graph_replays(device):
+    """Two calls at once on streams of their own, and a captured training step
+    replayed beside eager calls."""
+
+    texts = [Texts(s, [100, 50], 4, 2, 64, torch.float16) for s in (15, 16)]
+    want = [run_grads(t, device, softcap=30.0) for t in texts]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in texts]
+    got = []
+    for s, t in zip(streams, texts):
+        with torch.cuda.stream(s):
+            got.append(run_grads(t, device, softcap=30.0))
+    torch.cuda.synchronize()
+    for (o, g), (wo, wg) in zip(got, want):
+        assert torch.equal(o, wo) and all(torch.equal(x, y) for x, y in zip(g, wg))
+    held = [x.to(device) for x in (texts[0].q, texts[0].k, texts[0].v, texts[0].d)]
+    leaves = [x.clone().requires_grad_() for x in held[:3]]
+    starts = texts[0].starts.to(device)
+
+    def step():
+        out = jkv.packed_attention(*leaves, starts, softcap=30.0)
+        return out.detach(), torch.autograd.grad(out, leaves, held[3])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, grads = step()
+    for n in (1, 0, 1):
+        with torch.no_grad():
+            for x, source in zip((*leaves, held[3]), (texts[n].q, texts[n].k, texts[n].v, texts[n].d)):
+                x.copy_(source)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[n][0]) and all(torch.equal(x, y) for x, y in zip(grads, want[n][1]))
+        run_grads(texts[n], device, softcap=30.0)
+
+
+def test_a_step_from_turned_queries_to_gradients(device):
+    """Rotary, attention and their gradients together, against differences of the
+    64-bit definition along random directions."""
+
+    texts = Texts(17, [40, 25], 4, 2, 64, torch.bfloat16)
+    rule = jkv.RotaryRule(layout="interleaved", dims=32, scaling="linear", factor=2.0)
+    q, k, v = (x.to(device).requires_grad_() for x in (texts.q, texts.k, texts.v))
+    starts = texts.starts.to(device)
+    tq, tk = jkv.rotary(q, k, rule, starts=starts)
+    out = jkv.packed_attention(tq, tk, v, starts, softcap=10.0, window=30)
+    grads = torch.autograd.grad(out, (q, k, v), texts.d.to(device))
+    rates = ref.rates(32, 10000.0, "linear", 2.0)
+    at = list(range(40)) + list(range(25))
+
+    def loss(q, k, v):
+        total = 0.0
+        q, k = (ref.turn(x, at, rates, layout="interleaved") for x in (q, k))
+        for a, b in texts.spans:
+            total += (ref.attend(q[a:b], k[a:b], v[a:b], window=30, cap=10.0)["out"] * texts.d[a:b].double()).sum()
+        return float(total)
+
+    gen = torch.Generator().manual_seed(1)
+    x = [t.double() for t in (texts.q, texts.k, texts.v)]
+    for i, g in enumerate(grads):
+        way = torch.randn(x[i].shape, generator=gen, dtype=torch.float64)
+        step = 1e-4
+        moved = [[t + (s * step * way if j == i else 0) for j, t in enumerate(x)] for s in (1, -1)]
+        slope = (loss(*moved[0]) - loss(*moved[1])) / (2 * step)
+        # bf16 inputs to the products and results: four roundings of 2^-9 in the mean square over
+        # all elements' sum, here at eight times its size
+        size = float((g.cpu().double() * way).pow(2).sum().sqrt())
+        assert abs(float((g.cpu().double() * way).sum()) - slope) <= 8 * 2.0**-8 * size + 1e-3 * abs(slope)

@@ -492,13 +492,16 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
       return *(lds_v8*)(size_t)(k_at[n % kSteps] + (uint32_t)(2 * buf * kTileBytes + 32 * (n / kSteps) * kRowBytes));
     };
     auto first = [&](int kb, int e) { sc[kb][e] = shape_first<FORM>(shape, sc[kb][e]); };
+    // Without a bias the first step's maximum is the scores', and the second step
+    // subtracts the reference too; with one, the second step comes before the maximum.
+    constexpr bool kLate = !(FORM & kFormBias);
     auto second = [&](int kb, int e) {
-      sc[kb][e] = shape_second<FORM>(shape, sc[kb][e], at + (float)(32 * kb + 8 * (e >> 2) + (e & 3)));
+      sc[kb][e] = shape_second<FORM>(shape, sc[kb][e], at + (float)(32 * kb + 8 * (e >> 2) + (e & 3)), shape.cap2);
     };
     V8 pf[4];
     float sums[4] = {0.f, 0.f, 0.f, 0.f};
     auto third = [&](int kb, int e) {
-      const float p = __builtin_amdgcn_exp2f(sc[kb][e] - from);
+      const float p = __builtin_amdgcn_exp2f(kLate ? shape_second<FORM>(shape, sc[kb][e], 0.f, shape.cap2 - from) : sc[kb][e] - from);
       sums[e & 3] += p;
       pf[2 * kb + (e >> 3)][e & 7] = (T)p;
     };
@@ -508,13 +511,14 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
         for (int e = 0; e < 16; ++e) {
           const int32_t j = e0 + 32 * kb + 8 * (e >> 2) + 4 * lh + (e & 3);
           const bool seen = j <= reach && (j > self - a.window || j < a.sinks);
-          sc[kb][e] = seen ? sc[kb][e] : -INFINITY;
+          sc[kb][e] = seen ? sc[kb][e] : kLate ? shape_masked<FORM>() : -INFINITY;
         }
       }
       float mx = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, sc[kb][e]), sc[kb][e + 1]);
       mx = lanes2_max(mx);
+      if constexpr (kLate) mx = shape_second<FORM>(shape, mx, 0.f, shape.cap2);
       const bool need = mx > limit;
       if (__any(need)) {
         const float to = need ? mx - kHeld : from;
@@ -539,7 +543,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
       if (kb == 1) {
 #pragma unroll
         for (int e = c * kEach; e < (c + 1) * kEach; ++e) first(0, e);
-        if (c > 0)
+        if (c > 0 && !kLate)
 #pragma unroll
           for (int e = (c - 1) * kEach; e < c * kEach; ++e) second(0, e);
       }
@@ -547,8 +551,9 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     }
     ring[0] = value_operand(0, 0, buf);
     ring[1] = value_operand(1, 0, buf);
+    if constexpr (!kLate)
 #pragma unroll
-    for (int e = 16 - kEach; e < 16; ++e) second(0, e);
+      for (int e = 16 - kEach; e < 16; ++e) second(0, e);
     reference(0);
 #pragma unroll
     for (int e = 0; e < 8; ++e) third(0, e);
@@ -565,7 +570,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
         if (kb == 0) {
 #pragma unroll
           for (int e = n * kBeside; e < (n + 1) * kBeside; ++e) first(1, e);
-          if (n > 0)
+          if (n > 0 && !kLate)
 #pragma unroll
             for (int e = (n - 1) * kBeside; e < n * kBeside; ++e) second(1, e);
         }
@@ -574,8 +579,9 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
       if (kb == 0) {
         ring[0] = value_operand(0, 2, buf);
         ring[1] = value_operand(1, 2, buf);
+        if constexpr (!kLate)
 #pragma unroll
-        for (int e = 16 - kBeside; e < 16; ++e) second(1, e);
+          for (int e = 16 - kBeside; e < 16; ++e) second(1, e);
         reference(1);
 #pragma unroll
         for (int e = 0; e < 8; ++e) third(1, e);

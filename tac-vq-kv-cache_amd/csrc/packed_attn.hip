@@ -97,8 +97,7 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   if (rc != JKV_OK) return rc;
   if (form == kFormPlain) {
     form = kFormShaped;
-    a.q_mul = 1.f;
-    a.scale2 = scale * 1.4426950408889634f;
+    paged_scale_args(&a, scale);
   }
   if (N == 0) return JKV_OK;
   JKV_CHECK_ARG(q && k && v && out && starts, "null buffer");
@@ -181,8 +180,8 @@ int jkv_packed_attention_backward(const void* q, int64_t q_stride_t, int64_t q_s
   a.window = (int32_t)(window > 0 && window < kPagedMost ? window : kPagedMost);
   a.sinks = (int32_t)(sinks < kPagedMost ? sinks : kPagedMost);
   a.scale = scale; a.scale2 = scale * 1.4426950408889634f;
-  a.cap_mul = shape.cap_mul; a.cap2 = shape.cap2; a.slopes = slopes;
-  a.lse2 = (float*)workspace;
+  a.cap_mul = softcap > 0.f ? 2.f * a.scale2 / softcap : 0.f; a.cap2 = shape.cap2; a.slopes = slopes;
+  a.bases = (float*)workspace;
   a.minus_delta = (float*)((uint8_t*)workspace + plan.stats_bytes);
   a.maxima = (float2*)((uint8_t*)workspace + 2 * plan.stats_bytes);
   a.part = (float*)((uint8_t*)workspace + plan.part_at);

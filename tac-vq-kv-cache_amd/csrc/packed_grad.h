@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void packed_rows_kernel(PackedGradArgs a) {
         const float lse = a.lse[(int64_t)n[i] * a.QH + head[i]];
         // (a row that saw nothing weighs nothing)
         const int64_t at = (int64_t)head[i] * a.N + n[i];
-        a.lse2[at] = lse == -INFINITY ? INFINITY : fmaf(lse, 1.4426950408889634f, -10.f);
+        a.bases[at] = lse == -INFINITY ? -INFINITY : fmaf(lse, -1.4426950408889634f, 10.f + a.cap2);
         a.minus_delta[at] = -sum;
       }
     }
@@ -181,13 +181,16 @@ __device__ __forceinline__ bool packed_block(const PackedGradArgs& a, int32_t pe
   return false;
 }
 
-// Of what shape_first left of a score: its weight's exponent, and the cap's slope.
+// Of what shape_first left of a score: its weight's exponent, and a quarter of the
+// cap's slope.  `base` is cap2 less the log-sum-exp.
 template <int FORM>
-__device__ __forceinline__ float shape_and_slant(const ScoreShape& s, float x, float distance, float* slant) {
+__device__ __forceinline__ float shape_and_slant(const ScoreShape& s, float x, float distance, float base, float* slant) {
   if constexpr (FORM & kFormCap) {
     const float r = __builtin_amdgcn_rcpf(x);  // tanh = 1 - 2r
-    *slant = fmaf(-r, r, r);  // a quarter of it
-    x = fmaf(s.twice, r, s.cap2);
+    *slant = fmaf(-r, r, r);
+    x = fmaf(s.twice, r, base);
+  } else {
+    x = fmaf(x, s.mul, base);
   }
   if constexpr (FORM & kFormBias) x = fmaf(-s.slope2, fabsf(distance), x);
   return x;
@@ -345,7 +348,7 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
                            (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)bytes), 0x00020000u};
       load_to_lds<4>(at_to, 4u * (uint32_t)lane, rsrc);
     };
-    if (ALONE || wave == 0) load_stats(a.lse2, to + 2 * kTile);
+    if (ALONE || wave == 0) load_stats(a.bases, to + 2 * kTile);
     if (ALONE || wave == 1) load_stats(a.minus_delta, to + 2 * kTile + 256);
   };
   float16v dk[kDims], dv[kDims];
@@ -377,7 +380,7 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
     // row 8 q4 + 4 lh + e's statistics: of 16 rows a lane
     const uint32_t stats_at = lds_base + 16u * (uint32_t)lh + stage_at + 2 * kTile;
     float16v sc = {}, dp;
-    float4v lse[4];
+    float4v bases[4];
     V8 pf[2], df[2], ring[3], values[3];
     auto read = [&](int n) {
       if (n < kSteps) ring[n % 3] = read_rows<DT, D>(rows, n, stage_at);
@@ -396,7 +399,7 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
       return ring[n % 3];
     };
     const uint32_t seen_at = (uint32_t)(t0 + 4 * lh - key_from);
-    auto read_lse = [&](int q4) { lse[q4] = *(lds_f4*)(size_t)(stats_at + 32 * q4); };
+    auto read_bases = [&](int q4) { bases[q4] = *(lds_f4*)(size_t)(stats_at + 32 * q4); };
     auto first = [&](int e) {
       if constexpr (MASKED) odd = fmaf(sc[e], 0.f, odd);
       sc[e] = shape_first<FORM>(shape, sc[e]);
@@ -404,7 +407,7 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
     // p, and what ds takes of it (in sc)
     auto weigh = [&](int e) {
       float slant = 1.f;
-      float x = shape_and_slant<FORM>(shape, sc[e], at + (float)(8 * (e >> 2) + (e & 3)), &slant) - lse[e >> 2][e & 3];
+      const float x = shape_and_slant<FORM>(shape, sc[e], at + (float)(8 * (e >> 2) + (e & 3)), bases[e >> 2][e & 3], &slant);
       float p = __builtin_amdgcn_exp2f(x);
       if constexpr (MASKED) {
         const bool seen = seen_at + (uint32_t)(8 * (e >> 2) + (e & 3)) < key_rows;
@@ -443,7 +446,7 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
       read(n + 2);
       if (n < kSteps) {
         sc = mfma32<DT>(ring[n % 3], kf[n], sc);
-        if (n == kSteps - 2) { read_lse(0); read_lse(1); }
+        if (n == kSteps - 2) { read_bases(0); read_bases(1); }
       } else if (n < 2 * kSteps) {
         constexpr int kFirst = 16 / kSteps, kWeigh = 8 / kSteps;
         const int c = n - kSteps;
@@ -456,8 +459,8 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
         if (c == kSteps - 1) {
 #pragma unroll
           for (int e = c * kWeigh; e < 8; ++e) weigh(e);
-          read_lse(2);
-          read_lse(3);
+          read_bases(2);
+          read_bases(3);
           if constexpr (MASKED) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) odd = fmaf(dp[e], 0.f, odd);
@@ -691,7 +694,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
       dof[c] = *(const V8*)(dp + 32 * c);
     }
   }
-  const float lse = a.lse2[(int64_t)head * a.N + row0 + self], minus_delta = a.minus_delta[(int64_t)head * a.N + row0 + self];
+  const float base = a.bases[(int64_t)head * a.N + row0 + self], minus_delta = a.minus_delta[(int64_t)head * a.N + row0 + self];
   const float factor = ds_factor<DT, D>(a);
   const ScoreShape shape = score_shape<FORM>(a, head);
 
@@ -733,7 +736,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
     };
     auto weigh = [&](int half, int e) {
       float slant = 1.f;
-      float x = shape_and_slant<FORM>(shape, sc[half][e], at + (float)(32 * half + 8 * (e >> 2) + (e & 3)), &slant) - lse;
+      const float x = shape_and_slant<FORM>(shape, sc[half][e], at + (float)(32 * half + 8 * (e >> 2) + (e & 3)), base, &slant);
       float p = __builtin_amdgcn_exp2f(x);
       if constexpr (MASKED) {
         const uint32_t from = seen_at + (uint32_t)(32 * half + 8 * (e >> 2) + (e & 3));

@@ -136,8 +136,8 @@ enum { kFormPlain = 0, kFormShaped = 1, kFormCap = 2, kFormBias = 4 };
 
 // A shaped score is cap * tanh(scale q k / cap) - slope * distance, in base 2.
 // With E = exp(2x), tanh x = 1 - 2 / (1 + E): two transcendental instructions of
-// 7 cycles each and three others, where a rational function of x^2 as exact
-// would take eleven of 2 and a reciprocal.  Of a cap c it is within 2e-7 c, and
+// 8 cycles each and three others of 4, where a rational function of x^2 as exact
+// would take eleven and a reciprocal.  Of a cap c it is within 2e-7 c, and
 // right at infinite scores.
 struct ScoreShape {
   float mul, cap2, twice, slope2;
@@ -146,26 +146,30 @@ template <int FORM, typename Args> __device__ __forceinline__ ScoreShape score_s
   ScoreShape s = {};
   if constexpr (FORM != kFormPlain) {
     s.mul = FORM & kFormCap ? a.cap_mul : a.scale2;
-    s.cap2 = a.cap2;
+    s.cap2 = a.cap2;  // (0 without a cap)
     s.twice = -2.f * a.cap2;
     if constexpr (FORM & kFormBias) s.slope2 = a.slopes[head] * 1.4426950408889634f;
   }
   return s;
 }
-// in two steps, so that a caller can put other work between them
+// In two steps, so that a caller can put other work between them.  The first, which
+// with a cap leaves 1 + E, grows with the score (the host makes `mul` positive); the
+// second adds `base`, cap2 less what the caller moves scores by.
 template <int FORM> __device__ __forceinline__ float shape_first(const ScoreShape& s, float x) {
-  x *= s.mul;
-  if constexpr (FORM & kFormCap) x = 1.f + __builtin_amdgcn_exp2f(x);
+  if constexpr (FORM & kFormCap) x = 1.f + __builtin_amdgcn_exp2f(x * s.mul);
   return x;
 }
-template <int FORM> __device__ __forceinline__ float shape_second(const ScoreShape& s, float x, float distance) {
-  if constexpr (FORM & kFormCap) x = fmaf(s.twice, __builtin_amdgcn_rcpf(x), s.cap2);
+template <int FORM> __device__ __forceinline__ float shape_second(const ScoreShape& s, float x, float distance, float base) {
+  if constexpr (FORM & kFormCap) x = fmaf(s.twice, __builtin_amdgcn_rcpf(x), base);
+  else x = fmaf(x, s.mul, base);
   if constexpr (FORM & kFormBias) x = fmaf(-s.slope2, fabsf(distance), x);
   return x;
 }
 template <int FORM> __device__ __forceinline__ float shape_score(const ScoreShape& s, float x, float distance) {
-  return shape_second<FORM>(s, shape_first<FORM>(s, x), distance);
+  return shape_second<FORM>(s, shape_first<FORM>(s, x), distance, s.cap2);
 }
+// What the first step of a masked score is: its second is -infinity.
+template <int FORM> __device__ __forceinline__ float shape_masked() { return FORM & kFormCap ? 0.f : -INFINITY; }
 
 // the first entries that all rows of a sequence see
 __device__ __forceinline__ int32_t paged_prefix(const int32_t* prefixes, int32_t b, int32_t length) {
@@ -274,6 +278,7 @@ int paged_cache_args(PagedCache* c, const void* k, const void* v, int64_t page_s
                      const int32_t* positions, int64_t N, int64_t B, int64_t KVH, int64_t D, int64_t max_length,
                      int32_t dtype);
 int paged_rope_args(RopeRates* r, double theta, int64_t D);
+void paged_scale_args(PagedAttnArgs* a, float scale);
 int paged_form_args(PagedAttnArgs* a, int* form, float scale, float softcap, const float* slopes, const int32_t* prefixes);
 
 }  // namespace jkv

@@ -125,6 +125,14 @@ static PagedPlan paged_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64
   return p;
 }
 
+// A shaped score's scale, above 0: a negative one turns the queries round, and one
+// of 0 is near it (a masked score is -infinity times it).
+void paged_scale_args(PagedAttnArgs* a, float scale) {
+  a->q_mul = a->rope.on ? 0.5f : 1.f;  // a rotated fp16 query reaches sqrt 2 of its size
+  a->scale2 = fmaxf(fabsf(scale) * 1.4426950408889634f / a->q_mul, 1e-37f);
+  if (scale < 0.f) a->q_mul = -a->q_mul;
+}
+
 // what becomes of a score: the form's bits and what its kernels take
 int paged_form_args(PagedAttnArgs* a, int* form, float scale, float softcap, const float* slopes, const int32_t* prefixes) {
   *form = kFormPlain;
@@ -134,9 +142,7 @@ int paged_form_args(PagedAttnArgs* a, int* form, float scale, float softcap, con
   *form = kFormShaped | (softcap > 0.f ? kFormCap : 0) | (slopes != nullptr ? kFormBias : 0);
   a->slopes = slopes;
   a->prefixes = prefixes;
-  // a rotated fp16 query reaches sqrt 2 of its size
-  a->q_mul = a->rope.on ? 0.5f : 1.f;
-  a->scale2 = scale * 1.4426950408889634f / a->q_mul;
+  paged_scale_args(a, scale);
   if (softcap > 0.f) {
     a->cap_mul = 2.f * a->scale2 / softcap;
     a->cap2 = softcap * 1.4426950408889634f;

@@ -368,3 +368,23 @@ def test_a_step_from_turned_queries_to_gradients(device):
         # all elements' sum, here at eight times its size
         size = float((g.cpu().double() * way).pow(2).sum().sqrt())
         assert abs(float((g.cpu().double() * way).sum()) - slope) <= 8 * 2.0**-8 * size + 1e-3 * abs(slope)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=NAMES)
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.5])
+def test_scales(device, form, scale):
+    """Any scale, a negative one and none at all."""
+
+    texts = Texts(18, [100, 70], 4, 2, 64, torch.float16, gain=0.7)
+    want, call = form_of(texts, form, 4, device)
+    out, grads = run_grads(texts, device, scale=scale, window=60, **call)
+    results = texts.expect(scale=scale, window=60, grads=True, **want)
+    check_out(texts, out, results, want["cap"], want["slopes"])
+    check_grads(texts, grads, results, want["cap"], want["slopes"])
+    if not form:
+        return  # (a paged call of plain scores rounds the scaled queries: tested with the others)
+    pages = jkv.PagedKVCache(1, 2, 20, 2, max_length=100, page_size=16, head_dim=64, device=device)
+    step = pages.begin([100, 70])
+    pages.append(0, step, texts.k.to(device), texts.v.to(device), rope_theta=None)
+    paged = pages.attention(0, step, texts.q.to(device), rope_theta=None, scale=scale, window=60, **call)
+    check_out(texts, paged, results, want["cap"], want["slopes"])

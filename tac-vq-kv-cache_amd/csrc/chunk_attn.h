@@ -358,6 +358,11 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   constexpr float kHeld = DT == JKV_F16 ? 6.f : 10.f, kRoom = DT == JKV_F16 ? 9.f : 24.f;
   float from = 0.f;
   const ScoreShape shape = score_shape<FORM>(a, head);
+  // a shaped row sees entries [seen_from, seen_from + seen_count), and those before
+  // `sunk` more (counted from seen_from on)
+  const int32_t seen_from = self >= a.window ? self - a.window + 1 : 0;
+  const uint32_t seen_count = reach >= seen_from ? (uint32_t)(reach - seen_from + 1) : 0u;
+  const int32_t sunk = reach >= 0 ? (a.sinks < seen_from ? a.sinks : seen_from) - seen_from : -kPagedMost - 1;
 #pragma unroll
   for (int d = 0; d < kDims; ++d) o[d] = float16v{};
   // LDS addresses: a few per lane, the rest are offsets known at compile time
@@ -507,10 +512,11 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     };
     auto reference = [&](int kb) {
       if (!(is & kWaveFull)) {
+        const uint32_t seen_at = (uint32_t)(e0 + 32 * kb + 4 * lh - seen_from);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int32_t j = e0 + 32 * kb + 8 * (e >> 2) + 4 * lh + (e & 3);
-          const bool seen = j <= reach && (j > self - a.window || j < a.sinks);
+          const uint32_t n = seen_at + (uint32_t)(8 * (e >> 2) + (e & 3));
+          const bool seen = n < seen_count || (int32_t)n < sunk;
           sc[kb][e] = seen ? sc[kb][e] : kLate ? shape_masked<FORM>() : -INFINITY;
         }
       }
@@ -595,7 +601,9 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     const int32_t is = __builtin_amdgcn_readlane(what, i - run0);
     meet();
     load_stage(i + 1, buf ^ 1);
-    if (!(is & kBlockFull)) clean(buf);
+    // (shaped scores: a value that is not finite, seen or not, makes the sums so, and
+    // the walk is made again with all tiles cleaned)
+    if (FORM == kFormPlain && !(is & kBlockFull)) clean(buf);
     if (is & kWaveSees) {
       if constexpr (FORM == kFormPlain) work(i, is, parity, std::false_type());
       else work_shaped(i, is, parity, std::false_type());

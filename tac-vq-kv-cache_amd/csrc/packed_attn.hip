@@ -58,7 +58,7 @@ PackedGradPlan packed_grad_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, i
     const int64_t splits = ceil_div(per, each);
     const double join = splits > 1 ? 6.0 + 16.0 * (double)splits * (double)(N * KVH * D) / 4.5e6 : 0.0;
     const double t = all / 512.0 + 0.5 * walk / (double)splits + join / step_us;
-    if (t < least) {
+    if (t < 0.95 * least) {
       least = t;
       p.heads_each = (int32_t)each;
       p.splits = (int32_t)splits;

@@ -76,8 +76,8 @@ __global__ __launch_bounds__(256) void packed_rows_kernel(PackedGradArgs a) {
       rest[i] = V8{};
       if (!on[i]) continue;
       dw[i] = *(const uint4v*)(a.d + n[i] * a.dst + head[i] * a.dsh + 16 * part);
-      o[i] = *(const V8*)(a.o + n[i] * a.ost + head[i] * a.osh + 16 * part);
-      if (a.rest != nullptr) rest[i] = *(const V8*)(a.rest + row * (2 * D) + 16 * part);
+      o[i] = __builtin_nontemporal_load((const V8*)(a.o + n[i] * a.ost + head[i] * a.osh + 16 * part));
+      if (a.rest != nullptr) rest[i] = __builtin_nontemporal_load((const V8*)(a.rest + row * (2 * D) + 16 * part));
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -626,8 +626,8 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedGradArgs a) {
   if (i >= all || to == nullptr) return;
   const int64_t n = i / ((int64_t)a.KVH * D);
   if (n < a.starts[0] || n >= a.starts[a.B]) return;  // nobody's: 0 already
-  float4v sum = *(const float4v*)(a.part + blockIdx.y * all + i);
-  for (int s = 1; s < a.splits; ++s) sum += *(const float4v*)(a.part + (2 * s + blockIdx.y) * all + i);
+  float4v sum = __builtin_nontemporal_load((const float4v*)(a.part + blockIdx.y * all + i));
+  for (int s = 1; s < a.splits; ++s) sum += __builtin_nontemporal_load((const float4v*)(a.part + (2 * s + blockIdx.y) * all + i));
   V4 h;
 #pragma unroll
   for (int e = 0; e < 4; ++e) h[e] = (T)sum[e];

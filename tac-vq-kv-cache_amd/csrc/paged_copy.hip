@@ -3,7 +3,10 @@
 //
 // Memory bounds it: each byte that counts is read and written once, in 16-byte
 // pieces, of keys and values both.  A workgroup takes a run of one page's rows
-// (head, slot) in one layer.  Only the rows below a pair's entry count move.
+// (head, slot) in one layer.  Only the rows below a pair's entry count move.  Loads
+// and stores that the caches need not keep: 402 MB of whole pages 187 -> 140 us
+// (5.7 TB/s of both), the used parts of eight pages in 32 layers, 33 MB, 28 -> 15;
+// two pieces a thread 138 and 15.6, eight 247 and 36.
 #include "paged.h"
 
 namespace jkv {
@@ -24,7 +27,7 @@ __global__ __launch_bounds__(kCopyThreads) void paged_copy_kernel(CopyArgs a) {
   if ((uint32_t)src >= (uint32_t)a.c.n_pages || (uint32_t)dst >= (uint32_t)a.c.n_pages || src == dst) return;
   const int32_t count = a.entries != nullptr ? clamp_i32(a.entries[pair], 0, size) : size;
   const int64_t layer = blockIdx.y * a.layer_bytes, from = layer + src * a.c.page_bytes, to = layer + dst * a.c.page_bytes;
-  uint4 k[kCopyEach], v[kCopyEach];
+  uint4v k[kCopyEach], v[kCopyEach];
   int64_t off[kCopyEach];
 #pragma unroll
   for (int e = 0; e < kCopyEach; ++e) {
@@ -34,15 +37,15 @@ __global__ __launch_bounds__(kCopyThreads) void paged_copy_kernel(CopyArgs a) {
     const bool on = i < a.pieces && slot < count;
     off[e] = on ? (i >> (a.row_shift + a.c.page_shift)) * a.c.head_bytes + slot * a.c.slot_bytes + 16 * part : -1;
     if (on) {
-      k[e] = *(const uint4*)(a.c.k + from + off[e]);
-      v[e] = *(const uint4*)(a.c.v + from + off[e]);
+      k[e] = __builtin_nontemporal_load((const uint4v*)(a.c.k + from + off[e]));
+      v[e] = __builtin_nontemporal_load((const uint4v*)(a.c.v + from + off[e]));
     }
   }
 #pragma unroll
   for (int e = 0; e < kCopyEach; ++e)
     if (off[e] >= 0) {
-      *(uint4*)(a.c.k + to + off[e]) = k[e];
-      *(uint4*)(a.c.v + to + off[e]) = v[e];
+      __builtin_nontemporal_store(k[e], (uint4v*)(a.c.k + to + off[e]));
+      __builtin_nontemporal_store(v[e], (uint4v*)(a.c.v + to + off[e]));
     }
 }
 

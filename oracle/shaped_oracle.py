@@ -68,7 +68,7 @@ def scores(query, key, *, scale, cap, slope, first):
         raw, steep = cap * bent, 1 - bent**2
     if slope is not None:
         i = torch.arange(query.shape[0])[:, None] + first
-        raw = raw - slope * (i - torch.arange(key.shape[0])[None]).abs()
+        raw = raw - slope * (i - torch.arange(key.shape[0])[None]).abs().double()
     return raw, steep
 
 

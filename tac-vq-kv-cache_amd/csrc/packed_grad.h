@@ -36,15 +36,21 @@ template <int N, typename F> __device__ __forceinline__ void each_to(F&& f) {
   each_of(f, std::make_integer_sequence<int, N>());
 }
 
-// max of |x| over the finite halves of w, 0 if there are none
-template <int DT>
-__device__ __forceinline__ float largest_finite(uint4v w, float most) {
-  typedef typename Half16<DT>::T T;
-  typedef typename Half16<DT>::V8 V8;
-  const V8 v = finite_part<DT>(__builtin_bit_cast(V8, w));
+// The largest |x| over finite fp16 halves, as halves of bits plus 2^10: those of
+// infinities and NaN become negative and lose every comparison.
+typedef short short2v __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ short2v largest_finite(uint4v w, short2v most) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf((float)v[e]));
+  for (int e = 0; e < 4; ++e) {
+    const ushort2v bits = __builtin_bit_cast(ushort2v, w[e] & 0x7fff7fffu) + (unsigned short)0x0400;
+    most = __builtin_elementwise_max(most, __builtin_bit_cast(short2v, bits));
+  }
   return most;
+}
+__device__ __forceinline__ float largest_value(short2v most) {
+  const short m = most[0] > most[1] ? most[0] : most[1];
+  return (float)__builtin_bit_cast(_Float16, (short)(m - 0x0400));
 }
 
 // Per row: delta, and the log-sum-exp as the walks take it.  Rows that no sequence
@@ -56,7 +62,7 @@ __global__ __launch_bounds__(256) void packed_rows_kernel(PackedGradArgs a) {
   const int tid = threadIdx.x, part = tid % kLanes, r = tid / kLanes;
   int32_t lead = clamp_i32(a.starts[0], 0, a.N), from = clamp_i32(a.starts[a.B], 0, a.N);
   if (from < lead) from = lead;
-  float most_d = 0.f, most_v = 0.f;
+  short2v most_d = {0x0400, 0x0400}, most_v = {0x0400, 0x0400};
   const int64_t rows = (int64_t)a.N * a.QH, stride = (int64_t)gridDim.x * kRows;
   // (four rows' loads in flight)
   for (int64_t row0 = (int64_t)blockIdx.x * kRows + r; row0 < rows; row0 += 4 * stride) {
@@ -89,7 +95,7 @@ __global__ __launch_bounds__(256) void packed_rows_kernel(PackedGradArgs a) {
       for (int e = 0; e < 8; ++e) sum = fmaf((float)d[e], (float)o[i][e], sum);
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = fmaf((float)d[e], (float)rest[i][e], sum);
-      if constexpr (DT == JKV_F16) most_d = largest_finite<DT>(dw[i], most_d);
+      if constexpr (DT == JKV_F16) most_d = largest_finite(dw[i], most_d);
 #pragma unroll
       for (int off = kLanes / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
       if (on[i] && part == 0) {
@@ -109,17 +115,18 @@ __global__ __launch_bounds__(256) void packed_rows_kernel(PackedGradArgs a) {
         if (a.dk != nullptr) *(uint4v*)(a.dk + row * (2 * D) + 16 * part) = uint4v{0u, 0u, 0u, 0u};
         if (a.dv != nullptr) *(uint4v*)(a.dv + row * (2 * D) + 16 * part) = uint4v{0u, 0u, 0u, 0u};
       } else if constexpr (DT == JKV_F16) {
-        most_v = largest_finite<DT>(*(const uint4v*)(a.v + n * a.vst + head * a.vsh + 16 * part), most_v);
+        most_v = largest_finite(*(const uint4v*)(a.v + n * a.vst + head * a.vsh + 16 * part), most_v);
       }
     }
   if constexpr (DT == JKV_F16) {
     __shared__ float2 waves[4];
+    float d = largest_value(most_d), v = largest_value(most_v);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) {
-      most_d = fmaxf(most_d, __shfl_xor(most_d, off, 64));
-      most_v = fmaxf(most_v, __shfl_xor(most_v, off, 64));
+      d = fmaxf(d, __shfl_xor(d, off, 64));
+      v = fmaxf(v, __shfl_xor(v, off, 64));
     }
-    if ((tid & 63) == 0) waves[tid >> 6] = float2{most_d, most_v};
+    if ((tid & 63) == 0) waves[tid >> 6] = float2{d, v};
     __syncthreads();
     if (tid == 0)
       a.maxima[blockIdx.x] = float2{fmaxf(fmaxf(waves[0].x, waves[1].x), fmaxf(waves[2].x, waves[3].x)),

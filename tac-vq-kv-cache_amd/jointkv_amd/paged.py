@@ -703,7 +703,8 @@ class PagedKVCache:
         them: both list the same pages, and :meth:`begin` copies a half-written
         one before either writes to it.  The weights that the entries received
         are taken over.  Only sequences without evicted entries have a first
-        ``length``."""
+        ``length``.  To be called between steps: what the latest one's layers
+        have yet to append, a page copied by the next ``begin`` would miss."""
 
         have = self._lengths[source]
         length = have if length is None else int(length)

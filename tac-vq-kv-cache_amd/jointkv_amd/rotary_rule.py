@@ -90,6 +90,9 @@ def _rates(rule: RotaryRule, head_dim: int) -> tuple[float, ...]:
     if rule.scaling == "base":
         if dims <= 2:
             raise ValueError("scaling the base needs more than one pair")
+        grown = math.log(theta) + math.log(rule.factor) * dims / (dims - 2)
+        if abs(grown) > 700.0:
+            raise ValueError("the scaled rotary base passes 64 bits")
         theta *= rule.factor ** (dims / (dims - 2))
     rates = [theta ** (-2.0 * i / dims) for i in range(dims // 2)]
     if rule.scaling == "linear":

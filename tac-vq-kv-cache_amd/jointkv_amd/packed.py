@@ -78,7 +78,8 @@ class _PackedAttention(torch.autograd.Function):
                  for x, need in zip((query, key, value), ctx.needs_input_grad)]
         places = [_place(x) for x in (query, key, value, out, d_out)]  # (copies live until the launches are queued)
         with _current(device):
-            ws_bytes = getattr(_lib.load(), "jkv_packed_backward_workspace_bytes")(rows, starts.shape[0] - 1, qheads, key.shape[1], dim, span)
+            ws_bytes = _lib.workspace_bytes("jkv_packed_backward_workspace_bytes", rows, starts.shape[0] - 1, qheads,
+                                            key.shape[1], dim, span)
             workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
             _lib.check(_lib.load().jkv_packed_attention_backward(
                 *(x for _tensor, at in places[:4] for x in at), rest.data_ptr(), *places[4][1], lse.data_ptr(), _lib.dtype_code(query.dtype),

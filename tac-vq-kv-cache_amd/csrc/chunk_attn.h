@@ -46,6 +46,18 @@ namespace jkv {
 
 static const int kChunkTile = 64;
 
+// sum + a + b in 32 bits (ones times both)
+template <int DT>
+__device__ __forceinline__ float add_pair(typename Half16<DT>::T a, typename Half16<DT>::T b, float sum) {
+  if constexpr (DT == JKV_F16) {
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(half2v{a, b}, half2v{(_Float16)1.f, (_Float16)1.f}, sum, false);
+  } else {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(bf16x2{a, b}, bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false);
+  }
+}
+
 template <int DT>
 __device__ __forceinline__ float16v mfma32(typename Half16<DT>::V8 a, typename Half16<DT>::V8 b, float16v c) {
   if constexpr (DT == JKV_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -168,8 +180,9 @@ template <int FORM> __device__ __forceinline__ int32_t row_reach(int32_t i, int3
 
 // LINEAR: keys and values lie packed as the queries do, a sequence's rows are its
 // entries (the cache's head and slot strides are the keys', v_head_bytes and
-// v_slot_bytes the values').  Rows that no sequence owns get zeros.
-template <int DT, int D, bool EXACT, int kChunkWaves, int FORM = kFormPlain, bool LINEAR = false>
+// v_slot_bytes the values').  Rows that no sequence owns get zeros.  LSE: the
+// logarithms of the rows' sums are wanted.
+template <int DT, int D, bool EXACT, int kChunkWaves, int FORM = kFormPlain, bool LINEAR = false, bool LSE = EXACT>
 __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedAttnArgs a) {
   typedef typename Half16<DT>::T T;
   typedef typename Half16<DT>::V8 V8;
@@ -348,13 +361,17 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   // holds weights of 2^-34.  (In units of scale2, a power of two that only
   // large scales need.)
   float16v shift = {}, o[kDims];
-  float l = 0.f, limit = -INFINITY;
+  float l = 0.f, kept = 0.f, limit = -INFINITY;
   // Shaped scores are moved by `from` instead, the reference less kHeld, which
   // moves when a maximum passes it by kRoom: sharp heads move it often, and each
   // time costs a rescaling (with 10 and 4, a quarter of the vector instructions of
   // capped 8,192-token texts).  fp16 p stay below 2^15 and hold weights of 2^-30,
   // bf16 ones below 2^34 (values past 2^93 over the number of entries can pass 32
-  // bits).
+  // bits).  Their outputs are divided by `kept`, the sum of the p as rounded for the
+  // products, not by `l`, which only a row's lse takes (LSE): where one entry holds
+  // most of a row its rounding cancels, in the output and in the do out that gradients
+  // subtract (queries four times a unit normal, bf16: outputs 1.9e-3 off instead of
+  // 2.4e-3, dq 2.6e-3 instead of 3.5e-3).  Both sums are 6 % of a training chunk.
   constexpr float kHeld = DT == JKV_F16 ? 6.f : 10.f, kRoom = DT == JKV_F16 ? 9.f : 24.f;
   float from = 0.f;
   const ScoreShape shape = score_shape<FORM>(a, head);
@@ -504,11 +521,16 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
       sc[kb][e] = shape_second<FORM>(shape, sc[kb][e], at + (float)(32 * kb + 8 * (e >> 2) + (e & 3)), shape.cap2);
     };
     V8 pf[4];
-    float sums[4] = {0.f, 0.f, 0.f, 0.f};
+    float sums[4] = {0.f, 0.f, 0.f, 0.f}, keeps[2] = {0.f, 0.f};
+    auto keep = [&](int kb, int e) {
+      const V8& p8 = pf[2 * kb + (e >> 3)];
+      keeps[e >> 1 & 1] = add_pair<DT>(p8[e & 7], p8[(e & 7) + 1], keeps[e >> 1 & 1]);
+    };
     auto third = [&](int kb, int e) {
       const float p = __builtin_amdgcn_exp2f(kLate ? shape_second<FORM>(shape, sc[kb][e], 0.f, shape.cap2 - from) : sc[kb][e] - from);
-      sums[e & 3] += p;
+      if constexpr (LSE) sums[e & 3] += p;
       pf[2 * kb + (e >> 3)][e & 7] = (T)p;
+      if (e & 1) keep(kb, e - 1);
     };
     auto reference = [&](int kb) {
       if (!(is & kWaveFull)) {
@@ -531,9 +553,13 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
         const float alpha = limit == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(from - to);
         limit = need ? mx + kRoom : limit;
         from = to;
-        l *= alpha;
+        if constexpr (LSE) l *= alpha;
+        kept *= alpha;
+        if constexpr (LSE)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) sums[t] *= alpha;
+          for (int t = 0; t < 4; ++t) sums[t] *= alpha;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) keeps[t] *= alpha;
 #pragma unroll
         for (int x = 0; x < kDims; ++x) o[x] *= alpha;
       }
@@ -594,7 +620,8 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    if constexpr (LSE) l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    kept += keeps[0] + keeps[1];
   };
   auto step = [&](int32_t i, auto parity) {
     constexpr int buf = decltype(parity)::value;
@@ -618,7 +645,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   // query's trailing part: 0 times infinity or the other infinity, NaN where
   // there is a result.  What these go into is not finite, so a walk that ends in
   // finite sums needs no second.
-  float odd = l * 0.f;
+  float odd = (FORM == kFormPlain ? l : kept) * 0.f;
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
@@ -626,7 +653,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   const bool again = __syncthreads_or(odd != 0.f);
   if (again) {
     shift = float16v{};
-    l = 0.f;
+    l = kept = 0.f;
     limit = -INFINITY;
     from = 0.f;
 #pragma unroll
@@ -680,20 +707,27 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   meet();  // (loads ahead of the last tile land before the LDS is given back)
 
   // ---- out, or this split's part of it: lane holds dims 32d + 8(e/4) + 4lh + e%4 of row ln ----
-  const float lt = lanes2_sum(l);
+  const float kt = lanes2_sum(FORM == kFormPlain ? l : kept), lt = FORM == kFormPlain || !LSE ? kt : lanes2_sum(l);
   if (!row_ok) return;
   const int64_t n = s.row0 + row_t, row = n * a.QH + head;
   const float moved = FORM == kFormPlain ? -shift[0] * a.scale2 : from;
   if (a.splits > 1) {
     const int64_t at = (int64_t)split * a.c.N * a.QH + row;
     if (lh == 0) a.part_ml[at] = float2{limit == -INFINITY ? -INFINITY : moved, lt};
-    if (tile0 < tile1)
+    if (tile0 < tile1) {
+      // (the join divides by the sum of the splits' lt)
+      if constexpr (FORM != kFormPlain && LSE) {
+        const float to = lt == 0.f ? 0.f : lt / kt;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) o[d] *= to;
+      }
 #pragma unroll
       for (int d = 0; d < kDims; ++d)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
           *(float4v*)(a.part_o + at * D + 32 * d + 8 * q4 + 4 * lh) =
               float4v{o[d][4 * q4], o[d][4 * q4 + 1], o[d][4 * q4 + 2], o[d][4 * q4 + 3]};
+    }
     return;
   }
   const bool none = lt == 0.f;  // sees nothing
@@ -702,7 +736,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
     if (a.lse != nullptr) a.lse[row] = l2 * 0.6931471805599453f;
     if (a.lse2 != nullptr) a.lse2[((int64_t)kvh * a.c.N + s.row0) * a.per + wr0 + ln] = l2;
   }
-  const float inv = 1.0f / lt;
+  const float inv = 1.0f / kt;
   uint8_t* op = a.out + n * a.ost + (int64_t)head * a.osh;
 #pragma unroll
   for (int d = 0; d < kDims; ++d)

@@ -7,7 +7,8 @@ namespace jkv {
 template <int D, int FORM>
 static void launch_packed(const PagedAttnArgs& a, hipStream_t stream) {
   const dim3 grid((uint32_t)((int64_t)a.items * a.KVH));
-  hipLaunchKernelGGL((paged_chunk_kernel<JKV_F16, D, false, 4, FORM, true>), grid, dim3(256), 0, stream, a);
+  if (a.lse != nullptr) hipLaunchKernelGGL((paged_chunk_kernel<JKV_F16, D, false, 4, FORM, true, true>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((paged_chunk_kernel<JKV_F16, D, false, 4, FORM, true, false>), grid, dim3(256), 0, stream, a);
 }
 
 void packed_launch_f16(const PagedAttnArgs& a, int form, int64_t D, hipStream_t stream) {

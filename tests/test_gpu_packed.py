@@ -388,3 +388,37 @@ def test_scales(device, form, scale):
     pages.append(0, step, texts.k.to(device), texts.v.to(device), rope_theta=None)
     paged = pages.attention(0, step, texts.q.to(device), rope_theta=None, scale=scale, window=60, **call)
     check_out(texts, paged, results, want["cap"], want["slopes"])
+
+
+@pytest.mark.parametrize("cap,bias", [(None, False), (7.0, False), (None, True), (20.0, True)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_row_that_sees_one_entry(device, dtype, dim, cap, bias):
+    """Its output is the value itself, its score has no gradient.
+
+    The rounded weight divides itself out, and the quotient's 2^-22 is far below half a
+    step.  do v and do out are sums of dim products in 32 bits, the second one of two
+    parts whose second is rounded (2^-8 of 2^-22): they differ by at most (3 dim + 8)
+    2^-24 of the products' magnitudes; ds may round to twice its value, and dq and dk
+    add half a step of the smallest numbers.
+    """
+    texts = Texts(31, [150, 1, 64], 6, 2, dim, dtype, gain=2.0)
+    slopes = slopes_of(6).to(device) if bias else None
+    q, k, v = (x.to(device).requires_grad_() for x in (texts.q, texts.k, texts.v))
+    scale = dim**-0.5
+    for training in (False, True):
+        with torch.set_grad_enabled(training):
+            out = jkv.packed_attention(q, k, v, texts.starts.to(device), softcap=cap, slopes=slopes, window=1)
+        torch.testing.assert_close(out.detach().cpu(), texts.v.repeat_interleave(3, dim=1), rtol=0, atol=0)
+    out.backward(texts.d.to(device))
+    d, key, query = texts.d.double(), texts.k.double().repeat_interleave(3, dim=1), texts.q.double()
+    ds = 2 * (3 * dim + 8) * 2.0**-24 * (d * texts.v.double().repeat_interleave(3, dim=1)).abs().sum(-1, keepdim=True)
+    least = 2.0**-25 if dtype == torch.float16 else 0.0
+    assert (q.grad.cpu().double().abs() <= ds * scale * key.abs() + least).all()
+    grouped = (ds * scale * query.abs()).reshape(-1, 2, 3, dim).sum(2)
+    assert (k.grad.cpu().double().abs() <= grouped + least).all()
+    # p is within 2^-18 of 1 (its score's fraction in 32 bits) and rounds to 1 or beside
+    # it; three heads' sum, then half a step
+    h = half_step(dtype)
+    sums, sizes = d.reshape(-1, 2, 3, dim).sum(2), d.abs().reshape(-1, 2, 3, dim).sum(2)
+    assert ((v.grad.cpu().double() - sums).abs() <= h * sums.abs() + (h + 2.0**-18) * 1.01 * sizes + least).all()

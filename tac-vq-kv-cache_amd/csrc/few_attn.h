@@ -10,7 +10,8 @@
 // meet no barrier (where eight of them make a workgroup, they meet once, at its
 // end), and four of them a CU hold 64 KiB of loads in flight.  16 sequences of
 // 4,096 entries, 32/8 heads of 128: 55 us, 4.9 TB/s; four of up to 65,536: 115
-// us, 4.8 TB/s (a large copy reaches 5.15).
+// us, 4.8 TB/s (a large copy reaches 5.15).  Caps and biases hide behind the loads:
+// 50 and 116 us with capped and with biased scores.
 //
 // On v_mfma_f32_16x16x32: S^T[entry][row] = K Q^T, O^T[dim][row] += V^T P^T
 // (V^T by transposing reads of the row-major tile; the contraction order of

@@ -122,7 +122,8 @@ def packed_attention(
     Returns ``[N,QH,D]`` (``out``, if given); rows that no sequence owns are 0,
     their ``lse`` and gradients -inf and 0.  Rows and gradients depend on what
     they see alone, whatever lies in other places.  Scores and sums are 32-bit,
-    weights enter the second product rounded once to the inputs' type.
+    weights enter the second product rounded once to the inputs' type, and their
+    sum as rounded divides it.
     Differentiable in ``query``, ``key`` and ``value`` (not with a given ``out``);
     a call repeats bit for bit, its gradients too.
     """

@@ -82,8 +82,8 @@ class _PackedAttention(torch.autograd.Function):
                                             key.shape[1], dim, span)
             workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
             _lib.check(_lib.load().jkv_packed_attention_backward(
-                *(x for _tensor, at in places[:4] for x in at), rest.data_ptr(), *places[4][1], lse.data_ptr(), _lib.dtype_code(query.dtype),
-                starts.data_ptr(), _lib.ptr(prefixes), rows, starts.shape[0] - 1, qheads, key.shape[1], dim,
+                *(x for _tensor, at in places[:4] for x in at), rest.data_ptr(), *places[4][1], lse.data_ptr(),
+                _lib.dtype_code(query.dtype), starts.data_ptr(), _lib.ptr(prefixes), rows, starts.shape[0] - 1, qheads, key.shape[1], dim,
                 span, sinks, scale, softcap, _lib.ptr(slopes), *map(_lib.ptr, grads), workspace.data_ptr(),
                 ws_bytes, _lib.stream_handle(device)))
         return (*grads, *(None,) * 8)
@@ -119,11 +119,11 @@ def packed_attention(
     without gradients) then takes ``slopes[h] |i - j|`` off.  ``lse`` (fp32
     ``[N,QH]``) receives each row's log-sum-exp.
 
-    Returns ``[N,QH,D]`` (``out``, if given); rows that no sequence owns are 0,
-    their ``lse`` and gradients -inf and 0.  Rows and gradients depend on what
-    they see alone, whatever lies in other places.  Scores and sums are 32-bit,
-    weights enter the second product rounded once to the inputs' type, and their
-    sum as rounded divides it.
+    Returns ``[N,QH,D]`` (``out``, if given, which must not share memory with the
+    inputs); rows that no sequence owns are 0, their ``lse`` and gradients -inf
+    and 0.  Rows and gradients depend on what they see alone, whatever lies in
+    other places.  Scores and sums are 32-bit, weights enter the second product
+    rounded once to the inputs' type, and their sum as rounded divides it.
     Differentiable in ``query``, ``key`` and ``value`` (not with a given ``out``);
     a call repeats bit for bit, its gradients too.
     """

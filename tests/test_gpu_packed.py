@@ -422,3 +422,46 @@ def test_a_row_that_sees_one_entry(device, dtype, dim, cap, bias):
     h = half_step(dtype)
     sums, sizes = d.reshape(-1, 2, 3, dim).sum(2), d.abs().reshape(-1, 2, 3, dim).sum(2)
     assert ((v.grad.cpu().double() - sums).abs() <= h * sums.abs() + (h + 2.0**-18) * 1.01 * sizes + least).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rows_without_sequences(device, dtype):
+    texts = Texts(32, [], 4, 2, 64, dtype, lead=70)
+    x = [t.to(device).requires_grad_() for t in (texts.q, texts.k, texts.v)]
+    lse = torch.zeros(70, 4, device=device)
+    out = jkv.packed_attention(*x, texts.starts.to(device), lse=lse)
+    assert (out == 0).all() and (lse == float("-inf")).all()
+    out.backward(texts.d.to(device))
+    assert all((t.grad == 0).all() for t in x)
+    none = [t.detach()[:0].requires_grad_() for t in x]
+    out = jkv.packed_attention(*none, torch.zeros(3, dtype=torch.int32, device=device))
+    out.sum().backward()
+    assert out.shape == (0, 4, 64) and all(t.grad.shape == t.shape for t in none)
+
+
+def test_rows_past_32_bits(device):
+    """Rows 2^22 bytes apart give what rows one behind another give."""
+    texts = Texts(33, [600, 440], 4, 2, 64, torch.float16)
+    far = torch.zeros(1040, 1 << 21, dtype=torch.float16, device=device)
+    starts = texts.starts.to(device)
+    near = [t.to(device) for t in (texts.q, texts.k, texts.v, texts.d)]
+    apart, at = [], 0
+    for t in near:
+        place = far[:, at : at + t[0].numel()].view(t.shape)
+        place.copy_(t)
+        apart.append(place)
+        at += t[0].numel()
+    results = []
+    for q, k, v, d in (near, apart):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        assert q.stride(0) in (256, 1 << 21)
+        out = jkv.packed_attention(q, k, v, starts, softcap=20.0)
+        results.append((out.detach(), *torch.autograd.grad(out, (q, k, v), d)))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    target = far[:, at : at + 256].view(1040, 4, 64)
+    jkv.packed_attention(*(t.detach() for t in apart[:3]), starts, softcap=20.0, out=target)
+    assert torch.equal(target, results[0][0])
+    turned = [jkv.rotary(t, starts=starts) for t in (near[0], apart[0])]
+    assert torch.equal(*turned)
+    jkv.rotary(apart[0], starts=starts, out=target)
+    assert torch.equal(target, turned[0])

@@ -213,46 +213,47 @@ __device__ __forceinline__ float shape_and_slant(const ScoreShape& s, float x, f
   return x;
 }
 
-// 32 rows of D elements into LDS, row r's chunk j in slot chunk_both_slot(r, j),
-// 16 rows (D = 128) or 32 a load of the four waves.  Rows at or behind `left` land
-// as zeros.  Two groups of 16 rows share their slots, so one offset a lane serves
-// both.
+// A resource of up to `most` rows of D elements, those at or behind `left` outside it.
+// (One for all of a tile's loads: one a load is a hundred scalar instructions a step.)
+template <int D>
+__device__ __forceinline__ uint4v rows_resource(const uint8_t* base, int32_t left, int32_t most, uint32_t stride) {
+  const int32_t rows = left < most ? left : most;
+  const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * stride + 2 * D : 0u;
+  const uint64_t at = (uint64_t)base;
+  return uint4v{(uint32_t)__builtin_amdgcn_readfirstlane((int32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)(at >> 32)) & 0xffffu,
+                (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)bytes), 0x00020000u};
+}
+
+// ROWS rows into LDS, row r's chunk j in slot chunk_both_slot(r, j), 16 rows (D = 128)
+// or 32 a load of the four waves.  Rows at or behind `left` land as zeros.  Two groups
+// of 16 rows share their slots, so one offset a lane serves both.
 template <int D>
 __device__ __forceinline__ uint32_t rows32_offset(uint32_t stride, int wave, int lane) {
   constexpr int kRowsPerLoad = 1024 / (2 * D);
   const int r = kRowsPerLoad * wave + lane / (64 / kRowsPerLoad), slot = lane % (64 / kRowsPerLoad);
   return (uint32_t)r * stride + 16u * (uint32_t)chunk_both_slot<D>(r, slot);
 }
-template <int D>
-__device__ __forceinline__ void load_rows32(const uint8_t* base, int32_t left, uint32_t stride, uint32_t offset, uint32_t to, int wave) {
-  constexpr int kRowBytes = 2 * D, kEach = 4096 / kRowBytes;
+template <int D, int ROWS>
+__device__ __forceinline__ void load_rows(const uint8_t* base, int32_t left, uint32_t stride, uint32_t offset, uint32_t to, int wave) {
+  constexpr int kEach = 4096 / (2 * D);
+  const uint4v rsrc = rows_resource<D>(base, left, ROWS, stride);
+  asm volatile("" : "+v"(offset));  // (what is made from it is not kept)
 #pragma unroll
-  for (int j = 0; j < 32 / kEach; ++j) {
-    const int32_t rows = left - j * kEach;
-    const uint32_t bytes = rows > 0 ? (uint32_t)((rows < kEach ? rows : kEach) - 1) * stride + kRowBytes : 0u;
-    const uint64_t at = (uint64_t)base + (uint64_t)(j * kEach) * stride;
-    const uint4v rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)(at >> 32)) & 0xffffu,
-                         (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)bytes), 0x00020000u};
-    load_to_lds<16>(to + 4096u * j + 1024u * (uint32_t)wave, offset, rsrc);
-  }
+  for (int j = 0; j < ROWS / kEach; ++j) load_to_lds<16>(to + 4096u * j + 1024u * (uint32_t)wave, offset + (uint32_t)(j * kEach) * stride, rsrc);
 }
 
-// The same by one wave.
+// 32 rows by one wave.
 template <int D>
 __device__ __forceinline__ void load_rows32_alone(const uint8_t* base, int32_t left, uint32_t stride, uint32_t to, int lane) {
   constexpr int kRowBytes = 2 * D, kEach = 1024 / kRowBytes;
   const int r = lane / (64 / kEach), slot = lane % (64 / kEach);
-  const uint32_t row = (uint32_t)r * stride, part = 16u * (uint32_t)chunk_both_slot<D>(r, slot);
+  uint32_t row = (uint32_t)r * stride, part = 16u * (uint32_t)chunk_both_slot<D>(r, slot);
+  const uint4v rsrc = rows_resource<D>(base, left, 32, stride);
+  asm volatile("" : "+v"(row), "+v"(part));
+  // (row r + 4 or 8's slots)
 #pragma unroll
-  for (int j = 0; j < 32 / kEach; ++j) {
-    const int32_t rows = left - j * kEach;
-    const uint32_t bytes = rows > 0 ? (uint32_t)((rows < kEach ? rows : kEach) - 1) * stride + kRowBytes : 0u;
-    const uint64_t at = (uint64_t)base + (uint64_t)(j * kEach) * stride;
-    const uint4v rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)(at >> 32)) & 0xffffu,
-                         (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)bytes), 0x00020000u};
-    // (row r + 4 or 8's slots)
-    load_to_lds<16>(to + 1024u * j, row + (part ^ (D == 128 ? 16u * (j & 3) : 32u * (j & 1))), rsrc);
-  }
+  for (int j = 0; j < 32 / kEach; ++j)
+    load_to_lds<16>(to + 1024u * j, row + (uint32_t)(j * kEach) * stride + (part ^ (D == 128 ? 16u * (j & 3) : 32u * (j & 1))), rsrc);
 }
 
 // A lane's LDS addresses in a tile of 32 rows.  Row ln's 16-byte chunk 2c + lh (an
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
   // values into LDS, the wave's keys into registers (B operand: 8 dims of key ln)
 #pragma unroll
   for (int w = 0; w < kKeys / 32; ++w)
-    load_rows32<D>(a.v + (int64_t)(row0 + j0 + 32 * w) * a.vst + (int64_t)kvh * a.vsh, T0 - j0 - 32 * w, (uint32_t)a.vst,
+    load_rows<D, 32>(a.v + (int64_t)(row0 + j0 + 32 * w) * a.vst + (int64_t)kvh * a.vsh, T0 - j0 - 32 * w, (uint32_t)a.vst,
                    rows32_offset<D>((uint32_t)a.vst, wave, lane), lds_base + w * kTile, wave);
   V8 kf[kSteps];
   {
@@ -355,8 +356,8 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
       load_rows32_alone<D>(q_at, left, (uint32_t)a.qst, to, lane);
       load_rows32_alone<D>(d_at, left, (uint32_t)a.dst, to + kTile, lane);
     } else {
-      load_rows32<D>(q_at, left, (uint32_t)a.qst, q_off, to, wave);
-      load_rows32<D>(d_at, left, (uint32_t)a.dst, d_off, to + kTile, wave);
+      load_rows<D, 32>(q_at, left, (uint32_t)a.qst, q_off, to, wave);
+      load_rows<D, 32>(d_at, left, (uint32_t)a.dst, d_off, to + kTile, wave);
     }
     const uint32_t bytes = 4u * (uint32_t)(left < 32 ? (left > 0 ? left : 0) : 32);
     auto load_stats = [&](const float* from, uint32_t at_to) {
@@ -527,18 +528,11 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
   // it at about the same time (8,192 causal bf16 tokens in one sequence, 32/8 heads:
   // 2,260 us from the first on)
   auto advance = [&](Step& s, int32_t by) {
-    for (; by > 0; --by) {
-      if (++s.g < heads) continue;
-      s.g = 0;
+    for (s.g += by; s.g >= heads; s.g -= heads)
       if (++s.tile == full0) s.tile = full1;
-    }
   };
   auto go_back = [&](Step& s, int32_t by) {
-    for (; by > 0; --by) {
-      if (++s.g < heads) continue;
-      s.g = 0;
-      --s.tile;
-    }
+    for (s.g += by; s.g >= heads; s.g -= heads) --s.tile;
   };
   Step now = {tile0 == full0 ? full1 : tile0, 0}, first_plain = {full1 - 1, 0};
   if constexpr (ALONE) {  // a wave's share: every fourth
@@ -691,13 +685,9 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   auto load_step = [&](int32_t i, int stage) {
     const int32_t e0 = entry_of(i);
     const int64_t n = row0 + e0;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int32_t rows = T0 - e0 - 32 * half;
-      const uint32_t to = lds_base + 2 * stage * kTile + half * (kTile / 2);
-      load_rows32<D>(a.k + (n + 32 * half) * a.kst + (int64_t)kvh * a.ksh, rows, (uint32_t)a.kst, k_off, to, wave);
-      load_rows32<D>(a.v + (n + 32 * half) * a.vst + (int64_t)kvh * a.vsh, rows, (uint32_t)a.vst, v_off, to + kTile, wave);
-    }
+    const uint32_t to = lds_base + 2 * stage * kTile;
+    load_rows<D, 64>(a.k + n * a.kst + (int64_t)kvh * a.ksh, T0 - e0, (uint32_t)a.kst, k_off, to, wave);
+    load_rows<D, 64>(a.v + n * a.vst + (int64_t)kvh * a.vsh, T0 - e0, (uint32_t)a.vst, v_off, to + kTile, wave);
   };
 
   // the wave's queries and output gradients (B operands: 8 dims of row ln)

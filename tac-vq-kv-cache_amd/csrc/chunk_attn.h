@@ -325,7 +325,16 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
       qf[c][e] = (T)v;
       if constexpr (EXACT) ql[c][e] = __builtin_isfinite((float)(T)v) ? (T)(v - (float)(T)v) : (T)0.f;
     };
-    if (a.rope.on) {
+    if constexpr (LINEAR) {  // as they are, or their negatives
+      const uint32_t kept_bits = row_ok ? 0xffffffffu : 0u, flip = a.q_mul < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        uint4v w = __builtin_bit_cast(uint4v, x[c]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = (w[e] ^ flip) & kept_bits;
+        qf[c] = __builtin_bit_cast(V8, w);
+      }
+    } else if (a.rope.on) {
 #pragma unroll
       for (int c = 0; c < kSteps / 2; ++c)
 #pragma unroll

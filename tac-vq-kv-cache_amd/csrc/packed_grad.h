@@ -170,17 +170,56 @@ __device__ __forceinline__ float ds_factor(const PackedGradArgs& a) {
   return __uint_as_float((uint32_t)(127 + 5 - e) << 23);
 }
 
+// Of 64 sequences with `own` blocks in a lane's (`upto` of it and those before), the
+// lane and rank (from a sequence's last block on) of the `item`-th (below their sum):
+// all sequences' highest ranks first, as key blocks that are seen by many rows and
+// start last are waited for by all CUs; where a sequence has more than 64, one sequence
+// after another.  dk and dv of 48 texts of up to 511, 28/4 heads of 64, 131 -> 115 us,
+// of three of up to 8,192, 32/8 of 128, window 4,096, 2,470 -> 2,350.  Row blocks (the
+// attention's and dq's) are shorter and gain nothing, and prompts that see a prefix
+// lose what they share of it in the caches (180 -> 214 us).
+__device__ __forceinline__ int ranked_block(int32_t own, int32_t upto, int32_t item, int32_t* rank) {
+  const int lane = threadIdx.x & 63;
+  int32_t most = own;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    const int32_t other = __shfl_xor(most, off, 64);
+    most = other > most ? other : most;
+  }
+  most = __builtin_amdgcn_readfirstlane(most);
+  if (most > 64) {
+    const int at = __builtin_ctzll(__ballot(item < upto));
+    *rank = __builtin_amdgcn_readlane(upto, at) - 1 - item;
+    return at;
+  }
+  uint64_t have = 0;
+  int32_t r = most;
+  while (r > 0) {
+    have = __ballot(own >= r);
+    const int32_t count = __builtin_popcountll(have);
+    --r;
+    if (item < count) break;
+    item -= count;
+  }
+  *rank = r;
+  // the item-th of those that have one
+  const bool is = (have >> lane & 1) && __builtin_popcountll(have & ((uint64_t{1} << lane) - 1)) == item;
+  return __builtin_ctzll(__ballot(is));
+}
+
 // Blocks of `rows` of the sequences' rows times `per`: the sequence and block of
-// an item, blocks in their order.
+// an item, blocks in their order (RANKED: in that of ranked_block).
+template <bool RANKED>
 __device__ __forceinline__ bool packed_block(const PackedGradArgs& a, int32_t per, int32_t rows, int32_t item, int32_t* b, int32_t* block) {
   const int lane = threadIdx.x & 63;
   int32_t before = 0;
   for (int32_t b0 = 0; b0 < a.B; b0 += 64) {
-    int32_t upto = 0;
+    int32_t own = 0;
     if (b0 + lane < a.B) {
       const int32_t row0 = clamp_i32(a.starts[b0 + lane], 0, a.N), tokens = clamp_i32(a.starts[b0 + lane + 1], row0, a.N) - row0;
-      upto = (tokens * per + rows - 1) / rows;
+      own = (tokens * per + rows - 1) / rows;
     }
+    int32_t upto = own;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const int32_t up = __shfl_up(upto, off, 64);
@@ -188,9 +227,16 @@ __device__ __forceinline__ bool packed_block(const PackedGradArgs& a, int32_t pe
     }
     const int32_t all = __builtin_amdgcn_readlane(upto, 63);
     if (item < before + all) {
-      const int at = __builtin_ctzll(__ballot(item < before + upto));
-      *b = b0 + at;
-      *block = item - before - (at > 0 ? __builtin_amdgcn_readlane(upto, at > 0 ? at - 1 : 0) : 0);
+      if constexpr (RANKED) {
+        int32_t rank;
+        const int at = ranked_block(own, upto, item - before, &rank);
+        *b = b0 + at;
+        *block = __builtin_amdgcn_readlane(own, at) - 1 - rank;
+      } else {
+        const int at = __builtin_ctzll(__ballot(item < before + upto));
+        *b = b0 + at;
+        *block = item - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(own, at));
+      }
       return true;
     }
     before += all;
@@ -312,7 +358,7 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
   // the heads of the group that it walks
   const int32_t g0 = split * a.heads_each, heads = a.per - g0 < a.heads_each ? a.per - g0 : a.heads_each;
   int32_t b, block;
-  if (!packed_block(a, 1, kKeys, (int32_t)at_item, &b, &block)) return;
+  if (!packed_block<true>(a, 1, kKeys, (int32_t)at_item, &b, &block)) return;
   b = __builtin_amdgcn_readfirstlane(b);
   block = __builtin_amdgcn_readfirstlane(block);
   const int32_t row0 = clamp_i32(a.starts[b], 0, a.N), T0 = clamp_i32(a.starts[b + 1], row0, a.N) - row0;
@@ -334,10 +380,8 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
       kf[c] = V8{};
       if (ok) kf[c] = *(const V8*)(kp + 32 * c);
     }
-#pragma unroll
-    for (int c = 0; c < kSteps; ++c) asm volatile("" : "+v"(kf[c]));  // waited for here
   }
-  const float factor = ds_factor<DT, D>(a);
+  float factor = 1.f;
 
   // the rows that see some key of the block
   const int32_t i0 = prefix > j0 ? 0 : j0;
@@ -559,6 +603,9 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
     load_next(other);
   };
   load_next(edge & 1);  // (so that the full tiles start in stage 0)
+  factor = ds_factor<DT, D>(a);
+#pragma unroll
+  for (int c = 0; c < kSteps; ++c) asm volatile("" : "+v"(kf[c]));  // waited for here, with all loads before
   if constexpr (ALONE) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the values have landed
   for (int32_t n = edge; n > 0; --n) {
     turn_over((n & 1) ^ 1);
@@ -660,7 +707,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   const uint32_t at_item = blockIdx.x / (uint32_t)a.KVH;
   const int32_t kvh = (int32_t)(blockIdx.x - at_item * (uint32_t)a.KVH);
   int32_t b, block;
-  if (!packed_block(a, a.per, 128, (int32_t)at_item, &b, &block)) return;
+  if (!packed_block<false>(a, a.per, 128, (int32_t)at_item, &b, &block)) return;
   b = __builtin_amdgcn_readfirstlane(b);
   block = __builtin_amdgcn_readfirstlane(block);
   const int32_t row0 = clamp_i32(a.starts[b], 0, a.N), T0 = clamp_i32(a.starts[b + 1], row0, a.N) - row0;

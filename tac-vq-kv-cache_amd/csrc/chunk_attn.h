@@ -106,11 +106,38 @@ template <int D> __device__ __forceinline__ int chunk_both_slot(int r, int j) {
 }
 
 // The sequence and row block of an item: items are the row blocks of all
-// sequences in turn, a sequence's last one first (it sees most).  From item
+// sequences in turn (SORTED: by length where there are few), a sequence's last one
+// first (it sees most).  From item
 // `fold` on the order runs backwards, so that where all workgroups are resident
 // at once, two a CU, one that sees much shares a CU with one that sees little.
+template <bool SORTED>
 __device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int32_t item, int32_t fold, int32_t* b, int32_t* block) {
   const int lane = threadIdx.x & 63;
+  // The longest of up to eight sequences first, so that short walks come last (four
+  // biased prompts of 670 to 2,047, 179 -> 173 us).  Of more, the last is a small part
+  // of all, and finding its place takes an instruction or three a sequence.
+  if (SORTED && a.c.B <= 8) {
+    int32_t own = 0, mine = 0, total = 0;
+    if (lane < a.c.B) {
+      int32_t row0, tokens;
+      paged_rows(a.c, lane, &row0, &tokens);
+      if (tokens > a.max_new) tokens = a.max_new;
+      own = (tokens * a.per + a.item_rows - 1) / a.item_rows;
+    }
+    for (int32_t j = 0; j < a.c.B; ++j) {
+      const int32_t other = __builtin_amdgcn_readlane(own, j);
+      total += other;
+      if (other > own || (other == own && j < lane)) mine += other;
+    }
+    if (item >= fold && item < total) item = fold + (total - 1 - item);
+    const uint64_t is = __ballot(item >= mine && item < mine + own);
+    *block = total;
+    if (is == 0) return false;
+    const int at = __builtin_ctzll(is);
+    *b = at;
+    *block = __builtin_amdgcn_readlane(mine, at) + __builtin_amdgcn_readlane(own, at) - 1 - item;
+    return true;
+  }
   auto blocks_upto = [&](int32_t b0) -> int32_t {  // of sequences b0 to b0 + lane
     int32_t upto = 0;
     if (b0 + lane < a.c.B) {
@@ -201,7 +228,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   const int32_t kvh = (int32_t)(bid - at_item * (uint32_t)a.KVH);
   const int32_t item = (int32_t)(at_item / (uint32_t)a.splits), split = (int32_t)(at_item - (uint32_t)item * (uint32_t)a.splits);
   int32_t b, block;
-  if (!paged_item(a, item, a.fold, &b, &block)) {
+  if (!paged_item<LINEAR>(a, item, a.fold, &b, &block)) {
     if constexpr (LINEAR) clear_unowned<DT, D>(a, item - block, a.items - block, kvh, 64 * kChunkWaves);
     return;
   }

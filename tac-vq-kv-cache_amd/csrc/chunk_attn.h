@@ -107,9 +107,9 @@ template <int D> __device__ __forceinline__ int chunk_both_slot(int r, int j) {
 
 // The sequence and row block of an item: items are the row blocks of all
 // sequences in turn (SORTED: by length where there are few), a sequence's last one
-// first (it sees most).  From item
-// `fold` on the order runs backwards, so that where all workgroups are resident
-// at once, two a CU, one that sees much shares a CU with one that sees little.
+// first (it sees most).  From item `fold` on the order runs backwards, so that where
+// all workgroups are resident at once, two a CU, one that sees much shares a CU with
+// one that sees little.
 template <bool SORTED>
 __device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int32_t item, int32_t fold, int32_t* b, int32_t* block) {
   const int lane = threadIdx.x & 63;
@@ -539,8 +539,8 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   // beside the products of the other half's scores or of the values, a product
   // and a few scores at a time, fenced, as the compiler else gathers each kind.
   // Three capped texts of 21,760 bf16 tokens in all, window 4,096, 32/8 heads of 128:
-  // 1,495 us, 700 TFLOP/s, vector instructions 69 % of the cycles, products 37 %, both
-  // at once 18 %, 1.85 GHz; 2,048 capped tokens over 8,192 entries in pages 363 us, 660.
+  // 1,480 us, 705 TFLOP/s, vector instructions 69 % of the cycles, products 37 %, both
+  // at once 18 %, 1.85 GHz; 2,048 capped tokens over 8,192 entries in pages 357 us, 670.
   auto work_shaped = [&](int32_t i, int32_t is, auto parity, auto again) {
     constexpr int buf = decltype(parity)::value;
     constexpr bool AGAIN = decltype(again)::value;

@@ -12,13 +12,13 @@
 // order of atomics.
 //
 // 21,760 bf16 tokens of three texts, 32/8 heads of 128, capped scores, window 4,096
-// (5.2e11 flops a product): rows 117 us (560 MB, 4.8 TB/s), dk and dv 2,345 (four
-// products, 894 TFLOP/s), dq 1,680 (three, 936).  Products fill 48 and 52 % of their
-// cycles, vector instructions 53 and 69, both at once 21 and 30; the clock falls to
+// (5.2e11 flops a product): rows 115 us (560 MB, 4.9 TB/s), dk and dv 2,255 to 2,350
+// (four products, 930 TFLOP/s), dq 1,680 (three, 936).  Products fill 52 % of their
+// cycles, vector instructions 58 and 72, both at once 23 and 30; the clock falls to
 // 1.75 GHz, so more of either at once brings less than it seems.  dk and dv read 5.7
 // GB; walks that start at one place of the window for all blocks read 2.3 GB and take
-// as long.  48 texts of up to 511 fp16 tokens, 28/4 heads of 64: 42, 145 and 92 us,
-// vector instructions, and masked tiles at both ends of short walks.
+// as long.  48 texts of up to 511 fp16 tokens, 28/4 heads of 64: 40, 114 to 120 and 89
+// us, vector instructions, and masked tiles at both ends of short walks.
 //
 // p and ds enter their products rounded once to the inputs' type, p as 2^10 of
 // itself (fp16 holds 2^-34 of it then), ds in fp16 times a power of two that keeps

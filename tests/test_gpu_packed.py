@@ -465,3 +465,18 @@ def test_rows_past_32_bits(device):
     assert torch.equal(*turned)
     jkv.rotary(apart[0], starts=starts, out=target)
     assert torch.equal(target, turned[0])
+
+
+@pytest.mark.parametrize("form", [FORMS[0], FORMS[4]], ids=["plain", "all"])
+@pytest.mark.parametrize("sizes,qh,kvh,dim", [
+    ([17, 0, 40, 1, 33] * 15, 2, 1, 64),  # more than 64 sequences
+    ([5, 2200, 130], 1, 1, 64),  # one of more than 64 blocks of keys
+    ([300, 700, 0, 500], 24, 8, 64),  # few, in an order of lengths, two workgroups a CU
+])
+def test_orders_of_the_blocks(device, form, sizes, qh, kvh, dim):
+    texts = Texts(34, sizes, qh, kvh, dim, torch.bfloat16, lead=2, tail=3)
+    want, call = form_of(texts, form, qh, device)
+    out, grads = run_grads(texts, device, **call)
+    results = texts.expect(grads=True, **want)
+    check_out(texts, out, results, want["cap"], want["slopes"])
+    check_grads(texts, grads, results, want["cap"], want["slopes"])

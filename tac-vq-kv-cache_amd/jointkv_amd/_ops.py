@@ -59,6 +59,15 @@ def _overlaps(tensor: torch.Tensor) -> bool:
     return False
 
 
+def _written(*given: torch.Tensor | None) -> None:
+    """A kernel wrote to these tensors of the caller's: a backward pass that saved
+    one of them before refuses, as after torch's own writes in place."""
+
+    for tensor in given:
+        if tensor is not None and not tensor.is_inference():
+            torch.autograd.graph.increment_version(tensor)
+
+
 def _refuse_second_derivative(name: str) -> None:
     """In a backward pass: gradients are recorded there if they are to be
     differentiated again.  (A check of 0.1 us; ``once_differentiable`` costs a

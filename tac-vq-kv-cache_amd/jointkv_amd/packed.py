@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._ops import _current, _overlaps, _plain, _refuse_second_derivative
+from ._ops import _current, _overlaps, _plain, _refuse_second_derivative, _written
 from .paged import _rows, _shape_args
 
 PACKED_TYPES = (torch.float16, torch.bfloat16)
@@ -58,10 +58,11 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, query, key, value, starts, prefixes, slopes, softcap, window, sinks, scale, lse):
-        if lse is None:
-            lse = torch.empty(query.shape[:2], dtype=torch.float32, device=query.device)
+        given, lse = lse, torch.empty(query.shape[:2], dtype=torch.float32, device=query.device)
         rest = _plain(query)(tuple(query.shape))
         out = _forward(query, key, value, starts, prefixes, slopes, softcap, window, sinks, scale, lse, None, rest)
+        if given is not None:
+            given.copy_(lse)  # (the caller may use its own again before the backward)
         ctx.params = (softcap, window, sinks, scale)
         ctx.save_for_backward(query, key, value, out, rest, lse, starts, prefixes, slopes)
         return out
@@ -161,4 +162,7 @@ def packed_attention(
             raise ValueError("a given out is not differentiable")
         _lib.require_device(query, key, value, starts, prefixes, slopes, lse)
         return _PackedAttention.apply(query, key, value, *args)
-    return _forward(query, key, value, *args, out)
+    result = _forward(query, key, value, *args, out)
+    if out is not None or lse is not None:
+        _written(out, lse)
+    return result

@@ -20,7 +20,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._ops import _current, _overlaps, _plain, _refuse_second_derivative
+from ._ops import _current, _overlaps, _plain, _refuse_second_derivative, _written
 from .attention import MISTRAL_ROPE_THETA
 
 MOST_DIMS = 256
@@ -221,4 +221,7 @@ def rotary(
         if out is not None or key_out is not None:
             raise ValueError("given outputs are not differentiable")
         return _Rotary.apply(query, key, rule, starts, positions)
-    return _turn(query, key, rule, starts, positions, False, out, key_out)
+    turned = _turn(query, key, rule, starts, positions, False, out, key_out)
+    if out is not None or key_out is not None:
+        _written(out, key_out)
+    return turned

@@ -480,3 +480,33 @@ def test_orders_of_the_blocks(device, form, sizes, qh, kvh, dim):
     results = texts.expect(grads=True, **want)
     check_out(texts, out, results, want["cap"], want["slopes"])
     check_grads(texts, grads, results, want["cap"], want["slopes"])
+
+
+def test_buffers_given_beside_autograd(device):
+    """An lse buffer may serve two calls before the first's backward; what a kernel
+    writes over a saved tensor makes the backward refuse."""
+    texts = Texts(35, [40, 90], 4, 2, 64, torch.float16)
+    starts, d = texts.starts.to(device), texts.d.to(device)
+    x = [t.to(device).requires_grad_() for t in (texts.q, texts.k, texts.v)]
+    want = torch.autograd.grad(jkv.packed_attention(*x, starts), x, d)
+    lse = torch.empty(130, 4, device=device)
+    first = jkv.packed_attention(*x, starts, lse=lse)
+    held = lse.clone()
+    jkv.packed_attention(*x, starts, softcap=5.0, lse=lse)
+    assert not torch.equal(held, lse)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(first, x, d), want))
+
+    out = jkv.packed_attention(*x, starts)
+    with torch.no_grad():
+        jkv.packed_attention(*x, starts, softcap=5.0, out=out)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.backward(d)
+    y = x[0].sigmoid()  # (its backward takes its output)
+    with torch.no_grad():
+        jkv.rotary(y, starts=starts, out=y)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    with torch.inference_mode():
+        z = x[0].clone()
+        assert jkv.rotary(z, starts=starts, out=z) is z
+        assert jkv.packed_attention(z, x[1], x[2], starts, out=torch.empty_like(z)).shape == z.shape

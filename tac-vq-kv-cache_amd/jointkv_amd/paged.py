@@ -535,7 +535,7 @@ class PagedKVCache:
         more = [-(-a // self.page_size) - len(row) for a, row in zip(after, self._pages)]
         # half-written last pages that another sequence still reads: whoever
         # writes first, until one is left, takes a copy
-        uses, copied = {}, []
+        uses, copied, kept = {}, [], {}
         for b, (length, n, row) in enumerate(zip(self._lengths, new, self._pages)):
             if n and length % self.page_size:
                 page = row[-1]
@@ -543,10 +543,13 @@ class PagedKVCache:
                 if count > 1:
                     uses[page] = count - 1
                     copied.append(b)
+                else:
+                    kept[page] = length % self.page_size
         if sum(more) + len(copied) > len(self._free):
             raise ValueError(f"the step needs {sum(more) + len(copied)} pages, {len(self._free)} are free")
         before = self._lengths, self._positions, self._pages
         left = [self._pages[b][-1] for b in copied]
+        held = [self._lengths[b] % self.page_size for b in copied]
         taken = self._free[: -sum(more) - len(copied) - 1 : -1]
         if taken:
             free = iter(taken)
@@ -555,7 +558,6 @@ class PagedKVCache:
                 pages[b] = pages[b][:-1] + [next(free)]
             pages = [row + [next(free) for _ in range(n)] for row, n in zip(pages, more)]
             if copied:
-                held = [self._lengths[b] % self.page_size for b in copied]
                 ints = self._on_device(left + taken[: len(copied)] + held).view(3, -1)
                 copy_pages(self.key, self.value, ints[0], ints[1], entries=ints[2])
             self._upload(pages)
@@ -575,18 +577,28 @@ class PagedKVCache:
         self._positions = [p + n for p, n in zip(self._positions, new)]
         step = PagedStep(self.block_tables, ints[:batch], None if single else ints[2 * batch :],
                          ints[batch : 2 * batch], starts[-1], max(new), max(after))
-        self._begun = (step.lengths, *before, taken, left)
+        # Who keeps a page may have fewer entries there than who left it, and writes over
+        # theirs: a cancelled step takes them from the longest copy.
+        back = {}
+        for page, copy, n in sorted(zip(left, taken, held), key=lambda x: x[2]):
+            if n > kept.get(page, n):
+                back[page] = copy, page, n
+        self._begun = (step.lengths, *before, taken, left, list(back.values()))
         return step
 
     def cancel(self, step: PagedStep) -> None:
         """Take back ``step``, the latest one, before an eviction or release:
-        lengths, positions and pages are again those before it, and its own
-        entries' weights 0.  What its attention added to the weights of earlier
-        entries stays."""
+        lengths, positions, pages and the entries in them are again those before
+        it, and its own entries' weights 0.  What its attention added to the
+        weights of earlier entries stays."""
 
         if self._begun is None or step.lengths is not self._begun[0]:
             raise ValueError("only the latest step can be taken back, before an eviction or release")
-        lengths, positions, pages, taken, left = self._begun[1:]
+        lengths, positions, pages, taken, left, back = self._begun[1:]
+        if back:
+            copies, shared, held = zip(*back)
+            ints = self._on_device([*copies, *shared, *held]).view(3, -1)
+            copy_pages(self.key, self.value, ints[0], ints[1], entries=ints[2])
         if taken:
             self._upload(pages)
         if self.weights is not None:

@@ -329,3 +329,23 @@ def test_rule_in_a_cache(device):
                 slack = 2 * (r["reach"] * 2.0**-10)[..., None] * r["spread"]
                 assert ((out[at : at + n].cpu().double() - r["out"]).abs() <= 2.0**-10 * r["spread"] + slack + 1e-6).all()
             at += n
+
+
+@pytest.mark.parametrize("owner", [0, 1])
+def test_cancel_after_a_shorter_sharer_kept_the_page(device, owner):
+    """What a cancelled step wrote over entries that others have is undone, in both
+    pools and all layers: every later attention still matches its own rows."""
+
+    twin = Twin(device)
+    new = [0] * 5
+    new[owner] = 40
+    twin.step(new)
+    twin.fork(owner, 1 - owner, 35)
+    twin.fork(owner, 2, 33)
+    held = [[list(x) for x in layer] for layer in twin.held]
+    for count in ([1, 1, 1, 0, 0], [2, 9, 4, 0, 0], [1, 1, 0, 0, 0]):
+        step, _ = twin.step(count)
+        twin.cache.cancel(step)
+        twin.held = [[list(x) for x in layer] for layer in held]
+    twin.step([1, 1, 1, 0, 0])
+    twin.step([2, 1, 3, 0, 0])

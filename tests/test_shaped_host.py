@@ -387,3 +387,58 @@ def test_distances_and_prefixes_after_an_eviction_are_refused(copies):
     for form in (dict(slopes=torch.zeros(2)), dict(prefixes=ints(0, 0, 0, 0))):
         with pytest.raises(ValueError, match="evicted"):
             cache.attention(0, step, torch.zeros(20, 2, 64).half(), **form)
+
+
+def rows_of(cache, sequence):
+    """A sequence's stored keys of all layers, entry after entry (the copies made on the
+    CPU are of keys)."""
+
+    at = [(page, slot) for page in cache._pages[sequence] for slot in range(cache.page_size)][: cache.lengths[sequence]]
+    return torch.stack([cache.key[:, page, 0, slot] for page, slot in at])
+
+
+def write(cache, step, before, marks):
+    """What a step's appends do: sequence b's new rows, all of the number ``marks[b]``."""
+
+    tables = step.block_tables.tolist()
+    for b, (old, now) in enumerate(zip(before, cache.lengths)):
+        for j in range(old, now):
+            cache.key[:, tables[b][j // cache.page_size], :, j % cache.page_size] = marks[b]
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (2, 1, 0), (1, 2, 0), (2, 0, 1)])
+@pytest.mark.parametrize("new", [(1, 1, 1), (9, 1, 4), (1, 14, 2), (1, 1, 0), (0, 3, 1)])
+def test_a_cancelled_step_leaves_the_entries_of_all_sharers(copies, order, new):
+    """A prompt's owner and forks of parts of it, in every order of their lengths:
+    what a step wrote before it was taken back is nobody's."""
+
+    owner, part, less = order
+    cache = cache_of(dtype=torch.bfloat16)
+    cache.key.zero_()
+    count = [0, 0, 0, 0]
+    count[owner] = 40
+    cache.begin(count)
+    for j in range(40):
+        cache.key[:, cache._pages[owner][j // 16], :, j % 16] = 100 + j
+    cache.fork(owner, part, 35)
+    cache.fork(owner, less, 33)
+    held = [rows_of(cache, b).clone() for b in range(3)]
+    lengths = cache.lengths
+    for _ in range(2):
+        step = cache.begin([*new, 0])
+        listed(cache)
+        write(cache, step, lengths, [1, 2, 3, 0])
+        for b in range(3):  # each has its own rows behind what it had
+            rows = rows_of(cache, b)
+            assert torch.equal(rows[: lengths[b]], held[b]) and (rows[lengths[b] :] == b + 1).all()
+        cache.cancel(step)
+        listed(cache)
+        assert cache.lengths == lengths
+        for b in range(3):
+            assert torch.equal(rows_of(cache, b), held[b]), b
+    # and taken up again
+    step = cache.begin([*new, 0])
+    write(cache, step, lengths, [1, 2, 3, 0])
+    for b in range(3):
+        rows = rows_of(cache, b)
+        assert torch.equal(rows[: lengths[b]], held[b]) and (rows[lengths[b] :] == b + 1).all()

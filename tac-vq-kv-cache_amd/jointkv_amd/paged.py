@@ -653,7 +653,7 @@ class PagedKVCache:
         old ones, a shared prompt, is not disturbed) and the old pages are
         freed.  The pages of one sequence's ``budget`` have to be free; where
         those of all do not fit, sequences follow one another into the pages
-        that the ones before left."""
+        that the ones before left, those that share pages last."""
 
         if self.weights is None:
             raise ValueError("the cache does not track weights")
@@ -661,21 +661,42 @@ class PagedKVCache:
             raise ValueError("the budget must be positive and hold the first and the last entries that stay")
         over = [b for b, length in enumerate(self._lengths) if length > budget]
         each = -(-budget // self.page_size)
-        # (a round frees what it takes and more, but for pages that others list)
-        rounds, free, uses = [], len(self._free), {}
-        while over:
-            now = over[: free // each]
+        rounds, free = [], len(self._free)
+        order = self._eviction_order(over, each)
+        while order:
+            now = order[: free // each]
             if not now:
                 raise ValueError(f"the eviction needs {each} pages, {free} are free")
-            free -= each * len(now)
-            for b in now:
-                for page in self._pages[b]:
-                    uses[page] = uses.get(page, self._uses[page]) - 1
-                    free += not uses[page]
-            rounds.append(now)
-            over = over[len(now) :]
+            rounds.append([b for b, _freed in now])
+            # (a round frees what it takes and more, but for pages that others list)
+            free += sum(freed for _b, freed in now) - each * len(now)
+            order = order[len(now) :]
         for now in rounds:
             self._evict(now, each, budget, sinks, recent)
+
+    def _eviction_order(self, over: list[int], each: int) -> list[tuple[int, int]]:
+        """The sequences in the order of their moves, and the pages that each frees:
+        first those that share none, then whoever costs fewest free pages, of equals
+        a sharer of what has the fewest users left (its last one frees it)."""
+
+        freed = {b: sum(self._uses[page] == 1 for page in self._pages[b]) for b in over}
+        order = [(b, freed[b]) for b in over if freed[b] == len(self._pages[b])]
+        sharers = [b for b in over if freed[b] < len(self._pages[b])]
+        uses, listers = {}, {}
+        for b in sharers:
+            for page in self._pages[b]:
+                uses[page] = self._uses[page]
+                listers.setdefault(page, []).append(b)
+        while sharers:
+            b = min(sharers, key=lambda b: (max(0, each - freed[b]), uses[self._pages[b][0]]))
+            sharers.remove(b)
+            order.append((b, freed[b]))
+            for page in self._pages[b]:
+                uses[page] -= 1
+                if uses[page] == 1:
+                    for other in listers[page]:
+                        freed[other] += other in sharers
+        return order
 
     def _evict(self, over: list[int], each: int, budget: int, sinks: int, recent: int) -> None:
         taken = self._free[-each * len(over) :]

@@ -442,3 +442,39 @@ def test_a_cancelled_step_leaves_the_entries_of_all_sharers(copies, order, new):
     for b in range(3):
         rows = rows_of(cache, b)
         assert torch.equal(rows[: lengths[b]], held[b]) and (rows[lengths[b] :] == b + 1).all()
+
+
+@pytest.mark.parametrize("private", [0, 2])
+def test_an_eviction_begins_with_what_frees_pages(copies, monkeypatch, private):
+    """Sharers of a prompt beside a sequence with pages of its own, two pages free: the
+    latter's move makes room for the others', whatever their order."""
+
+    monkeypatch.setattr(jkv.paged, "select_entries", lambda w, n, budget, **_: (torch.zeros(len(n), 1, budget, dtype=torch.int32), n))
+    monkeypatch.setattr(jkv.paged, "compact_pages", lambda k, v, old, kept, new, weights: weights.clone())
+    cache = cache_of(track_weights=True, pages=13)
+    owner, fork = [b for b in range(3) if b != private]
+    count = [0] * 4
+    count[owner], count[private] = 96, 80
+    cache.begin(count)
+    cache.fork(owner, fork)
+    assert cache.free_pages == 2
+    cache.evict(32)
+    listed(cache)
+    assert cache.lengths == (32, 32, 32, 0) and cache.free_pages == 13 - 6
+
+
+def test_an_eviction_finishes_one_prompts_sharers_first(copies, monkeypatch):
+    """Two prompts with sharers each and pages for three moves: the last sharer's is
+    what frees a prompt."""
+
+    monkeypatch.setattr(jkv.paged, "select_entries", lambda w, n, budget, **_: (torch.zeros(len(n), 1, budget, dtype=torch.int32), n))
+    monkeypatch.setattr(jkv.paged, "compact_pages", lambda k, v, old, kept, new, weights: weights.clone())
+    cache = cache_of(track_weights=True, pages=14, sequences=5)
+    cache.begin([64, 64, 0, 0, 0])
+    cache.fork(0, 2)
+    cache.fork(0, 3)
+    cache.fork(1, 4)
+    assert cache.free_pages == 6
+    cache.evict(32)  # (the first three to move would free nothing)
+    listed(cache)
+    assert cache.lengths == (32,) * 5 and cache.free_pages == 4

@@ -13,6 +13,7 @@ import functools
 from typing import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -66,6 +67,17 @@ def _written(*given: torch.Tensor | None) -> None:
     for tensor in given:
         if tensor is not None and not tensor.is_inference():
             torch.autograd.graph.increment_version(tensor)
+
+
+def _refuse_tangents(name: str, *given: torch.Tensor | None) -> None:
+    """Tangents of forward mode would be lost where no autograd function is applied.
+    (No cost outside of forward mode.)"""
+
+    if forward_ad._current_level < 0:
+        return
+    for tensor in given:
+        if tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def _refuse_second_derivative(name: str) -> None:

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._ops import _current, _overlaps, _plain, _refuse_second_derivative, _written
+from ._ops import _current, _overlaps, _plain, _refuse_second_derivative, _refuse_tangents, _written
 from .paged import _rows, _shape_args
 
 PACKED_TYPES = (torch.float16, torch.bfloat16)
@@ -125,8 +125,9 @@ def packed_attention(
     and 0.  Rows and gradients depend on what they see alone, whatever lies in
     other places.  Scores and sums are 32-bit, weights enter the second product
     rounded once to the inputs' type, and their sum as rounded divides it.
-    Differentiable in ``query``, ``key`` and ``value`` (not with a given ``out``);
-    a call repeats bit for bit, its gradients too.
+    Differentiable in ``query``, ``key`` and ``value`` (not with a given ``out``), once
+    and in reverse: ``create_graph`` and tangents are refused.  A call repeats bit for
+    bit, its gradients too.
     """
 
     if query.ndim != 3 or query.dtype not in PACKED_TYPES:
@@ -157,6 +158,7 @@ def packed_attention(
     scale = dim ** -0.5 if scale is None else float(scale)
     starts = starts.contiguous()
     args = (starts, prefixes, slopes, softcap, window, sinks, scale, lse)
+    _refuse_tangents("packed_attention", query, key, value, slopes)
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         if out is not None:
             raise ValueError("a given out is not differentiable")

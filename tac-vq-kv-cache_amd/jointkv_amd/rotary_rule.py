@@ -20,7 +20,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._ops import _current, _overlaps, _plain, _refuse_second_derivative, _written
+from ._ops import _current, _overlaps, _plain, _refuse_second_derivative, _refuse_tangents, _written
 from .attention import MISTRAL_ROPE_THETA
 
 MOST_DIMS = 256
@@ -195,8 +195,8 @@ def rotary(
 
     Returns the turned query, or the pair (query, key); into ``out`` and
     ``key_out`` if given, which may be the inputs themselves but overlap them in
-    no other way.  Differentiable in both (not with given outputs); a call
-    repeats bit for bit.
+    no other way.  Differentiable in both (not with given outputs), once and in
+    reverse: ``create_graph`` and tangents are refused.  A call repeats bit for bit.
     """
 
     if query.ndim != 3 or query.dtype not in (torch.float16, torch.bfloat16, torch.float32):
@@ -217,6 +217,7 @@ def rotary(
         if positions.dtype != torch.int32 or positions.shape != (count,):
             raise ValueError("positions must be int32 [N], or [B] beside starts")
         positions = positions.contiguous()
+    _refuse_tangents("rotary", query, key)
     if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
         if out is not None or key_out is not None:
             raise ValueError("given outputs are not differentiable")

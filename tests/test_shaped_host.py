@@ -478,3 +478,26 @@ def test_an_eviction_finishes_one_prompts_sharers_first(copies, monkeypatch):
     cache.evict(32)  # (the first three to move would free nothing)
     listed(cache)
     assert cache.lengths == (32,) * 5 and cache.free_pages == 4
+
+
+def test_tangents_are_refused():
+    """Forward mode: a dual tensor would give a result without its tangent."""
+
+    q, k = torch.zeros(4, 2, 64).half(), torch.zeros(4, 1, 64).half()
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda x: torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for args in ((dual(q),), (q, dual(k)), (dual(q), k)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    jkv.rotary(*args)
+        for args in ((dual(q), k, k), (q, dual(k), k), (q, k, dual(k))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                jkv.packed_attention(*args, ints(0, 4))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            jkv.packed_attention(q, k, k, ints(0, 4), slopes=dual(torch.zeros(2)))
+        with pytest.raises(ValueError, match="HIP"):  # (none has a tangent)
+            jkv.packed_attention(q, k, k, ints(0, 4))
+        with pytest.raises(ValueError, match="HIP"):
+            jkv.rotary(q, k)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda x: jkv.rotary(x), (q,), (q,))

@@ -24,11 +24,12 @@
 // itself (fp16 holds 2^-34 of it then), ds in fp16 times a power of two that keeps
 // the largest that inputs of their sizes could give below 2^15.
 //
-// A masked weight is 0, but 0 times an infinite or NaN row is not.  Such a row makes
-// its raw scores (or do's products) in a tile not finite, seen or not: in tiles with
-// masked places these are tested, and if one is odd the second operands are read
-// with such elements as 0.  Where they are seen, p or delta are not finite and
-// carry it.
+// A masked weight is 0, but 0 times an infinite or NaN row is not: whatever is not
+// finite in a tile, seen or not, makes the sums so.  A walk that ends in finite sums
+// needs no second; after another, the walk is made again with the masked p and ds
+// selected, all tiles alike, the last products' operands with such elements as 0, and
+// what they are added where they are seen: do's to dv with their sign, NaN for those of q
+// and k (their scores are not finite: their ds is 0 or NaN).
 #pragma once
 
 #include <utility>
@@ -330,6 +331,9 @@ __device__ __forceinline__ typename Half16<DT>::V8 read_cols(uint32_t cols, int 
   return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
+// How a walk takes a tile.
+enum { kSeenInPart, kSeenWhole, kWalkedAgain };
+
 // dk and dv of 128 keys: a wave's 32 are columns of S = Q K^T and dP = dO V^T
 // (v_mfma_f32_32x32x16; 16 of 32 rows a lane), and rows of dv += P^T dO and dk +=
 // dS^T Q, which take P and dS from those registers and dO and Q by transposing
@@ -429,8 +433,8 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
   // A step's products in turn: S, dP, dv, dk, and beside each a few places' vector
   // instructions, fenced (the compiler else gathers each kind, and they overlap
   // little).  Operands are read two products ahead.
-  auto work = [&](int32_t tile, int32_t g, auto stage, auto masked) {
-    constexpr bool MASKED = decltype(masked)::value;
+  auto work = [&](int32_t tile, int32_t g, auto stage, auto kind) {
+    constexpr bool MASKED = decltype(kind)::value != kSeenWhole, AGAIN = decltype(kind)::value == kWalkedAgain;
     constexpr int kOps = 2 * kSteps + 4 * kDims;
     const uint32_t stage_at = stages_at + (uint32_t)(stage * kStage);
     const int32_t t0 = 32 * tile;
@@ -454,45 +458,28 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
         ring[n % 3] = read_cols<DT, D>(cols, m % kDims, stage_at + (n < 2 * kSteps + 2 * kDims ? kTile : 0) + 16 * (m / kDims) * kRowBytes);
       }
     };
-    float odd = 0.f;
-    bool clean = false;
     auto operand = [&](int n) -> V8 {
-      if (MASKED && clean) return finite_part<DT>(ring[n % 3]);
+      if constexpr (AGAIN) return finite_part<DT>(ring[n % 3]);
       return ring[n % 3];
     };
     const uint32_t seen_at = (uint32_t)(t0 + 4 * lh - key_from);
+    auto is_seen = [&](int e) { return seen_at + (uint32_t)(8 * (e >> 2) + (e & 3)) < key_rows; };
     auto read_bases = [&](int q4) { bases[q4] = *(lds_f4*)(size_t)(stats_at + 32 * q4); };
-    auto first = [&](int e) {
-      if constexpr (MASKED) odd = fmaf(sc[e], 0.f, odd);
-      sc[e] = shape_first<FORM>(shape, sc[e]);
-    };
+    auto first = [&](int e) { sc[e] = shape_first<FORM>(shape, sc[e]); };
     // p, and what ds takes of it (in sc)
     auto weigh = [&](int e) {
       float slant = 1.f;
       const float x = shape_and_slant<FORM>(shape, sc[e], at + (float)(8 * (e >> 2) + (e & 3)), bases[e >> 2][e & 3], &slant);
       float p = __builtin_amdgcn_exp2f(x);
-      if constexpr (MASKED) {
-        const bool seen = seen_at + (uint32_t)(8 * (e >> 2) + (e & 3)) < key_rows;
-        p = seen ? p : 0.f;
-        if constexpr (FORM & kFormCap) slant = seen ? slant : 0.f;
-      }
+      if constexpr (MASKED) p = is_seen(e) ? p : 0.f;
       pf[e >> 3][e & 7] = (T)p;
       if constexpr (FORM & kFormCap) p *= slant;
       if constexpr (DT == JKV_F16) p *= factor;
       sc[e] = p;
     };
-    // where do is not finite, delta is not, and what sees it takes a NaN
-    auto poison = [&](int e) {
-      const float minus_delta = *(__attribute__((address_space(3))) const float*)(size_t)(stats_at + 256 + 32 * (e >> 2) + 4 * (e & 3));
-      const bool seen = seen_at + (uint32_t)(8 * (e >> 2) + (e & 3)) < key_rows;
-      if (seen && !__builtin_isfinite(minus_delta)) {
-        pf[e >> 3][e & 7] = (T)NAN;
-        sc[e] = NAN;
-      }
-    };
     auto lean = [&](int e) {
       float ds = sc[e] * dp[e];
-      if constexpr (MASKED) ds = sc[e] == 0.f ? 0.f : ds;
+      if constexpr (AGAIN) ds = is_seen(e) ? ds : 0.f;
       df[e >> 3][e & 7] = (T)ds;
     };
     read(0);
@@ -523,14 +510,6 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
           for (int e = c * kWeigh; e < 8; ++e) weigh(e);
           read_bases(2);
           read_bases(3);
-          if constexpr (MASKED) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) odd = fmaf(dp[e], 0.f, odd);
-            clean = __any(odd != 0.f);
-            if (clean)
-#pragma unroll
-              for (int e = 0; e < 8; ++e) poison(e);
-          }
         }
       } else {
         constexpr int kEach = 8 / kDims;
@@ -539,12 +518,8 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
           dv[d] = mfma32<DT>(pf[st], operand(n), dv[d]);
 #pragma unroll
           for (int e = d * kEach; e < (d + 1) * kEach; ++e) {
-            if (st == 0) {
-              weigh(8 + e);
-              if (MASKED && clean) poison(8 + e);
-            } else {
-              lean(e);
-            }
+            if (st == 0) weigh(8 + e);
+            else lean(e);
           }
         } else {
           dk[d] = mfma32<DT>(df[st], operand(n), dk[d]);
@@ -555,6 +530,28 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
       }
       __builtin_amdgcn_sched_barrier(0);
     });
+    if constexpr (AGAIN) {
+      V8 seen[2];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) seen[e >> 3][e & 7] = is_seen(e) ? (T)1.f : (T)0.f;
+#pragma unroll
+      for (int n = 0; n < 2 * kDims; ++n) {  // rows of do, then of q
+        const int d = n % kDims;
+        float16v up = {}, down = {};
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          V8 vu, vd;
+          non_finite_marks<DT>(read_cols<DT, D>(cols, d, stage_at + (n < kDims ? kTile : 0) + 16 * st * kRowBytes), &vu, &vd);
+          up = mfma32<DT>(seen[st], vu, up);
+          down = mfma32<DT>(seen[st], vd, down);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (n < kDims) dv[d][e] = marked(dv[d][e], up[e], down[e]);
+          else dk[d][e] = up[e] + down[e] > 0.f ? NAN : dk[d][e];
+        }
+      }
+    }
   };
 
   // Row tiles that all of the block's keys are seen by, [full0, full1), come last and
@@ -579,12 +576,15 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
     for (s.g += by; s.g >= heads; s.g -= heads) --s.tile;
   };
   Step now = {tile0 == full0 ? full1 : tile0, 0}, first_plain = {full1 - 1, 0};
+  constexpr auto kPart = std::integral_constant<int, kSeenInPart>();
+  constexpr auto kWhole = std::integral_constant<int, kSeenWhole>();
   if constexpr (ALONE) {  // a wave's share: every fourth
     advance(now, wave);
     go_back(first_plain, wave);
     edge = (edge - wave + 3) / 4;
     plain = (plain - wave + 3) / 4;
   }
+  const Step first_edge = now;
   Step next = now;
   int32_t loaded = 0;
   auto load_next = [&](int stage) {
@@ -607,24 +607,55 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
 #pragma unroll
   for (int c = 0; c < kSteps; ++c) asm volatile("" : "+v"(kf[c]));  // waited for here, with all loads before
   if constexpr (ALONE) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the values have landed
+  auto is_on = [&](int32_t tile) {
+    const int32_t t0 = 32 * tile;
+    return wj0 < T0 && (wj0 <= t0 + 31 || wj0 < prefix) && (wj0 + 31 > t0 - a.window || wj0 < a.sinks);
+  };
   for (int32_t n = edge; n > 0; --n) {
     turn_over((n & 1) ^ 1);
-    const int32_t t0 = 32 * now.tile;
-    if (wj0 < T0 && (wj0 <= t0 + 31 || wj0 < prefix) && (wj0 + 31 > t0 - a.window || wj0 < a.sinks))
-      work(now.tile, now.g, n & 1, std::true_type());
+    if (is_on(now.tile)) work(now.tile, now.g, n & 1, kPart);
     advance(now, kStride);
   }
   now = first_plain;
   for (int32_t n = 0; n < plain; n += 2) {
     turn_over(1);
-    work(now.tile, now.g, std::integral_constant<int, 0>(), std::false_type());
+    work(now.tile, now.g, std::integral_constant<int, 0>(), kWhole);
     go_back(now, kStride);
     if (n + 1 >= plain) break;
     turn_over(0);
-    work(now.tile, now.g, std::integral_constant<int, 1>(), std::false_type());
+    work(now.tile, now.g, std::integral_constant<int, 1>(), kWhole);
     go_back(now, kStride);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  // (see the head of this file; the same steps in the same order, a stage's loads
+  // waited for)
+  float odd = 0.f;
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) odd = fmaf(dv[d][e], 0.f, fmaf(dk[d][e], 0.f, odd));
+  if (ALONE ? __any(odd != 0.f) : __syncthreads_or(odd != 0.f)) {
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) {
+      dk[d] = float16v{};
+      dv[d] = float16v{};
+    }
+    auto meet = [&]() {
+      if constexpr (ALONE) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    now = first_edge;
+    for (int32_t n = 0; n < edge + plain; ++n) {
+      if (n == edge) now = first_plain;
+      meet();
+      load_step(now.tile, now.g, 0);
+      meet();
+      if (is_on(now.tile)) work(now.tile, now.g, std::integral_constant<int, 0>(), std::integral_constant<int, kWalkedAgain>());
+      if (n < edge) advance(now, kStride);
+      else go_back(now, kStride);
+    }
+  }
 
   // lane holds dim 32d + ln of keys 8(e/4) + 4lh + e%4
   const float dv_mul = 0x1p-10f, dk_mul = a.scale * (FORM & kFormCap ? 4.f : 1.f) * 0x1p-10f / factor;
@@ -762,8 +793,8 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
 #pragma unroll
   for (int d = 0; d < kDims; ++d) dq[d] = float16v{};
   const TileAt tile_lane = tile_at<D>(lds_base, lane);
-  auto work = [&](int32_t e0, auto stage, auto masked) {
-    constexpr bool MASKED = decltype(masked)::value;
+  auto work = [&](int32_t e0, auto stage, auto kind) {
+    constexpr bool MASKED = decltype(kind)::value != kSeenWhole, AGAIN = decltype(kind)::value == kWalkedAgain;
     const uint32_t stage_at = (uint32_t)(stage * 2 * kTile);
     uint32_t rows = tile_lane.rows, cols = tile_lane.cols;
     asm volatile("" : "+v"(rows), "+v"(cols));
@@ -780,32 +811,25 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
         ring[n % 3] = read_cols<DT, D>(cols, m % kDims, stage_at + 16 * (m / kDims) * kRowBytes);
       }
     };
-    float odd = 0.f;
-    bool clean = false;
     const uint32_t seen_at = (uint32_t)(e0 + 4 * lh - seen_from);
-    const float at = (float)(e0 + 4 * lh - self);
-    auto first = [&](int half, int e) {
-      if constexpr (MASKED) odd = fmaf(sc[half][e], 0.f, odd);
-      sc[half][e] = shape_first<FORM>(shape, sc[half][e]);
+    auto is_seen = [&](int half, int e) {  // entries of the window, or first ones before it
+      const uint32_t from = seen_at + (uint32_t)(32 * half + 8 * (e >> 2) + (e & 3));
+      return from < seen_count || (int32_t)from < sunk;
     };
+    const float at = (float)(e0 + 4 * lh - self);
+    auto first = [&](int half, int e) { sc[half][e] = shape_first<FORM>(shape, sc[half][e]); };
     auto weigh = [&](int half, int e) {
       float slant = 1.f;
       const float x = shape_and_slant<FORM>(shape, sc[half][e], at + (float)(32 * half + 8 * (e >> 2) + (e & 3)), base, &slant);
       float p = __builtin_amdgcn_exp2f(x);
-      if constexpr (MASKED) {
-        const uint32_t from = seen_at + (uint32_t)(32 * half + 8 * (e >> 2) + (e & 3));
-        // (entries of the window, or first ones before it)
-        const bool seen = from < seen_count || (int32_t)from < sunk;
-        p = seen ? p : 0.f;
-        if constexpr (FORM & kFormCap) slant = seen ? slant : 0.f;
-      }
+      if constexpr (MASKED) p = is_seen(half, e) ? p : 0.f;
       if constexpr (FORM & kFormCap) p *= slant;
       if constexpr (DT == JKV_F16) p *= factor;
       sc[half][e] = p;
     };
     auto lean = [&](int half, int e) {
       float ds = sc[half][e] * (dp[half][e] + minus_delta);
-      if constexpr (MASKED) ds = sc[half][e] == 0.f ? 0.f : ds;
+      if constexpr (AGAIN) ds = is_seen(half, e) ? ds : 0.f;
       df[half][e >> 3][e & 7] = (T)ds;
     };
     read(0);
@@ -826,8 +850,9 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
         }
       } else {
         const int m = n - 4 * kSteps, d = m % kDims, st = m / kDims;
-        if (m == 0 && MASKED) clean = __any(odd != 0.f);
-        dq[d] = mfma32<DT>(MASKED && clean ? finite_part<DT>(ring[n % 3]) : ring[n % 3], df[st / 2][st % 2], dq[d]);
+        V8 keys = ring[n % 3];
+        if constexpr (AGAIN) keys = finite_part<DT>(keys);
+        dq[d] = mfma32<DT>(keys, df[st / 2][st % 2], dq[d]);
 #pragma unroll
         for (int e = d * kBeside; e < (d + 1) * kBeside; ++e) {
           if (st == 0) weigh(1, e);
@@ -837,6 +862,23 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
       }
       __builtin_amdgcn_sched_barrier(0);
     });
+    if constexpr (AGAIN) {
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) {
+        float16v some = {};
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          V8 vu, vd, seen;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) seen[e] = is_seen(st / 2, 8 * (st % 2) + e) ? (T)1.f : (T)0.f;
+          non_finite_marks<DT>(read_cols<DT, D>(cols, d, stage_at + 16 * st * kRowBytes), &vu, &vd);
+          some = mfma32<DT>(vu, seen, some);
+          some = mfma32<DT>(vd, seen, some);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dq[d][e] = some[e] > 0.f ? NAN : dq[d][e];
+      }
+    }
   };
   // as above: the tiles that all rows see, [full0, full1), come last
   int32_t full1 = pt.lead + (row_reach<FORM>(first, prefix) + 1) / 64 - pt.main, full0 = pt.lead;
@@ -846,6 +888,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   const int32_t plain = full1 - full0, edge = pt.count - plain;
   int32_t now = full0 == 0 ? full1 : 0;
   if (now >= pt.count) now = full0;
+  const int32_t start = now;
   int32_t next = now, left = pt.count;
   auto advance = [&](int32_t& i) {
     const bool in_full = i >= full0 && i < full1;
@@ -867,22 +910,44 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
     advance(next);
     --left;
   }
+  auto is_on = [&](int32_t e0) { return e0 <= row_reach<FORM>(wlast, prefix) && (e0 + 63 > wfirst - a.window || e0 < a.sinks); };
   for (int32_t n = edge; n > 0; --n) {
     turn_over((n & 1) ^ 1);
     const int32_t e0 = entry_of(now);
-    if (e0 <= row_reach<FORM>(wlast, prefix) && (e0 + 63 > wfirst - a.window || e0 < a.sinks)) work(e0, n & 1, std::true_type());
+    if (is_on(e0)) work(e0, n & 1, std::integral_constant<int, kSeenInPart>());
     advance(now);
   }
+  constexpr auto kWhole = std::integral_constant<int, kSeenWhole>();
   for (int32_t n = 0; n < plain; n += 2) {
     turn_over(1);
-    work(entry_of(now), std::integral_constant<int, 0>(), std::false_type());
+    work(entry_of(now), std::integral_constant<int, 0>(), kWhole);
     advance(now);
     if (n + 1 >= plain) break;
     turn_over(0);
-    work(entry_of(now), std::integral_constant<int, 1>(), std::false_type());
+    work(entry_of(now), std::integral_constant<int, 1>(), kWhole);
     advance(now);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  float odd = 0.f;  // as above
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) odd = fmaf(dq[d][e], 0.f, odd);
+  if (__syncthreads_or(odd != 0.f)) {
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) dq[d] = float16v{};
+    auto meet = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    now = start;
+    for (int32_t n = 0; n < pt.count; ++n) {
+      const int32_t e0 = entry_of(now);
+      meet();
+      load_step(now, 0);
+      meet();
+      if (is_on(e0)) work(e0, std::integral_constant<int, 0>(), std::integral_constant<int, kWalkedAgain>());
+      advance(now);
+    }
+  }
   if (!row_ok) return;
   // lane holds dims 32d + 8(e/4) + 4lh + e%4 of row ln
   const float mul = a.scale * (FORM & kFormCap ? 4.f : 1.f) * 0x1p-10f / factor;

@@ -510,3 +510,95 @@ def test_buffers_given_beside_autograd(device):
         z = x[0].clone()
         assert jkv.rotary(z, starts=starts, out=z) is z
         assert jkv.packed_attention(z, x[1], x[2], starts, out=torch.empty_like(z)).shape == z.shape
+
+
+def _sum_seen(weights, seen, rows):
+    """``sum_i weights[i,j] rows[i]`` over the i that j counts for, infinities and NaN
+    among them as they come."""
+
+    weights = torch.where(seen, weights, 0.0)
+    odd = ~torch.isfinite(rows).all(-1)
+    total = weights[~odd].T @ rows[~odd]
+    for i in odd.nonzero()[:, 0].tolist():
+        total = total + torch.where(seen[i][:, None], weights[i][:, None] * rows[i], 0.0)
+    return total
+
+
+def defined_gradients(q, k, v, d, *, cap, window, prefix, h):
+    """The gradients of one kv head's sequence from their formulas in 64 bits, also
+    where rows are not finite, and by how much roundings of h may change what is."""
+
+    q, k, v, d = (x.double() for x in (q, k, v, d))
+    rows, heads, dim = q.shape
+    seen = ref.visible(rows, rows, window, 0, prefix)
+    grads = [torch.zeros_like(x) for x in (q, k, v)]
+    bounds = [torch.zeros_like(x) for x in (q, k, v)]
+    tame = lambda x: torch.nan_to_num(x.abs(), 0.0, 0.0, 0.0)
+    for g in range(heads):
+        x, steep = ref.scores(q[:, g], k, scale=dim**-0.5, cap=cap, slope=None, first=0)
+        x = torch.where(seen, x, -torch.inf)
+        e = torch.exp(x - x.amax(-1, keepdim=True))
+        p = e / e.sum(-1, keepdim=True)
+        out = _sum_seen(p.T, seen.T, v)
+        dp, delta = d[:, g] @ v.T, (d[:, g] * out).sum(-1, keepdim=True)
+        slant = steep * dim**-0.5
+        ds = p * (dp - delta) * slant
+        grads[0][:, g] = _sum_seen(ds.T, seen.T, k)
+        grads[1] += _sum_seen(ds, seen, q[:, g])
+        grads[2] += _sum_seen(p, seen, d[:, g])
+        # p and ds rounded to h each, delta's own rounding, scores off as elsewhere here
+        size = float((tame(q[:, g]) @ tame(k).T).max()) * dim**-0.5
+        off = 2 * (size * (dim + 2) * 2.0**-23 + 8 * (cap or 0.0) * 2.0**-23 + 2.0**-20) + (dim + rows) * 2.0**-23
+        reach = tame(d[:, g]) @ tame(v).T + (tame(d[:, g]) * tame(out)).sum(-1, keepdim=True)
+        much = tame(p) * tame(slant) * (h * (2 * tame(dp - delta) + tame(delta)) + (h * h + off) * reach)
+        bounds[0][:, g] = _sum_seen(much.T, seen.T, tame(k))
+        bounds[1] += _sum_seen(much, seen, tame(q[:, g]))
+        bounds[2] += _sum_seen(tame(p) * (h + off) * 1.01, seen, tame(d[:, g]))
+    for g, b in zip(grads, bounds):
+        b += h * tame(g) + 1e-7 * b.max() + 2.0**-24
+    return grads, bounds
+
+
+@pytest.mark.parametrize("cap", [30.0, None])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sizes,qh,kvh,dim,window,prefix", [
+    ([330], 4, 2, 64, None, 0),              # 32 keys a workgroup
+    ([100, 330], 4, 2, 128, 150, 40),
+    ([600], 16, 2, 128, None, 0),            # heads in splits
+    ([330, 250] * 6, 12, 12, 128, None, 0),  # 128 keys a workgroup, all heads
+])
+def test_what_odd_elements_reach(device, cap, dtype, sizes, qh, kvh, dim, window, prefix):
+    """One infinite or NaN element: every gradient is finite where its formula is, in
+    tiles with and without masked places, has its value there, and is the same as
+    without the element where that takes no part."""
+
+    per = qh // kvh
+    at = sum(sizes[: len(sizes) - 1 - len(sizes) // 2]) + 170
+    prefixes = torch.full((len(sizes),), prefix, dtype=torch.int32, device=device)
+    args = dict(window=window, softcap=cap, prefixes=prefixes)
+    base = Texts(41, sizes, qh, kvh, dim, dtype, gain=1.5)
+    span = next(slice(a, b) for a, b in base.spans if a <= at < b)
+    _, clean = run_grads(base, device, **args)
+    for name in ("q", "k", "v", "d"):
+        for bad in (float("inf"), float("-inf"), float("nan")):
+            odd = Texts(41, sizes, qh, kvh, dim, dtype, gain=1.5)
+            getattr(odd, name)[at, 1 if name in "kv" else per, 3] = bad
+            _, grads = run_grads(odd, device, **args)
+            heads = slice(per, 2 * per)
+            want, bounds = defined_gradients(odd.q[span, heads], odd.k[span, 1], odd.v[span, 1], odd.d[span, heads], cap=cap,
+                                             window=window, prefix=prefix, h=half_step(dtype))
+            # beside the sequence and the group nothing changes
+            for got, same, of in zip(grads, clean, (heads, 1, 1)):
+                got, same = got.clone(), same.clone()
+                got[span, of] = 0
+                same[span, of] = 0
+                assert torch.equal(got, same), (name, bad)
+            if name == "v":  # p does not depend on values
+                assert torch.equal(grads[2], clean[2]), bad
+            for part, got, w, bound in zip(("dq", "dk", "dv"), (grads[0][span, heads], grads[1][span, 1], grads[2][span, 1]), want, bounds):
+                got = got.cpu().double()
+                finite = torch.isfinite(w)
+                assert torch.equal(torch.isfinite(got), finite), (name, bad, part)
+                assert ((got - w).abs() <= bound)[finite].all(), (name, bad, part)
+                if (name, part) == ("d", "dv"):
+                    assert torch.equal(torch.isnan(got), torch.isnan(w)) and torch.equal(got[~finite & ~torch.isnan(w)], w[~finite & ~torch.isnan(w)])

@@ -17,7 +17,6 @@ struct PackedGradArgs {
   float scale, scale2, cap_mul, cap2;
   const float* slopes;
   float *bases, *minus_delta;  // [QH][N]: 10 and the cap (base 2) less the base-2 log-sum-exp, -rowsum(do o)
-  float2* maxima;  // [kGradBlocks]: largest finite |do| and |v| (fp16)
   // dk and dv: 32 keys a workgroup instead of 128; or the group's heads in splits
   // of heads_each, whose sums a last launch adds up
   int32_t alone, splits, heads_each;

@@ -71,7 +71,7 @@ PackedGradPlan packed_grad_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, i
     p.splits = 1;
   }
   p.stats_bytes = ceil_div(N * QH * 4, 256) * 256;
-  p.part_at = 2 * p.stats_bytes + kGradBlocks * 8;
+  p.part_at = 2 * p.stats_bytes;
   p.bytes = p.part_at + (p.splits > 1 ? 2 * p.splits * N * KVH * D * 4 : 0);
   return p;
 }
@@ -184,7 +184,6 @@ int jkv_packed_attention_backward(const void* q, int64_t q_stride_t, int64_t q_s
   a.cap_mul = softcap > 0.f ? 2.f * a.scale2 / softcap : 0.f; a.cap2 = shape.cap2; a.slopes = slopes;
   a.bases = (float*)workspace;
   a.minus_delta = (float*)((uint8_t*)workspace + plan.stats_bytes);
-  a.maxima = (float2*)((uint8_t*)workspace + 2 * plan.stats_bytes);
   a.part = (float*)((uint8_t*)workspace + plan.part_at);
   a.alone = plan.alone; a.splits = plan.splits; a.heads_each = plan.heads_each;
   if (form == kFormPlain) form = kFormShaped;

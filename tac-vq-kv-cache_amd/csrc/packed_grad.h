@@ -21,8 +21,10 @@
 // us, vector instructions, and masked tiles at both ends of short walks.
 //
 // p and ds enter their products rounded once to the inputs' type, p as 2^10 of
-// itself (fp16 holds 2^-34 of it then), ds in fp16 times a power of two that keeps
-// the largest that inputs of their sizes could give below 2^15.
+// itself (fp16 holds 2^-34 of it then), ds in fp16 times a power of two of its row
+// (dq) or key (dk): from 2^64 on it falls as the largest ds passes 2^15, which then
+// is 2^7 to 2^8, and the sums with it.  So it follows from what a row sees, or what
+// sees a key, alone, and holds 2^-32 of the largest.
 //
 // A masked weight is 0, but 0 times an infinite or NaN row is not: whatever is not
 // finite in a tile, seen or not, makes the sums so.  A walk that ends in finite sums
@@ -47,23 +49,6 @@ template <int N, typename F> __device__ __forceinline__ void each_to(F&& f) {
   each_of(f, std::make_integer_sequence<int, N>());
 }
 
-// The largest |x| over finite fp16 halves, as halves of bits plus 2^10: those of
-// infinities and NaN become negative and lose every comparison.
-typedef short short2v __attribute__((ext_vector_type(2)));
-typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ short2v largest_finite(uint4v w, short2v most) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const ushort2v bits = __builtin_bit_cast(ushort2v, w[e] & 0x7fff7fffu) + (unsigned short)0x0400;
-    most = __builtin_elementwise_max(most, __builtin_bit_cast(short2v, bits));
-  }
-  return most;
-}
-__device__ __forceinline__ float largest_value(short2v most) {
-  const short m = most[0] > most[1] ? most[0] : most[1];
-  return (float)__builtin_bit_cast(_Float16, (short)(m - 0x0400));
-}
-
 // Per row: delta, and the log-sum-exp as the walks take it.  Rows that no sequence
 // owns get gradients of 0 here.
 template <int DT, int D>
@@ -73,12 +58,10 @@ __global__ __launch_bounds__(256) void packed_rows_kernel(PackedGradArgs a) {
   const int tid = threadIdx.x, part = tid % kLanes, r = tid / kLanes;
   int32_t lead = clamp_i32(a.starts[0], 0, a.N), from = clamp_i32(a.starts[a.B], 0, a.N);
   if (from < lead) from = lead;
-  short2v most_d = {0x0400, 0x0400}, most_v = {0x0400, 0x0400};
   const int64_t rows = (int64_t)a.N * a.QH, stride = (int64_t)gridDim.x * kRows;
   // (four rows' loads in flight)
   for (int64_t row0 = (int64_t)blockIdx.x * kRows + r; row0 < rows; row0 += 4 * stride) {
-    uint4v dw[4];
-    V8 o[4], rest[4];
+    V8 d[4], o[4], rest[4];
     int32_t n[4], head[4];
     bool on[4];
 #pragma unroll
@@ -88,25 +71,23 @@ __global__ __launch_bounds__(256) void packed_rows_kernel(PackedGradArgs a) {
       head[i] = (int32_t)(row - (int64_t)n[i] * a.QH);
       on[i] = row < rows && n[i] >= lead && n[i] < from;
       if (row < rows && !on[i] && a.dq != nullptr) *(uint4v*)(a.dq + row * (2 * D) + 16 * part) = uint4v{0u, 0u, 0u, 0u};
-      dw[i] = uint4v{0u, 0u, 0u, 0u};
+      d[i] = V8{};
       o[i] = V8{};
       rest[i] = V8{};
       if (!on[i]) continue;
-      dw[i] = *(const uint4v*)(a.d + n[i] * a.dst + head[i] * a.dsh + 16 * part);
+      d[i] = *(const V8*)(a.d + n[i] * a.dst + head[i] * a.dsh + 16 * part);
       o[i] = __builtin_nontemporal_load((const V8*)(a.o + n[i] * a.ost + head[i] * a.osh + 16 * part));
       if (a.rest != nullptr) rest[i] = __builtin_nontemporal_load((const V8*)(a.rest + row * (2 * D) + 16 * part));
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const V8 d = __builtin_bit_cast(V8, dw[i]);
       // (where one place holds most of a row's weight, do v and delta are near each
       // other: without the rest the gradients of bf16 rows are 3.6e-3 off, with it 2.5e-3)
       float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf((float)d[e], (float)o[i][e], sum);
+      for (int e = 0; e < 8; ++e) sum = fmaf((float)d[i][e], (float)o[i][e], sum);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf((float)d[e], (float)rest[i][e], sum);
-      if constexpr (DT == JKV_F16) most_d = largest_finite(dw[i], most_d);
+      for (int e = 0; e < 8; ++e) sum = fmaf((float)d[i][e], (float)rest[i][e], sum);
 #pragma unroll
       for (int off = kLanes / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
       if (on[i] && part == 0) {
@@ -118,57 +99,22 @@ __global__ __launch_bounds__(256) void packed_rows_kernel(PackedGradArgs a) {
       }
     }
   }
+  if (a.dk == nullptr && a.dv == nullptr) return;
   const int64_t kv_rows = (int64_t)a.N * a.KVH;
-  if (DT == JKV_F16 || a.dk != nullptr || a.dv != nullptr)
-    for (int64_t row = (int64_t)blockIdx.x * kRows + r; row < kv_rows; row += stride) {
-      const int32_t n = (int32_t)((uint32_t)row / (uint32_t)a.KVH), head = (int32_t)(row - (int64_t)n * a.KVH);
-      if (n < lead || n >= from) {
-        if (a.dk != nullptr) *(uint4v*)(a.dk + row * (2 * D) + 16 * part) = uint4v{0u, 0u, 0u, 0u};
-        if (a.dv != nullptr) *(uint4v*)(a.dv + row * (2 * D) + 16 * part) = uint4v{0u, 0u, 0u, 0u};
-      } else if constexpr (DT == JKV_F16) {
-        most_v = largest_finite(*(const uint4v*)(a.v + n * a.vst + head * a.vsh + 16 * part), most_v);
-      }
-    }
-  if constexpr (DT == JKV_F16) {
-    __shared__ float2 waves[4];
-    float d = largest_value(most_d), v = largest_value(most_v);
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-      d = fmaxf(d, __shfl_xor(d, off, 64));
-      v = fmaxf(v, __shfl_xor(v, off, 64));
-    }
-    if ((tid & 63) == 0) waves[tid >> 6] = float2{d, v};
-    __syncthreads();
-    if (tid == 0)
-      a.maxima[blockIdx.x] = float2{fmaxf(fmaxf(waves[0].x, waves[1].x), fmaxf(waves[2].x, waves[3].x)),
-                                    fmaxf(fmaxf(waves[0].y, waves[1].y), fmaxf(waves[2].y, waves[3].y))};
+  for (int64_t row = (int64_t)blockIdx.x * kRows + r; row < kv_rows; row += stride) {
+    const int32_t n = (int32_t)((uint32_t)row / (uint32_t)a.KVH);
+    if (n >= lead && n < from) continue;
+    if (a.dk != nullptr) *(uint4v*)(a.dk + row * (2 * D) + 16 * part) = uint4v{0u, 0u, 0u, 0u};
+    if (a.dv != nullptr) *(uint4v*)(a.dv + row * (2 * D) + 16 * part) = uint4v{0u, 0u, 0u, 0u};
   }
 }
 
-// The power of two that ds takes (with p's 2^10) so that it stays below 2^15:
-// |do v - delta| is at most 2 D max|do| max|v|.
-template <int DT, int D>
-__device__ __forceinline__ float ds_factor(const PackedGradArgs& a) {
-  if constexpr (DT != JKV_F16) return 1.f;
-  const int lane = threadIdx.x & 63;
-  float most_d = 0.f, most_v = 0.f;
-#pragma unroll
-  for (int i = 0; i < kGradBlocks / 64; ++i) {
-    const float2 m = a.maxima[64 * i + lane];
-    most_d = fmaxf(most_d, m.x);
-    most_v = fmaxf(most_v, m.y);
-  }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    most_d = fmaxf(most_d, __shfl_xor(most_d, off, 64));
-    most_v = fmaxf(most_v, __shfl_xor(most_v, off, 64));
-  }
-  const float most = 2.f * D * most_d * most_v;
-  if (!(most > 0.f)) return 1.f;
-  // (fp16 values: 2^-48 to 2^32 times 2^8; with a cap, its slope's 4 comes last)
-  int e;
-  frexpf(most, &e);  // most < 2^e
-  return __uint_as_float((uint32_t)(127 + 5 - e) << 23);
+// What ds takes in fp16 at first (with p's 2^10, 2^64: |do v - delta| of finite rows is
+// below 2^41), and what brings it, `most` at the largest, to 2^7 to 2^8 once it has
+// passed 2^15 (1 before, and where it is not finite).
+static constexpr float kMostDs = 0x1p15f, kFirstDs = 0x1p54f;
+__device__ __forceinline__ float ds_shrink(float most) {
+  return most > kMostDs && most < INFINITY ? __builtin_amdgcn_ldexpf(1.f, 8 - __builtin_amdgcn_frexp_expf(most)) : 1.f;
 }
 
 // Of 64 sequences with `own` blocks in a lane's (`upto` of it and those before), the
@@ -385,7 +331,6 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
       if (ok) kf[c] = *(const V8*)(kp + 32 * c);
     }
   }
-  float factor = 1.f;
 
   // the rows that see some key of the block
   const int32_t i0 = prefix > j0 ? 0 : j0;
@@ -423,12 +368,27 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
     dk[d] = float16v{};
     dv[d] = float16v{};
   }
+  float factor = DT == JKV_F16 ? kFirstDs : 1.f;  // of the lane's key
   const TileAt tile_lane = tile_at<D>(lds_base, lane);
   const int32_t key = wj0 + ln;
   // rows [key_from, key_from + key_rows) see the lane's key
   const int32_t key_from = key < prefix ? 0 : key;
   int32_t key_upto = key >= a.sinks && key + a.window < T0 ? key + a.window : T0;
   const uint32_t key_rows = key_upto > key_from ? (uint32_t)(key_upto - key_from) : 0u;
+
+  // dk times what the keys' lanes hold: sums are of key 8(e/4) + 4lh + e%4
+  auto scale_keys = [&](float by) {
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+#pragma unroll
+      for (int e = 4 * q4; e < 4 * q4 + 4; ++e) {
+        const float of = __uint_as_float((uint32_t)__builtin_amdgcn_ds_bpermute(16 * lh + 4 * (8 * q4 + (e & 3)), (int)__float_as_uint(by)));
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) dk[d][e] *= of;
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (four at a time: all would take 16 registers)
+    }
+  };
 
   // A step's products in turn: S, dP, dv, dk, and beside each a few places' vector
   // instructions, fenced (the compiler else gathers each kind, and they overlap
@@ -480,8 +440,26 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
     auto lean = [&](int e) {
       float ds = sc[e] * dp[e];
       if constexpr (AGAIN) ds = is_seen(e) ? ds : 0.f;
-      df[e >> 3][e & 7] = (T)ds;
+      if constexpr (DT == JKV_F16) dp[e] = ds;
+      else df[e >> 3][e & 7] = (T)ds;
     };
+    // the keys' factors less where a ds is too large for them
+    auto fit = [&]() {
+      float most = 0.f, other = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        most = fmaxf(fmaxf(most, fabsf(dp[e])), fabsf(dp[e + 1]));
+        other = fmaxf(fmaxf(other, fabsf(dp[e + 2])), fabsf(dp[e + 3]));
+      }
+      most = fmaxf(most, other);
+      if (__any(most > kMostDs)) {
+        const float by = ds_shrink(lanes2_max(most));
+        factor *= by;
+        dp *= by;
+        scale_keys(by);
+      }
+    };
+    auto round = [&](int e) { df[e >> 3][e & 7] = (T)dp[e]; };
     read(0);
     read(1);
 #pragma unroll
@@ -513,19 +491,31 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
         }
       } else {
         constexpr int kEach = 8 / kDims;
-        const int m = (n - 2 * kSteps) % (2 * kDims), d = m % kDims, st = m / kDims;
+        constexpr int m = (n - 2 * kSteps) % (2 * kDims), d = m % kDims, st = m / kDims;
         if (n < 2 * kSteps + 2 * kDims) {
           dv[d] = mfma32<DT>(pf[st], operand(n), dv[d]);
 #pragma unroll
           for (int e = d * kEach; e < (d + 1) * kEach; ++e) {
-            if (st == 0) weigh(8 + e);
-            else lean(e);
+            if (st == 0) {
+              weigh(8 + e);
+            } else {
+              lean(e);
+              if constexpr (DT == JKV_F16) lean(8 + e);
+            }
+          }
+          if constexpr (DT == JKV_F16 && m == 2 * kDims - 1) {
+            fit();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) round(e);
           }
         } else {
           dk[d] = mfma32<DT>(df[st], operand(n), dk[d]);
           if (st == 0)
 #pragma unroll
-            for (int e = d * kEach; e < (d + 1) * kEach; ++e) lean(8 + e);
+            for (int e = d * kEach; e < (d + 1) * kEach; ++e) {
+              if constexpr (DT == JKV_F16) round(8 + e);
+              else lean(8 + e);
+            }
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -603,7 +593,6 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
     load_next(other);
   };
   load_next(edge & 1);  // (so that the full tiles start in stage 0)
-  factor = ds_factor<DT, D>(a);
 #pragma unroll
   for (int c = 0; c < kSteps; ++c) asm volatile("" : "+v"(kf[c]));  // waited for here, with all loads before
   if constexpr (ALONE) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the values have landed
@@ -641,6 +630,7 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
       dk[d] = float16v{};
       dv[d] = float16v{};
     }
+    if constexpr (DT == JKV_F16) factor = kFirstDs;
     auto meet = [&]() {
       if constexpr (ALONE) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -658,7 +648,10 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
   }
 
   // lane holds dim 32d + ln of keys 8(e/4) + 4lh + e%4
-  const float dv_mul = 0x1p-10f, dk_mul = a.scale * (FORM & kFormCap ? 4.f : 1.f) * 0x1p-10f / factor;
+  const float dv_mul = 0x1p-10f, dk_mul = a.scale * (FORM & kFormCap ? 4.f : 1.f) * 0x1p-10f;
+  if constexpr (DT == JKV_F16) {
+    scale_keys(1.f / factor);
+  }
   if constexpr (ALONE) {
     __syncthreads();
     float* sums = (float*)(lds + kValues);  // [wave][dk, dv][dims / 32][e][lane]
@@ -779,8 +772,11 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
       dof[c] = *(const V8*)(dp + 32 * c);
     }
   }
-  const float base = a.bases[(int64_t)head * a.N + row0 + self], minus_delta = a.minus_delta[(int64_t)head * a.N + row0 + self];
-  const float factor = ds_factor<DT, D>(a);
+  float base = a.bases[(int64_t)head * a.N + row0 + self];
+  const float minus_delta = a.minus_delta[(int64_t)head * a.N + row0 + self];
+  const float first_base = DT == JKV_F16 ? base + 54.f : base;
+  base = first_base;
+  float factor = DT == JKV_F16 ? kFirstDs : 1.f;  // what of base is ds's, of the lane's row
   const ScoreShape shape = score_shape<FORM>(a, head);
 
   // entries [seen_from, seen_from + seen_count) are seen, and those before `sunk`
@@ -824,13 +820,37 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
       float p = __builtin_amdgcn_exp2f(x);
       if constexpr (MASKED) p = is_seen(half, e) ? p : 0.f;
       if constexpr (FORM & kFormCap) p *= slant;
-      if constexpr (DT == JKV_F16) p *= factor;
       sc[half][e] = p;
     };
     auto lean = [&](int half, int e) {
       float ds = sc[half][e] * (dp[half][e] + minus_delta);
       if constexpr (AGAIN) ds = is_seen(half, e) ? ds : 0.f;
-      df[half][e >> 3][e & 7] = (T)ds;
+      if constexpr (DT == JKV_F16) dp[half][e] = ds;
+      else df[half][e >> 3][e & 7] = (T)ds;
+    };
+    // 8 places' ds as fp16, the rows' factors less where they are too large
+    auto fit = [&](int half, int st) {
+      float most = 0.f;
+#pragma unroll
+      for (int e = 8 * st; e < 8 * st + 8; e += 2) most = fmaxf(fmaxf(most, fabsf(dp[half][e])), fabsf(dp[half][e + 1]));
+      if (__any(most > kMostDs)) {
+        const float by = ds_shrink(lanes2_max(most));
+        factor *= by;
+        base = first_base + (float)(__builtin_amdgcn_frexp_expf(factor) - 55);
+#pragma unroll
+        for (int e = 8 * st; e < 8 * st + 8; ++e) dp[half][e] *= by;
+        // what was weighed and not leaned yet, and what waits for its product
+        if (st == 0)
+#pragma unroll
+          for (int e = 8; e < 16; ++e) sc[half][e] *= by;
+        if (half == 0 && st == 1)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) df[0][0][e] = (T)((float)df[0][0][e] * by);
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) dq[d] *= by;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) df[half][st][e] = (T)dp[half][8 * st + e];
     };
     read(0);
     read(1);
@@ -839,7 +859,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
       constexpr int kEach = 16 / kSteps, kBeside = 8 / kDims;
       read(n + 2);
       if (n < 4 * kSteps) {
-        const int half = n / kBoth, m = n % kBoth, c = m % kSteps;
+        constexpr int half = n / kBoth, m = n % kBoth, c = m % kSteps;
         if (m < kSteps) sc[half] = mfma32<DT>(ring[n % 3], qf[c], sc[half]);
         else dp[half] = mfma32<DT>(ring[n % 3], dof[c], dp[half]);
 #pragma unroll
@@ -848,8 +868,9 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
           if (half == 1 && m < kSteps) weigh(0, e);
           if (half == 1 && m >= kSteps) lean(0, e);
         }
+        if constexpr (DT == JKV_F16 && half == 1 && m >= kSteps && (c + 1) * kEach % 8 == 0) fit(0, (c + 1) * kEach / 8 - 1);
       } else {
-        const int m = n - 4 * kSteps, d = m % kDims, st = m / kDims;
+        constexpr int m = n - 4 * kSteps, d = m % kDims, st = m / kDims;
         V8 keys = ring[n % 3];
         if constexpr (AGAIN) keys = finite_part<DT>(keys);
         dq[d] = mfma32<DT>(keys, df[st / 2][st % 2], dq[d]);
@@ -859,6 +880,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
           if (st == 1) { weigh(1, 8 + e); lean(1, e); }
           if (st == 2) lean(1, 8 + e);
         }
+        if constexpr (DT == JKV_F16 && (st == 1 || st == 2) && d == kDims - 1) fit(1, st - 1);
       }
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -937,6 +959,8 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   if (__syncthreads_or(odd != 0.f)) {
 #pragma unroll
     for (int d = 0; d < kDims; ++d) dq[d] = float16v{};
+    base = first_base;
+    if constexpr (DT == JKV_F16) factor = kFirstDs;
     auto meet = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     now = start;
     for (int32_t n = 0; n < pt.count; ++n) {

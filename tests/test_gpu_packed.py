@@ -602,3 +602,85 @@ def test_what_odd_elements_reach(device, cap, dtype, sizes, qh, kvh, dim, window
                 assert ((got - w).abs() <= bound)[finite].all(), (name, bad, part)
                 if (name, part) == ("d", "dv"):
                     assert torch.equal(torch.isnan(got), torch.isnan(w)) and torch.equal(got[~finite & ~torch.isnan(w)], w[~finite & ~torch.isnan(w)])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sizes,qh,kvh,dim", [
+    ([150, 90], 4, 2, 64),
+    ([200, 290], 4, 2, 128),
+    ([600, 40], 16, 2, 128),            # heads in splits
+    ([330, 250] * 6, 12, 12, 128),      # 128 keys a workgroup
+])
+@pytest.mark.parametrize("size", [2.0**-12, 1000.0])
+def test_gradients_beside_small_and_large_ones(device, dtype, sizes, qh, kvh, dim, size):
+    """A neighbour's sizes, a head's, or those of rows that are not seen change no bit."""
+
+    texts = Texts(51, sizes, qh, kvh, dim, dtype)
+    args = dict(window=100, softcap=25.0)
+    _, want = run_grads(texts, device, **args)
+
+    def moved(change):
+        other = Texts(51, sizes, qh, kvh, dim, dtype)
+        change(other)
+        return run_grads(other, device, **args)[1]
+
+    def neighbour(t):
+        for a, b in t.spans[1::2]:
+            t.d[a:b] *= size
+            t.v[a:b] *= min(size, 100.0)
+
+    got = moved(neighbour)
+    for x, y in zip(got, want):
+        for a, b in texts.spans[::2]:
+            assert torch.equal(x[a:b], y[a:b])
+    # heads of the other kv head
+    got = moved(lambda t: (t.d[:, qh // kvh :].mul_(size), t.v[:, 1:].mul_(min(size, 100.0))))
+    assert torch.equal(got[0][:, : qh // kvh], want[0][:, : qh // kvh])
+    assert torch.equal(got[1][:, 0], want[1][:, 0]) and torch.equal(got[2][:, 0], want[2][:, 0])
+    # do of the last rows of the first sequence: of the others' dq, and of keys out of their window
+    a, b = texts.spans[0]
+    cut = b - 25
+
+    def late(t):
+        t.d[cut:b] *= size
+
+    got = moved(late)
+    assert torch.equal(got[0][a:cut], want[0][a:cut])
+    for x, y in zip(got[1:], want[1:]):
+        assert torch.equal(x[a : cut - 99], y[a : cut - 99])
+
+    def late_values(t):
+        t.v[cut:b] *= min(size, 100.0)
+
+    got = moved(late_values)
+    assert torch.equal(got[0][a:cut], want[0][a:cut]) and torch.equal(got[1][a : cut - 99], want[1][a : cut - 99])
+
+
+@pytest.mark.parametrize("cap", [None, 25.0])
+@pytest.mark.parametrize("qh,kvh,dim,rows", [(4, 2, 64, 400), (16, 2, 128, 600)])
+def test_gradients_keep_their_digits_beside_outliers(device, cap, qh, kvh, dim, rows):
+    """fp16: one row of do at the end of its type's range, one of values far above the
+    others; what neither reaches is as exact as without them (the largest of a row's or
+    key's own ds is the measure: 2^-32 of it, and half a step of a result below 2^-14)."""
+
+    texts = Texts(52, [rows], qh, kvh, dim, torch.float16)
+    texts.d *= 2.0**-4
+    texts.d[200] = 60000.0 * torch.sign(texts.d[200].float()).half()
+    texts.v[50] *= 2000.0
+    out, grads = run_grads(texts, device, window=60, softcap=cap)
+    r = texts.expect(grads=True, cap=cap, window=60)[0]
+    far = torch.ones(rows, dtype=torch.bool)
+    far[50:110] = False   # rows that see the values
+    far[200] = False
+    keys = torch.ones(rows, dtype=torch.bool)
+    keys[0:110] = False   # keys that those rows see
+    keys[141:201] = False
+    h = half_step(torch.float16)
+    for name, got, kept in zip(("dq", "dk", "dv"), grads, (far, keys, keys)):
+        off = float(score_slack(r, dim, cap, None, rows)[far].max()) * 2 + (dim + rows) * 2.0**-23 + (2.0**-21 if cap else 0.0)
+        size = r[name + "_size"][kept]
+        bound = h * r[name][kept].abs() + (h + 2.0**-22) * r[name + "_slack"][kept] + (off + 1e-7) * size + 2.0**-25 + (
+            (2.0**-32 * 60 * size.amax() if name != "dv" else 2.0**-34 * size.amax()))
+        assert ((got.cpu().double()[kept] - r[name][kept]).abs() <= bound).all(), name
+        # and in the mean a rounding or two of 2^-11
+        assert float((got.cpu().double()[kept] - r[name][kept]).norm() / r[name][kept].norm()) < 2.0**-11

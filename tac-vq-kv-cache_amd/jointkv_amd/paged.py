@@ -424,6 +424,7 @@ class PagedStep:
     tokens: int
     max_new: int
     max_length: int
+    new: tuple[int, ...] | None = None  # new tokens of every sequence
 
 
 def _turned(tensor: torch.Tensor, rule: RotaryRule, step: PagedStep) -> torch.Tensor:
@@ -576,7 +577,7 @@ class PagedKVCache:
         self._lengths = after
         self._positions = [p + n for p, n in zip(self._positions, new)]
         step = PagedStep(self.block_tables, ints[:batch], None if single else ints[2 * batch :],
-                         ints[batch : 2 * batch], starts[-1], max(new), max(after))
+                         ints[batch : 2 * batch], starts[-1], max(new), max(after), tuple(new))
         # Who keeps a page may have fewer entries there than who left it, and writes over
         # theirs: a cancelled step takes them from the longest copy.
         back = {}
@@ -636,7 +637,9 @@ class PagedKVCache:
 
         if query.shape[0] != step.tokens:
             raise ValueError(f"the step has {step.tokens} new tokens, got {query.shape[0]}")
-        if (slopes is not None or prefixes is not None) and self._lengths != self._positions:
+        if (slopes is not None or prefixes is not None) and self._lengths != self._positions and any(
+                length != position and (step.new is None or step.new[b])
+                for b, (length, position) in enumerate(zip(self._lengths, self._positions))):
             raise ValueError("distances and prefixes count entries: not of sequences that had some evicted")
         if rule is not None:
             query, rope_theta = _turned(query, rule, step), None

@@ -501,3 +501,21 @@ def test_tangents_are_refused():
             jkv.rotary(q, k)
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(lambda x: jkv.rotary(x), (q,), (q,))
+
+
+def test_distances_beside_an_idle_sequence_with_evicted_entries(copies, monkeypatch):
+    """Only the sequences that a step attends for must have all their entries."""
+
+    calls = []
+    monkeypatch.setattr(jkv.paged, "paged_attention", lambda *args, **form: calls.append(form))
+    cache = cache_of()
+    cache.begin([20, 20, 0, 0])
+    cache._positions = [25, 20, 0, 0]  # (as an eviction leaves them)
+    step = cache.begin([0, 3, 5, 0])
+    for form in (dict(slopes=torch.zeros(2)), dict(prefixes=ints(0, 0, 0, 0))):
+        cache.attention(0, step, torch.zeros(8, 2, 64).half(), **form)
+    assert len(calls) == 2
+    step = cache.begin([1, 0, 1, 0])
+    for form in (dict(slopes=torch.zeros(2)), dict(prefixes=ints(0, 0, 0, 0))):
+        with pytest.raises(ValueError, match="evicted"):
+            cache.attention(0, step, torch.zeros(2, 2, 64).half(), **form)

@@ -479,6 +479,7 @@ class PagedKVCache:
                          for _ in range(layers)] if track_weights else None)
         self._free = list(range(pages - 1, -1, -1))
         self._uses = [0] * pages  # sequences that list a page
+        self._shared = 0  # sum of the uses beyond each page's first
         self._pages: list[list[int]] = [[] for _ in range(sequences)]
         self._lengths = [0] * sequences
         self._positions = [0] * sequences
@@ -519,6 +520,8 @@ class PagedKVCache:
             self._uses[page] -= 1
             if not self._uses[page]:
                 self._free.append(page)
+            else:
+                self._shared -= 1
 
     def begin(self, new_tokens: Sequence[int]) -> PagedStep:
         """Take pages for ``new_tokens[b]`` more entries of every sequence b
@@ -537,7 +540,7 @@ class PagedKVCache:
         # half-written last pages that another sequence still reads: whoever
         # writes first, until one is left, takes a copy
         uses, copied, kept = {}, [], {}
-        for b, (length, n, row) in enumerate(zip(self._lengths, new, self._pages)):
+        for b, (length, n, row) in enumerate(zip(self._lengths, new, self._pages) if self._shared else ()):
             if n and length % self.page_size:
                 page = row[-1]
                 count = uses.get(page, self._uses[page])
@@ -568,6 +571,7 @@ class PagedKVCache:
                 self._uses[page] -= 1
             for page in taken:
                 self._uses[page] = 1
+            self._shared -= len(left)
         starts = [0]
         for n in new:
             starts.append(starts[-1] + n)
@@ -581,9 +585,10 @@ class PagedKVCache:
         # Who keeps a page may have fewer entries there than who left it, and writes over
         # theirs: a cancelled step takes them from the longest copy.
         back = {}
-        for page, copy, n in sorted(zip(left, taken, held), key=lambda x: x[2]):
-            if n > kept.get(page, n):
-                back[page] = copy, page, n
+        if kept:
+            for page, copy, n in sorted(zip(left, taken, held), key=lambda x: x[2]):
+                if n > kept.get(page, n):
+                    back[page] = copy, page, n
         self._begun = (step.lengths, *before, taken, left, list(back.values()))
         return step
 
@@ -612,6 +617,7 @@ class PagedKVCache:
             self._uses[page] = 0
         for page in left:
             self._uses[page] += 1
+        self._shared += len(left)
         self._lengths, self._positions, self._pages, self._begun = lengths, positions, pages, None
 
     def append(self, layer: int, step: PagedStep, key: torch.Tensor, value: torch.Tensor, *,
@@ -757,6 +763,7 @@ class PagedKVCache:
         self._pages = pages
         for page in pages[target]:
             self._uses[page] += 1
+        self._shared += len(pages[target])
         self._lengths = list(self._lengths)
         self._positions = list(self._positions)
         self._lengths[target] = length

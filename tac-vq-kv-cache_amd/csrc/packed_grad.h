@@ -7,8 +7,8 @@
 // Three launches: the rows' delta and base-2 log-sum-exps; dk and dv, a workgroup
 // a block of keys that walks the rows that see it, of all heads of the group in
 // turn; dq, a workgroup a block of (token, head) rows that walks the keys.  A fourth
-// joins the heads' sums where they were split.  Scores are formed in both walks:
-// seven products in place of five, and no sum waits on another workgroup or on the
+// joins the heads' sums where they were split.  Scores are formed in both walks, and ds
+// has two parts: nine products in place of five, and no sum waits on another workgroup or on the
 // order of atomics.
 //
 // 21,760 bf16 tokens of three texts, 32/8 heads of 128, capped scores, window 4,096
@@ -20,11 +20,15 @@
 // as long.  48 texts of up to 511 fp16 tokens, 28/4 heads of 64: 40, 114 to 120 and 89
 // us, vector instructions, and masked tiles at both ends of short walks.
 //
-// p and ds enter their products rounded once to the inputs' type, p as 2^10 of
-// itself (fp16 holds 2^-34 of it then), ds in fp16 times a power of two of its row
-// (dq) or key (dk): from 2^64 on it falls as the largest ds passes 2^15, which then
-// is 2^7 to 2^8, and the sums with it.  So it follows from what a row sees, or what
-// sees a key, alone, and holds 2^-32 of the largest.
+// p enters its product rounded once to the inputs' type, as 2^10 of itself (fp16
+// holds 2^-34 of it then): dv is 1.35 to 1.45 times as far off as its own rounding.  ds
+// enters as a sum of two parts: a row's ds cancel, and one part's rounding left dq of
+// sharp heads 1.5 to 1.9 times its own off and dk 1.4 to 1.55; with two 1.0 to 1.4 and
+// 1.1 (the rest is delta's, from the rounded weights of the forward), for a product
+// more in each walk.  In fp16 ds takes a power of two of its row (dq) or key (dk): from
+// 2^64 on it falls as the largest ds passes 2^15, which then is 2^7 to 2^8, and the sums
+// with it.  So it follows from what a row sees, or what sees a key, alone, and holds
+// 2^-32 of the largest.
 //
 // A masked weight is 0, but 0 times an infinite or NaN row is not: whatever is not
 // finite in a tile, seen or not, makes the sums so.  A walk that ends in finite sums
@@ -407,7 +411,7 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
     const uint32_t stats_at = lds_base + 16u * (uint32_t)lh + stage_at + 2 * kTile;
     float16v sc = {}, dp;
     float4v bases[4];
-    V8 pf[2], df[2], ring[3], values[3];
+    V8 pf[2], df[2], dl[2], ring[3], values[3];
     auto read = [&](int n) {
       if (n < kSteps) ring[n % 3] = read_rows<DT, D>(rows, n, stage_at);
       else if (n < 2 * kSteps) {
@@ -437,11 +441,16 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
       if constexpr (DT == JKV_F16) p *= factor;
       sc[e] = p;
     };
+    // ds (in dp), and its two parts
     auto lean = [&](int e) {
-      float ds = sc[e] * dp[e];
-      if constexpr (AGAIN) ds = is_seen(e) ? ds : 0.f;
-      if constexpr (DT == JKV_F16) dp[e] = ds;
-      else df[e >> 3][e & 7] = (T)ds;
+      dp[e] *= sc[e];
+      if constexpr (AGAIN) dp[e] = is_seen(e) ? dp[e] : 0.f;
+    };
+    auto part = [&](int e) {
+#pragma clang fp contract(off)  // (fused with ds's product in one kind of tile, it would differ in another)
+      const T lead = (T)dp[e];
+      df[e >> 3][e & 7] = lead;
+      dl[e >> 3][e & 7] = (T)(dp[e] - (float)lead);
     };
     // the keys' factors less where a ds is too large for them
     auto fit = [&]() {
@@ -459,7 +468,6 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
         scale_keys(by);
       }
     };
-    auto round = [&](int e) { df[e >> 3][e & 7] = (T)dp[e]; };
     read(0);
     read(1);
 #pragma unroll
@@ -501,20 +509,22 @@ __global__ __launch_bounds__(256, ALONE && D == 128 ? 1 : 2) void packed_kv_grad
             } else {
               lean(e);
               if constexpr (DT == JKV_F16) lean(8 + e);
+              else part(e);
             }
           }
           if constexpr (DT == JKV_F16 && m == 2 * kDims - 1) {
             fit();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) round(e);
+            for (int e = 0; e < 8; ++e) part(e);
           }
         } else {
           dk[d] = mfma32<DT>(df[st], operand(n), dk[d]);
+          dk[d] = mfma32<DT>(dl[st], operand(n), dk[d]);
           if (st == 0)
 #pragma unroll
             for (int e = d * kEach; e < (d + 1) * kEach; ++e) {
-              if constexpr (DT == JKV_F16) round(8 + e);
-              else lean(8 + e);
+              if constexpr (DT != JKV_F16) lean(8 + e);
+              part(8 + e);
             }
         }
       }
@@ -797,7 +807,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
     // S^T and dP^T of each half of 32 entries, then its part of dq; fenced as above
     constexpr int kOps = 4 * kSteps + 4 * kDims, kBoth = 2 * kSteps;
     float16v sc[2] = {}, dp[2] = {};
-    V8 df[2][2], ring[3];
+    V8 df[2][2], dl[2][2], ring[3];
     auto read = [&](int n) {
       if (n < 4 * kSteps) {
         const int half = n / kBoth, m = n % kBoth;
@@ -822,13 +832,18 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
       if constexpr (FORM & kFormCap) p *= slant;
       sc[half][e] = p;
     };
-    auto lean = [&](int half, int e) {
-      float ds = sc[half][e] * (dp[half][e] + minus_delta);
-      if constexpr (AGAIN) ds = is_seen(half, e) ? ds : 0.f;
-      if constexpr (DT == JKV_F16) dp[half][e] = ds;
-      else df[half][e >> 3][e & 7] = (T)ds;
+    auto part = [&](int half, int e) {
+#pragma clang fp contract(off)
+      const T lead = (T)dp[half][e];
+      df[half][e >> 3][e & 7] = lead;
+      dl[half][e >> 3][e & 7] = (T)(dp[half][e] - (float)lead);
     };
-    // 8 places' ds as fp16, the rows' factors less where they are too large
+    auto lean = [&](int half, int e) {
+      dp[half][e] = sc[half][e] * (dp[half][e] + minus_delta);
+      if constexpr (AGAIN) dp[half][e] = is_seen(half, e) ? dp[half][e] : 0.f;
+      if constexpr (DT != JKV_F16) part(half, e);
+    };
+    // 8 places' ds in parts, the rows' factors less where they are too large
     auto fit = [&](int half, int st) {
       float most = 0.f;
 #pragma unroll
@@ -845,12 +860,15 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
           for (int e = 8; e < 16; ++e) sc[half][e] *= by;
         if (half == 0 && st == 1)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) df[0][0][e] = (T)((float)df[0][0][e] * by);
+          for (int e = 0; e < 8; ++e) {
+            df[0][0][e] = (T)((float)df[0][0][e] * by);
+            dl[0][0][e] = (T)((float)dl[0][0][e] * by);
+          }
 #pragma unroll
         for (int d = 0; d < kDims; ++d) dq[d] *= by;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) df[half][st][e] = (T)dp[half][8 * st + e];
+      for (int e = 8 * st; e < 8 * st + 8; ++e) part(half, e);
     };
     read(0);
     read(1);
@@ -874,6 +892,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
         V8 keys = ring[n % 3];
         if constexpr (AGAIN) keys = finite_part<DT>(keys);
         dq[d] = mfma32<DT>(keys, df[st / 2][st % 2], dq[d]);
+        dq[d] = mfma32<DT>(keys, dl[st / 2][st % 2], dq[d]);
 #pragma unroll
         for (int e = d * kBeside; e < (d + 1) * kBeside; ++e) {
           if (st == 0) weigh(1, e);

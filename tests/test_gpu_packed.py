@@ -684,3 +684,24 @@ def test_gradients_keep_their_digits_beside_outliers(device, cap, qh, kvh, dim, 
         assert ((got.cpu().double()[kept] - r[name][kept]).abs() <= bound).all(), name
         # and in the mean a rounding or two of 2^-11
         assert float((got.cpu().double()[kept] - r[name][kept]).norm() / r[name][kept].norm()) < 2.0**-11
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sizes,qh,kvh,dim,form,gain", [
+    ([129], 32, 8, 128, 1, 4.0), ([700], 8, 2, 128, 0, 8.0), ([700, 200], 7, 1, 64, 4, 6.0), ([60] * 10, 4, 4, 64, 2, 4.0)])
+def test_gradients_in_the_mean(device, dtype, sizes, qh, kvh, dim, form, gain):
+    """The error's norm against that of the exact results' own rounding.  For sharp heads
+    too, dq and dk add no rounding of that size (ds has two parts; delta takes the
+    forward's weights, whose roundings meet in one sum a row), out and dv one, of p:
+    the root of 2 where, as here, terms have signs at random."""
+
+    texts = Texts(61, sizes, qh, kvh, dim, dtype, gain=1.0)
+    texts.q = (texts.q.float() * gain).to(dtype)
+    texts.d = (texts.d.float() * 0.05).to(dtype)
+    want, call = form_of(texts, FORMS[form], qh, device)
+    out, grads = run_grads(texts, device, **call)
+    results = texts.expect(grads=True, **want)
+    for name, got, most in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), (1.5, 1.45, 1.3, 1.5)):
+        exact = torch.cat([r[name] for r in results])
+        own = (exact.to(dtype).double() - exact).norm()
+        assert (got.cpu().double() - exact).norm() <= most * own, (name, float((got.cpu().double() - exact).norm() / own))

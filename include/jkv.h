@@ -767,7 +767,9 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  * type (fp32 sums, one rounding), each NULL if not wanted.  o, lse and
  * rest (or NULL: gradients of bf16 rows are half as far off again) are the
  * forward's, d_out the gradient of o.  Rows that no sequence owns get 0.  Every
- * sum has one order.
+ * sum has one order.  Weights enter dv's products rounded to the inputs' type,
+ * score gradients theirs as two parts of it; a row's and a key's gradients follow
+ * from what it sees, or what sees it, alone.
  *   workspace    jkv_packed_backward_workspace_bytes() bytes, 16-byte aligned
  */
 int jkv_packed_attention_backward(

@@ -539,8 +539,9 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(PagedA
   // beside the products of the other half's scores or of the values, a product
   // and a few scores at a time, fenced, as the compiler else gathers each kind.
   // Three capped texts of 21,760 bf16 tokens in all, window 4,096, 32/8 heads of 128:
-  // 1,480 us, 705 TFLOP/s, vector instructions 69 % of the cycles, products 37 %, both
-  // at once 18 %, 1.85 GHz; 2,048 capped tokens over 8,192 entries in pages 357 us, 670.
+  // 1,440 to 1,480 us, 705 to 725 TFLOP/s, vector instructions 69 % of the cycles,
+  // products 37 %, both at once 18 %, 1.85 GHz; in pages 2,048 capped tokens over 8,192
+  // entries and one over 3,436 353 us, 680.
   auto work_shaped = [&](int32_t i, int32_t is, auto parity, auto again) {
     constexpr int buf = decltype(parity)::value;
     constexpr bool AGAIN = decltype(again)::value;

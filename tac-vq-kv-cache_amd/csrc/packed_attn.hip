@@ -40,11 +40,11 @@ static int packed_strides(const int64_t* strides, int count) {
 // traffic).  In steps of one head's 32 rows: the CUs' share of all walks, half the
 // longest walk for the end where not all CUs have one, and the join.  us of the
 // gradients of k and v with 1, 2 and 4 splits and with 32 keys, 32/8 heads of 128,
-// bf16: one sequence of 8,192 2,295, 2,079, 2,017 and 2,329; of 2,048 393, 254, 199
-// and 205; of 512 121, 83, 64 and 60; four of 2,048 657, 633, 645 and 739; eight of
-// 1,000 377, 384, 414 and 453; one of 4,096 with 8/8 heads 276 and (32 keys) 260; 48
-// texts of up to 511, 28/4 heads of 64, fp16, 259, 268, 278 and 229; 16/16 heads 181
-// and (32 keys) 244.  The choice is within 2 % of the least in 25 of 26 such, and 10 %
+// bf16: one sequence of 8,192 2,609, 2,370, 2,300 and 2,633; of 2,048 440, 282, 222
+// and 230; of 512 125, 87, 83 and 73; four of 2,048 742, 714, 723 and 808; eight of
+// 1,000 416, 423, 452 and 485; one of 4,096 with 8/8 heads 316 and (32 keys) 291; 48
+// texts of up to 511, 28/4 heads of 64, fp16, 275, 286, 300 and 248; 16/16 heads 191
+// and (32 keys) 258.  The choice is within 1 % of the least in 25 of 26 such, and 5 %
 // off it for two sequences of 8,192 with a window of 256 and heads of 64.
 PackedGradPlan packed_grad_plan(int64_t N, int64_t B, int64_t QH, int64_t KVH, int64_t D, int64_t window) {
   PackedGradPlan p = {};
@@ -119,8 +119,8 @@ int jkv_packed_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   // Blocks of 128 rows: vector instructions bound shaped scores, and two
   // workgroups a CU, which meet apart, overlap them with products better than one
   // of eight waves does (1.55 -> 1.46 ms for 21,760 bf16 tokens with a window of
-  // 4,096, 198 -> 180 us for four biased prompts; 1.48 and 173 since).  At most those of all sequences,
-  // and one that clears unowned rows.
+  // 4,096, 198 -> 180 us for four biased prompts; 1.44 and 175 now).  At most those of
+  // all sequences, and one that clears unowned rows.
   a.item_rows = 128;
   const int64_t items = std::min<int64_t>(B * ceil_div(N * a.per, 128), N * a.per / 128 + B) + 1;
   JKV_CHECK_GRID(items * KVH, 2 * a.item_rows);

@@ -12,13 +12,13 @@
 // order of atomics.
 //
 // 21,760 bf16 tokens of three texts, 32/8 heads of 128, capped scores, window 4,096
-// (5.2e11 flops a product): rows 115 us (560 MB, 4.9 TB/s), dk and dv 2,255 to 2,350
-// (four products, 930 TFLOP/s), dq 1,680 (three, 936).  Products fill 52 % of their
-// cycles, vector instructions 58 and 72, both at once 23 and 30; the clock falls to
-// 1.75 GHz, so more of either at once brings less than it seems.  dk and dv read 5.7
-// GB; walks that start at one place of the window for all blocks read 2.3 GB and take
-// as long.  48 texts of up to 511 fp16 tokens, 28/4 heads of 64: 40, 114 to 120 and 89
-// us, vector instructions, and masked tiles at both ends of short walks.
+// (5.2e11 flops a product): rows 115 us (560 MB, 4.9 TB/s), dk and dv 2,510 (five
+// products, 1,035 TFLOP/s), dq 1,945 (four, 1,070).  Products fill 57 and 59 % of their
+// cycles, vector instructions 62 and 75, both at once 26 and 34; the clock falls to
+// 1.77 GHz, so more of either at once brings less than it seems.  dk and dv read 5.8
+// GB; walks that start at one place of the window for all blocks read 2.3 GB and took
+// as long.  48 texts of up to 511 fp16 tokens, 28/4 heads of 64: 40, 128 and 123 us,
+// vector instructions, and masked tiles at both ends of short walks.
 //
 // p enters its product rounded once to the inputs' type, as 2^10 of itself (fp16
 // holds 2^-34 of it then): dv is 1.35 to 1.45 times as far off as its own rounding.  ds

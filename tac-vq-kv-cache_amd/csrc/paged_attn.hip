@@ -217,9 +217,13 @@ int jkv_paged_attention_shaped(const void* q, int64_t q_stride_t, int64_t q_stri
                 "paged attention needs an aligned workspace of %lld bytes, got %lld", (long long)p.bytes,
                 (long long)workspace_bytes);
   if (form != kFormPlain && p.item_rows == 256) {
-    // Shaped scores are bound by vector instructions, and four-wave blocks, two a
-    // CU, overlap those with products better (2 x 2,048 capped bf16 tokens over 8,192
-    // entries 374 -> 343 us); they are enough to need no splits.
+    // Shaped scores are bound by vector instructions, and four-wave blocks, two a CU,
+    // overlap those with products where the blocks of 256 rows are few or part full.  us
+    // with 128 rows and with 256, capped bf16, 32/8 heads of 128: 2,048 tokens over 8,192
+    // entries 304 and 319, with one token over 3,436 beside them 332 and 326, 2 x 2,048
+    // over 8,192 584 and 565, 40 x 10 over 4,096 157 and 195, 60 x 10 over 16,384 694 and
+    // 764.  Without the two splits that the plan may have made for blocks of 256, and
+    // with them: 2,048 over 8,192 304 and 338, 40 x 10 over 16,384 590 and 573.
     p.item_rows = 128;
     p.items = std::min<int64_t>(B * ceil_div(max_new * (QH / KVH), 128), N * (QH / KVH) / 128 + B);
     p.splits = 1;

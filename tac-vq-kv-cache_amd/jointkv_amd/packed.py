@@ -7,7 +7,8 @@ length packed without padding (each sees itself alone), fp16 or bf16, scores
 capped or biased by distance, prefixes seen from both sides, first tokens that
 stay visible behind a window.  Queries and keys come turned
 (:func:`jointkv_amd.rotary`).  It is what a prompt needs before there is a cache,
-and differentiable, what calibration needs.
+and differentiable, for a caller's own training or calibration loop (the
+closed-loop modules of this package call :func:`jointkv_amd.prefill_attention`).
 """
 
 from __future__ import annotations
@@ -123,8 +124,12 @@ def packed_attention(
     Returns ``[N,QH,D]`` (``out``, if given, which must not share memory with the
     inputs); rows that no sequence owns are 0, their ``lse`` and gradients -inf
     and 0.  Rows and gradients depend on what they see alone, whatever lies in
-    other places.  Scores and sums are 32-bit, weights enter the second product
-    rounded once to the inputs' type, and their sum as rounded divides it.
+    other places; infinite and NaN elements reach what the formulas say.  Scores
+    and sums are 32-bit, a cap c within 2e-7 c.  Weights enter the second product
+    rounded once to the inputs' type, and their sum as rounded divides it; so they
+    do in the values' gradient, and score gradients enter theirs as two parts:
+    outputs and gradients are at most about 1.5 times as far off, in norm, as
+    their own rounding.
     Differentiable in ``query``, ``key`` and ``value`` (not with a given ``out``), once
     and in reverse: ``create_graph`` and tangents are refused.  A call repeats bit for
     bit, its gradients too.

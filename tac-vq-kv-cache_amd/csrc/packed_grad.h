@@ -8,8 +8,8 @@
 // a block of keys that walks the rows that see it, of all heads of the group in
 // turn; dq, a workgroup a block of (token, head) rows that walks the keys.  A fourth
 // joins the heads' sums where they were split.  Scores are formed in both walks, and ds
-// has two parts: nine products in place of five, and no sum waits on another workgroup or on the
-// order of atomics.
+// has two parts: nine products in place of five, and no sum waits on another workgroup
+// or on the order of atomics.
 //
 // 21,760 bf16 tokens of three texts, 32/8 heads of 128, capped scores, window 4,096
 // (5.2e11 flops a product): rows 115 us (560 MB, 4.9 TB/s), dk and dv 2,510 (five
@@ -782,7 +782,8 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
       dof[c] = *(const V8*)(dp + 32 * c);
     }
   }
-  float base = a.bases[(int64_t)head * a.N + row0 + self];
+  // (lanes without a row weigh nothing)
+  float base = row_ok ? a.bases[(int64_t)head * a.N + row0 + self] : -INFINITY;
   const float minus_delta = a.minus_delta[(int64_t)head * a.N + row0 + self];
   const float first_base = DT == JKV_F16 ? base + 54.f : base;
   base = first_base;
@@ -975,7 +976,7 @@ __global__ __launch_bounds__(256, 2) void packed_q_grad_kernel(PackedGradArgs a)
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) odd = fmaf(dq[d][e], 0.f, odd);
-  if (__syncthreads_or(odd != 0.f)) {
+  if (__syncthreads_or(row_ok && odd != 0.f)) {
 #pragma unroll
     for (int d = 0; d < kDims; ++d) dq[d] = float16v{};
     base = first_base;
